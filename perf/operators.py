@@ -1,0 +1,372 @@
+"""What the operators next to the GEMM are timed on: the products of a layer and of its training step.
+
+A case is one pass through one operator, as a program calls it through ``Loader``:
+
+``linear``           C = act(A B + bias) + residual, the sum before the activation kept on request
+``linear_backward``  its gradients: of A, of B and of the bias
+``experts``          the same product for groups of rows, each with its own B (rows sorted by expert)
+``experts_backward`` its gradients
+``orthogonal``       an update brought near the closest orthogonal matrix by Newton-Schulz steps,
+                     alone or for a batch of matrices
+
+Sizes are those of the library's own configurations, tests and benchmark (projections, decode-like
+skinny shapes, ragged shapes, batches) and generic powers of two; ``draw`` spreads over the same
+ranges.
+"""
+import math
+import random
+
+import torch
+
+own = False
+
+DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+PAIRS = (("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"))  # (A and B, C)
+ACTIVATIONS = ("none", "relu", "silu", "gelu")
+#: the coefficients of the Newton-Schulz step: x -> a x + b x^3 + c x^5 on the singular values
+STEP = (3.4445, -4.7750, 2.0315)
+STEPS = 5
+MOST_FLOPS = 6e11  # no drawn case costs more than the largest listed one
+
+
+def _linear(kind, m, n, k, ab, c, layout, act, bias=True, residual=False, preact=False, groups=0, routing=0):
+    """layout: of B (K x N); c = column-major, weights stored N x K, r = row-major, stored K x N.
+    groups and routing (a seed): of the experts; the rows that each gets follow from the two and m."""
+    return {"kind": kind, "m": m, "n": n, "k": k, "ab": ab, "c": c, "layout": layout, "act": act, "bias": bias,
+            "residual": residual, "preact": preact, "groups": groups, "routing": routing}
+
+
+def _orthogonal(m, n, batch, given, c):
+    return {"kind": "orthogonal", "m": m, "n": n, "batch": batch, "ab": given, "c": c}
+
+
+def listed():
+    return [
+        # one token through an attention output projection: a call's latency
+        dict(_linear("linear", 1, 1024, 1024, "f16", "f16", "c", "none", residual=True),
+             name="linear_token_1x1024x1024_f16"),
+        # decode: a batch of sequences through a down projection, weights from memory
+        dict(_linear("linear", 32, 4096, 14336, "bf16", "bf16", "c", "none", bias=False, residual=True),
+             name="linear_decode_32x4096x14336_bf16"),
+        # prefill of one prompt of an odd length through an up projection
+        dict(_linear("linear", 777, 28672, 8192, "bf16", "bf16", "c", "gelu"),
+             name="linear_prefill_777x28672x8192_bf16"),
+        # odd in every extent, weights stored K x N, logits kept in 32 bits
+        dict(_linear("linear", 1999, 1001, 999, "f16", "f32", "r", "relu"),
+             name="linear_ragged_1999x1001x999_f16_f32"),
+        # training: the backward of a projection with its activation
+        dict(_linear("linear_backward", 4096, 5120, 5120, "bf16", "bf16", "c", "gelu"),
+             name="linear_backward_4096x5120x5120_bf16"),
+        # decode: a few tokens, most experts without a row
+        dict(_linear("experts", 16, 2048, 4096, "f16", "f16", "c", "silu", bias=False, groups=64, routing=1),
+             name="experts_decode_16_of_64_2048x4096_f16"),
+        # prefill of an odd number of tokens over many small experts
+        dict(_linear("experts", 4099, 2048, 4096, "bf16", "bf16", "c", "silu", groups=32, routing=2),
+             name="experts_prefill_4099_32_2048x4096_bf16"),
+        # training: forward of a few large experts, the sums before the activation kept
+        dict(_linear("experts", 8192, 8192, 4096, "f16", "f16", "r", "gelu", preact=True, groups=8, routing=3),
+             name="experts_train_8192_8_8192x4096_f16"),
+        # training: backward of the experts
+        dict(_linear("experts_backward", 8192, 4096, 2048, "bf16", "bf16", "c", "silu", groups=16, routing=4),
+             name="experts_backward_8192_16_4096x2048_bf16"),
+        # training with gradients kept in 32 bits, rows that leave some experts nearly empty
+        dict(_linear("experts_backward", 3001, 1024, 512, "bf16", "f32", "r", "none", groups=24, routing=5),
+             name="experts_backward_3001_24_1024x512_bf16_f32"),
+        # an optimiser's step on a square weight
+        dict(_orthogonal(4096, 4096, 1, "f32", "bf16"), name="orthogonal_4096x4096_f32_bf16"),
+        # and on a batch of small ones, of odd sizes
+        dict(_orthogonal(1001, 520, 16, "bf16", "bf16"), name="orthogonal_16x1001x520_bf16"),
+    ]
+
+
+def _spread(rng, low, high, grain=1):
+    """A size between low and high, spread over its logarithm, a multiple of grain."""
+    x = 0
+    while x in (0, 3072):
+        x = max(grain, int(round(math.exp(rng.uniform(math.log(low), math.log(high))) / grain)) * grain)
+    return x
+
+
+def draw(rng):
+    ab, c = PAIRS[rng.randrange(4)]
+    # most programs keep features on multiples of 64; some only on 8; a few not at all
+    grain = rng.choice((64, 64, 64, 8, 8, 1))
+    kind = rng.choice(("linear", "linear", "linear_backward", "experts", "experts", "experts_backward", "orthogonal"))
+    if kind == "orthogonal":
+        batch = rng.choice((1, 1, _spread(rng, 2, 32)))
+        m, n = (_spread(rng, 64, 4096, grain) for _ in range(2))
+        while batch > 1 and (batch * m * n > 1 << 24 or _flops_orthogonal(m, n, batch) > MOST_FLOPS):
+            batch -= 1
+        return _orthogonal(m, n, batch, rng.choice(("f32", "bf16", "f16")), rng.choice(("bf16", "f16")))
+    backward = kind.endswith("backward")
+    act = rng.choice(ACTIVATIONS)
+    if backward and c == "f32":
+        # what the activation lets through is rounded to A's type before it is multiplied
+        act = "none"
+    groups, routing = 0, 0
+    if kind.startswith("experts"):
+        groups, routing = _spread(rng, 2, 128), rng.randrange(1 << 20)
+        n, k = (_spread(rng, 256, 8192, grain) for _ in range(2))
+        while groups * n * k > 1 << 29:
+            n, k = (n // 2, k) if n > k else (n, k // 2)
+            n, k = (max(grain, x // grain * grain) for x in (n, k))
+        m = _spread(rng, 128, 16384) if backward or rng.random() < 0.6 else _spread(rng, 1, 127)
+    else:
+        n, k = (_spread(rng, 512, 16384, grain) for _ in range(2))
+        m = _spread(rng, 128, 8192) if backward or rng.random() < 0.5 else _spread(rng, 1, 127)
+    while (4.0 if backward else 2.0) * m * n * k > MOST_FLOPS:
+        m = max(1, m // 2)
+    return _linear(kind, m, n, k, ab, c, rng.choice("rc"), act, bias=rng.random() < 0.7,
+                   residual=not backward and rng.random() < 0.5,
+                   preact=not backward and act != "none" and rng.random() < 0.4, groups=groups, routing=routing)
+
+
+def _rows_of(case):
+    """How many of the rows each expert gets: a popularity that differs from expert to expert, then chance."""
+    rng = random.Random("%d %d %d" % (case["groups"], case["routing"], case["m"]))
+    popular = [math.exp(rng.gauss(0.0, 0.7)) for _ in range(case["groups"])]
+    rows = [0] * case["groups"]
+    for e in rng.choices(range(case["groups"]), popular, k=case["m"]):
+        rows[e] += 1
+    return rows
+
+
+def _normal(generator, shape, dtype, scale=1.0):
+    x = torch.empty(shape, dtype=torch.float32, device="cuda").normal_(0.0, scale, generator=generator)
+    return x.to(dtype)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    ab, c = DTYPES[case["ab"]], DTYPES[case["c"]]
+    state = dict(case)
+    if own:
+        import rocm_wmma_gemm_amd as R
+
+        state["loader"] = R.Loader()
+        state["codes"] = {"r": R.row_major, "c": R.col_major}
+        state["activations"] = {name: R.activation[name] for name in ACTIVATIONS}
+    m, n = case["m"], case["n"]
+    if case["kind"] == "orthogonal":
+        # a momentum: a few strong directions over noise
+        rank = max(1, min(m, n) // 32)
+        strong = _normal(g, (case["batch"], m, rank), torch.float32) @ _normal(g, (case["batch"], rank, n), torch.float32)
+        state["given"] = (1e-3 * (strong / math.sqrt(rank) + _normal(g, (case["batch"], m, n), torch.float32))).to(ab)
+        state["out"] = torch.empty((case["batch"], m, n), dtype=c, device="cuda")
+        return state
+    k, groups = case["k"], case["groups"]
+    lead = (groups,) if groups else ()
+    weight = (n, k) if case["layout"] == "c" else (k, n)
+    backward = case["kind"].endswith("backward")
+    state["a"] = _normal(g, (m, k), ab)
+    state["b"] = _normal(g, lead + weight, ab, 1.0 / math.sqrt(k))
+    state["bias"] = _normal(g, lead + (n,), ab, 0.5) if case["bias"] and not backward else None
+    state["residual"] = _normal(g, (m, n), c) if case["residual"] else None
+    if groups:
+        rows = _rows_of(case)
+        ends = [0]
+        for r in rows:
+            ends.append(ends[-1] + r)
+        state["offsets"] = torch.tensor(ends, dtype=torch.int32, device="cuda")
+        state["most"] = max(rows)
+    if backward:
+        state["dc"] = _normal(g, (m, n), ab)
+        state["z"] = _normal(g, (m, n), ab) if case["act"] != "none" else None
+    if backward:
+        state["da"] = torch.empty((m, k), dtype=c, device="cuda")
+        state["db"] = torch.empty(lead + weight, dtype=c, device="cuda")
+        state["dbias"] = torch.empty(lead + (n,), dtype=c, device="cuda") if case["bias"] else None
+    else:
+        state["out"] = torch.empty((m, n), dtype=c, device="cuda")
+        state["kept"] = torch.empty((m, n), dtype=ab, device="cuda") if case["preact"] else None
+    return state
+
+
+def _run_own(s):
+    loader = s["loader"]
+    if s["kind"] == "orthogonal":
+        loader.orthogonalize(s["out"], s["given"], s["m"], s["n"], s["batch"], steps=STEPS, coefficients=STEP)
+        return s["out"]
+    layout, act = s["codes"][s["layout"]], s["activations"][s["act"]]
+    m, n, k = s["m"], s["n"], s["k"]
+    if s["kind"] == "linear":
+        loader.linear(s["out"], s["a"], s["b"], m, n, k, layout, bias=s["bias"], residual=s["residual"],
+                      preact=s["kept"], activation=act)
+        return [s["out"], s["kept"]]
+    if s["kind"] == "experts":
+        loader.grouped(s["out"], s["a"], s["b"], s["offsets"], m, n, k, layout, bias=s["bias"],
+                       residual=s["residual"], preact=s["kept"], activation=act)
+        return [s["out"], s["kept"]]
+    if s["kind"] == "linear_backward":
+        loader.linear_backward(s["da"], s["db"], s["dbias"], s["dc"], s["a"], s["b"], m, n, k, layout,
+                               preact=s["z"], activation=act)
+    else:
+        loader.grouped_backward(s["da"], s["db"], s["dbias"], s["dc"], s["a"], s["b"], s["offsets"], m, n, k, layout,
+                                preact=s["z"], activation=act)
+    return [s["da"], s["db"], s["dbias"]]
+
+
+def _act(z, name):
+    if name == "relu":
+        return z.clamp_min(0.0)
+    if name == "silu":
+        return z * torch.sigmoid(z)
+    if name == "gelu":
+        return 0.5 * z * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * (z + 0.044715 * z * z * z)))
+    return z
+
+
+def _act_slope(z, name):
+    if name == "relu":
+        return (z > 0).to(z.dtype)
+    if name == "silu":
+        s = torch.sigmoid(z)
+        return s * (1.0 + z * (1.0 - s))
+    r = math.sqrt(2.0 / math.pi)
+    t = torch.tanh(r * (z + 0.044715 * z * z * z))
+    return 0.5 * (1.0 + t) + 0.5 * z * (1.0 - t * t) * r * (1.0 + 3.0 * 0.044715 * z * z)
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    s = state
+    ab, c = DTYPES[s["ab"]], DTYPES[s["c"]]
+    if s["kind"] == "orthogonal":
+        return _steps(s["given"].float()).to(c)
+    a, b = s["a"].float(), s["b"].float()
+    if s["layout"] == "c":
+        b = b.transpose(-1, -2)
+    groups, most = s["groups"], s.get("most")
+    if groups:
+        # every group padded to the longest: rows of `a` and their places there
+        row = torch.arange(s["m"], device="cuda")
+        group = torch.bucketize(row, s["offsets"][1:], right=True)
+        place = group * most + row - s["offsets"][group]
+
+        def pad(x):
+            wide = torch.zeros((groups * most, x.shape[1]), dtype=x.dtype, device="cuda")
+            wide[place] = x
+            return wide.view(groups, most, x.shape[1])
+
+        def unpad(x):
+            return x.reshape(groups * most, x.shape[2])[place]
+    if not s["kind"].endswith("backward"):
+        z = unpad(torch.bmm(pad(a), b)) if groups else a @ b
+        if s["bias"] is not None:
+            z = z + (s["bias"].float()[group] if groups else s["bias"].float())
+        y = _act(z, s["act"])
+        if s["residual"] is not None:
+            y = y + s["residual"].float()
+        return [y.to(c), z.to(ab) if s["preact"] else None]
+    dz = s["dc"].float()
+    if s["z"] is not None:
+        dz = dz * _act_slope(s["z"].float(), s["act"])
+    if groups:
+        wide = pad(dz)
+        da = unpad(torch.bmm(wide, b.transpose(1, 2)))
+        db = torch.bmm(pad(a).transpose(1, 2), wide)
+        dbias = wide.sum(1)
+    else:
+        da, db, dbias = dz @ b.t(), a.t() @ dz, dz.sum(0)
+    if s["layout"] == "c":
+        db = db.transpose(-1, -2).contiguous()
+    return [da.to(c), db.to(c), dbias.to(c) if s["bias"] else None]
+
+
+def _steps(x):
+    """The Newton-Schulz steps in x's own type, over a batch of matrices."""
+    a, b, c = STEP
+    x = x / (x.square().sum((1, 2), keepdim=True).sqrt() + 1e-7)
+    tall = x.shape[1] > x.shape[2]
+    x = x.transpose(1, 2).contiguous() if tall else x
+    for _ in range(STEPS):
+        s = torch.bmm(x, x.transpose(1, 2))
+        x = a * x + torch.bmm(b * s + c * torch.bmm(s, s), x)
+    return x.transpose(1, 2).contiguous() if tall else x
+
+
+def _flops_orthogonal(m, n, batch):
+    # per step: X X^T and its square are symmetric (half of each is enough), their sum times X is not
+    low, high = min(m, n), max(m, n)
+    return float(STEPS) * batch * (low * low * high + low * low * low + 2.0 * low * low * high)
+
+
+def work(case):
+    m, n = case["m"], case["n"]
+    out, given = (4 if case["c"] == "f32" else 2), (4 if case["ab"] == "f32" else 2)
+    if case["kind"] == "orthogonal":
+        return {"bytes": case["batch"] * m * n * (given + out), "flops": _flops_orthogonal(m, n, case["batch"])}
+    k, groups = case["k"], case["groups"]
+    used = sum(r > 0 for r in _rows_of(case)) if groups else 1
+    lead = groups or 1
+    if case["kind"].endswith("backward"):
+        read = 2 * (m * k + used * n * k + m * n * (1 if case["act"] == "none" else 2))
+        written = out * (m * k + lead * n * k + (lead * n if case["bias"] else 0))
+        return {"bytes": read + written, "flops": 4.0 * m * n * k}
+    read = 2 * (m * k + used * n * k + (used * n if case["bias"] else 0)) + (out * m * n if case["residual"] else 0)
+    return {"bytes": read + m * n * (out + (2 if case["preact"] else 0)), "flops": 2.0 * m * n * k}
+
+
+def exact(case, seed):
+    """What run() returns for these inputs by the definitions in float64, group by group."""
+    s = prepare(case, seed)
+    if case["kind"] == "orthogonal":
+        out = torch.empty(s["given"].shape, dtype=torch.float64, device="cuda")
+        for i in range(case["batch"]):
+            x = s["given"][i].double()
+            x = x / (torch.linalg.norm(x) + 1e-7)
+            for _ in range(STEPS):
+                if x.shape[0] <= x.shape[1]:
+                    p = x @ x.t()
+                    x = STEP[0] * x + STEP[1] * (p @ x) + STEP[2] * (p @ (p @ x))
+                else:
+                    p = x.t() @ x
+                    x = STEP[0] * x + STEP[1] * (x @ p) + STEP[2] * ((x @ p) @ p)
+            out[i] = x
+        return out
+    m, n, k, groups = case["m"], case["n"], case["k"], case["groups"]
+    rows = _rows_of(case) if groups else [m]
+    ends = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    b = s["b"].view((len(rows),) + s["b"].shape[-2:])
+    backward = case["kind"].endswith("backward")
+    new = lambda *shape: torch.zeros(shape, dtype=torch.float64, device="cuda")  # noqa: E731
+    slope = {"none": torch.ones_like, "relu": lambda z: torch.where(z > 0, 1.0, 0.0),
+             "silu": lambda z: (lambda e: (1 + e + z * e) / (1 + e) ** 2)(torch.exp(-z)),
+             "gelu": _gelu_slope}[case["act"]]
+    act = {"none": lambda z: z, "relu": lambda z: torch.where(z > 0, z, 0.0), "silu": lambda z: z / (1 + torch.exp(-z)),
+           "gelu": lambda z: z / (1 + torch.exp(-_gelu_inner(z)))}[case["act"]]
+    y, z_all, da, db, dbias = new(m, n), new(m, n), new(m, k), new(*b.shape), new(len(rows), n)
+    for e in range(len(rows)):
+        at = slice(ends[e], ends[e + 1])
+        a = s["a"][at].double()
+        w = b[e].double() if case["layout"] == "r" else b[e].double().t()
+        if backward:
+            dz = s["dc"][at].double()
+            if s["z"] is not None:
+                dz = dz * slope(s["z"][at].double())
+            da[at] = dz @ w.t()
+            db[e] = a.t() @ dz if case["layout"] == "r" else dz.t() @ a
+            dbias[e] = dz.sum(0)
+            continue
+        z = a @ w
+        if s["bias"] is not None:
+            z = z + s["bias"].view(len(rows), n)[e].double()
+        z_all[at] = z
+        y[at] = act(z)
+    if backward:
+        return [da, db.view(s["b"].shape), dbias.view(s["b"].shape[:-2] + (n,)) if case["bias"] else None]
+    if s["residual"] is not None:
+        y = y + s["residual"].double()
+    return [y, z_all if case["preact"] else None]
+
+
+def _gelu_inner(z):
+    return 2.0 * math.sqrt(2.0 / math.pi) * (z + 0.044715 * z ** 3)
+
+
+def _gelu_slope(z):
+    e = torch.exp(-_gelu_inner(z))
+    inner = 2.0 * math.sqrt(2.0 / math.pi) * (1.0 + 3.0 * 0.044715 * z ** 2)
+    return 1.0 / (1.0 + e) + z * inner * e / (1.0 + e) ** 2
