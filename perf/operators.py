@@ -272,7 +272,7 @@ def run(state):
         da, db, dbias = dz @ b.t(), a.t() @ dz, dz.sum(0)
     if s["layout"] == "c":
         db = db.transpose(-1, -2).contiguous()
-    return [da.to(c), db.to(c), dbias.to(c) if s["bias"] else None]
+    return [da.to(c), db.to(c), dbias.to(c) if s["dbias"] is not None else None]
 
 
 def _steps(x):
