@@ -208,6 +208,70 @@ int rocm_wmma_gemm_noalloc(int type_idx, void* C, void* A, void* B, size_t M, si
                            size_t batch_count, int layout_c, int layout_a, int layout_b,
                            void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Layer products: additions with no counterpart in the reference.
+ *
+ * A linear layer C = act(A B + bias) + residual on rows of activations, the same for groups of
+ * rows with a weight each (experts), and their gradients.  A (M x K), C (M x N) and the
+ * gradients of both are row-major; B (K x N) is row-major (layout_b 0) or column-major (1: weights
+ * stored N x K).  type_idx names the types of C and of A and B as above; bias has A's type,
+ * residual and dbias C's, preact (the sum before the activation, M x N) A's, as dC.  Everything is added up
+ * and activated in fp32, each output rounded once.  `stream` is the address of a hipStream_t;
+ * the calls enqueue and return.  M, N, K below 2^31; a size of 0 leaves the sums empty.
+ * --------------------------------------------------------------------------------------- */
+#define ROCM_WMMA_GEMM_ACT_NONE 0
+#define ROCM_WMMA_GEMM_ACT_RELU 1
+#define ROCM_WMMA_GEMM_ACT_SILU 2 /* x / (1 + e^-x) */
+#define ROCM_WMMA_GEMM_ACT_GELU 3 /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
+
+/* Most groups of one grouped call. */
+#define ROCM_WMMA_GEMM_MAX_GROUPS 1024
+
+typedef struct rocm_wmma_gemm_epilogue
+{
+    const void* bias; /* N values (grouped: N per group), or NULL */
+    const void* residual; /* M x N, added behind the activation, or NULL; may be C itself */
+    void*       preact; /* M x N, receives A B + bias, or NULL */
+    int         activation; /* ROCM_WMMA_GEMM_ACT_* */
+} rocm_wmma_gemm_epilogue;
+
+/* C = act(A B + bias) + residual.  epilogue may be NULL: C = A B. */
+int rocm_wmma_gemm_linear(int type_idx, void* C, const void* A, const void* B, size_t M, size_t N, size_t K,
+                          int layout_b, const rocm_wmma_gemm_epilogue* epilogue, void* stream);
+
+/* With dZ = dC act'(preact) (preact may be NULL for ROCM_WMMA_GEMM_ACT_NONE):
+ * dA = dZ B^T (M x K), dB = A^T dZ (in B's layout), dbias = sum of dZ's rows (N); a NULL result is not
+ * computed.  accumulate 1: dB and dbias are added to.  dZ is rounded to A's type before it is
+ * multiplied (not in dbias); it and the partial sums of dbias live in the library's scratch buffer, so a call
+ * on a capturing stream for which that buffer is too small returns ROCM_WMMA_GEMM_ERR_SCRATCH.
+ * (The gradient of the residual is dC.) */
+int rocm_wmma_gemm_linear_backward(int type_idx, void* dA, void* dB, void* dbias, const void* dC, const void* A,
+                                   const void* B, const void* preact, size_t M, size_t N, size_t K, int layout_b,
+                                   int activation, int accumulate, void* stream);
+
+/* The same for `groups` weights (B: groups x K x N, one after the other) and rows sorted by group:
+ * group e has rows offsets[e] .. offsets[e+1] - 1 of A and C.  offsets: groups + 1 ints on the
+ * device, not decreasing, within 0 .. M (values that break this are clamped).  A group may be empty:
+ * its weight is not read, its gradients are zero.  Rows before offsets[0] and from offsets[groups] on are not
+ * touched. */
+int rocm_wmma_gemm_grouped(int type_idx, void* C, const void* A, const void* B, const int* offsets, size_t groups,
+                           size_t M, size_t N, size_t K, int layout_b, const rocm_wmma_gemm_epilogue* epilogue,
+                           void* stream);
+int rocm_wmma_gemm_grouped_backward(int type_idx, void* dA, void* dB, void* dbias, const void* dC, const void* A,
+                                    const void* B, const void* preact, const int* offsets, size_t groups, size_t M,
+                                    size_t N, size_t K, int layout_b, int activation, int accumulate, void* stream);
+
+/* Newton-Schulz steps that bring an update near the closest matrix with orthonormal rows or
+ * columns (all singular values near 1): X = G / (|G|_F + epsilon), then `steps` times
+ * X = a X + (b S + c S^2) X with S = X X^T, coefficients = {a, b, c}; O = X.  G and O: batch_count
+ * row-major M x N matrices; G of type F16, BF16 or F32, O of type F16 or BF16.  M and N up to 2^20.
+ * Works in the library's scratch buffer (8 bytes an element and 4 min(M, N)^2 per matrix). */
+#define ROCM_WMMA_GEMM_ELEMENT_F16 0
+#define ROCM_WMMA_GEMM_ELEMENT_BF16 1
+#define ROCM_WMMA_GEMM_ELEMENT_F32 2
+int rocm_wmma_gemm_orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M, size_t N,
+                                 size_t batch_count, int steps, const float* coefficients, float epsilon, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,6 +10,7 @@ from .loader import (  # noqa: F401
     GemmLibraryError,
     Loader,
     VariantInfo,
+    activation,
     build_library,
     col_major,
     library_path,
@@ -18,5 +19,5 @@ from .loader import (  # noqa: F401
     source_stamp,
 )
 
-__all__ = ["Loader", "GemmLibraryError", "VariantInfo", "m_layout", "row_major", "col_major",
+__all__ = ["Loader", "GemmLibraryError", "VariantInfo", "m_layout", "row_major", "col_major", "activation",
            "library_path", "build_library", "source_stamp"]

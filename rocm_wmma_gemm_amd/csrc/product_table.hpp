@@ -1,0 +1,57 @@
+// Host-side view of the compiled layer-product kernels: entry points by type set, operand
+// layouts and form.  Defined in product_slice.hip, one translation unit per type set.
+#ifndef ROCM_WMMA_GEMM_PRODUCT_TABLE_HPP
+#define ROCM_WMMA_GEMM_PRODUCT_TABLE_HPP
+
+#include "kernel/product_common.hpp"
+
+namespace rocm_wmma_gemm
+{
+namespace host
+{
+
+using product_fn = void (*)(const device::product_args);
+
+// Types of (A and B, C, residual).  The first four are the library's type pairs, in their order;
+// the last four are the products of the Newton-Schulz steps.
+enum product_types
+{
+    types_f16_f16 = 0,
+    types_f32_f16,
+    types_bf16_bf16,
+    types_f32_bf16,
+    types_steps_square, // f16 -> f16, f16 residual
+    types_steps_next, // f16 -> fp32, fp32 residual
+    types_steps_f16, // f16 -> f16, fp32 residual
+    types_steps_bf16, // f16 -> bf16, fp32 residual
+    num_product_types
+};
+
+// Operand layouts: which of A and B have the summed dimension contiguous.
+enum product_layout
+{
+    layout_kk = 0, // both
+    layout_kn, // A; B is contiguous along N
+    layout_mn, // neither
+    num_product_layouts
+};
+
+enum product_form
+{
+    form_general_128 = 0, // 128 x 128 tiles, any alignment
+    form_general_64, // 64 x 64 tiles, any alignment
+    num_product_forms
+};
+
+struct product_kernel
+{
+    product_fn fn; // nullptr: not built
+    int        block_m, block_n, threads;
+};
+
+product_kernel find_product(int types, int layout, int form);
+
+} // namespace host
+} // namespace rocm_wmma_gemm
+
+#endif // ROCM_WMMA_GEMM_PRODUCT_TABLE_HPP

@@ -43,6 +43,23 @@ row_major = m_layout.row_major
 col_major = m_layout.col_major
 
 
+class activation(enum.IntEnum):
+    """What a linear layer applies to its sums (the codes of include/rocm_wmma_gemm_c.h)."""
+
+    none = 0
+    relu = 1
+    silu = 2  # x / (1 + e^-x)
+    gelu = 3  # the tanh form
+
+
+class _EpilogueC(ctypes.Structure):
+    _fields_ = [("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("preact", ctypes.c_void_p),
+                ("activation", ctypes.c_int)]
+
+
+MAX_GROUPS = 1024
+
+
 class _VariantInfoC(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in (
         "block_m", "block_n", "block_k", "warps_m", "warps_n", "warp_tile_m", "warp_tile_n",
@@ -188,6 +205,17 @@ class Loader:
         if hasattr(L, "rocm_wmma_gemm_noalloc"):
             L.rocm_wmma_gemm_noalloc.restype = ctypes.c_int
             L.rocm_wmma_gemm_noalloc.argtypes = [ctypes.c_int] + self._ENTRY_ARGS
+        if hasattr(L, "rocm_wmma_gemm_linear"):
+            p, z, i = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int
+            for name, args in (
+                    ("linear", [i, p, p, p, z, z, z, i, p, p]),
+                    ("linear_backward", [i] + [p] * 7 + [z] * 3 + [i] * 3 + [p]),
+                    ("grouped", [i, p, p, p, p, z, z, z, z, i, p, p]),
+                    ("grouped_backward", [i] + [p] * 8 + [z] * 4 + [i] * 3 + [p]),
+                    ("orthogonalize", [i, i, p, p, z, z, z, i, p, ctypes.c_float, p])):
+                fn = getattr(L, "rocm_wmma_gemm_" + name)
+                fn.restype = ctypes.c_int
+                fn.argtypes = args
 
     def library_arch(self) -> str:
         return self._lib.rocm_wmma_gemm_arch().decode()
@@ -296,3 +324,144 @@ class Loader:
         return self._lib.rocm_wmma_gemm_run_variant_ex(
             slot, variant, swizzle, split_k, touch_ahead, C.data_ptr(), A.data_ptr(), B.data_ptr(),
             M, N, K, batch_count, int(layout_c), int(layout_a), int(layout_b), ctypes.byref(handle))
+
+    # ------------------------------------------------------------------ layer products
+    _STATUS = {ERR_VARIANT: "no kernel for this problem", ERR_ARGUMENT: "an argument is out of range or missing",
+               ERR_SCRATCH: "no scratch memory (too much asked for, or the stream is capturing: size the "
+                            "library's buffer with one eager call first)",
+               ERR_RUNTIME: "the HIP runtime reported an error", ERR_LIMIT: "a size is beyond the library's limits"}
+
+    def _done(self, name, status):
+        if status != OK:
+            raise GemmLibraryError(f"rocm_wmma_gemm_{name}: {self._STATUS.get(status, status)}")
+
+    @staticmethod
+    def _held(name, t, need, dtype, like=None):
+        """Address of a packed device tensor that holds `need` elements of `dtype` (None: NULL)."""
+        if t is None:
+            return None
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a device tensor")
+        if like is not None and t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, the other operands on {like.device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be densely packed")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if t.numel() < need:
+            raise ValueError(f"{name} holds {t.numel()} elements, the problem needs {need}")
+        return t.data_ptr()
+
+    @staticmethod
+    def _sizes(**sizes):
+        for name, v in sizes.items():
+            if v < 0 or v > 0x7FFFFFFF:
+                raise ValueError(f"{name} = {v} does not fit in 31 bits")
+
+    def _groups(self, offsets, M, like):
+        import torch
+
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets must hold groups + 1 row offsets")
+        groups = offsets.numel() - 1
+        if groups > MAX_GROUPS:
+            raise ValueError(f"{groups} groups: at most {MAX_GROUPS} in one call")
+        return self._held("offsets", offsets, groups + 1, torch.int32, like), groups
+
+    def _forward(self, name, C, A, B, offsets, M, N, K, layout_b, bias, residual, preact, act, stream):
+        self._sizes(M=M, N=N, K=K)
+        slot = _type_slot(C.dtype, A.dtype)
+        act, layout_b = activation(act), m_layout(layout_b)
+        groups, where = 1, ()
+        if offsets is not None:
+            address, groups = self._groups(offsets, M, C)
+            where = (address, groups)
+        c = self._held("C", C, M * N, C.dtype)
+        a = self._held("A", A, M * K, A.dtype, C)
+        b = self._held("B", B, groups * K * N, A.dtype, C)
+        e = _EpilogueC(self._held("bias", bias, groups * N, A.dtype, C),
+                       self._held("residual", residual, M * N, C.dtype, C),
+                       self._held("preact", preact, M * N, A.dtype, C), int(act))
+        handle = ctypes.c_void_p(self._stream_handle(stream))
+        fn = getattr(self._lib, "rocm_wmma_gemm_" + name)
+        self._done(name, fn(slot, c, a, b, *where, M, N, K, int(layout_b), ctypes.byref(e), ctypes.byref(handle)))
+
+    def _backward(self, name, dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, act, accumulate, stream):
+        self._sizes(M=M, N=N, K=K)
+        wanted = [t for t in (dA, dB, dbias) if t is not None]
+        if not wanted:
+            raise ValueError("none of dA, dB and dbias is wanted")
+        if any(t.dtype != wanted[0].dtype for t in wanted):
+            raise TypeError("dA, dB and dbias must share an element type")
+        slot = _type_slot(wanted[0].dtype, dC.dtype)
+        act, layout_b = activation(act), m_layout(layout_b)
+        if act != activation.none and preact is None:
+            raise ValueError(f"the gradient of {act.name} needs preact")
+        if act == activation.none:
+            preact = None
+        if dB is not None and A is None or dA is not None and B is None:
+            raise ValueError("dA needs B, and dB needs A")
+        groups, where = 1, ()
+        if offsets is not None:
+            address, groups = self._groups(offsets, M, dC)
+            where = (address, groups)
+        out = wanted[0].dtype
+        args = (self._held("dA", dA, M * K, out, dC), self._held("dB", dB, groups * K * N, out, dC),
+                self._held("dbias", dbias, groups * N, out, dC), self._held("dC", dC, M * N, dC.dtype),
+                self._held("A", A, M * K, dC.dtype, dC), self._held("B", B, groups * K * N, dC.dtype, dC),
+                self._held("preact", preact, M * N, dC.dtype, dC))
+        handle = ctypes.c_void_p(self._stream_handle(stream))
+        fn = getattr(self._lib, "rocm_wmma_gemm_" + name)
+        self._done(name, fn(slot, *args, *where, M, N, K, int(layout_b), int(act), int(bool(accumulate)),
+                            ctypes.byref(handle)))
+
+    def linear(self, C, A, B, M: int, N: int, K: int, layout_b=col_major, bias=None, residual=None, preact=None,
+               activation=activation.none, stream=None) -> None:
+        """C = activation(A B + bias) + residual on ``stream`` (default: torch's current stream).
+
+        A (M x K) and C (M x N) are row-major; B (K x N) is column-major (weights stored N x K)
+        or row-major.  bias: N values of A's type; residual: M x N of C's type, may be C itself;
+        preact: M x N of A's type, receives A B + bias for the backward pass."""
+        self._forward("linear", C, A, B, None, M, N, K, layout_b, bias, residual, preact, activation, stream)
+
+    def linear_backward(self, dA, dB, dbias, dC, A, B, M: int, N: int, K: int, layout_b=col_major, preact=None,
+                        activation=activation.none, accumulate: bool = False, stream=None) -> None:
+        """The gradients of linear() from dC (M x N, A's type): dA = dZ B^T, dB = A^T dZ in B's
+        layout and dbias = the sum of dZ's rows, with dZ = dC activation'(preact).  A result that
+        is None is not computed.  accumulate: dB and dbias are added to."""
+        self._backward("linear_backward", dA, dB, dbias, dC, A, B, None, M, N, K, layout_b, preact, activation,
+                       accumulate, stream)
+
+    def grouped(self, C, A, B, offsets, M: int, N: int, K: int, layout_b=col_major, bias=None, residual=None,
+                preact=None, activation=activation.none, stream=None) -> None:
+        """linear() for groups of rows with a weight (and bias) each: rows offsets[e] ..
+        offsets[e+1] - 1 of A and C belong to weight e of B (groups x K x N).  offsets: groups + 1
+        int32 on the device; they are read there, never by the host.  Rows outside the groups are
+        not touched."""
+        self._forward("grouped", C, A, B, offsets, M, N, K, layout_b, bias, residual, preact, activation, stream)
+
+    def grouped_backward(self, dA, dB, dbias, dC, A, B, offsets, M: int, N: int, K: int, layout_b=col_major,
+                         preact=None, activation=activation.none, accumulate: bool = False, stream=None) -> None:
+        """The gradients of grouped(); an empty group's are zero (unchanged with accumulate)."""
+        self._backward("grouped_backward", dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, activation,
+                       accumulate, stream)
+
+    def orthogonalize(self, O, G, M: int, N: int, batch_count: int = 1, steps: int = 5,
+                      coefficients=(3.4445, -4.7750, 2.0315), epsilon: float = 1e-7, stream=None) -> None:
+        """O = G / (|G| + epsilon) after ``steps`` Newton-Schulz steps x -> a x + b x^3 + c x^5 on
+        its singular values, for a batch of row-major M x N matrices: an update with singular
+        values near 1.  G: f16, bf16 or f32; O: f16 or bf16."""
+        import torch
+
+        self._sizes(M=M, N=N, batch_count=batch_count)
+        codes = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+        if G.dtype not in codes or codes.get(O.dtype, 2) == 2:
+            raise TypeError(f"Unsupported type pair for orthogonalize: O={O.dtype}, G={G.dtype}")
+        if steps < 1 or len(coefficients) != 3:
+            raise ValueError("at least one step, and three coefficients")
+        o = self._held("O", O, batch_count * M * N, O.dtype)
+        g = self._held("G", G, batch_count * M * N, G.dtype, O)
+        handle = ctypes.c_void_p(self._stream_handle(stream))
+        self._done("orthogonalize", self._lib.rocm_wmma_gemm_orthogonalize(
+            codes[G.dtype], codes[O.dtype], o, g, M, N, batch_count, steps, (ctypes.c_float * 3)(*coefficients),
+            epsilon, ctypes.byref(handle)))
