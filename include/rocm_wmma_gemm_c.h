@@ -225,7 +225,7 @@ int rocm_wmma_gemm_noalloc(int type_idx, void* C, void* A, void* B, size_t M, si
 #define ROCM_WMMA_GEMM_ACT_GELU 3 /* 0.5 x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) */
 
 /* Most groups of one grouped call. */
-#define ROCM_WMMA_GEMM_MAX_GROUPS 1024
+#define ROCM_WMMA_GEMM_MAX_GROUPS 512
 
 typedef struct rocm_wmma_gemm_epilogue
 {

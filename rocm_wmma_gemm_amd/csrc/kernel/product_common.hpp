@@ -52,7 +52,7 @@ struct act_args
     float    k1, k3;
 };
 
-constexpr int max_groups = 1024; // two tables of this many integers fit beside every ring in LDS
+constexpr int max_groups = 512; // two tables of this many integers fit beside every ring in LDS
 
 struct product_args
 {

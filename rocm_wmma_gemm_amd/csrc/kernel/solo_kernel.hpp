@@ -155,11 +155,12 @@ struct solo_gemm
     // part that depends on i is a scalar offset i * stride, and the lane's own part is
     // a vector offset that is the same for every i (K-contiguous: the swizzle of row
     // RPL*(wave + 4i) + lane/CH does not depend on i) or alternates between two values
-    // with the parity of i (M/N-contiguous: the swizzle term 2*((kg/2)%2) does).
+    // with the parity of i (M/N-contiguous, 256 rows: the swizzle term 2*((kg/2)%2) does; with
+    // 128 rows a k group is one block, kg = wave + 4i, and the term is the same for every i).
     template<bool KMAJOR, int ROWS>
     struct load_addr
     {
-        static_assert(WAVES == 4 && (KMAJOR || ROWS == 256), "derived for this tile and wave count");
+        static_assert(WAVES == 4 && (KMAJOR || ROWS == 256 || ROWS == 128), "derived for this tile and wave count");
         static constexpr int CH  = BK / 8; // 16-byte chunks of a K-contiguous row
         static constexpr int RPL = 64 / CH; // rows of it that one load fills
         unsigned int voff[KMAJOR ? 1 : 2]; // bytes
@@ -173,6 +174,12 @@ struct solo_gemm
                 const int c = (lane % CH) ^ swizzle_of_row<CH, MI>(r);
                 voff[0]     = (unsigned int)((r * ld + c * 8) * 2);
                 stride      = (unsigned int)(WAVES * RPL * ld * 2);
+            }
+            else if constexpr(ROWS == 128)
+            {
+                const int j = lane / 16, c = (lane % 16) ^ (4 * j) ^ (2 * ((wave >> 1) & 1));
+                voff[0] = voff[1] = (unsigned int)(((wave * 4 + j) * ld + c * 8) * 2);
+                stride            = (unsigned int)(16 * ld * 2);
             }
             else
             {

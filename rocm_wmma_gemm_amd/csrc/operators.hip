@@ -17,10 +17,10 @@ namespace host
 {
 
 template<int TYPES>
-product_kernel product_of(int layout, int form);
+product_kernel product_of(int layout, int form, int finish);
 #define RWG_TYPES(T) \
     template<>       \
-    product_kernel product_of<T>(int layout, int form);
+    product_kernel product_of<T>(int layout, int form, int finish);
 RWG_TYPES(0)
 RWG_TYPES(1)
 RWG_TYPES(2)
@@ -31,19 +31,19 @@ RWG_TYPES(6)
 RWG_TYPES(7)
 #undef RWG_TYPES
 
-product_kernel find_product(int types, int layout, int form)
+product_kernel find_product(int types, int layout, int form, int finish)
 {
     switch(types)
     {
-        case 0: return product_of<0>(layout, form);
-        case 1: return product_of<1>(layout, form);
-        case 2: return product_of<2>(layout, form);
-        case 3: return product_of<3>(layout, form);
-        case 4: return product_of<4>(layout, form);
-        case 5: return product_of<5>(layout, form);
-        case 6: return product_of<6>(layout, form);
-        case 7: return product_of<7>(layout, form);
-        default: return {nullptr, 0, 0, 0};
+        case 0: return product_of<0>(layout, form, finish);
+        case 1: return product_of<1>(layout, form, finish);
+        case 2: return product_of<2>(layout, form, finish);
+        case 3: return product_of<3>(layout, form, finish);
+        case 4: return product_of<4>(layout, form, finish);
+        case 5: return product_of<5>(layout, form, finish);
+        case 6: return product_of<6>(layout, form, finish);
+        case 7: return product_of<7>(layout, form, finish);
+        default: return {nullptr, 0, 0, 0, 0};
     }
 }
 
@@ -119,34 +119,64 @@ int with_status(Body&& body)
     }
 }
 
+// Whether the kernels that load 16 bytes at a time, straight to LDS, can take the operands: every row,
+// and every group's first, starts on 16 bytes, and a tile's span fits the 31 bits of their offsets.
+bool aligned_rows(const product_args& a, int layout)
+{
+    const bool k_contiguous = layout != layout_mn;
+    return a.lda % 8 == 0 && a.ldb % 8 == 0 && a.ldc % 8 == 0 && a.N % 8 == 0 && (k_contiguous ? a.K % 8 == 0 : a.M % 8 == 0)
+           && a.stride_a % 8 == 0 && a.stride_b % 8 == 0 && a.stride_c % 8 == 0 && aligned16(a.A) && aligned16(a.B)
+           && aligned16(a.C) && aligned16(a.kept) && aligned16(a.residual) && aligned16(a.bias) && a.K > 0
+           && std::max({a.lda, a.ldb, a.ldc}) < (1 << 21);
+}
+
+// Which kernel a product runs on.
+int choose_form(int types, int layout, int finish, const product_args& args, size_t cus)
+{
+    auto tiles = [&](size_t edge) {
+        const size_t n = ceil_div(args.N, edge);
+        return args.kind == product_kind::rows ? (args.M / edge + std::min<size_t>(args.groups, args.M)) * n
+                                               : args.groups * ceil_div(args.M, edge) * n;
+    };
+    if(!aligned_rows(args, layout))
+    {
+        return tiles(128) < cus ? form_general_64 : form_general_128;
+    }
+    const size_t rows = args.kind == product_kind::rows ? ceil_div(args.M, std::min<size_t>(args.groups, args.M)) : args.M;
+    if(args.kind == product_kind::rows && rows <= 64
+       && (layout == layout_kk || static_cast<long long>(args.K) * args.ldb < (1ll << 30)))
+    {
+        return rows <= 16 ? form_skinny_16x32 : rows <= 32 ? form_skinny_32x32 : form_skinny_64x32;
+    }
+    return rows <= 160 || tiles(256) < cus ? form_tiled_128 : form_tiled_256;
+}
+
 // One product: picks the kernel and launches it.
-int launch_product(int types, int layout, product_args args, hipStream_t stream)
+int launch_product(int types, int layout, int finish, product_args args, hipStream_t stream)
 {
     if(args.N == 0 || args.M == 0 || args.groups == 0)
     {
         return ROCM_WMMA_GEMM_OK;
     }
-    const size_t cus = std::max<size_t>(compute_units_of_current_device(), 1);
-    auto         tiles_of = [&](const product_kernel& k) {
-        const size_t grid_n = ceil_div(args.N, k.block_n);
-        // (rows: how many of its tiles are there is only known on the device; at most this many)
-        return args.kind == product_kind::rows
-                           ? (args.M / k.block_m + std::min<size_t>(args.groups, args.M)) * grid_n
-                           : args.groups * ceil_div(args.M, k.block_m) * grid_n;
-    };
-    product_kernel kernel = find_product(types, layout, form_general_128);
-    if(tiles_of(kernel) < cus)
+    const size_t         cus    = std::max<size_t>(compute_units_of_current_device(), 1);
+    const product_kernel kernel = find_product(types, layout, choose_form(types, layout, finish, args, cus), finish);
+    if(kernel.fn == nullptr)
     {
-        kernel = find_product(types, layout, form_general_64);
+        return ROCM_WMMA_GEMM_ERR_LIMIT;
     }
-    const size_t items = tiles_of(kernel);
+    const size_t grid_m = ceil_div(args.M, kernel.block_m), grid_n = ceil_div(args.N, kernel.block_n);
+    // (rows: how many tiles there are is only known on the device; at most this many)
+    const size_t items = args.kind == product_kind::rows
+                             ? (args.M / kernel.block_m + std::min<size_t>(args.groups, args.M)) * grid_n
+                             : args.groups * grid_m * grid_n;
     if(items > most_extent)
     {
         return ROCM_WMMA_GEMM_ERR_LIMIT;
     }
-    args.grid_m = static_cast<int>(ceil_div(args.M, kernel.block_m));
-    args.grid_n = static_cast<int>(ceil_div(args.N, kernel.block_n));
-    enqueue(kernel.fn, dim3(static_cast<unsigned>(std::min(items, 8 * cus))), dim3(kernel.threads), stream, args);
+    args.grid_m = static_cast<int>(grid_m);
+    args.grid_n = static_cast<int>(grid_n);
+    const size_t blocks = kernel.per_cu == 0 ? items : std::min(items, kernel.per_cu * cus);
+    enqueue(kernel.fn, dim3(static_cast<unsigned>(blocks)), dim3(kernel.threads), stream, args);
     return ROCM_WMMA_GEMM_OK;
 }
 
@@ -213,7 +243,10 @@ int forward(const layer& p, void* C, const void* A, const void* B, const rocm_wm
     a.ldc          = p.N;
     a.stride_b     = static_cast<long long>(p.N * p.K);
     a.stride_bias  = p.N;
-    return launch_product(p.type_idx, p.layout_b == 1 ? layout_kk : layout_kn, a, stream);
+    const int finish = p.act.kind == act_kind::logistic ? finish_logistic
+                       : p.act.kind == act_kind::relu || e.bias || e.residual || e.preact ? finish_layer
+                                                                                          : finish_plain;
+    return launch_product(p.type_idx, p.layout_b == 1 ? layout_kk : layout_kn, finish, a, stream);
 }
 
 template<class InT>
@@ -311,7 +344,7 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
         a.ldb          = p.layout_b == 1 ? p.K : p.N;
         a.ldc          = p.K;
         a.stride_b     = static_cast<long long>(p.N * p.K);
-        rc             = launch_product(p.type_idx, p.layout_b == 1 ? layout_kn : layout_kk, a, stream);
+        rc             = launch_product(p.type_idx, p.layout_b == 1 ? layout_kn : layout_kk, finish_plain, a, stream);
     }
     if(rc == ROCM_WMMA_GEMM_OK && dB != nullptr)
     {
@@ -330,7 +363,7 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
         a.ldb           = a.N;
         a.ldc           = a.N;
         a.stride_c      = static_cast<long long>(p.N * p.K);
-        rc              = launch_product(p.type_idx, layout_mn, a, stream);
+        rc              = launch_product(p.type_idx, layout_mn, accumulate ? finish_add : finish_plain, a, stream);
     }
     return rc;
 }
@@ -431,7 +464,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         p.lda = p.ldb = np, p.ldc = lp;
         p.stride_a = p.stride_b = each, p.stride_c = square;
         p.alpha = 1.0f / (scale * scale), p.beta = 0.0f, p.diagonal_is = device::diagonal_use::none;
-        rc = launch_product(types_steps_square, tall ? layout_mn : layout_kk, p, stream);
+        rc = launch_product(types_steps_square, tall ? layout_mn : layout_kk, finish_square, p, stream);
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             break;
@@ -440,7 +473,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         p.C = q, p.A = p.B = s, p.residual = s;
         p.K = static_cast<int>(lp), p.lda = p.ldb = lp, p.stride_a = p.stride_b = square;
         p.alpha = c, p.beta = b, p.diagonal_is = device::diagonal_use::split;
-        rc = launch_product(types_steps_square, layout_kk, p, stream);
+        rc = launch_product(types_steps_square, layout_kk, finish_poly, p, stream);
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             break;
@@ -456,7 +489,9 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         p.kept = last ? nullptr : x16[(step + 1) & 1], p.keep_sum = 1;
         rc = launch_product(!last ? types_steps_next
                             : out_type == ROCM_WMMA_GEMM_ELEMENT_F16 ? types_steps_f16 : types_steps_bf16,
-                            tall ? layout_kk : layout_kn, p, stream);
+                            tall ? layout_kk : layout_kn,
+                            last ? (tall ? finish_last_cols : finish_last_rows) : tall ? finish_next_cols : finish_next_rows,
+                            p, stream);
         p.keep_sum = 0;
     }
     if(rc == ROCM_WMMA_GEMM_OK && !direct)

@@ -1,6 +1,8 @@
 // The layer-product kernels of one type set (-DRWG_PRODUCT_TYPES=<product_types>), so that the
 // sets build in parallel.
 #include "kernel/general_product.hpp"
+#include "kernel/skinny_product.hpp"
+#include "kernel/tiled_product.hpp"
 #include "product_table.hpp"
 
 namespace rocm_wmma_gemm
@@ -18,37 +20,148 @@ using out_t = std::conditional_t<
     std::conditional_t<kTypes == types_bf16_bf16 || kTypes == types_steps_bf16, __bf16, float>>;
 using res_t = std::conditional_t<kTypes == types_steps_f16 || kTypes == types_steps_bf16, float, out_t>;
 
+constexpr product_kernel kNone{nullptr, 0, 0, 0, 0};
+constexpr bool           kSteps = kTypes >= types_steps_square;
+
 template<class Impl>
-product_kernel made(int block_m, int block_n)
+product_kernel made(int block_m, int block_n, int per_cu)
 {
-    return {&device::product_entry<Impl>, block_m, block_n, Impl::THREADS};
+    return {&device::product_entry<Impl>, block_m, block_n, Impl::THREADS, per_cu};
+}
+
+template<int LAYOUT, int EDGE, class EPI>
+product_kernel tiled()
+{
+    constexpr bool AK = LAYOUT != layout_mn, BK = LAYOUT == layout_kk;
+    using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, EDGE, EDGE, EPI>;
+    return {&device::tiled_product_entry<impl>, EDGE, EDGE, impl::THREADS, impl::PER_CU};
+}
+
+// Only what some call asks for is built.
+template<int LAYOUT, int EDGE>
+product_kernel tiled_finish(int finish)
+{
+    if constexpr(!kSteps && LAYOUT == layout_mn) // gradients of weights
+    {
+        switch(finish)
+        {
+            case finish_plain: return tiled<LAYOUT, EDGE, device::epilogue_plain>();
+            case finish_add: return tiled<LAYOUT, EDGE, device::epilogue_add>();
+            default: return kNone;
+        }
+    }
+    else if constexpr(!kSteps)
+    {
+        switch(finish)
+        {
+            case finish_plain: return tiled<LAYOUT, EDGE, device::epilogue_plain>();
+            case finish_layer: return tiled<LAYOUT, EDGE, device::epilogue_layer>();
+            case finish_logistic: return tiled<LAYOUT, EDGE, device::epilogue_logistic>();
+            default: return kNone;
+        }
+    }
+    else if constexpr(kTypes == types_steps_square)
+    {
+        if constexpr(LAYOUT != layout_kn)
+        {
+            if(finish == finish_square)
+            {
+                return tiled<LAYOUT, EDGE, device::epilogue_square>();
+            }
+        }
+        if constexpr(LAYOUT == layout_kk)
+        {
+            if(finish == finish_poly)
+            {
+                return tiled<LAYOUT, EDGE, device::epilogue_poly>();
+            }
+        }
+        return kNone;
+    }
+    else if constexpr(LAYOUT != layout_mn)
+    {
+        // Q X: rows of the residual meet the diagonal; X Q: columns
+        constexpr bool ROWS = LAYOUT == layout_kn;
+        if constexpr(kTypes == types_steps_next)
+        {
+            using epi = std::conditional_t<ROWS, device::epilogue_next_rows, device::epilogue_next_cols>;
+            return finish == (ROWS ? finish_next_rows : finish_next_cols) ? tiled<LAYOUT, EDGE, epi>() : kNone;
+        }
+        else
+        {
+            using epi = std::conditional_t<ROWS, device::epilogue_last_rows, device::epilogue_last_cols>;
+            return finish == (ROWS ? finish_last_rows : finish_last_cols) ? tiled<LAYOUT, EDGE, epi>() : kNone;
+        }
+    }
+    else
+    {
+        return kNone;
+    }
+}
+
+template<int LAYOUT, int BM, int BN>
+product_kernel skinny()
+{
+    if constexpr(!kSteps && LAYOUT != layout_mn)
+    {
+        return made<device::skinny_product<kIn, out_t, BM, BN, LAYOUT == layout_kk>>(BM, BN, 0);
+    }
+    else
+    {
+        return kNone;
+    }
 }
 
 template<int LAYOUT>
-product_kernel in_layout(int form)
+product_kernel general(int form)
 {
     constexpr bool AK = LAYOUT != layout_mn, BK = LAYOUT == layout_kk;
+    if constexpr(kSteps)
+    {
+        return kNone; // (their operands are the library's own, always aligned)
+    }
+    else if(form == form_general_128)
+    {
+        return made<device::general_product<kIn, out_t, res_t, AK, BK, 128, 128, 32>>(128, 128, 8);
+    }
+    else
+    {
+        return made<device::general_product<kIn, out_t, res_t, AK, BK, 64, 64, 64>>(64, 64, 8);
+    }
+}
+
+template<int LAYOUT>
+product_kernel in_layout(int form, int finish)
+{
     switch(form)
     {
-        case form_general_128: return made<device::general_product<kIn, out_t, res_t, AK, BK, 128, 128, 32>>(128, 128);
-        case form_general_64: return made<device::general_product<kIn, out_t, res_t, AK, BK, 64, 64, 64>>(64, 64);
-        default: return {nullptr, 0, 0, 0};
+        case form_general_128:
+        case form_general_64: return general<LAYOUT>(form);
+        case form_tiled_256: return tiled_finish<LAYOUT, 256>(finish);
+        case form_tiled_128: return tiled_finish<LAYOUT, 128>(finish);
+        case form_skinny_16x32: return skinny<LAYOUT, 16, 32>();
+        case form_skinny_16x64: return skinny<LAYOUT, 16, 64>();
+        case form_skinny_32x32: return skinny<LAYOUT, 32, 32>();
+        case form_skinny_32x64: return skinny<LAYOUT, 32, 64>();
+        case form_skinny_64x32: return skinny<LAYOUT, 64, 32>();
+        case form_skinny_64x64: return skinny<LAYOUT, 64, 64>();
+        default: return kNone;
     }
 }
 } // namespace
 
 template<int TYPES>
-product_kernel product_of(int layout, int form);
+product_kernel product_of(int layout, int form, int finish);
 
 template<>
-product_kernel product_of<kTypes>(int layout, int form)
+product_kernel product_of<kTypes>(int layout, int form, int finish)
 {
     switch(layout)
     {
-        case layout_kk: return in_layout<layout_kk>(form);
-        case layout_kn: return in_layout<layout_kn>(form);
-        case layout_mn: return in_layout<layout_mn>(form);
-        default: return {nullptr, 0, 0, 0};
+        case layout_kk: return in_layout<layout_kk>(form, finish);
+        case layout_kn: return in_layout<layout_kn>(form, finish);
+        case layout_mn: return in_layout<layout_mn>(form, finish);
+        default: return kNone;
     }
 }
 

@@ -40,16 +40,42 @@ enum product_form
 {
     form_general_128 = 0, // 128 x 128 tiles, any alignment
     form_general_64, // 64 x 64 tiles, any alignment
+    // rows that start on 16 bytes:
+    form_tiled_256, // persistent 256 x 256 tiles
+    form_tiled_128, // persistent 128 x 128 tiles
+    form_skinny_16x32, // whole sums of few rows, rows x columns of a tile
+    form_skinny_16x64,
+    form_skinny_32x32,
+    form_skinny_32x64,
+    form_skinny_64x32,
+    form_skinny_64x64,
     num_product_forms
+};
+
+// What happens to a finished tile (tiled forms; the others read it from the arguments).
+enum product_finish
+{
+    finish_plain = 0, // alpha = 1, nothing added
+    finish_add, // a residual is added
+    finish_layer, // bias, nothing or relu, residual, the sum kept
+    finish_logistic, // the same with silu or gelu
+    finish_square, // symmetric
+    finish_poly, // symmetric, with a residual and the diagonal held apart
+    finish_next_rows, // + diagonal times residual, kept in A's type as well
+    finish_next_cols,
+    finish_last_rows, // the same without
+    finish_last_cols,
+    num_product_finishes
 };
 
 struct product_kernel
 {
     product_fn fn; // nullptr: not built
     int        block_m, block_n, threads;
+    int        per_cu; // workgroups of a compute unit, for a persistent kernel; 0: a workgroup per tile
 };
 
-product_kernel find_product(int types, int layout, int form);
+product_kernel find_product(int types, int layout, int form, int finish);
 
 } // namespace host
 } // namespace rocm_wmma_gemm

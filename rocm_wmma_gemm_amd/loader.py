@@ -57,7 +57,7 @@ class _EpilogueC(ctypes.Structure):
                 ("activation", ctypes.c_int)]
 
 
-MAX_GROUPS = 1024
+MAX_GROUPS = 512
 
 
 class _VariantInfoC(ctypes.Structure):
