@@ -144,13 +144,15 @@ size_t out_bytes(int type_idx)
 // never count in the same slots at the same time), one for the entry point that allocates
 // nothing, which takes no lease (its calls are ordered by the caller, like their scratch
 // array); a call of one kind never meets a call of the other in a counter.
-constexpr size_t stream_arrival_slots = 4096;
 __attribute__((used)) static __device__ unsigned int stream_arrivals[stream_arrival_slots];
 __attribute__((used)) static __device__ unsigned int noalloc_arrivals[stream_arrival_slots];
 std::mutex            arrivals_mutex;
 unsigned int*         arrivals_address[64][2] = {};
 std::atomic<unsigned> arrival_epoch{0};
 
+} // namespace
+
+// (host_services.hpp)
 unsigned int* arrivals_of_current_device(bool noalloc)
 {
     int dev = -1;
@@ -184,6 +186,9 @@ unsigned int next_arrival_epoch()
     } while(e == 0);
     return e;
 }
+
+namespace
+{
 
 // Scratch memory that a call brings along instead of leasing the library's buffer (the
 // entry point that allocates nothing): the call takes what it needs from the front, or

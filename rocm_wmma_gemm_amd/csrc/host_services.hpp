@@ -170,6 +170,12 @@ private:
     bool                         ordered_ = false;
 };
 
+// Counters of the workgroups that share a tile, and a tag for one launch that counts in them (see
+// gemm.hip); nullptr without a device.  A caller holds the lease while its launches count.
+constexpr size_t stream_arrival_slots = 4096;
+unsigned int*    arrivals_of_current_device(bool noalloc);
+unsigned int     next_arrival_epoch();
+
 inline bool aligned16(const void* p)
 {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;

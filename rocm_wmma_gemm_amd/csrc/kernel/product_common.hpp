@@ -77,7 +77,44 @@ struct product_args
     float*       diagonal; // stride_diagonal values from group to group
     long long    stride_diagonal;
     int          grid_m, grid_n; // tiles of a problem (rows: grid_m is not used)
+    float*       partials; // tiled kernels: nullptr, or room for a tile of fp32 per workgroup of the
+                           // grid; the tiles of the last round may then be cut along K (cut_tail)
+    int          workgroups; // of the grid that writes them
+    int           k_slices; // few-row kernel: workgroups that share a tile, each with a run of K; 1: none do
+    unsigned int* arrivals; // with k_slices > 1: a counter per tile, and this launch's tag in them
+    unsigned int  arrival_epoch;
 };
+
+// How the tiles of a launch are dealt to its persistent workgroups: whole tiles round by round, and
+// where the last round has tiles for at most half of them, each of those in `slices` runs of `each` K
+// tiles that another kernel adds up.
+struct tail_cut
+{
+    int whole; // tiles before the cut ones
+    int cut; // tiles that are cut
+    int slices, each;
+    RWG_HD int positions() const
+    {
+        return whole + cut * slices;
+    }
+};
+
+// A slice shorter than this many K tiles costs more to write and add up than it saves.
+constexpr int least_slice = 4, most_slices = 16;
+
+RWG_HD inline tail_cut cut_tail(int tiles, int workgroups, int k_tiles, bool may_cut)
+{
+    const int rest   = tiles % workgroups;
+    int       slices = may_cut && rest > 0 ? workgroups / rest : 1;
+    slices           = slices < most_slices ? slices : most_slices;
+    slices           = slices < k_tiles / least_slice ? slices : k_tiles / least_slice;
+    if(slices < 2)
+    {
+        return {tiles, 0, 1, k_tiles};
+    }
+    const int each = (k_tiles + slices - 1) / slices;
+    return {tiles - rest, rest, (k_tiles + each - 1) / each, each};
+}
 
 __device__ __forceinline__ int clamped_offset(int v, int rows)
 {
@@ -131,6 +168,27 @@ __device__ __forceinline__ void build_group_table(const int* offsets, int groups
             carry_off  = __shfl(v, 63);
             carry_tile = __shfl(t, 63);
         }
+    }
+    __syncthreads();
+}
+
+// order[0 .. groups]: the groups by falling size (ties by number), for launches whose groups cost as
+// much as they have rows: dealt in this order, round by round, the persistent workgroups end nearly
+// together.  Ready behind its barrier.
+template<class IntPtr>
+__device__ __forceinline__ void order_groups(int groups, IntPtr off, IntPtr order)
+{
+    for(int e = threadIdx.x; e < groups; e += blockDim.x)
+    {
+        const int own  = off[e + 1] - off[e];
+        int       rank = 0;
+#pragma unroll 8
+        for(int j = 0; j < groups; ++j)
+        {
+            const int other = off[j + 1] - off[j];
+            rank += other > own || (other == own && j < e);
+        }
+        order[rank] = e;
     }
     __syncthreads();
 }
@@ -274,6 +332,66 @@ __device__ __forceinline__ void finish_element(const product_args& args, const p
         static_cast<InT*>(args.kept)[at] = to_out<InT>(args.keep_sum ? y : z);
     }
     static_cast<OutT*>(args.C)[at] = to_out<OutT>(y);
+}
+
+// Eight consecutive elements of a row, as 16-byte pieces: for operands whose rows start on 16 bytes.
+template<class InT, class OutT, class ResT>
+__device__ __forceinline__ void finish_piece(const product_args& args, const product_item& x, int row, int col,
+                                             const float (&sum)[8])
+{
+    typedef InT     in8 __attribute__((ext_vector_type(8)));
+    typedef OutT    out8 __attribute__((ext_vector_type(8)));
+    typedef ResT    res8 __attribute__((ext_vector_type(8)));
+    const long long at = x.c_at + row * args.ldc + col;
+    float           z[8], y[8];
+#pragma unroll
+    for(int e = 0; e < 8; ++e)
+    {
+        z[e] = args.alpha * sum[e];
+    }
+    if(args.bias != nullptr)
+    {
+        const in8 b = *reinterpret_cast<const in8*>(static_cast<const InT*>(args.bias) + x.group * args.stride_bias + col);
+#pragma unroll
+        for(int e = 0; e < 8; ++e)
+        {
+            z[e] += (float)b[e];
+        }
+    }
+#pragma unroll
+    for(int e = 0; e < 8; ++e)
+    {
+        y[e] = activate(args.act, z[e]);
+    }
+    if(args.residual != nullptr)
+    {
+        const res8 r = *reinterpret_cast<const res8*>(static_cast<const ResT*>(args.residual) + at);
+        const bool rows = args.diagonal_is == diagonal_use::rows, cols = args.diagonal_is == diagonal_use::cols;
+        const float* d = args.diagonal + x.group * args.stride_diagonal;
+        const float  by_row = rows ? args.beta + args.alpha * d[row] : args.beta;
+#pragma unroll
+        for(int e = 0; e < 8; ++e)
+        {
+            y[e] += (cols ? args.beta + args.alpha * d[col + e] : by_row) * (float)r[e];
+        }
+    }
+    if(args.kept != nullptr)
+    {
+        in8 k;
+#pragma unroll
+        for(int e = 0; e < 8; ++e)
+        {
+            k[e] = to_out<InT>(args.keep_sum ? y[e] : z[e]);
+        }
+        *reinterpret_cast<in8*>(static_cast<InT*>(args.kept) + at) = k;
+    }
+    out8 o;
+#pragma unroll
+    for(int e = 0; e < 8; ++e)
+    {
+        o[e] = to_out<OutT>(y[e]);
+    }
+    *reinterpret_cast<out8*>(static_cast<OutT*>(args.C) + at) = o;
 }
 
 template<class Impl>

@@ -12,7 +12,7 @@ namespace device
 {
 
 // dZ = dC * act'(Z), and the sums of its columns over runs of slope_rows rows of a group.
-constexpr int slope_rows = 128; // rows of a run (a workgroup's); a group's last run is shorter
+constexpr int slope_rows = 32; // rows of a run (a workgroup's); a group's last run is shorter
 
 struct slope_args
 {
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
     }
     if(col < args.cols)
     {
-#pragma unroll 4
+#pragma unroll 8
         for(int row = row0 + wave; row < row1; row += 4)
         {
             const long long at = (long long)row * args.cols + col;
@@ -105,58 +105,73 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
     }
 }
 
-// The sums of a group's runs, in their order: the gradient of its bias (blockIdx.y: the group).
+// The sums of a group's runs: the gradient of its bias (blockIdx.y: the group).  Each of four waves
+// adds up a quarter of the runs in their order, then the quarters are added in theirs.
 template<class OutT>
-__global__ void __launch_bounds__(64) column_sums(const slope_args args, OutT* __restrict__ dbias,
-                                                  int accumulate)
+__global__ void __launch_bounds__(256) column_sums(const slope_args args, OutT* __restrict__ dbias, int accumulate)
 {
-    __shared__ int off[max_groups + 1], first[max_groups + 1];
+    __shared__ int   off[max_groups + 1], first[max_groups + 1];
+    __shared__ float part[4][64];
     build_group_table(args.offsets, args.groups, args.rows, slope_rows, &off[0], &first[0]);
-    const int group = blockIdx.y, col = blockIdx.x * 64 + threadIdx.x;
-    if(col >= args.cols)
+    const int group = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+    const int run0 = first[group], runs = first[group + 1] - run0, each = (runs + 3) / 4;
+    const int begin = run0 + wave * each, end = run0 + ((wave + 1) * each < runs ? (wave + 1) * each : runs);
+    float     s = 0.0f;
+    if(col < args.cols)
     {
-        return;
-    }
-    float s = 0.0f;
 #pragma unroll 8
-    for(int run = first[group]; run < first[group + 1]; ++run)
-    {
-        s += args.sums[(long long)run * args.cols + col];
+        for(int run = begin; run < end; ++run)
+        {
+            s += args.sums[(long long)run * args.cols + col];
+        }
     }
-    OutT& to = dbias[(long long)group * args.cols + col];
-    to       = to_out<OutT>(accumulate ? s + (float)to : s);
+    part[wave][lane] = s;
+    __syncthreads();
+    if(wave == 0 && col < args.cols)
+    {
+        s        = ((part[0][lane] + part[1][lane]) + part[2][lane]) + part[3][lane];
+        OutT& to = dbias[(long long)group * args.cols + col];
+        to       = to_out<OutT>(accumulate ? s + (float)to : s);
+    }
 }
 
 // ---------------------------------------------------------------------------
 // Newton-Schulz steps: X is held twice, scaled by a power of two, with rows and columns padded with zeros
 // to multiples of 8: in fp32 (its linear term, see operators.hip) and in f16 (what is multiplied).
 // ---------------------------------------------------------------------------
-constexpr int square_parts = 64; // workgroups that add up the squares of one matrix
+constexpr int square_parts = 1024; // the most workgroups that add up the squares of one matrix
 
-// blockIdx.y: the matrix.  One partial sum per workgroup, in a fixed order.
-template<class GivenT>
+// blockIdx.y: the matrix, blockIdx.x: one of `parts` runs of it.  One partial sum per workgroup, in a
+// fixed order.  WIDTH elements at a time (16 bytes where the matrices are aligned, else one).
+template<class GivenT, int WIDTH>
 __global__ void __launch_bounds__(256) sum_squares(const GivenT* __restrict__ given, long long count,
                                                    float* __restrict__ parts)
 {
-    const GivenT* g = given + blockIdx.y * count;
-    float         s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    long long     i    = (long long)blockIdx.x * 256 + threadIdx.x;
-    constexpr long long hop = 256 * square_parts;
-    for(; i + 3 * hop < count; i += 4 * hop)
-    {
+    typedef GivenT given_t __attribute__((ext_vector_type(WIDTH)));
+    const given_t* g    = reinterpret_cast<const given_t*>(given + blockIdx.y * count);
+    const long long n   = count / WIDTH, hop = 256ll * gridDim.x;
+    float           s[WIDTH];
 #pragma unroll
-        for(int u = 0; u < 4; ++u)
+    for(int v = 0; v < WIDTH; ++v)
+    {
+        s[v] = 0.0f;
+    }
+#pragma unroll 4
+    for(long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += hop)
+    {
+        const given_t x = g[i];
+#pragma unroll
+        for(int v = 0; v < WIDTH; ++v)
         {
-            const float v = (float)g[i + u * hop];
-            s[u] += v * v;
+            s[v] += (float)x[v] * (float)x[v];
         }
     }
-    for(; i < count; i += hop)
+    float t = 0.0f;
+#pragma unroll
+    for(int v = 0; v < WIDTH; ++v)
     {
-        const float v = (float)g[i];
-        s[0] += v * v;
+        t += s[v];
     }
-    float t = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
     for(int d = 32; d > 0; d /= 2)
     {
@@ -170,53 +185,75 @@ __global__ void __launch_bounds__(256) sum_squares(const GivenT* __restrict__ gi
     __syncthreads();
     if(threadIdx.x == 0)
     {
-        parts[blockIdx.y * square_parts + blockIdx.x]
-            = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+        parts[blockIdx.y * square_parts + blockIdx.x] = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
     }
 }
 
-// X = G scale / (|G| + epsilon), padded; a thread writes 8 elements of a row.
-template<class GivenT>
+// X = G scale / (|G| + epsilon), padded.  A thread writes 8 elements of a row at a time; WIDE: G's
+// rows are whole pieces of 8 that start on 16 bytes.
+template<class GivenT, bool WIDE>
 __global__ void __launch_bounds__(256) orthogonal_start(const GivenT* __restrict__ given,
                                                         const float* __restrict__ parts,
-                                                        float*     x32,
-                                                        _Float16*  x16,
-                                                        int        rows,
-                                                        int        cols,
-                                                        int        rows_pad,
-                                                        int        cols_pad,
-                                                        float      scale,
-                                                        float      epsilon)
+                                                        float*    x32,
+                                                        _Float16* x16,
+                                                        int       rows,
+                                                        int       cols,
+                                                        int       rows_pad,
+                                                        int       cols_pad,
+                                                        float     scale,
+                                                        float     epsilon,
+                                                        int       used_parts)
 {
     const long long matrix = blockIdx.y;
-    float           t      = parts[matrix * square_parts + (threadIdx.x & 63)];
+    float           t      = 0.0f;
+    for(int i = threadIdx.x & 63; i < used_parts; i += 64)
+    {
+        t += parts[matrix * square_parts + i];
+    }
 #pragma unroll
     for(int d = 32; d > 0; d /= 2)
     {
         t += __shfl_xor(t, d);
     }
-    const float     f      = scale / (sqrtf(t) + epsilon);
-    const int       pieces = cols_pad / 8;
-    const long long piece  = (long long)blockIdx.x * 256 + threadIdx.x;
-    if(piece >= (long long)rows_pad * pieces)
+    const float   f      = scale / (sqrtf(t) + epsilon);
+    const int     pieces = cols_pad / 8;
+    const GivenT* g      = given + matrix * rows * cols;
+    for(int row = blockIdx.x; row < rows_pad; row += gridDim.x)
     {
-        return;
-    }
-    const int     row = (int)(piece / pieces), col = (int)(piece - (long long)row * pieces) * 8;
-    const GivenT* g   = given + matrix * rows * cols + (long long)row * cols + col;
-    f32x4         lo, hi;
-    f16x8         h;
+        for(int piece = threadIdx.x; piece < pieces; piece += 256)
+        {
+            typedef GivenT given8 __attribute__((ext_vector_type(8)));
+            const int      col = piece * 8;
+            float          y[8];
+            if constexpr(WIDE)
+            {
+                const given8 v = *reinterpret_cast<const given8*>(g + (long long)row * cols + col);
 #pragma unroll
-    for(int v = 0; v < 8; ++v)
-    {
-        const float y = row < rows && col + v < cols ? (float)g[v] * f : 0.0f;
-        (v < 4 ? lo : hi)[v & 3] = y;
-        h[v]                     = (_Float16)y;
+                for(int e = 0; e < 8; ++e)
+                {
+                    y[e] = (float)v[e] * f;
+                }
+            }
+            else
+            {
+#pragma unroll
+                for(int e = 0; e < 8; ++e)
+                {
+                    y[e] = row < rows && col + e < cols ? (float)g[(long long)row * cols + col + e] * f : 0.0f;
+                }
+            }
+            f16x8 h;
+#pragma unroll
+            for(int e = 0; e < 8; ++e)
+            {
+                h[e] = (_Float16)y[e];
+            }
+            const long long at = (matrix * rows_pad + row) * cols_pad + col;
+            *reinterpret_cast<f32x4*>(x32 + at)     = f32x4{y[0], y[1], y[2], y[3]};
+            *reinterpret_cast<f32x4*>(x32 + at + 4) = f32x4{y[4], y[5], y[6], y[7]};
+            *reinterpret_cast<f16x8*>(x16 + at)     = h;
+        }
     }
-    const long long at = (matrix * rows_pad + row) * cols_pad + col;
-    *reinterpret_cast<f32x4*>(x32 + at)     = lo;
-    *reinterpret_cast<f32x4*>(x32 + at + 4) = hi;
-    *reinterpret_cast<f16x8*>(x16 + at)     = h;
 }
 
 // All steps of one small matrix (smaller side up to 64, larger up to 256) in one workgroup, in
@@ -371,11 +408,13 @@ template<class OutT>
 __global__ void __launch_bounds__(256) orthogonal_end(const OutT* __restrict__ padded, OutT* __restrict__ out, int rows,
                                                       int cols, int rows_pad, int cols_pad)
 {
-    const long long count = (long long)rows * cols, matrix = blockIdx.y;
-    for(long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256)
+    const long long matrix = blockIdx.y;
+    for(int row = blockIdx.x; row < rows; row += gridDim.x)
     {
-        const long long row = i / cols;
-        out[matrix * count + i] = padded[(matrix * rows_pad + row) * cols_pad + (i - row * cols)];
+        for(int col = threadIdx.x; col < cols; col += 256)
+        {
+            out[(matrix * rows + row) * cols + col] = padded[(matrix * rows_pad + row) * cols_pad + col];
+        }
     }
 }
 

@@ -7,6 +7,10 @@
 // waits are the streaming kernel's; the four waves split K and their partial tiles meet in LDS,
 // where bias, activation and residual join them.  The row tiles that share a slice of a weight are
 // neighbours on one XCD.
+//
+// Where the tiles are too few for the compute units, args.k_slices workgroups share one, as in the
+// streaming kernel: each leaves its part in args.partials, counts itself in, and the last to arrive
+// adds the parts up in slice order and finishes the tile.
 #ifndef ROCM_WMMA_GEMM_SKINNY_PRODUCT_HPP
 #define ROCM_WMMA_GEMM_SKINNY_PRODUCT_HPP
 
@@ -18,7 +22,8 @@ namespace rocm_wmma_gemm
 namespace device
 {
 
-template<in_kind IN, class OutT, int BM, int BN, bool B_KMAJOR>
+// ONCE: the weight's loads carry the non-temporal hint (product_kernel::once).
+template<in_kind IN, class OutT, int BM, int BN, bool B_KMAJOR, bool ONCE>
 struct skinny_product
 {
     using S   = stream_gemm<IN, OutT, BM, BN, true, B_KMAJOR>;
@@ -36,7 +41,7 @@ struct skinny_product
 
         // Which tile.  The group table is built in the ring, which is empty yet.
         product_item x;
-        int          tm, tn;
+        int          tm, tn, slice, tile;
         {
             using lds_int  = __attribute__((address_space(3))) int;
             lds_int* off   = reinterpret_cast<lds_int*>(lds);
@@ -44,11 +49,15 @@ struct skinny_product
             static_assert(2 * (max_groups + 1) * 4 <= S::LDS_BYTES, "the table fits the ring");
             build_group_table(args.offsets, args.groups, args.M, BM, off, first);
             const int total = __builtin_amdgcn_readfirstlane(first[args.groups]) * args.grid_n;
-            if((int)blockIdx.x >= total)
+            // (slices outermost over the grid's tiles, so that a tile's slices have one counter)
+            const int most = gridDim.x / args.k_slices;
+            slice          = blockIdx.x / most;
+            tile           = blockIdx.x - slice * most;
+            if(tile >= total)
             {
                 return; // (the grid covers the most tiles that this many rows can have)
             }
-            const int item = xcd_remap(blockIdx.x, total);
+            const int item = xcd_remap(tile, total);
             x.group        = group_of_tile(first, args.groups, item / args.grid_n);
             const int f    = __builtin_amdgcn_readfirstlane(first[x.group]);
             const int high = __builtin_amdgcn_readfirstlane(first[x.group + 1]) - f;
@@ -78,10 +87,13 @@ struct skinny_product
         const unsigned int past    = 0x80000000u;
         const unsigned int voff_a_tail = k_tail != 0 && chunk * 8 >= k_tail ? past : voff_a;
         const unsigned int voff_b_tail = B_KMAJOR && k_tail != 0 && chunk * 8 >= k_tail ? past : voff_b;
-        const int          stages      = (args.K + BK - 1) / BK;
-        auto issue = [&](int stage, int at) {
+        // this workgroup's run of the stages
+        const int all = (args.K + BK - 1) / BK, each = (all + args.k_slices - 1) / args.k_slices, from = slice * each;
+        const int stages = all - from < each ? all - from : each; // >= 1 (host)
+        auto issue = [&](int run_stage, int at) {
+            const int          stage = from + run_stage;
             const unsigned int base = lds_addr + at * S::STAGE + wave * 1024;
-            const bool         last = stage == stages - 1; // the stage that K may cut short
+            const bool         last = stage == all - 1; // the stage that K may cut short
             const unsigned int va = last ? voff_a_tail : voff_a, vb = last ? voff_b_tail : voff_b;
 #pragma unroll
             for(int i = 0; i < S::LOADS_A; ++i)
@@ -93,7 +105,7 @@ struct skinny_product
 #pragma unroll
             for(int i = 0; i < S::LOADS_B; ++i)
             {
-                S::template load_block<false>(base + S::A_BYTES + i * 4096, vb, rsrc_b,
+                S::template load_block<ONCE>(base + S::A_BYTES + i * 4096, vb, rsrc_b,
                                               __builtin_amdgcn_readfirstlane((unsigned int)stage * stage_b + i * step_b));
             }
         };
@@ -182,16 +194,86 @@ struct skinny_product
             }
         }
         __syncthreads();
-#pragma unroll 4
-        for(int m = 0; m < MINE; ++m)
-        {
-            const int e = threadIdx.x + m * THREADS, row = x.row0 + e / BN, col = x.col0 + e % BN;
-            if(e < BM * BN && row < x.m && col < args.N)
+        // (wave order: the sum of an element is the same in every run)
+        auto tile_sum = [&](int e) {
+            return ((part[e] + part[BM * BN + e]) + part[2 * BM * BN + e]) + part[3 * BM * BN + e];
+        };
+        auto finish = [&](int e, float sum) {
+            const int row = x.row0 + e / BN, col = x.col0 + e % BN;
+            if(row < x.m && col < args.N)
             {
-                // (wave order: the sum of an element is the same in every run)
-                const float s = ((part[e] + part[BM * BN + e]) + part[2 * BM * BN + e]) + part[3 * BM * BN + e];
-                finish_element<InT, OutT, OutT>(args, x, row, col, s);
+                finish_element<InT, OutT, OutT>(args, x, row, col, sum);
             }
+        };
+        if(args.k_slices == 1)
+        {
+#pragma unroll 4
+            for(int m = 0; m < MINE; ++m)
+            {
+                const int e = threadIdx.x + m * THREADS;
+                if(e < BM * BN)
+                {
+                    finish(e, tile_sum(e));
+                }
+            }
+            return;
+        }
+        // Parts travel at device scope, past the XCD's own L2; a workgroup counts itself in when its
+        // stores have been acknowledged (see stream_gemm::run, whose exchange this is).
+        constexpr int DEVICE_SCOPE = 16, TILE = BM * BN, MAX_SLICES = S::MAX_SLICES;
+        const __amdgpu_buffer_rsrc_t shared = __builtin_amdgcn_make_buffer_rsrc(
+            args.partials + (long long)tile * args.k_slices * TILE, 0, args.k_slices * TILE * 4, 0x00020000);
+        for(int e = threadIdx.x; e < TILE; e += THREADS)
+        {
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, tile_sum(e)), shared,
+                                                  (slice * TILE + e) * 4, 0, DEVICE_SCOPE);
+        }
+        __builtin_amdgcn_s_waitcnt(S::vmcnt_imm(0));
+        __syncthreads();
+        __shared__ unsigned int arrived_before;
+        if(threadIdx.x == 0)
+        {
+            // the counter holds (epoch << 8 | arrivals); a count under another epoch starts from zero
+            unsigned int seen = __hip_atomic_load(args.arrivals + tile, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for(;;)
+            {
+                const unsigned int count = (seen >> 8) == args.arrival_epoch ? (seen & 255u) : 0u;
+                if(__hip_atomic_compare_exchange_strong(args.arrivals + tile, &seen,
+                                                        (args.arrival_epoch << 8) | (count + 1u), __ATOMIC_RELAXED,
+                                                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+                {
+                    arrived_before = count;
+                    break;
+                }
+            }
+        }
+        __syncthreads();
+        if(arrived_before != (unsigned int)(args.k_slices - 1))
+        {
+            return; // the last one to arrive finishes the tile
+        }
+        for(int e = threadIdx.x; e < TILE; e += THREADS)
+        {
+            float v[MAX_SLICES];
+#pragma unroll
+            for(int q = 0; q < MAX_SLICES; ++q)
+            {
+                v[q] = q < args.k_slices ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                                                         shared, (q * TILE + e) * 4, 0, DEVICE_SCOPE))
+                                         : 0.0f;
+            }
+            float sum = v[0];
+#pragma unroll
+            for(int q = 1; q < MAX_SLICES; ++q)
+            {
+                sum = q < args.k_slices ? sum + v[q] : sum;
+            }
+            finish(e, sum);
+        }
+        if(threadIdx.x == 0)
+        {
+            // back to zero arrivals, for a replay of this launch (same epoch)
+            __hip_atomic_store(args.arrivals + tile, args.arrival_epoch << 8, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
 };

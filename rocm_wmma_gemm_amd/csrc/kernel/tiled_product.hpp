@@ -57,13 +57,17 @@ struct tiled_product
     using InT  = typename loop::InT;
     static constexpr int THREADS = loop::THREADS, TM = loop::TM, TN = loop::TN, BK = 64;
     static constexpr int STAGE = loop::STAGE, VM_LOADS = loop::VM_LOADS;
-    // a wave's strip: 16 rows of half the columns of its tile in fp32, 16 bytes of padding a row
-    static constexpr int HALF = TN / 2, ROW_BYTES = HALF * 64, PITCH = ROW_BYTES + 16, STRIP = 16 * PITCH;
-    static constexpr int TABLE = 2 * (max_groups + 1) * 4;
-    static constexpr int LDS_BYTES = loop::LDS_BYTES + 4 * STRIP + TABLE;
+    // The ring: 2 stages, as the GEMM; 3 for 128 x 256 tiles, whose groups have few rows for a weight that
+    // comes from memory: the loads of two K tiles are then always on their way.
+    static constexpr int RING = BM == 128 && BN == 256 ? 3 : 2, RING_BYTES = RING * STAGE;
+    // a wave's strip: 16 rows of a part of the columns of its tile in fp32, 16 bytes of padding a row
+    static constexpr int PASSES = RING == 3 ? 4 : 2;
+    static constexpr int HALF = TN / PASSES, ROW_BYTES = HALF * 64, PITCH = ROW_BYTES + 16, STRIP = 16 * PITCH;
+    static constexpr int TABLE = 3 * (max_groups + 1) * 4;
+    static constexpr int LDS_BYTES = RING_BYTES + 4 * STRIP + TABLE;
     // workgroups per compute unit: what the LDS holds
     static constexpr int PER_CU = LDS_BYTES <= 80 * 1024 ? 2 : 1;
-    static_assert(LDS_BYTES <= 160 * 1024 && TN % 2 == 0 && TM % 2 == 0, "tile");
+    static_assert(LDS_BYTES <= 160 * 1024 && TN % PASSES == 0 && TM % 2 == 0, "tile");
     static_assert(!EPI::mirror || (TM == TN && BM == BN), "a mirrored tile is square");
 
     using lds_int   = __attribute__((address_space(3))) int;
@@ -75,7 +79,16 @@ struct tiled_product
     {
         product_item x;
         int          nk; // K tiles, at least one
+        bool         ends_k; // its last one is the last of K
+        float*       partial; // nullptr: a whole tile; else where its [BM][BN] of fp32 goes
         const InT *  a, *b, *a_end, *b_end;
+    };
+
+    // The groups' tables and how the launch's tiles are dealt.
+    struct plan
+    {
+        const lds_int *off, *first, *order;
+        tail_cut       cut;
     };
 
     __device__ __forceinline__ static int tiles_per_group(const product_args& args)
@@ -83,32 +96,56 @@ struct tiled_product
         return EPI::mirror ? args.grid_n * (args.grid_n + 1) / 2 : args.grid_m * args.grid_n;
     }
 
-    __device__ __forceinline__ static int total_items(const product_args& args, const lds_int* first)
+    __device__ __forceinline__ static plan make_plan(const product_args& args, lds_int* table, int workgroups)
     {
-        return args.kind == product_kind::rows ? __builtin_amdgcn_readfirstlane(first[args.groups]) * args.grid_n
-                                               : args.groups * tiles_per_group(args);
+        lds_int *off = table, *first = off + max_groups + 1, *order = first + max_groups + 1;
+        int      tiles = args.groups * tiles_per_group(args);
+        if(args.kind != product_kind::batch)
+        {
+            build_group_table(args.offsets, args.groups, args.kind == product_kind::rows ? args.M : args.K, BM, off,
+                              first);
+            if(args.kind == product_kind::rows)
+            {
+                tiles = __builtin_amdgcn_readfirstlane(first[args.groups]) * args.grid_n;
+            }
+            else if(args.groups > 1)
+            {
+                order_groups(args.groups, off, order);
+            }
+        }
+        // (where groups differ in K the slices would too: those launches are not cut)
+        const bool may_cut = args.partials != nullptr && !EPI::mirror && (args.kind != product_kind::sum || args.groups == 1);
+        tail_cut   cut     = cut_tail(tiles, workgroups, (args.K + BK - 1) / BK, may_cut);
+        cut.whole          = __builtin_amdgcn_readfirstlane(cut.whole);
+        cut.cut            = __builtin_amdgcn_readfirstlane(cut.cut);
+        cut.slices         = __builtin_amdgcn_readfirstlane(cut.slices);
+        cut.each           = __builtin_amdgcn_readfirstlane(cut.each);
+        return {off, first, order, cut};
     }
 
-    // Positions congruent mod 8 run on one XCD: it takes a contiguous run of items, the tiles of
-    // a group in bands of 4 tile rows, so that its L2 serves the panels that its workgroups share.
-    __device__ __forceinline__ static work decode(const product_args& args, const lds_int* off, const lds_int* first,
-                                                  int pos, int total)
+    // Tile number `tile` of the launch: its group and place.
+    __device__ __forceinline__ static product_item locate(const product_args& args, const plan& pl, int tile)
     {
-        work      w;
-        const int item = xcd_remap(pos, total);
-        int       local, grid_m = args.grid_m;
+        product_item x;
+        int          local, grid_m = args.grid_m;
         if(args.kind == product_kind::rows)
         {
-            w.x.group   = group_of_tile(first, args.groups, item / args.grid_n);
-            const int f = __builtin_amdgcn_readfirstlane(first[w.x.group]);
-            grid_m      = __builtin_amdgcn_readfirstlane(first[w.x.group + 1]) - f;
-            local       = item - f * args.grid_n;
+            x.group     = group_of_tile(pl.first, args.groups, tile / args.grid_n);
+            const int f = __builtin_amdgcn_readfirstlane(pl.first[x.group]);
+            grid_m      = __builtin_amdgcn_readfirstlane(pl.first[x.group + 1]) - f;
+            local       = tile - f * args.grid_n;
         }
         else
         {
             const int tiles = tiles_per_group(args);
-            w.x.group       = item / tiles;
-            local           = item - w.x.group * tiles;
+            x.group         = tile / tiles;
+            local           = tile - x.group * tiles;
+            if(args.kind == product_kind::sum && args.groups > 1)
+            {
+                // (one group after the other over the whole GPU, an XCD on neighbouring tiles)
+                x.group = pl.order[x.group];
+                local   = xcd_remap(local, tiles);
+            }
         }
         tile_coord t;
         if constexpr(EPI::mirror)
@@ -122,16 +159,44 @@ struct tiled_product
         {
             t = banded_tile(local, grid_m, args.grid_n, 4);
         }
-        w.x.group = __builtin_amdgcn_readfirstlane(w.x.group);
-        w.x.row0  = __builtin_amdgcn_readfirstlane(t.m * BM);
-        w.x.col0  = __builtin_amdgcn_readfirstlane(t.n * BN);
-        place_group(args, off, w.x);
-        w.nk = w.x.k > BK ? (w.x.k + BK - 1) / BK : 1;
+        x.group = __builtin_amdgcn_readfirstlane(x.group);
+        x.row0  = __builtin_amdgcn_readfirstlane(t.m * BM);
+        x.col0  = __builtin_amdgcn_readfirstlane(t.n * BN);
+        place_group(args, pl.off, x);
+        return x;
+    }
 
-        const InT* A = static_cast<const InT*>(args.A);
-        const InT* B = static_cast<const InT*>(args.B);
-        w.a = loop::scalar_pointer(A + w.x.a_at + (A_KMAJOR ? w.x.row0 * args.lda : (long long)w.x.row0));
-        w.b = loop::scalar_pointer(B + w.x.b_at + (B_KMAJOR ? w.x.col0 * args.ldb : (long long)w.x.col0));
+    // Positions congruent mod 8 run on one XCD: it takes a contiguous run of tiles, those of a
+    // group in bands of 4 tile rows, so that its L2 serves the panels that its workgroups share (of
+    // the cut tiles, a contiguous run of slices over all tiles).
+    __device__ __forceinline__ static work decode(const product_args& args, const plan& pl, int pos)
+    {
+        work w;
+        int  tile, k0 = 0;
+        w.partial = nullptr;
+        if(pos < pl.cut.whole)
+        {
+            tile = args.kind == product_kind::sum && args.groups > 1 ? pos : xcd_remap(pos, pl.cut.whole);
+        }
+        else
+        {
+            const int p = xcd_remap(pos - pl.cut.whole, pl.cut.cut * pl.cut.slices), slice = p / pl.cut.cut;
+            const int t = p - slice * pl.cut.cut;
+            tile        = pl.cut.whole + t;
+            k0          = slice * pl.cut.each;
+            w.partial   = args.partials + (long long)(t * pl.cut.slices + slice) * (BM * BN);
+        }
+        w.x         = locate(args, pl, tile);
+        const int k = w.x.k > BK ? (w.x.k + BK - 1) / BK : 1;
+        w.nk        = w.partial == nullptr ? k : (k - k0 < pl.cut.each ? k - k0 : pl.cut.each);
+        w.nk        = __builtin_amdgcn_readfirstlane(w.nk);
+        w.ends_k    = k0 + w.nk == k;
+
+        const InT*      A    = static_cast<const InT*>(args.A);
+        const InT*      B    = static_cast<const InT*>(args.B);
+        const long long from = (long long)k0 * BK;
+        w.a = loop::scalar_pointer(A + w.x.a_at + (A_KMAJOR ? w.x.row0 * args.lda + from : w.x.row0 + from * args.lda));
+        w.b = loop::scalar_pointer(B + w.x.b_at + (B_KMAJOR ? w.x.col0 * args.ldb + from : w.x.col0 + from * args.ldb));
         // Where the loads' range ends.  K-contiguous: with the operand's last row (rows past the
         // group's only reach rows of C that are not stored).  Else: with the group's K rows, so that
         // the rows of a last K tile past them read zeros, also those of the next group.
@@ -194,7 +259,8 @@ struct tiled_product
     __device__ __forceinline__ static void store(const float (&y)[PIECE], __amdgpu_buffer_rsrc_t to, unsigned int at,
                                                  unsigned int wave_at)
     {
-        constexpr int NT = 2; // C is not read again here
+        // (a layer's C is not read again here; what a Newton-Schulz step leaves the next one reads)
+        constexpr int NT = EPI::scaled ? 0 : 2;
         if constexpr(sizeof(T) == 4)
         {
             static_assert(PIECE == 4, "one 16-byte piece");
@@ -280,10 +346,10 @@ struct tiled_product
                 (unsigned int)((row_w + 16 * block) * args.ldc + col_w + p * HALF * 16) * size);
         };
 
-        float bias[2][READS][EPI::layer ? PIECE : 1];
-        float by_col[2][READS][EPI::diagonal == diagonal_use::cols ? PIECE : 1];
+        float bias[PASSES][READS][EPI::layer ? PIECE : 1];
+        float by_col[PASSES][READS][EPI::diagonal == diagonal_use::cols ? PIECE : 1];
 #pragma unroll
-        for(int p = 0; p < 2; ++p)
+        for(int p = 0; p < PASSES; ++p)
         {
 #pragma unroll
             for(int q = 0; q < READS; ++q)
@@ -327,13 +393,13 @@ struct tiled_product
         // residual pieces (and, by rows, what they are multiplied by) of AHEAD blocks are on their way
         constexpr int WANT = sizeof(OutT) == 4 || sizeof(ResT) == 4 || PER_CU > 1 || EPI::mirror ? 2 : 4;
         constexpr int AHEAD = BLOCKS < WANT ? BLOCKS : WANT;
-        piece<ResT, PIECE> residual[EPI::residual ? AHEAD : 1][2][READS];
+        piece<ResT, PIECE> residual[EPI::residual ? AHEAD : 1][PASSES][READS];
         float              by_row[EPI::diagonal == diagonal_use::rows ? AHEAD : 1][READS];
         auto fetch = [&](int block) {
             if constexpr(EPI::residual)
             {
 #pragma unroll
-                for(int p = 0; p < 2; ++p)
+                for(int p = 0; p < PASSES; ++p)
                 {
 #pragma unroll
                     for(int q = 0; q < READS; ++q)
@@ -369,7 +435,7 @@ struct tiled_product
                 loop::pin_row(acc[block]);
             }
 #pragma unroll
-            for(int p = 0; p < 2; ++p)
+            for(int p = 0; p < PASSES; ++p)
             {
 #pragma unroll
                 for(int t = 0; t < HALF; ++t)
@@ -479,24 +545,87 @@ struct tiled_product
         }
     }
 
-    // The K loop and its load stream: see solo_gemm::run, whose ring of 2 this is.
+    // A slice's part of a tile, in fp32: [BM][BN].
+    __device__ __forceinline__ static void write_partial(const work& w, f32x4 (&acc)[TM][TN], int row_w, int col_w,
+                                                         int lane, lds_char_ptr strip)
+    {
+        constexpr int PR = HALF * 4, READS = 16 * PR / 64; // pieces of 4 columns
+        static_assert(16 * PR % 64 == 0, "whole reads");
+        const int                    r16 = lane & 15, g = lane >> 4;
+        const __amdgpu_buffer_rsrc_t to = window(w.partial, true);
+        const int                    row = lane / PR, col = lane % PR * 4;
+        const unsigned int           at = (unsigned int)((row * BN + col) * 4);
+#pragma unroll
+        for(int block = 0; block < TM; ++block)
+        {
+            loop::pin_row(acc[block]);
+#pragma unroll
+            for(int p = 0; p < PASSES; ++p)
+            {
+#pragma unroll
+                for(int t = 0; t < HALF; ++t)
+                {
+                    *reinterpret_cast<lds_f32x4*>(strip + r16 * PITCH + (16 * t + 4 * g) * 4) = acc[block][p * HALF + t];
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                const unsigned int wave_at
+                    = (unsigned int)__builtin_amdgcn_readfirstlane(((row_w + 16 * block) * BN + col_w + p * HALF * 16) * 4);
+#pragma unroll
+                for(int q = 0; q < READS; ++q)
+                {
+                    const f32x4 v = *reinterpret_cast<const lds_f32x4*>(strip + (q * (64 / PR) + row) * PITCH + col * 4);
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to, at + q * (64 / PR) * BN * 4,
+                                                           wave_at, 0);
+                }
+                asm volatile("" ::: "memory");
+            }
+        }
+    }
+
+    // Adds up the slices of the cut tiles, in their order, and finishes them.  A thread takes 8
+    // columns of a row; a workgroup FINISH_ROWS rows of a tile.
+    static constexpr int FINISH_ROWS = THREADS * 8 / BN, FINISH_PARTS = BM / FINISH_ROWS;
+    __device__ __forceinline__ static void finish_cut(const product_args& args)
+    {
+        __shared__ int table_raw[3 * (max_groups + 1)];
+        lds_int*       table = (lds_int*)table_raw;
+        const plan     pl = make_plan(args, table, args.workgroups);
+        const int      parts = pl.cut.cut * FINISH_PARTS;
+        for(int part = blockIdx.x; part < parts; part += gridDim.x)
+        {
+            const int          t = part / FINISH_PARTS;
+            const product_item x = locate(args, pl, pl.cut.whole + t);
+            const int          r = (part - t * FINISH_PARTS) * FINISH_ROWS + (int)threadIdx.x / (BN / 8);
+            const int          c = (int)threadIdx.x % (BN / 8) * 8, row = x.row0 + r, col = x.col0 + c;
+            if(row >= x.m || col >= args.N)
+            {
+                continue;
+            }
+            const float* from = args.partials + (long long)t * pl.cut.slices * (BM * BN) + r * BN + c;
+            f32x4        lo{0.0f, 0.0f, 0.0f, 0.0f}, hi{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for(int s = 0; s < pl.cut.slices; ++s)
+            {
+                lo += *reinterpret_cast<const f32x4*>(from + (long long)s * (BM * BN));
+                hi += *reinterpret_cast<const f32x4*>(from + (long long)s * (BM * BN) + 4);
+            }
+            const float sum[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            finish_piece<InT, OutT, ResT>(args, x, row, col, sum);
+        }
+    }
+
+    // The K loop and its load stream: see solo_gemm::run; here with a ring of 2 or 3.
     __device__ __forceinline__ static void run(const product_args& args)
     {
         __shared__ __attribute__((aligned(1024))) char lds_raw[LDS_BYTES];
         lds_char_ptr lds   = (lds_char_ptr)lds_raw;
-        lds_int*     off   = reinterpret_cast<lds_int*>(lds + loop::LDS_BYTES + 4 * STRIP);
-        lds_int*     first = off + max_groups + 1;
 
         const int lane = threadIdx.x & 63;
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wave_m = wave / 2, wave_n = wave % 2;
-        if(args.kind != product_kind::batch)
-        {
-            build_group_table(args.offsets, args.groups, args.kind == product_kind::rows ? args.M : args.K, BM, off,
-                              first);
-        }
-        const int total = total_items(args, first), hop = (int)gridDim.x;
-        int       pos = (int)blockIdx.x;
+        const plan pl = make_plan(args, reinterpret_cast<lds_int*>(lds + RING_BYTES + 4 * STRIP), (int)gridDim.x);
+        const int  total = pl.cut.positions(), hop = (int)gridDim.x;
+        int        pos = (int)blockIdx.x;
         if(pos >= total)
         {
             return;
@@ -518,32 +647,34 @@ struct tiled_product
         const typename loop::addr_a la_tail = la.for_tail(lane, wave, k_tail);
         const typename loop::addr_b lb_tail = lb.for_tail(lane, wave, k_tail);
 
-        work       cur  = decode(args, off, first, pos, total);
+        work       cur  = decode(args, pl, pos);
         const InT* a_src = cur.a;
         const InT* b_src = cur.b;
         const InT* a_end = cur.a_end;
         const InT* b_end = cur.b_end;
         int        stream_left = cur.nk, stream_pos = pos + hop;
+        bool       stream_ends = cur.ends_k;
         auto advance = [&]() {
             a_src += a_step;
             b_src += b_step;
             if(--stream_left == 0)
             {
                 // (past its last item the stream starts over: the loads go where nobody reads)
-                const work nx = decode(args, off, first, stream_pos < total ? stream_pos : (int)blockIdx.x, total);
+                const work nx = decode(args, pl, stream_pos < total ? stream_pos : (int)blockIdx.x);
                 a_src         = nx.a;
                 b_src         = nx.b;
                 a_end         = nx.a_end;
                 b_end         = nx.b_end;
                 stream_left   = nx.nk;
+                stream_ends   = nx.ends_k;
                 stream_pos += hop;
             }
         };
-        auto partial_tile = [&]() { return k_ragged && stream_left == 1; };
+        auto partial_tile = [&]() { return k_ragged && stream_ends && stream_left == 1; };
 
         const unsigned int lds_addr   = (unsigned int)(size_t)lds;
         const unsigned int wave_block = lds_addr + wave * 1024;
-        lds_char_ptr       strip      = lds + loop::LDS_BYTES + wave * STRIP;
+        lds_char_ptr       strip      = lds + RING_BYTES + wave * STRIP;
         u32x4              fa[2][TM], fb[2][TN];
         constexpr int LOADS_A = VM_LOADS / 4, LOADS_B = VM_LOADS - LOADS_A, MFMAS = loop::MFMAS;
         using plan_b = typename loop::template load_plan<2, (MFMAS - 2) / LOADS_B, 0, LOADS_B>;
@@ -555,21 +686,30 @@ struct tiled_product
                               loop::descriptor(b_src, b_end));
         }
         advance();
+        if constexpr(RING == 3)
+        {
+            const bool part = partial_tile();
+            loop::issue_loads(std::make_integer_sequence<int, VM_LOADS>{}, la.or_else(part, la_tail),
+                              lb.or_else(part, lb_tail), wave_block + STAGE, loop::descriptor(a_src, a_end),
+                              loop::descriptor(b_src, b_end));
+            advance();
+        }
         bool part_prev = partial_tile();
         loop::issue_loads(std::make_integer_sequence<int, LOADS_B>{}, la.or_else(part_prev, la_tail),
-                          lb.or_else(part_prev, lb_tail), wave_block + STAGE, loop::descriptor(a_src, a_end),
-                          loop::descriptor(b_src, b_end));
+                          lb.or_else(part_prev, lb_tail), wave_block + (RING - 1) * STAGE,
+                          loop::descriptor(a_src, a_end), loop::descriptor(b_src, b_end));
         const InT* a_prev     = a_src;
         const InT* b_prev     = b_src;
         const InT* a_end_prev = a_end;
         const InT* b_end_prev = b_end;
         advance();
-        __builtin_amdgcn_s_waitcnt(loop::waitcnt_imm(LOADS_B));
+        // (behind tile 0, the first: the loads of the ring's other tiles may still be in flight)
+        __builtin_amdgcn_s_waitcnt(loop::waitcnt_imm((RING - 2) * VM_LOADS + LOADS_B));
         __builtin_amdgcn_s_barrier();
         loop::read_first(std::make_integer_sequence<int, TM>{}, std::make_integer_sequence<int, TN>{}, oa, ob, lds_addr,
                          fa[0], fb[0]);
 
-        unsigned int here = 0;
+        unsigned int here = 0; // stage (byte offset) of the tile the MFMAs are on
         for(;;)
         {
             f32x4 acc[TM][TN];
@@ -589,18 +729,20 @@ struct tiled_product
             }
             for(int it = 0; it < cur.nk; ++it)
             {
-                const unsigned int there = STAGE - here;
+                const unsigned int there = here + STAGE == RING_BYTES ? 0 : here + STAGE;
+                const unsigned int late  = here == 0 ? RING_BYTES - STAGE : here - STAGE; // of the last tile on its way
                 const bool         part  = partial_tile();
                 const auto la0 = la.or_else(part_prev, la_tail), la1 = la.or_else(part, la_tail);
                 const auto lb0 = lb.or_else(part_prev, lb_tail), lb1 = lb.or_else(part, lb_tail);
-                const typename loop::step_ctx c0{oa, ob, la0, lb0, lds_addr + here, wave_block + there,
+                const typename loop::step_ctx c0{oa, ob, la0, lb0, lds_addr + here, wave_block + late,
                                                  loop::descriptor(a_prev, a_end_prev),
                                                  loop::descriptor(b_prev, b_end_prev)};
                 const typename loop::step_ctx c1{oa, ob, la1, lb1, lds_addr + there, wave_block + here,
                                                  loop::descriptor(a_src, a_end), loop::descriptor(b_src, b_end)};
                 __builtin_amdgcn_s_waitcnt(loop::waitcnt_imm(63));
                 loop::template step<1, plan_a>(c0, fa[0], fb[0], fa[1], fb[1], acc);
-                __builtin_amdgcn_s_waitcnt(loop::waitcnt_imm(0));
+                // (the next tile has landed; with a ring of 3 the one behind it may be in flight)
+                __builtin_amdgcn_s_waitcnt(loop::waitcnt_imm((RING - 2) * VM_LOADS));
                 __builtin_amdgcn_s_barrier();
                 loop::template step<0, plan_b>(c1, fa[1], fb[1], fa[0], fb[0], acc);
                 a_prev     = a_src;
@@ -613,9 +755,21 @@ struct tiled_product
             }
             // (the MFMAs are invisible to the compiler: their result latency is covered by hand)
             asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-            write<false>(args, cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
-            if constexpr(EPI::mirror)
+            if constexpr(!EPI::mirror)
             {
+                if(cur.partial != nullptr)
+                {
+                    // (read next by the kernel that adds the slices up: no streaming hint)
+                    write_partial(cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
+                }
+                else
+                {
+                    write<false>(args, cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
+                }
+            }
+            else
+            {
+                write<false>(args, cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
                 write<true>(args, cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
             }
             pos += hop;
@@ -623,7 +777,7 @@ struct tiled_product
             {
                 break;
             }
-            cur = decode(args, off, first, pos, total);
+            cur = decode(args, pl, pos);
             loop::read_first(std::make_integer_sequence<int, TM>{}, std::make_integer_sequence<int, TN>{}, oa, ob,
                              lds_addr + here, fa[0], fb[0]);
         }
@@ -631,6 +785,12 @@ struct tiled_product
         __builtin_amdgcn_s_waitcnt(loop::waitcnt_imm(0));
     }
 };
+
+template<class Impl>
+__global__ void __launch_bounds__(Impl::THREADS) tiled_finish_entry(const product_args args)
+{
+    Impl::finish_cut(args);
+}
 
 template<class Impl>
 __global__ void __launch_bounds__(Impl::THREADS, Impl::PER_CU) tiled_product_entry(const product_args args)

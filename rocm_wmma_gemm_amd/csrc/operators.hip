@@ -43,7 +43,7 @@ product_kernel find_product(int types, int layout, int form, int finish)
         case 5: return product_of<5>(layout, form, finish);
         case 6: return product_of<6>(layout, form, finish);
         case 7: return product_of<7>(layout, form, finish);
-        default: return {nullptr, 0, 0, 0, 0};
+        default: return {nullptr, 0, 0, 0, nullptr, nullptr, 0};
     }
 }
 
@@ -130,54 +130,238 @@ bool aligned_rows(const product_args& a, int layout)
            && std::max({a.lda, a.ldb, a.ldc}) < (1 << 21);
 }
 
-// Which kernel a product runs on.
-int choose_form(int types, int layout, int finish, const product_args& args, size_t cus)
+// A product's kernel, and how the tiles that would leave compute units idle are cut along K.
+struct launch_choice
 {
-    auto tiles = [&](size_t edge) {
-        const size_t n = ceil_div(args.N, edge);
-        return args.kind == product_kind::rows ? (args.M / edge + std::min<size_t>(args.groups, args.M)) * n
-                                               : args.groups * ceil_div(args.M, edge) * n;
+    product_kernel kernel{nullptr, 0, 0, 0, nullptr, nullptr, 0};
+    size_t         items = 0; // tiles, or the most there can be (rows: the device knows how many)
+    size_t         workgroups = 0;
+    size_t         partial_bytes = 0; // room that cutting needs; 0: nothing is cut
+    int            k_slices = 1; // workgroups that share a tile of the few-row kernel
+    bool           once = false; // B's loads carry the non-temporal hint
+};
+
+// Tiles of a product: at most (`most`), and about (rows of several groups end inside a tile, half
+// full on average).
+size_t tiles_of(const product_args& a, size_t bm, size_t bn, bool symmetric, bool most)
+{
+    const size_t n = ceil_div(a.N, bn);
+    if(a.kind == product_kind::rows)
+    {
+        if(a.groups == 1 && a.offsets == nullptr)
+        {
+            return ceil_div(a.M, bm) * n;
+        }
+        const size_t used = std::min<size_t>(a.groups, a.M);
+        return (a.M / bm + (most || static_cast<size_t>(a.M) < bm * used ? used : (used + 1) / 2)) * n;
+    }
+    return a.groups * (symmetric ? n * (n + 1) / 2 : ceil_div(a.M, bm) * n);
+}
+
+// What a form costs, in microseconds: a round of tiles takes `fixed` plus, per 64 of K, `alone` where
+// few compute units work (and where each has one workgroup of the two it holds) up to `full` where
+// all do.  Measured in bf16 over 60 shapes from 1 x 1024 x 1024 to 8192 x 8192 x 1024, in the three pairs of
+// operand layouts (tiled: within 15 % of the measured time for all but the smallest; `full` is what
+// the clock under the power limit leaves).
+struct form_cost
+{
+    int   form;
+    float fixed, alone, full;
+    float stream; // bytes per us at which a weight comes from memory that no cache holds
+};
+constexpr form_cost tiled_costs[] = {
+    {form_tiled_256, 9.0f, 1.10f, 1.45f, 2.3e6f},
+    {form_tiled_128x256, 6.0f, 0.64f, 0.85f, 3.5e6f},
+    {form_tiled_128, 4.5f, 0.64f, 1.0f, 2.9e6f},
+    {form_tiled_192, 8.0f, 0.70f, 0.90f, 2.9e6f},
+};
+// (both operands K-contiguous)
+constexpr form_cost skinny_costs_kk[] = {
+    {form_skinny_16x32, 3.5f, 0.09f, 0.20f, 5.2e6f},  {form_skinny_32x16, 3.5f, 0.085f, 0.20f, 5.2e6f},
+    {form_skinny_32x32, 3.5f, 0.11f, 0.25f, 5.2e6f},  {form_skinny_64x32, 4.0f, 0.16f, 0.29f, 4.5e6f},
+    {form_skinny_64x64, 4.5f, 0.24f, 0.25f, 4.0e6f},
+};
+// (B contiguous along N: a k row of 32 columns is half a cache line)
+constexpr form_cost skinny_costs_kn[] = {
+    {form_skinny_16x32, 3.5f, 0.15f, 0.24f, 3.2e6f}, {form_skinny_16x64, 4.0f, 0.15f, 0.26f, 4.5e6f},
+    {form_skinny_32x32, 3.5f, 0.16f, 0.24f, 3.0e6f}, {form_skinny_32x64, 4.0f, 0.19f, 0.30f, 4.2e6f},
+    {form_skinny_64x32, 4.0f, 0.21f, 0.34f, 2.8e6f}, {form_skinny_64x64, 4.5f, 0.25f, 0.28f, 4.0e6f},
+};
+constexpr float bytes_per_us = 4.5e6f; // of partial tiles, written and read once each
+constexpr float join_us      = 9.0f; // the scratch buffer's lease and a second launch, or the exchange in one
+// A weight of this many bytes is not in the 256 MB memory-side cache when it is read again, behind
+// the others of its model; non-temporal loads then stream 6..15 % faster (16 x 8192 x 8192: 25.6 -> 23.4 us,
+// 16 x 8192 x 28672 79 -> 71), but lose what that cache holds of smaller ones (64 x 4096 x 4096: 10.9 -> 14.0).
+constexpr size_t once_bytes = size_t{96} << 20;
+
+// One round's time on `tiles` workgroups of a form.
+float round_us(const form_cost& f, size_t tiles, size_t cus, int per_cu, float k64)
+{
+    const float busy = per_cu > 1 ? (tiles > cus ? std::min(1.0f, float(tiles - cus) / cus * 2.0f) : 0.0f)
+                                  : std::min(1.0f, float(tiles) / cus);
+    return f.fixed + k64 * (f.alone + (f.full - f.alone) * busy);
+}
+
+// Which kernel a product runs on: the least estimated time of the forms that can take it.
+launch_choice choose(int types, int layout, int finish, const product_args& args, size_t cus)
+{
+    const bool symmetric = finish == finish_square || finish == finish_poly;
+    auto       made = [&](int form) {
+        launch_choice c;
+        c.kernel = find_product(types, layout, form, finish);
+        if(c.kernel.fn != nullptr)
+        {
+            c.items      = tiles_of(args, c.kernel.block_m, c.kernel.block_n, symmetric, true);
+            c.workgroups = c.kernel.per_cu == 0 ? c.items : std::min(c.items, c.kernel.per_cu * cus);
+        }
+        return c;
+    };
+    auto with_cut = [&](launch_choice c) {
+        const size_t all = c.kernel.per_cu * cus, tile_bytes = size_t{4} * c.kernel.block_m * c.kernel.block_n;
+        c.workgroups    = all;
+        c.partial_bytes = all * tile_bytes;
+        return c;
+    };
+    const size_t stages      = ceil_div(args.K, 128); // of the few-row kernel
+    auto         with_slices = [&](launch_choice c, size_t slices) {
+        // (every slice has a stage, and the counters have a place for every tile)
+        slices = std::max<size_t>(1, std::min(slices, stages));
+        slices = ceil_div(stages, ceil_div(stages, slices));
+        if(c.kernel.per_cu == 0 && slices > 1 && c.items <= stream_arrival_slots)
+        {
+            c.k_slices      = static_cast<int>(slices);
+            c.partial_bytes = c.items * slices * c.kernel.block_m * c.kernel.block_n * 4;
+        }
+        return c;
     };
     if(!aligned_rows(args, layout))
     {
-        return tiles(128) < cus ? form_general_64 : form_general_128;
+        return made(tiles_of(args, 128, 128, false, true) < cus ? form_general_64 : form_general_128);
     }
-    const size_t rows = args.kind == product_kind::rows ? ceil_div(args.M, std::min<size_t>(args.groups, args.M)) : args.M;
-    if(args.kind == product_kind::rows && rows <= 64
-       && (layout == layout_kk || static_cast<long long>(args.K) * args.ldb < (1ll << 30)))
+    launch_choice best;
+    float         least = 1e30f;
+    auto          offer = [&](const launch_choice& c, float us) {
+        if(us < least)
+        {
+            least = us;
+            best  = c;
+        }
+    };
+    const bool  several = args.kind == product_kind::sum && args.groups > 1; // sums of different lengths
+    const bool  rows_kind = args.kind == product_kind::rows;
+    // (rows: a group's weight is read if it has a row)
+    const size_t used   = rows_kind ? std::min<size_t>(args.groups, args.M) : args.groups;
+    const float  weight = rows_kind ? float(used) * args.N * args.K * 2 : 0.0f;
+    const float k64     = std::max(1.0f, (several ? float(args.K) / args.groups : float(args.K)) / 64.0f);
+    for(const form_cost& f : tiled_costs)
     {
-        return rows <= 16 ? form_skinny_16x32 : rows <= 32 ? form_skinny_32x32 : form_skinny_64x32;
+        const launch_choice c = made(f.form);
+        if(c.kernel.fn == nullptr)
+        {
+            continue;
+        }
+        const size_t tiles = tiles_of(args, c.kernel.block_m, c.kernel.block_n, symmetric, false);
+        const size_t slots = c.kernel.per_cu * cus, rounds = tiles / slots, rest = tiles % slots;
+        const float  whole = rounds * round_us(f, slots, cus, c.kernel.per_cu, k64), least_us = weight / f.stream;
+        offer(c, std::max(least_us, whole + (rest ? round_us(f, rest, cus, c.kernel.per_cu, k64) : 0.0f)));
+        const device::tail_cut cut = device::cut_tail(static_cast<int>(tiles), static_cast<int>(slots),
+                                                      static_cast<int>(std::ceil(k64)), !several && c.kernel.finish != nullptr);
+        if(cut.cut != 0)
+        {
+            const size_t parts = size_t(cut.cut) * cut.slices;
+            offer(with_cut(c), std::max(least_us, whole + round_us(f, parts, cus, c.kernel.per_cu, float(cut.each))) + join_us
+                                   + 2.0f * parts * 4 * c.kernel.block_m * c.kernel.block_n / bytes_per_us);
+        }
     }
-    return rows <= 160 || tiles(256) < cus ? form_tiled_128 : form_tiled_256;
+    // (the few-row kernel's offsets within a weight that is contiguous along N have 31 bits)
+    if(rows_kind && (layout == layout_kk || static_cast<long long>(args.K) * args.ldb < (1ll << 30)))
+    {
+        const size_t rows = ceil_div(args.M, used);
+        auto         consider = [&](const form_cost& f) {
+            launch_choice c = made(f.form);
+            if(c.kernel.fn == nullptr)
+            {
+                return;
+            }
+            const size_t tiles = tiles_of(args, c.kernel.block_m, c.kernel.block_n, false, false);
+            const int    per_cu = f.form == form_skinny_64x64 ? 1 : 2;
+            const size_t slots = per_cu * cus;
+            const bool   one_high = rows <= static_cast<size_t>(c.kernel.block_m);
+            c.once                = one_high && weight >= once_bytes;
+            for(const size_t slices : {1, 2, 4})
+            {
+                const launch_choice s = slices == 1 ? c : with_slices(c, slices);
+                if(slices > 1 && (s.k_slices == 1 || tiles * slices > slots))
+                {
+                    continue;
+                }
+                const size_t workgroups = tiles * s.k_slices, rounds = workgroups / slots, rest = workgroups % slots;
+                const float  k = k64 / s.k_slices;
+                float us = rounds * round_us(f, slots, cus, per_cu, k) + (rest ? round_us(f, rest, cus, per_cu, k) : 0.0f);
+                // (row tiles that share a weight do not all find it in L2)
+                us = std::max(us, weight / (one_high ? f.stream : 0.65f * f.stream));
+                offer(s, us + (s.k_slices > 1 ? join_us : 0.0f));
+            }
+        };
+        if(layout == layout_kk)
+        {
+            for(const form_cost& f : skinny_costs_kk)
+            {
+                consider(f);
+            }
+        }
+        else
+        {
+            for(const form_cost& f : skinny_costs_kn)
+            {
+                consider(f);
+            }
+        }
+    }
+    return best;
 }
 
-// One product: picks the kernel and launches it.
-int launch_product(int types, int layout, int finish, product_args args, hipStream_t stream)
+// One product on the kernel chosen for it.  partials: the room that the choice asked for, or nullptr:
+// nothing is cut then.
+int launch_product(const launch_choice& c, product_args args, void* partials, hipStream_t stream)
 {
     if(args.N == 0 || args.M == 0 || args.groups == 0)
     {
         return ROCM_WMMA_GEMM_OK;
     }
-    const size_t         cus    = std::max<size_t>(compute_units_of_current_device(), 1);
-    const product_kernel kernel = find_product(types, layout, choose_form(types, layout, finish, args, cus), finish);
-    if(kernel.fn == nullptr)
+    if(c.kernel.fn == nullptr || c.items > most_extent)
     {
         return ROCM_WMMA_GEMM_ERR_LIMIT;
     }
-    const size_t grid_m = ceil_div(args.M, kernel.block_m), grid_n = ceil_div(args.N, kernel.block_n);
-    // (rows: how many tiles there are is only known on the device; at most this many)
-    const size_t items = args.kind == product_kind::rows
-                             ? (args.M / kernel.block_m + std::min<size_t>(args.groups, args.M)) * grid_n
-                             : args.groups * grid_m * grid_n;
-    if(items > most_extent)
+    const bool cuts = c.partial_bytes != 0 && partials != nullptr;
+    args.grid_m     = static_cast<int>(ceil_div(args.M, c.kernel.block_m));
+    args.grid_n     = static_cast<int>(ceil_div(args.N, c.kernel.block_n));
+    args.partials   = cuts ? static_cast<float*>(partials) : nullptr;
+    args.workgroups = static_cast<int>(c.workgroups);
+    args.k_slices   = 1;
+    if(cuts && c.k_slices > 1)
     {
-        return ROCM_WMMA_GEMM_ERR_LIMIT;
+        args.arrivals = arrivals_of_current_device(false);
+        if(args.arrivals == nullptr)
+        {
+            return ROCM_WMMA_GEMM_ERR_RUNTIME;
+        }
+        args.arrival_epoch = next_arrival_epoch();
+        args.k_slices      = c.k_slices;
     }
-    args.grid_m = static_cast<int>(grid_m);
-    args.grid_n = static_cast<int>(grid_n);
-    const size_t blocks = kernel.per_cu == 0 ? items : std::min(items, kernel.per_cu * cus);
-    enqueue(kernel.fn, dim3(static_cast<unsigned>(blocks)), dim3(kernel.threads), stream, args);
+    enqueue(c.once && c.kernel.once != nullptr ? c.kernel.once : c.kernel.fn,
+            dim3(static_cast<unsigned>(c.workgroups * args.k_slices)), dim3(c.kernel.threads), stream, args);
+    if(cuts && c.kernel.finish != nullptr)
+    {
+        enqueue(c.kernel.finish, dim3(static_cast<unsigned>(std::min<size_t>(2048, c.workgroups * 8))),
+                dim3(c.kernel.threads), stream, args);
+    }
     return ROCM_WMMA_GEMM_OK;
+}
+
+size_t compute_units()
+{
+    return std::max<size_t>(compute_units_of_current_device(), 1);
 }
 
 // A linear layer's problem, for one weight (groups = 1 and no offsets) or one per group of rows.
@@ -246,7 +430,10 @@ int forward(const layer& p, void* C, const void* A, const void* B, const rocm_wm
     const int finish = p.act.kind == act_kind::logistic ? finish_logistic
                        : p.act.kind == act_kind::relu || e.bias || e.residual || e.preact ? finish_layer
                                                                                           : finish_plain;
-    return launch_product(p.type_idx, p.layout_b == 1 ? layout_kk : layout_kn, finish, a, stream);
+    const launch_choice c = choose(p.type_idx, p.layout_b == 1 ? layout_kk : layout_kn, finish, a, compute_units());
+    workspace_lease     lease;
+    void* partials = c.partial_bytes != 0 ? lease.acquire(c.partial_bytes, stream) : nullptr; // (without: whole tiles)
+    return launch_product(c, a, partials, stream);
 }
 
 template<class InT>
@@ -261,7 +448,7 @@ template<class OutT>
 void launch_column_sums(const device::slope_args& s, void* dbias, int accumulate, hipStream_t stream)
 {
     enqueue(&device::column_sums<OutT>, dim3(static_cast<unsigned>(ceil_div(s.cols, 64)), static_cast<unsigned>(s.groups)),
-            dim3(64), stream, s, static_cast<OutT*>(dbias), accumulate);
+            dim3(256), stream, s, static_cast<OutT*>(dbias), accumulate);
 }
 
 // dZ = dC act'(Z); dA = dZ B^T, dB = A^T dZ, dbias = sum of dZ's rows, group by group
@@ -279,23 +466,78 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     {
         return ROCM_WMMA_GEMM_ERR_ARGUMENT;
     }
-    workspace_lease lease;
-    const void*     dz = dC;
-    if((sloped || dbias != nullptr) && p.N != 0)
+    const size_t       cus = compute_units();
+    const void*        dz  = dC;
+    product_args       to_a = arguments(p), to_b = arguments(p);
+    launch_choice      on_a, on_b;
+    device::slope_args s{};
+    // dZ and the sums of its columns live in the scratch buffer, and what the products ask for
+    const bool   passes = (sloped || dbias != nullptr) && p.N != 0;
+    const size_t runs   = p.M / device::slope_rows + std::min(p.groups, p.M);
+    const size_t dz_bytes = passes && sloped ? whole_lines(p.M * p.N * 2) : 0;
+    const size_t sums     = passes && dbias != nullptr ? whole_lines(runs * p.N * sizeof(float)) : 0;
+    if(runs > most_extent || ceil_div(p.N, 64) > 65535)
     {
-        const size_t runs     = p.M / device::slope_rows + std::min(p.groups, p.M);
-        const size_t dz_bytes = sloped ? whole_lines(p.M * p.N * 2) : 0;
-        const size_t sums     = dbias != nullptr ? runs * p.N * sizeof(float) : 0;
-        char*        ws       = nullptr;
-        if(dz_bytes + sums != 0)
+        return ROCM_WMMA_GEMM_ERR_LIMIT;
+    }
+    // (where the products find dZ is not known yet; the buffer is aligned for any kernel)
+    auto placed = [&](const void* at) {
+        to_a.A = at;
+        (p.layout_b == 1 ? to_b.A : to_b.B) = at;
+    };
+    if(dA != nullptr)
+    {
+        to_a.C        = dA;
+        to_a.B        = B;
+        to_a.kind     = product_kind::rows;
+        to_a.M        = static_cast<int>(p.M);
+        to_a.N        = static_cast<int>(p.K);
+        to_a.K        = static_cast<int>(p.N);
+        to_a.lda      = p.N;
+        to_a.ldb      = p.layout_b == 1 ? p.K : p.N;
+        to_a.ldc      = p.K;
+        to_a.stride_b = static_cast<long long>(p.N * p.K);
+    }
+    if(dB != nullptr)
+    {
+        // stored N x K: dZ^T A; stored K x N: A^T dZ
+        const bool nk = p.layout_b == 1;
+        to_b.C        = dB;
+        (nk ? to_b.B : to_b.A) = A;
+        to_b.residual = accumulate ? dB : nullptr;
+        to_b.kind     = product_kind::sum;
+        to_b.M        = static_cast<int>(nk ? p.N : p.K);
+        to_b.N        = static_cast<int>(nk ? p.K : p.N);
+        to_b.K        = static_cast<int>(p.M);
+        to_b.lda      = to_b.M;
+        to_b.ldb      = to_b.N;
+        to_b.ldc      = to_b.N;
+        to_b.stride_c = static_cast<long long>(p.N * p.K);
+    }
+    placed(dz_bytes != 0 ? nullptr : dC);
+    if(dA != nullptr && p.M != 0 && p.K != 0)
+    {
+        on_a = choose(p.type_idx, p.layout_b == 1 ? layout_kn : layout_kk, finish_plain, to_a, cus);
+    }
+    if(dB != nullptr && p.N != 0 && p.K != 0)
+    {
+        on_b = choose(p.type_idx, layout_mn, accumulate ? finish_add : finish_plain, to_b, cus);
+    }
+    workspace_lease lease;
+    const size_t    needed = dz_bytes + sums, cuts = std::max(on_a.partial_bytes, on_b.partial_bytes);
+    char*           ws = needed + cuts != 0 ? lease.acquire(needed + cuts, stream) : nullptr;
+    char*           partials = ws != nullptr ? ws + needed : nullptr;
+    if(ws == nullptr && needed != 0)
+    {
+        // (a capture forbids to allocate: perhaps there is room without cut tiles)
+        ws = cuts != 0 ? lease.acquire(needed, stream) : nullptr;
+        if(ws == nullptr)
         {
-            ws = lease.acquire(dz_bytes + sums, stream);
-            if(ws == nullptr)
-            {
-                return ROCM_WMMA_GEMM_ERR_SCRATCH;
-            }
+            return ROCM_WMMA_GEMM_ERR_SCRATCH;
         }
-        device::slope_args s{};
+    }
+    if(passes)
+    {
         s.dc      = dC;
         s.z       = sloped ? preact : nullptr;
         s.dz      = sloped ? ws : nullptr;
@@ -305,20 +547,13 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
         s.rows    = static_cast<int>(p.M);
         s.cols    = static_cast<int>(p.N);
         s.act     = p.act;
-        if(runs > most_extent || ceil_div(p.N, 64) > 65535)
-        {
-            return ROCM_WMMA_GEMM_ERR_LIMIT;
-        }
         if(runs != 0)
         {
             const bool wide = p.N % 8 == 0 && aligned16(dC) && (!sloped || aligned16(preact));
             is_bf16(p.type_idx) ? launch_slope<__bf16>(s, runs, wide, stream)
                                 : launch_slope<_Float16>(s, runs, wide, stream);
         }
-        if(sloped)
-        {
-            dz = ws;
-        }
+        dz = sloped ? ws : dC;
         if(dbias != nullptr)
         {
             switch(p.type_idx)
@@ -329,41 +564,15 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
             }
         }
     }
+    placed(dz);
     int rc = ROCM_WMMA_GEMM_OK;
-    if(dA != nullptr)
+    if(on_a.kernel.fn != nullptr)
     {
-        product_args a = arguments(p);
-        a.C            = dA;
-        a.A            = dz;
-        a.B            = B;
-        a.kind         = product_kind::rows;
-        a.M            = static_cast<int>(p.M);
-        a.N            = static_cast<int>(p.K);
-        a.K            = static_cast<int>(p.N);
-        a.lda          = p.N;
-        a.ldb          = p.layout_b == 1 ? p.K : p.N;
-        a.ldc          = p.K;
-        a.stride_b     = static_cast<long long>(p.N * p.K);
-        rc             = launch_product(p.type_idx, p.layout_b == 1 ? layout_kn : layout_kk, finish_plain, a, stream);
+        rc = launch_product(on_a, to_a, partials, stream);
     }
-    if(rc == ROCM_WMMA_GEMM_OK && dB != nullptr)
+    if(rc == ROCM_WMMA_GEMM_OK && on_b.kernel.fn != nullptr)
     {
-        // stored N x K: dZ^T A; stored K x N: A^T dZ
-        const bool   nk = p.layout_b == 1;
-        product_args a  = arguments(p);
-        a.C             = dB;
-        a.A             = nk ? dz : A;
-        a.B             = nk ? A : dz;
-        a.residual      = accumulate ? dB : nullptr;
-        a.kind          = product_kind::sum;
-        a.M             = static_cast<int>(nk ? p.N : p.K);
-        a.N             = static_cast<int>(nk ? p.K : p.N);
-        a.K             = static_cast<int>(p.M);
-        a.lda           = a.M;
-        a.ldb           = a.N;
-        a.ldc           = a.N;
-        a.stride_c      = static_cast<long long>(p.N * p.K);
-        rc              = launch_product(p.type_idx, layout_mn, accumulate ? finish_add : finish_plain, a, stream);
+        rc = launch_product(on_b, to_b, partials, stream);
     }
     return rc;
 }
@@ -440,15 +649,27 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
     auto start = [&](auto* typed) {
         using given_t = std::remove_pointer_t<decltype(typed)>;
         const given_t* given = static_cast<const given_t*>(G);
-        enqueue(&device::sum_squares<given_t>, dim3(device::square_parts, static_cast<unsigned>(batch)), dim3(256), stream,
-                given, static_cast<long long>(M * N), parts);
-        enqueue(&device::orthogonal_start<given_t>,
-                dim3(static_cast<unsigned>(ceil_div(each / 8, 256)), static_cast<unsigned>(batch)), dim3(256), stream, given,
+        constexpr int  wide   = 16 / sizeof(given_t);
+        const bool     vector = M * N % wide == 0 && aligned16(given);
+        // (a workgroup for every 4096 pieces, but at most eight to a compute unit over the batch)
+        const size_t used = std::max<size_t>(
+            1, std::min({ceil_div(M * N / (vector ? wide : 1), 4096), size_t{device::square_parts}, ceil_div(2048, batch)}));
+        enqueue(vector ? &device::sum_squares<given_t, wide> : &device::sum_squares<given_t, 1>,
+                dim3(static_cast<unsigned>(used), static_cast<unsigned>(batch)), dim3(256), stream, given,
+                static_cast<long long>(M * N), parts);
+        const bool   whole = mp == M && np == N && aligned16(given);
+        const size_t row_groups = std::min<size_t>(mp, std::max<size_t>(1, 2048 / batch));
+        enqueue(whole ? &device::orthogonal_start<given_t, true> : &device::orthogonal_start<given_t, false>,
+                dim3(static_cast<unsigned>(row_groups), static_cast<unsigned>(batch)), dim3(256), stream, given,
                 parts, x32, x16[0], static_cast<int>(M), static_cast<int>(N), static_cast<int>(mp), static_cast<int>(np),
-                scale, epsilon);
+                scale, epsilon, static_cast<int>(used));
     };
     by_element(given_type, start);
     const float a = coefficients[0], b = coefficients[1], c = coefficients[2];
+    const size_t cus     = compute_units();
+    auto         product = [&](int types, int layout, int finish, const product_args& args) {
+        return launch_product(choose(types, layout, finish, args, cus), args, nullptr, stream);
+    };
     product_args p{};
     p.kind   = product_kind::batch;
     p.groups = static_cast<int>(batch);
@@ -464,7 +685,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         p.lda = p.ldb = np, p.ldc = lp;
         p.stride_a = p.stride_b = each, p.stride_c = square;
         p.alpha = 1.0f / (scale * scale), p.beta = 0.0f, p.diagonal_is = device::diagonal_use::none;
-        rc = launch_product(types_steps_square, tall ? layout_mn : layout_kk, finish_square, p, stream);
+        rc = product(types_steps_square, tall ? layout_mn : layout_kk, finish_square, p);
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             break;
@@ -473,7 +694,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         p.C = q, p.A = p.B = s, p.residual = s;
         p.K = static_cast<int>(lp), p.lda = p.ldb = lp, p.stride_a = p.stride_b = square;
         p.alpha = c, p.beta = b, p.diagonal_is = device::diagonal_use::split;
-        rc = launch_product(types_steps_square, layout_kk, finish_poly, p, stream);
+        rc = product(types_steps_square, layout_kk, finish_poly, p);
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             break;
@@ -487,18 +708,18 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         p.diagonal_is = tall ? device::diagonal_use::cols : device::diagonal_use::rows;
         p.C = last ? (direct ? O : static_cast<void*>(x16[(step + 1) & 1])) : x32;
         p.kept = last ? nullptr : x16[(step + 1) & 1], p.keep_sum = 1;
-        rc = launch_product(!last ? types_steps_next
+        rc = product(!last ? types_steps_next
                             : out_type == ROCM_WMMA_GEMM_ELEMENT_F16 ? types_steps_f16 : types_steps_bf16,
                             tall ? layout_kk : layout_kn,
                             last ? (tall ? finish_last_cols : finish_last_rows) : tall ? finish_next_cols : finish_next_rows,
-                            p, stream);
+                     p);
         p.keep_sum = 0;
     }
     if(rc == ROCM_WMMA_GEMM_OK && !direct)
     {
         // (a 16-bit element is a 16-bit element)
         enqueue(&device::orthogonal_end<unsigned short>,
-                dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(M * N, 256), 4096)), static_cast<unsigned>(batch)),
+                dim3(static_cast<unsigned>(std::min<size_t>(M, 4096)), static_cast<unsigned>(batch)),
                 dim3(256), stream, reinterpret_cast<const unsigned short*>(x16[steps & 1]), static_cast<unsigned short*>(O),
                 static_cast<int>(M), static_cast<int>(N), static_cast<int>(mp), static_cast<int>(np));
     }

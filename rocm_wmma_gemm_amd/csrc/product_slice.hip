@@ -20,33 +20,38 @@ using out_t = std::conditional_t<
     std::conditional_t<kTypes == types_bf16_bf16 || kTypes == types_steps_bf16, __bf16, float>>;
 using res_t = std::conditional_t<kTypes == types_steps_f16 || kTypes == types_steps_bf16, float, out_t>;
 
-constexpr product_kernel kNone{nullptr, 0, 0, 0, 0};
+constexpr product_kernel kNone{nullptr, 0, 0, 0, nullptr, nullptr, 0};
 constexpr bool           kSteps = kTypes >= types_steps_square;
 
 template<class Impl>
 product_kernel made(int block_m, int block_n, int per_cu)
 {
-    return {&device::product_entry<Impl>, block_m, block_n, Impl::THREADS, per_cu};
+    return {&device::product_entry<Impl>, block_m, block_n, Impl::THREADS, nullptr, nullptr, per_cu};
 }
 
-template<int LAYOUT, int EDGE, class EPI>
+template<int LAYOUT, int BM, int BN, class EPI>
 product_kernel tiled()
 {
     constexpr bool AK = LAYOUT != layout_mn, BK = LAYOUT == layout_kk;
-    using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, EDGE, EDGE, EPI>;
-    return {&device::tiled_product_entry<impl>, EDGE, EDGE, impl::THREADS, impl::PER_CU};
+    using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, BM, BN, EPI>;
+    product_fn finish = nullptr;
+    if constexpr(!EPI::mirror)
+    {
+        finish = &device::tiled_finish_entry<impl>;
+    }
+    return {&device::tiled_product_entry<impl>, BM, BN, impl::THREADS, finish, nullptr, impl::PER_CU};
 }
 
 // Only what some call asks for is built.
-template<int LAYOUT, int EDGE>
+template<int LAYOUT, int BM, int BN>
 product_kernel tiled_finish(int finish)
 {
     if constexpr(!kSteps && LAYOUT == layout_mn) // gradients of weights
     {
         switch(finish)
         {
-            case finish_plain: return tiled<LAYOUT, EDGE, device::epilogue_plain>();
-            case finish_add: return tiled<LAYOUT, EDGE, device::epilogue_add>();
+            case finish_plain: return tiled<LAYOUT, BM, BN, device::epilogue_plain>();
+            case finish_add: return tiled<LAYOUT, BM, BN, device::epilogue_add>();
             default: return kNone;
         }
     }
@@ -54,9 +59,9 @@ product_kernel tiled_finish(int finish)
     {
         switch(finish)
         {
-            case finish_plain: return tiled<LAYOUT, EDGE, device::epilogue_plain>();
-            case finish_layer: return tiled<LAYOUT, EDGE, device::epilogue_layer>();
-            case finish_logistic: return tiled<LAYOUT, EDGE, device::epilogue_logistic>();
+            case finish_plain: return tiled<LAYOUT, BM, BN, device::epilogue_plain>();
+            case finish_layer: return tiled<LAYOUT, BM, BN, device::epilogue_layer>();
+            case finish_logistic: return tiled<LAYOUT, BM, BN, device::epilogue_logistic>();
             default: return kNone;
         }
     }
@@ -66,14 +71,14 @@ product_kernel tiled_finish(int finish)
         {
             if(finish == finish_square)
             {
-                return tiled<LAYOUT, EDGE, device::epilogue_square>();
+                return tiled<LAYOUT, BM, BN, device::epilogue_square>();
             }
         }
         if constexpr(LAYOUT == layout_kk)
         {
             if(finish == finish_poly)
             {
-                return tiled<LAYOUT, EDGE, device::epilogue_poly>();
+                return tiled<LAYOUT, BM, BN, device::epilogue_poly>();
             }
         }
         return kNone;
@@ -85,12 +90,12 @@ product_kernel tiled_finish(int finish)
         if constexpr(kTypes == types_steps_next)
         {
             using epi = std::conditional_t<ROWS, device::epilogue_next_rows, device::epilogue_next_cols>;
-            return finish == (ROWS ? finish_next_rows : finish_next_cols) ? tiled<LAYOUT, EDGE, epi>() : kNone;
+            return finish == (ROWS ? finish_next_rows : finish_next_cols) ? tiled<LAYOUT, BM, BN, epi>() : kNone;
         }
         else
         {
             using epi = std::conditional_t<ROWS, device::epilogue_last_rows, device::epilogue_last_cols>;
-            return finish == (ROWS ? finish_last_rows : finish_last_cols) ? tiled<LAYOUT, EDGE, epi>() : kNone;
+            return finish == (ROWS ? finish_last_rows : finish_last_cols) ? tiled<LAYOUT, BM, BN, epi>() : kNone;
         }
     }
     else
@@ -102,9 +107,14 @@ product_kernel tiled_finish(int finish)
 template<int LAYOUT, int BM, int BN>
 product_kernel skinny()
 {
-    if constexpr(!kSteps && LAYOUT != layout_mn)
+    constexpr bool built = (BN == 64 && BM < 64) ? LAYOUT == layout_kn : BN == 16 ? LAYOUT == layout_kk : true;
+    if constexpr(!kSteps && LAYOUT != layout_mn && built)
     {
-        return made<device::skinny_product<kIn, out_t, BM, BN, LAYOUT == layout_kk>>(BM, BN, 0);
+        using impl       = device::skinny_product<kIn, out_t, BM, BN, LAYOUT == layout_kk, false>;
+        using once       = device::skinny_product<kIn, out_t, BM, BN, LAYOUT == layout_kk, true>;
+        product_kernel k = made<impl>(BM, BN, 0);
+        k.once           = &device::product_entry<once>;
+        return k;
     }
     else
     {
@@ -137,14 +147,27 @@ product_kernel in_layout(int form, int finish)
     {
         case form_general_128:
         case form_general_64: return general<LAYOUT>(form);
-        case form_tiled_256: return tiled_finish<LAYOUT, 256>(finish);
-        case form_tiled_128: return tiled_finish<LAYOUT, 128>(finish);
+        case form_tiled_256: return tiled_finish<LAYOUT, 256, 256>(finish);
+        case form_tiled_128: return tiled_finish<LAYOUT, 128, 128>(finish);
+        case form_tiled_128x256:
+            if constexpr(!kSteps)
+            {
+                return tiled_finish<LAYOUT, 128, 256>(finish);
+            }
+            return kNone;
+        case form_tiled_192:
+            if constexpr(kTypes == types_steps_square && LAYOUT == layout_kk)
+            {
+                return tiled_finish<LAYOUT, 192, 192>(finish);
+            }
+            return kNone;
         case form_skinny_16x32: return skinny<LAYOUT, 16, 32>();
         case form_skinny_16x64: return skinny<LAYOUT, 16, 64>();
         case form_skinny_32x32: return skinny<LAYOUT, 32, 32>();
         case form_skinny_32x64: return skinny<LAYOUT, 32, 64>();
         case form_skinny_64x32: return skinny<LAYOUT, 64, 32>();
         case form_skinny_64x64: return skinny<LAYOUT, 64, 64>();
+        case form_skinny_32x16: return skinny<LAYOUT, 32, 16>();
         default: return kNone;
     }
 }

@@ -43,12 +43,16 @@ enum product_form
     // rows that start on 16 bytes:
     form_tiled_256, // persistent 256 x 256 tiles
     form_tiled_128, // persistent 128 x 128 tiles
-    form_skinny_16x32, // whole sums of few rows, rows x columns of a tile
-    form_skinny_16x64,
+    form_tiled_128x256,
+    form_tiled_192, // symmetric products of K-contiguous operands only
+    // whole sums of few rows, rows x columns of a tile
+    form_skinny_16x32,
+    form_skinny_16x64, // B contiguous along N only: a k row of 64 columns is a whole cache line
     form_skinny_32x32,
-    form_skinny_32x64,
+    form_skinny_32x64, // likewise
     form_skinny_64x32,
     form_skinny_64x64,
+    form_skinny_32x16, // B contiguous along K only
     num_product_forms
 };
 
@@ -72,6 +76,8 @@ struct product_kernel
 {
     product_fn fn; // nullptr: not built
     int        block_m, block_n, threads;
+    product_fn finish; // adds up and finishes the tiles that the kernel cut along K; nullptr: it cuts none
+    product_fn once; // its twin with non-temporal loads of B; nullptr: none
     int        per_cu; // workgroups of a compute unit, for a persistent kernel; 0: a workgroup per tile
 };
 

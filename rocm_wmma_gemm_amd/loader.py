@@ -128,15 +128,20 @@ def detect_arch() -> str:
     return name.split(":", 1)[0]
 
 
-def _type_slot(c_dtype, ab_dtype) -> int:
-    import torch
+_SLOTS = {}
 
-    table = {(torch.float16, torch.float16): 0, (torch.float32, torch.float16): 1,
-             (torch.bfloat16, torch.bfloat16): 2, (torch.float32, torch.bfloat16): 3}
-    try:
-        return table[(c_dtype, ab_dtype)]
-    except KeyError:
-        raise TypeError(f"Unsupported type pair for rocm_wmma_gemm loader: C={c_dtype}, A/B={ab_dtype}")
+
+def _type_slot(c_dtype, ab_dtype) -> int:
+    slot = _SLOTS.get((c_dtype, ab_dtype))
+    if slot is None:
+        import torch
+
+        _SLOTS.update({(torch.float16, torch.float16): 0, (torch.float32, torch.float16): 1,
+                       (torch.bfloat16, torch.bfloat16): 2, (torch.float32, torch.bfloat16): 3})
+        slot = _SLOTS.get((c_dtype, ab_dtype))
+        if slot is None:
+            raise TypeError(f"Unsupported type pair for rocm_wmma_gemm loader: C={c_dtype}, A/B={ab_dtype}")
+    return slot
 
 
 class Loader:
@@ -335,30 +340,47 @@ class Loader:
         if status != OK:
             raise GemmLibraryError(f"rocm_wmma_gemm_{name}: {self._STATUS.get(status, status)}")
 
+    # (A decode step is many small calls, each a few microseconds on the GPU: what is checked here is
+    # asked of each tensor once, in the cheapest form.)
     @staticmethod
-    def _held(name, t, need, dtype, like=None):
-        """Address of a packed device tensor that holds `need` elements of `dtype` (None: NULL)."""
-        if t is None:
-            return None
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a device tensor")
-        if like is not None and t.device != like.device:
-            raise ValueError(f"{name} is on {t.device}, the other operands on {like.device}")
+    def _held(name, t, need, dtype, device):
+        """Address of a packed tensor on `device` that holds `need` elements of `dtype`."""
+        if t.get_device() != device:
+            raise ValueError(f"{name} must be a device tensor" if not t.is_cuda else
+                             f"{name} is on device {t.get_device()}, the other operands on {device}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be densely packed")
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
         if t.numel() < need:
             raise ValueError(f"{name} holds {t.numel()} elements, the problem needs {need}")
         return t.data_ptr()
 
     @staticmethod
-    def _sizes(**sizes):
-        for name, v in sizes.items():
-            if v < 0 or v > 0x7FFFFFFF:
-                raise ValueError(f"{name} = {v} does not fit in 31 bits")
+    def _stream_on(stream, device):
+        """Handle of `stream`, or of torch's current one on `device` (whose stream object takes 3 us
+        to make, a third of a small call)."""
+        if stream is None:
+            import torch
 
-    def _groups(self, offsets, M, like):
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            return raw(device) if raw is not None else int(torch.cuda.current_stream(device).cuda_stream)
+        return Loader._stream_handle(stream)
+
+    @staticmethod
+    def _device_of(name, t):
+        device = t.get_device()
+        if device < 0:
+            raise ValueError(f"{name} must be a device tensor")
+        return device
+
+    @staticmethod
+    def _sizes(*sizes):
+        for v in sizes:
+            if v < 0 or v > 0x7FFFFFFF:
+                raise ValueError(f"a size of {v} does not fit in 31 bits")
+
+    def _groups(self, offsets, device):
         import torch
 
         if offsets.dim() != 1 or offsets.numel() < 1:
@@ -366,54 +388,59 @@ class Loader:
         groups = offsets.numel() - 1
         if groups > MAX_GROUPS:
             raise ValueError(f"{groups} groups: at most {MAX_GROUPS} in one call")
-        return self._held("offsets", offsets, groups + 1, torch.int32, like), groups
+        return self._held("offsets", offsets, groups + 1, torch.int32, device), groups
 
-    def _forward(self, name, C, A, B, offsets, M, N, K, layout_b, bias, residual, preact, act, stream):
-        self._sizes(M=M, N=N, K=K)
-        slot = _type_slot(C.dtype, A.dtype)
-        act, layout_b = activation(act), m_layout(layout_b)
+    def _forward(self, fn, name, C, A, B, offsets, M, N, K, layout_b, bias, residual, preact, act, stream):
+        self._sizes(M, N, K)
+        out, ab = C.dtype, A.dtype
+        slot = _type_slot(out, ab)
+        act = act if type(act) is activation else activation(act)
+        layout_b = layout_b if type(layout_b) is m_layout else m_layout(layout_b)
+        held, device = self._held, self._device_of("C", C)
         groups, where = 1, ()
         if offsets is not None:
-            address, groups = self._groups(offsets, M, C)
-            where = (address, groups)
-        c = self._held("C", C, M * N, C.dtype)
-        a = self._held("A", A, M * K, A.dtype, C)
-        b = self._held("B", B, groups * K * N, A.dtype, C)
-        e = _EpilogueC(self._held("bias", bias, groups * N, A.dtype, C),
-                       self._held("residual", residual, M * N, C.dtype, C),
-                       self._held("preact", preact, M * N, A.dtype, C), int(act))
-        handle = ctypes.c_void_p(self._stream_handle(stream))
-        fn = getattr(self._lib, "rocm_wmma_gemm_" + name)
-        self._done(name, fn(slot, c, a, b, *where, M, N, K, int(layout_b), ctypes.byref(e), ctypes.byref(handle)))
+            where = self._groups(offsets, device)
+            groups = where[1]
+        e = _EpilogueC(None if bias is None else held("bias", bias, groups * N, ab, device),
+                       None if residual is None else held("residual", residual, M * N, out, device),
+                       None if preact is None else held("preact", preact, M * N, ab, device), act)
+        status = fn(slot, held("C", C, M * N, out, device), held("A", A, M * K, ab, device),
+                    held("B", B, groups * K * N, ab, device), *where, M, N, K, layout_b, ctypes.byref(e),
+                    ctypes.byref(ctypes.c_void_p(self._stream_on(stream, device))))
+        if status != OK:
+            self._done(name, status)
 
-    def _backward(self, name, dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, act, accumulate, stream):
-        self._sizes(M=M, N=N, K=K)
+    def _backward(self, fn, name, dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, act, accumulate, stream):
+        self._sizes(M, N, K)
         wanted = [t for t in (dA, dB, dbias) if t is not None]
         if not wanted:
             raise ValueError("none of dA, dB and dbias is wanted")
-        if any(t.dtype != wanted[0].dtype for t in wanted):
+        out, ab = wanted[0].dtype, dC.dtype
+        if any(t.dtype is not out for t in wanted):
             raise TypeError("dA, dB and dbias must share an element type")
-        slot = _type_slot(wanted[0].dtype, dC.dtype)
-        act, layout_b = activation(act), m_layout(layout_b)
-        if act != activation.none and preact is None:
-            raise ValueError(f"the gradient of {act.name} needs preact")
-        if act == activation.none:
+        slot = _type_slot(out, ab)
+        act = act if type(act) is activation else activation(act)
+        layout_b = layout_b if type(layout_b) is m_layout else m_layout(layout_b)
+        if act is activation.none:
             preact = None
+        elif preact is None:
+            raise ValueError(f"the gradient of {act.name} needs preact")
         if dB is not None and A is None or dA is not None and B is None:
             raise ValueError("dA needs B, and dB needs A")
+        held, device = self._held, self._device_of("dC", dC)
         groups, where = 1, ()
         if offsets is not None:
-            address, groups = self._groups(offsets, M, dC)
-            where = (address, groups)
-        out = wanted[0].dtype
-        args = (self._held("dA", dA, M * K, out, dC), self._held("dB", dB, groups * K * N, out, dC),
-                self._held("dbias", dbias, groups * N, out, dC), self._held("dC", dC, M * N, dC.dtype),
-                self._held("A", A, M * K, dC.dtype, dC), self._held("B", B, groups * K * N, dC.dtype, dC),
-                self._held("preact", preact, M * N, dC.dtype, dC))
-        handle = ctypes.c_void_p(self._stream_handle(stream))
-        fn = getattr(self._lib, "rocm_wmma_gemm_" + name)
-        self._done(name, fn(slot, *args, *where, M, N, K, int(layout_b), int(act), int(bool(accumulate)),
-                            ctypes.byref(handle)))
+            where = self._groups(offsets, device)
+            groups = where[1]
+        args = [None if t is None else held(what, t, need, dtype, device)
+                for what, t, need, dtype in (("dA", dA, M * K, out), ("dB", dB, groups * K * N, out),
+                                             ("dbias", dbias, groups * N, out), ("dC", dC, M * N, ab),
+                                             ("A", A, M * K, ab), ("B", B, groups * K * N, ab),
+                                             ("preact", preact, M * N, ab))]
+        status = fn(slot, *args, *where, M, N, K, layout_b, act, 1 if accumulate else 0,
+                    ctypes.byref(ctypes.c_void_p(self._stream_on(stream, device))))
+        if status != OK:
+            self._done(name, status)
 
     def linear(self, C, A, B, M: int, N: int, K: int, layout_b=col_major, bias=None, residual=None, preact=None,
                activation=activation.none, stream=None) -> None:
@@ -422,14 +449,14 @@ class Loader:
         A (M x K) and C (M x N) are row-major; B (K x N) is column-major (weights stored N x K)
         or row-major.  bias: N values of A's type; residual: M x N of C's type, may be C itself;
         preact: M x N of A's type, receives A B + bias for the backward pass."""
-        self._forward("linear", C, A, B, None, M, N, K, layout_b, bias, residual, preact, activation, stream)
+        self._forward(self._lib.rocm_wmma_gemm_linear, "linear", C, A, B, None, M, N, K, layout_b, bias, residual, preact, activation, stream)
 
     def linear_backward(self, dA, dB, dbias, dC, A, B, M: int, N: int, K: int, layout_b=col_major, preact=None,
                         activation=activation.none, accumulate: bool = False, stream=None) -> None:
         """The gradients of linear() from dC (M x N, A's type): dA = dZ B^T, dB = A^T dZ in B's
         layout and dbias = the sum of dZ's rows, with dZ = dC activation'(preact).  A result that
         is None is not computed.  accumulate: dB and dbias are added to."""
-        self._backward("linear_backward", dA, dB, dbias, dC, A, B, None, M, N, K, layout_b, preact, activation,
+        self._backward(self._lib.rocm_wmma_gemm_linear_backward, "linear_backward", dA, dB, dbias, dC, A, B, None, M, N, K, layout_b, preact, activation,
                        accumulate, stream)
 
     def grouped(self, C, A, B, offsets, M: int, N: int, K: int, layout_b=col_major, bias=None, residual=None,
@@ -438,12 +465,12 @@ class Loader:
         offsets[e+1] - 1 of A and C belong to weight e of B (groups x K x N).  offsets: groups + 1
         int32 on the device; they are read there, never by the host.  Rows outside the groups are
         not touched."""
-        self._forward("grouped", C, A, B, offsets, M, N, K, layout_b, bias, residual, preact, activation, stream)
+        self._forward(self._lib.rocm_wmma_gemm_grouped, "grouped", C, A, B, offsets, M, N, K, layout_b, bias, residual, preact, activation, stream)
 
     def grouped_backward(self, dA, dB, dbias, dC, A, B, offsets, M: int, N: int, K: int, layout_b=col_major,
                          preact=None, activation=activation.none, accumulate: bool = False, stream=None) -> None:
         """The gradients of grouped(); an empty group's are zero (unchanged with accumulate)."""
-        self._backward("grouped_backward", dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, activation,
+        self._backward(self._lib.rocm_wmma_gemm_grouped_backward, "grouped_backward", dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, activation,
                        accumulate, stream)
 
     def orthogonalize(self, O, G, M: int, N: int, batch_count: int = 1, steps: int = 5,
@@ -453,15 +480,16 @@ class Loader:
         values near 1.  G: f16, bf16 or f32; O: f16 or bf16."""
         import torch
 
-        self._sizes(M=M, N=N, batch_count=batch_count)
+        self._sizes(M, N, batch_count)
         codes = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
         if G.dtype not in codes or codes.get(O.dtype, 2) == 2:
             raise TypeError(f"Unsupported type pair for orthogonalize: O={O.dtype}, G={G.dtype}")
         if steps < 1 or len(coefficients) != 3:
             raise ValueError("at least one step, and three coefficients")
-        o = self._held("O", O, batch_count * M * N, O.dtype)
-        g = self._held("G", G, batch_count * M * N, G.dtype, O)
-        handle = ctypes.c_void_p(self._stream_handle(stream))
+        device = self._device_of("O", O)
+        o = self._held("O", O, batch_count * M * N, O.dtype, device)
+        g = self._held("G", G, batch_count * M * N, G.dtype, device)
+        handle = ctypes.c_void_p(self._stream_on(stream, device))
         self._done("orthogonalize", self._lib.rocm_wmma_gemm_orthogonalize(
             codes[G.dtype], codes[O.dtype], o, g, M, N, batch_count, steps, (ctypes.c_float * 3)(*coefficients),
             epsilon, ctypes.byref(handle)))

@@ -4,8 +4,9 @@
 
 using namespace rocm_wmma_gemm;
 
-#define CHECKED(IN, OUT, RES, AK, BK, EDGE, EPI) \
-    template __global__ void device::tiled_product_entry<device::tiled_product<device::in_kind::IN, OUT, RES, AK, BK, EDGE, EDGE, device::EPI>>(device::product_args);
+#define SHAPED(IN, OUT, RES, AK, BK, BM, BN, EPI) \
+    template __global__ void device::tiled_product_entry<device::tiled_product<device::in_kind::IN, OUT, RES, AK, BK, BM, BN, device::EPI>>(device::product_args);
+#define CHECKED(IN, OUT, RES, AK, BK, EDGE, EPI) SHAPED(IN, OUT, RES, AK, BK, EDGE, EDGE, EPI)
 
 CHECKED(bf16, __bf16, __bf16, true, true, 256, epilogue_plain)
 CHECKED(bf16, __bf16, __bf16, true, true, 256, epilogue_logistic)
@@ -20,3 +21,5 @@ CHECKED(f16, _Float16, _Float16, true, true, 128, epilogue_poly)
 CHECKED(f16, float, float, true, false, 256, epilogue_next_rows)
 CHECKED(f16, float, float, true, true, 128, epilogue_next_cols)
 CHECKED(f16, __bf16, float, true, true, 256, epilogue_last_cols)
+SHAPED(bf16, __bf16, __bf16, true, true, 128, 256, epilogue_logistic)
+CHECKED(f16, _Float16, _Float16, true, true, 192, epilogue_poly)

@@ -10,7 +10,7 @@ import pytest
 import rocm_wmma_gemm_amd as R
 from test_host import ROOT, _mfma_loops
 
-INSTANTIATED = 13
+INSTANTIATED = 15
 
 
 def test_tiled_products_keep_accumulators_in_place(tmp_path):
@@ -34,7 +34,7 @@ def test_tiled_products_keep_accumulators_in_place(tmp_path):
     for func, body in loops.items():
         whole = text[text.index(func + ":"):]
         whole = whole[:whole.index(".Lfunc_end")]
-        expected = 32 if "Li128ELi128E" in func else 128  # two K steps of (edge / 32)^2 MFMAs
+        expected = 32 if "Li128ELi128E" in func else 64 if "Li128ELi256E" in func else 72 if "Li192E" in func else 128
         assert sum("v_mfma_f32_16x16x32" in b for b in body) == whole.count("v_mfma_f32_16x16x32") == expected, func
         bad = [b for b in body if re.search(r"v_accvgpr_|scratch_", b)]
         assert not bad, f"{func}: accumulator traffic or spills inside the MFMA loop: {bad[:3]}"
