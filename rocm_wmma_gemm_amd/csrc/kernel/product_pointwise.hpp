@@ -19,6 +19,7 @@ struct slope_args
     const void* dc; // rows x cols of 16-bit elements
     const void* z; // the same, or nullptr: dZ = dC
     void*       dz; // nullptr: not wanted (dZ = dC)
+    int         dz_pitch; // its row length, a multiple of 8: columns past cols are written as zeros
     float*      sums; // nullptr, or [run][cols]
     const int*  offsets; // groups + 1, or nullptr: one group
     int         groups, rows, cols;
@@ -51,6 +52,13 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
     {
         sum[v] = 0.0f;
     }
+    if(args.dz != nullptr && col >= args.cols && col < args.dz_pitch)
+    {
+        for(int row = row0 + wave; row < row1; row += 4)
+        {
+            static_cast<InT*>(args.dz)[(long long)row * args.dz_pitch + col] = to_out<InT>(0.0f);
+        }
+    }
     if(col < args.cols)
     {
 #pragma unroll 8
@@ -81,7 +89,7 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
             }
             if(args.dz != nullptr)
             {
-                *reinterpret_cast<in_t*>(static_cast<InT*>(args.dz) + at) = o;
+                *reinterpret_cast<in_t*>(static_cast<InT*>(args.dz) + (long long)row * args.dz_pitch + col) = o;
             }
         }
     }

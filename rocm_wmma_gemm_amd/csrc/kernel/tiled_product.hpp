@@ -50,7 +50,9 @@ using epilogue_next_cols = product_epilogue<false, false, true, true, true, fals
 using epilogue_last_rows = product_epilogue<false, false, true, false, true, false, diagonal_use::rows>;
 using epilogue_last_cols = product_epilogue<false, false, true, false, true, false, diagonal_use::cols>;
 
-template<in_kind IN, class OutT, class ResT, bool A_KMAJOR, bool B_KMAJOR, int BM, int BN, class EPI>
+// NARROW: rows of C, the residual, the second output or the bias do not start on 16 bytes: they go
+// element by element, a lane a column, so that a store instruction still writes runs of a row.
+template<in_kind IN, class OutT, class ResT, bool A_KMAJOR, bool B_KMAJOR, int BM, int BN, class EPI, bool NARROW = false>
 struct tiled_product
 {
     using loop = solo_gemm<IN, OutT, A_KMAJOR, B_KMAJOR, BM, BN, 64, 2, 2, 2, true>;
@@ -228,20 +230,41 @@ struct tiled_product
     struct piece
     {
         static constexpr int QUADS = PIECE * (int)sizeof(T) / 16;
-        static constexpr bool HALF_QUAD = QUADS == 0; // 8 bytes
-        u32x4 raw[QUADS > 0 ? QUADS : 1];
+        static_assert(PIECE == 1 || QUADS > 0, "one element, or 16 bytes at least");
+        typename std::conditional<PIECE == 1, unsigned int, u32x4>::type raw[QUADS > 0 ? QUADS : 1];
         __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t from, unsigned int at, unsigned int wave_at)
         {
-            static_assert(!HALF_QUAD, "16 bytes at least");
-#pragma unroll
-            for(int q = 0; q < QUADS; ++q)
+            if constexpr(PIECE == 1 && sizeof(T) == 2)
             {
-                raw[q] = __builtin_amdgcn_raw_buffer_load_b128(from, at + 16 * q, wave_at, 0);
+                raw[0] = __builtin_amdgcn_raw_buffer_load_b16(from, at, wave_at, 0);
+            }
+            else if constexpr(PIECE == 1)
+            {
+                raw[0] = __builtin_amdgcn_raw_buffer_load_b32(from, at, wave_at, 0);
+            }
+            else
+            {
+#pragma unroll
+                for(int q = 0; q < QUADS; ++q)
+                {
+                    raw[q] = __builtin_amdgcn_raw_buffer_load_b128(from, at + 16 * q, wave_at, 0);
+                }
             }
         }
         __device__ __forceinline__ float get(int e) const
         {
-            if constexpr(sizeof(T) == 4)
+            if constexpr(PIECE == 1)
+            {
+                if constexpr(sizeof(T) == 4)
+                {
+                    return __builtin_bit_cast(float, raw[0]);
+                }
+                else
+                {
+                    return (float)__builtin_bit_cast(T, (unsigned short)raw[0]);
+                }
+            }
+            else if constexpr(sizeof(T) == 4)
             {
                 // (a bit cast of a vector's element itself gives element 0: it goes through a variable)
                 const unsigned int bits = raw[e / 4][e % 4];
@@ -261,7 +284,15 @@ struct tiled_product
     {
         // (a layer's C is not read again here; what a Newton-Schulz step leaves the next one reads)
         constexpr int NT = EPI::scaled ? 0 : 2;
-        if constexpr(sizeof(T) == 4)
+        if constexpr(PIECE == 1 && sizeof(T) == 4)
+        {
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, y[0]), to, at, wave_at, NT);
+        }
+        else if constexpr(PIECE == 1)
+        {
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, to_out<T>(y[0])), to, at, wave_at, NT);
+        }
+        else if constexpr(sizeof(T) == 4)
         {
             static_assert(PIECE == 4, "one 16-byte piece");
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{y[0], y[1], y[2], y[3]}), to, at,
@@ -294,7 +325,7 @@ struct tiled_product
     __device__ __forceinline__ static void write(const product_args& args, const work& w, f32x4 (&acc)[TM][TN],
                                                  int row_w, int col_w, int lane, lds_char_ptr strip)
     {
-        constexpr int PIECE = 16 / (int)sizeof(OutT); // columns of a piece
+        constexpr int PIECE = NARROW ? 1 : 16 / (int)sizeof(OutT); // columns of a piece
         constexpr int PR    = HALF * 16 / PIECE; // pieces of a strip row
         constexpr int READS = (16 * PR + 63) / 64;
         constexpr bool UNEVEN = 16 * PR % 64 != 0; // the last read has lanes to spare
@@ -357,10 +388,14 @@ struct tiled_product
                 const int col = col_w + p * HALF * 16 + piece_col[q];
                 if constexpr(EPI::layer)
                 {
-                    // (8 columns of 16 bits, also where a piece has 4: the piece's 8 bytes start at a multiple of 8)
                     typedef unsigned int u2 __attribute__((ext_vector_type(2)));
                     constexpr int        PAIRS = PIECE / 4;
                     const unsigned int   from_at = col < cols ? (unsigned int)col * 2 : loop::STORE_RANGE;
+                    if constexpr(NARROW)
+                    {
+                        const unsigned short b = __builtin_amdgcn_raw_buffer_load_b16(bias_from, from_at, 0, 0);
+                        bias[p][q][0]          = (float)__builtin_bit_cast(InT, b);
+                    }
 #pragma unroll
                     for(int h = 0; h < PAIRS; ++h)
                     {
@@ -392,7 +427,7 @@ struct tiled_product
         }
         // residual pieces (and, by rows, what they are multiplied by) of AHEAD blocks are on their way
         constexpr int WANT = sizeof(OutT) == 4 || sizeof(ResT) == 4 || PER_CU > 1 || EPI::mirror ? 2 : 4;
-        constexpr int AHEAD = BLOCKS < WANT ? BLOCKS : WANT;
+        constexpr int AHEAD = NARROW ? 1 : BLOCKS < WANT ? BLOCKS : WANT;
         piece<ResT, PIECE> residual[EPI::residual ? AHEAD : 1][PASSES][READS];
         float              by_row[EPI::diagonal == diagonal_use::rows ? AHEAD : 1][READS];
         auto fetch = [&](int block) {
@@ -461,6 +496,11 @@ struct tiled_product
                 for(int q = 0; q < READS; ++q)
                 {
                     float z[PIECE], y[PIECE];
+                    if constexpr(NARROW)
+                    {
+                        const float v = *reinterpret_cast<const lds_float*>(strip + strip_at[q]);
+                        z[0]          = EPI::scaled ? args.alpha * v : v;
+                    }
 #pragma unroll
                     for(int h = 0; h < PIECE / 4; ++h)
                     {
@@ -610,7 +650,21 @@ struct tiled_product
                 hi += *reinterpret_cast<const f32x4*>(from + (long long)s * (BM * BN) + 4);
             }
             const float sum[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            finish_piece<InT, OutT, ResT>(args, x, row, col, sum);
+            if constexpr(NARROW)
+            {
+#pragma unroll
+                for(int e = 0; e < 8; ++e)
+                {
+                    if(col + e < args.N)
+                    {
+                        finish_element<InT, OutT, ResT>(args, x, row, col + e, sum[e]);
+                    }
+                }
+            }
+            else
+            {
+                finish_piece<InT, OutT, ResT>(args, x, row, col, sum);
+            }
         }
     }
 

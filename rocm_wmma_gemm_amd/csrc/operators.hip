@@ -119,15 +119,65 @@ int with_status(Body&& body)
     }
 }
 
-// Whether the kernels that load 16 bytes at a time, straight to LDS, can take the operands: every row,
-// and every group's first, starts on 16 bytes, and a tile's span fits the 31 bits of their offsets.
-bool aligned_rows(const product_args& a, int layout)
+// Which operands have rows (and groups) that all start on 16 bytes, as the kernels need them that
+// load 16 bytes at a time, straight to LDS, or store pieces of 16.
+struct starts_on_16
 {
-    const bool k_contiguous = layout != layout_mn;
-    return a.lda % 8 == 0 && a.ldb % 8 == 0 && a.ldc % 8 == 0 && a.N % 8 == 0 && (k_contiguous ? a.K % 8 == 0 : a.M % 8 == 0)
-           && a.stride_a % 8 == 0 && a.stride_b % 8 == 0 && a.stride_c % 8 == 0 && aligned16(a.A) && aligned16(a.B)
-           && aligned16(a.C) && aligned16(a.kept) && aligned16(a.residual) && aligned16(a.bias) && a.K > 0
-           && std::max({a.lda, a.ldb, a.ldc}) < (1 << 21);
+    bool a, b, c;
+};
+
+starts_on_16 alignment_of(const product_args& x)
+{
+    return {x.lda % 8 == 0 && x.stride_a % 8 == 0 && aligned16(x.A), x.ldb % 8 == 0 && x.stride_b % 8 == 0 && aligned16(x.B),
+            x.ldc % 8 == 0 && x.N % 8 == 0 && x.stride_c % 8 == 0 && aligned16(x.C) && aligned16(x.kept)
+                && aligned16(x.residual) && aligned16(x.bias)};
+}
+
+// An operand as a matrix of contiguous rows, groups one after the other.
+struct matrix_of_rows
+{
+    size_t rows, length;
+    size_t padded() const
+    {
+        return round_up8(length);
+    }
+    size_t bytes() const
+    {
+        return whole_lines(rows * padded() * 2);
+    }
+};
+
+matrix_of_rows rows_of_a(const product_args& x, int layout)
+{
+    // (rows and sum: A's rows are those of all groups)
+    return layout == layout_mn ? matrix_of_rows{size_t(x.K), size_t(x.M)} : matrix_of_rows{size_t(x.M), size_t(x.K)};
+}
+
+matrix_of_rows rows_of_b(const product_args& x, int layout)
+{
+    const size_t groups = x.kind == product_kind::rows ? x.groups : 1;
+    return layout == layout_kk ? matrix_of_rows{groups * x.N, size_t(x.K)} : matrix_of_rows{groups * x.K, size_t(x.N)};
+}
+
+// The product on copies whose rows are padded with zeros to multiples of 8.  (Where K is no multiple
+// of 8 both K-contiguous operands are such copies, or dZ, which is written that way, so that the
+// columns past K add zeros.)
+product_args on_copies(product_args x, int layout, bool copy_a, bool copy_b, char* at)
+{
+    if(copy_a)
+    {
+        x.lda = static_cast<long long>(rows_of_a(x, layout).padded());
+        x.A   = at;
+        at += at != nullptr ? rows_of_a(x, layout).bytes() : 0;
+    }
+    if(copy_b)
+    {
+        const matrix_of_rows m = rows_of_b(x, layout);
+        x.ldb                  = static_cast<long long>(m.padded());
+        x.stride_b             = static_cast<long long>(m.rows / (x.kind == product_kind::rows ? x.groups : 1) * m.padded());
+        x.B                    = at;
+    }
+    return x;
 }
 
 // A product's kernel, and how the tiles that would leave compute units idle are cut along K.
@@ -139,6 +189,13 @@ struct launch_choice
     size_t         partial_bytes = 0; // room that cutting needs; 0: nothing is cut
     int            k_slices = 1; // workgroups that share a tile of the few-row kernel
     bool           once = false; // B's loads carry the non-temporal hint
+    bool           copy_a = false, copy_b = false; // work on padded copies
+    size_t         copy_bytes = 0; // room for them
+    int            layout = 0;
+    size_t         scratch() const
+    {
+        return copy_bytes + partial_bytes;
+    }
 };
 
 // Tiles of a product: at most (`most`), and about (rows of several groups end inside a tile, half
@@ -175,6 +232,12 @@ constexpr form_cost tiled_costs[] = {
     {form_tiled_128, 4.5f, 0.64f, 1.0f, 2.9e6f},
     {form_tiled_192, 8.0f, 0.70f, 0.90f, 2.9e6f},
 };
+constexpr form_cost narrow_cost = {form_narrow_128, 6.0f, 0.64f, 1.0f, 2.9e6f};
+// The general kernel, by layout: FLOP per us where there is enough to do (it gathers operands that are contiguous
+// along M or N two bytes at a time), and us per 64 of K of a tile on its own.
+constexpr float general_flops[num_product_layouts] = {2.0e8f, 8.5e7f, 6.5e7f};
+constexpr float general_k64 = 1.5f;
+constexpr float copy_bytes_per_us = 4.2e6f; // read and written by the copies
 // (both operands K-contiguous)
 constexpr form_cost skinny_costs_kk[] = {
     {form_skinny_16x32, 3.5f, 0.09f, 0.20f, 5.2e6f},  {form_skinny_32x16, 3.5f, 0.085f, 0.20f, 5.2e6f},
@@ -203,11 +266,22 @@ float round_us(const form_cost& f, size_t tiles, size_t cus, int per_cu, float k
 }
 
 // Which kernel a product runs on: the least estimated time of the forms that can take it.
-launch_choice choose(int types, int layout, int finish, const product_args& args, size_t cus)
+launch_choice choose(int types, int layout, int finish, const product_args& given, size_t cus)
 {
-    const bool symmetric = finish == finish_square || finish == finish_poly;
-    auto       made = [&](int form) {
+    const bool         symmetric = finish == finish_square || finish == finish_poly;
+    const starts_on_16 aligned   = alignment_of(given);
+    const bool         copy_a = !aligned.a, copy_b = !aligned.b;
+    const product_args args = on_copies(given, layout, copy_a, copy_b, nullptr);
+    const matrix_of_rows am = rows_of_a(given, layout), bm = rows_of_b(given, layout);
+    auto                 made = [&](int form) {
         launch_choice c;
+        c.layout = layout;
+        if(form != form_general_64 && form != form_general_128)
+        {
+            c.copy_a     = copy_a;
+            c.copy_b     = copy_b;
+            c.copy_bytes = (copy_a ? am.bytes() : 0) + (copy_b ? bm.bytes() : 0);
+        }
         c.kernel = find_product(types, layout, form, finish);
         if(c.kernel.fn != nullptr)
         {
@@ -234,9 +308,11 @@ launch_choice choose(int types, int layout, int finish, const product_args& args
         }
         return c;
     };
-    if(!aligned_rows(args, layout))
+    const int general = tiles_of(args, 128, 128, false, true) < cus ? form_general_64 : form_general_128;
+    if(args.K == 0 || std::max({args.lda, args.ldb, args.ldc}) >= (1 << 21))
     {
-        return made(tiles_of(args, 128, 128, false, true) < cus ? form_general_64 : form_general_128);
+        // (no K tile to load; or a tile's span beyond the 31 bits of the other kernels' offsets)
+        return made(general);
     }
     launch_choice best;
     float         least = 1e30f;
@@ -253,25 +329,43 @@ launch_choice choose(int types, int layout, int finish, const product_args& args
     const size_t used   = rows_kind ? std::min<size_t>(args.groups, args.M) : args.groups;
     const float  weight = rows_kind ? float(used) * args.N * args.K * 2 : 0.0f;
     const float k64     = std::max(1.0f, (several ? float(args.K) / args.groups : float(args.K)) / 64.0f);
-    for(const form_cost& f : tiled_costs)
+    const float copies = copy_a || copy_b ? 3.0f + 2.0f * ((copy_a ? am.bytes() : 0) + (copy_b ? bm.bytes() : 0)) / copy_bytes_per_us
+                                          : 0.0f;
+    if(copy_a || copy_b)
     {
+        // (the copies pay against a large product only: a few rows read a weight as it is)
+        const float flops = 2.0f * tiles_of(args, 64, 64, false, false) * 4096 * k64 * 64;
+        offer(made(general), 5.0f + std::max(flops / general_flops[layout], k64 * general_k64));
+    }
+    auto consider_tiled = [&](const form_cost& f) {
         const launch_choice c = made(f.form);
         if(c.kernel.fn == nullptr)
         {
-            continue;
+            return;
         }
         const size_t tiles = tiles_of(args, c.kernel.block_m, c.kernel.block_n, symmetric, false);
         const size_t slots = c.kernel.per_cu * cus, rounds = tiles / slots, rest = tiles % slots;
         const float  whole = rounds * round_us(f, slots, cus, c.kernel.per_cu, k64), least_us = weight / f.stream;
-        offer(c, std::max(least_us, whole + (rest ? round_us(f, rest, cus, c.kernel.per_cu, k64) : 0.0f)));
+        offer(c, copies + std::max(least_us, whole + (rest ? round_us(f, rest, cus, c.kernel.per_cu, k64) : 0.0f)));
         const device::tail_cut cut = device::cut_tail(static_cast<int>(tiles), static_cast<int>(slots),
                                                       static_cast<int>(std::ceil(k64)), !several && c.kernel.finish != nullptr);
         if(cut.cut != 0)
         {
             const size_t parts = size_t(cut.cut) * cut.slices;
-            offer(with_cut(c), std::max(least_us, whole + round_us(f, parts, cus, c.kernel.per_cu, float(cut.each))) + join_us
+            offer(with_cut(c), copies + std::max(least_us, whole + round_us(f, parts, cus, c.kernel.per_cu, float(cut.each))) + join_us
                                    + 2.0f * parts * 4 * c.kernel.block_m * c.kernel.block_n / bytes_per_us);
         }
+    };
+    if(aligned.c)
+    {
+        for(const form_cost& f : tiled_costs)
+        {
+            consider_tiled(f);
+        }
+    }
+    else
+    {
+        consider_tiled(narrow_cost);
     }
     // (the few-row kernel's offsets within a weight that is contiguous along N have 31 bits)
     if(rows_kind && (layout == layout_kk || static_cast<long long>(args.K) * args.ldb < (1ll << 30)))
@@ -300,7 +394,7 @@ launch_choice choose(int types, int layout, int finish, const product_args& args
                 float us = rounds * round_us(f, slots, cus, per_cu, k) + (rest ? round_us(f, rest, cus, per_cu, k) : 0.0f);
                 // (row tiles that share a weight do not all find it in L2)
                 us = std::max(us, weight / (one_high ? f.stream : 0.65f * f.stream));
-                offer(s, us + (s.k_slices > 1 ? join_us : 0.0f));
+                offer(s, copies + us + (s.k_slices > 1 ? join_us : 0.0f));
             }
         };
         if(layout == layout_kk)
@@ -321,22 +415,46 @@ launch_choice choose(int types, int layout, int finish, const product_args& args
     return best;
 }
 
-// One product on the kernel chosen for it.  partials: the room that the choice asked for, or nullptr:
-// nothing is cut then.
-int launch_product(const launch_choice& c, product_args args, void* partials, hipStream_t stream)
+// One product on the kernel chosen for it.  scratch: the room that the choice asked for.  Without it (a
+// capture forbids to allocate) nothing is cut, and the general kernel stands in for one that needs copies.
+int launch_product(int types, int finish, launch_choice c, product_args args, char* scratch, hipStream_t stream)
 {
     if(args.N == 0 || args.M == 0 || args.groups == 0)
     {
         return ROCM_WMMA_GEMM_OK;
     }
+    if(c.copy_bytes != 0 && scratch == nullptr)
+    {
+        c.kernel     = find_product(types, c.layout, form_general_128, finish);
+        c.copy_bytes = 0;
+        c.copy_a = c.copy_b = c.once = false;
+        c.items      = tiles_of(args, 128, 128, false, true);
+        c.workgroups = std::min(c.items, c.kernel.per_cu * std::max<size_t>(compute_units_of_current_device(), 1));
+    }
     if(c.kernel.fn == nullptr || c.items > most_extent)
     {
         return ROCM_WMMA_GEMM_ERR_LIMIT;
     }
-    const bool cuts = c.partial_bytes != 0 && partials != nullptr;
+    if(c.copy_bytes != 0)
+    {
+        const product_args on = on_copies(args, c.layout, c.copy_a, c.copy_b, scratch);
+        auto job = [](const matrix_of_rows& m, const void* from, const void* to) {
+            return device::pack_job{from, const_cast<void*>(to), static_cast<int>(m.rows), static_cast<int>(m.length),
+                                    static_cast<int>(m.rows), static_cast<int>(m.padded()), 0, 0};
+        };
+        const matrix_of_rows   am = rows_of_a(args, c.layout), bm = rows_of_b(args, c.layout);
+        const device::pack_job ja = job(am, args.A, on.A), jb = job(bm, args.B, on.B);
+        const size_t pieces = std::max(c.copy_a ? am.rows * am.padded() / 8 : 0, c.copy_b ? bm.rows * bm.padded() / 8 : 0);
+        enqueue(&device::pack_padded<unsigned short>,
+                dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(pieces, 256), 8192)), c.copy_a && c.copy_b ? 2 : 1),
+                dim3(256), stream, c.copy_a ? ja : jb, c.copy_b ? jb : ja);
+        args = on;
+        scratch += c.copy_bytes;
+    }
+    const bool cuts = c.partial_bytes != 0 && scratch != nullptr;
     args.grid_m     = static_cast<int>(ceil_div(args.M, c.kernel.block_m));
     args.grid_n     = static_cast<int>(ceil_div(args.N, c.kernel.block_n));
-    args.partials   = cuts ? static_cast<float*>(partials) : nullptr;
+    args.partials   = cuts ? reinterpret_cast<float*>(scratch) : nullptr;
     args.workgroups = static_cast<int>(c.workgroups);
     args.k_slices   = 1;
     if(cuts && c.k_slices > 1)
@@ -432,8 +550,8 @@ int forward(const layer& p, void* C, const void* A, const void* B, const rocm_wm
                                                                                           : finish_plain;
     const launch_choice c = choose(p.type_idx, p.layout_b == 1 ? layout_kk : layout_kn, finish, a, compute_units());
     workspace_lease     lease;
-    void* partials = c.partial_bytes != 0 ? lease.acquire(c.partial_bytes, stream) : nullptr; // (without: whole tiles)
-    return launch_product(c, a, partials, stream);
+    char*               scratch = c.scratch() != 0 ? lease.acquire(c.scratch(), stream) : nullptr;
+    return launch_product(p.type_idx, finish, c, a, scratch, stream);
 }
 
 template<class InT>
@@ -472,9 +590,12 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     launch_choice      on_a, on_b;
     device::slope_args s{};
     // dZ and the sums of its columns live in the scratch buffer, and what the products ask for
-    const bool   passes = (sloped || dbias != nullptr) && p.N != 0;
+    // (a dC whose rows do not start on 16 bytes is copied to rows that do, as dZ is written)
+    const bool   pitched = sloped || p.N % 8 != 0 || !aligned16(dC);
+    const bool   passes  = (pitched || dbias != nullptr) && p.N != 0;
+    const size_t pitch   = pitched ? round_up8(p.N) : p.N;
     const size_t runs   = p.M / device::slope_rows + std::min(p.groups, p.M);
-    const size_t dz_bytes = passes && sloped ? whole_lines(p.M * p.N * 2) : 0;
+    const size_t dz_bytes = passes && pitched ? whole_lines(p.M * pitch * 2) : 0;
     const size_t sums     = passes && dbias != nullptr ? whole_lines(runs * p.N * sizeof(float)) : 0;
     if(runs > most_extent || ceil_div(p.N, 64) > 65535)
     {
@@ -493,7 +614,7 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
         to_a.M        = static_cast<int>(p.M);
         to_a.N        = static_cast<int>(p.K);
         to_a.K        = static_cast<int>(p.N);
-        to_a.lda      = p.N;
+        to_a.lda      = pitch;
         to_a.ldb      = p.layout_b == 1 ? p.K : p.N;
         to_a.ldc      = p.K;
         to_a.stride_b = static_cast<long long>(p.N * p.K);
@@ -509,27 +630,28 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
         to_b.M        = static_cast<int>(nk ? p.N : p.K);
         to_b.N        = static_cast<int>(nk ? p.K : p.N);
         to_b.K        = static_cast<int>(p.M);
-        to_b.lda      = to_b.M;
-        to_b.ldb      = to_b.N;
+        to_b.lda      = nk ? pitch : p.K;
+        to_b.ldb      = nk ? p.K : pitch;
         to_b.ldc      = to_b.N;
         to_b.stride_c = static_cast<long long>(p.N * p.K);
     }
     placed(dz_bytes != 0 ? nullptr : dC);
+    const int a_layout = p.layout_b == 1 ? layout_kn : layout_kk, b_finish = accumulate ? finish_add : finish_plain;
     if(dA != nullptr && p.M != 0 && p.K != 0)
     {
-        on_a = choose(p.type_idx, p.layout_b == 1 ? layout_kn : layout_kk, finish_plain, to_a, cus);
+        on_a = choose(p.type_idx, a_layout, finish_plain, to_a, cus);
     }
     if(dB != nullptr && p.N != 0 && p.K != 0)
     {
-        on_b = choose(p.type_idx, layout_mn, accumulate ? finish_add : finish_plain, to_b, cus);
+        on_b = choose(p.type_idx, layout_mn, b_finish, to_b, cus);
     }
     workspace_lease lease;
-    const size_t    needed = dz_bytes + sums, cuts = std::max(on_a.partial_bytes, on_b.partial_bytes);
+    const size_t    needed = dz_bytes + sums, cuts = std::max(on_a.scratch(), on_b.scratch());
     char*           ws = needed + cuts != 0 ? lease.acquire(needed + cuts, stream) : nullptr;
-    char*           partials = ws != nullptr ? ws + needed : nullptr;
+    char*           scratch = ws != nullptr && cuts != 0 ? ws + needed : nullptr;
     if(ws == nullptr && needed != 0)
     {
-        // (a capture forbids to allocate: perhaps there is room without cut tiles)
+        // (a capture forbids to allocate: perhaps there is room without cut tiles and copies)
         ws = cuts != 0 ? lease.acquire(needed, stream) : nullptr;
         if(ws == nullptr)
         {
@@ -540,7 +662,8 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     {
         s.dc      = dC;
         s.z       = sloped ? preact : nullptr;
-        s.dz      = sloped ? ws : nullptr;
+        s.dz      = pitched ? ws : nullptr;
+        s.dz_pitch = static_cast<int>(pitch);
         s.sums    = dbias != nullptr ? reinterpret_cast<float*>(ws + dz_bytes) : nullptr;
         s.offsets = p.offsets;
         s.groups  = static_cast<int>(p.groups);
@@ -553,7 +676,7 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
             is_bf16(p.type_idx) ? launch_slope<__bf16>(s, runs, wide, stream)
                                 : launch_slope<_Float16>(s, runs, wide, stream);
         }
-        dz = sloped ? ws : dC;
+        dz = pitched ? ws : dC;
         if(dbias != nullptr)
         {
             switch(p.type_idx)
@@ -568,11 +691,11 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     int rc = ROCM_WMMA_GEMM_OK;
     if(on_a.kernel.fn != nullptr)
     {
-        rc = launch_product(on_a, to_a, partials, stream);
+        rc = launch_product(p.type_idx, finish_plain, on_a, to_a, on_a.scratch() != 0 ? scratch : nullptr, stream);
     }
     if(rc == ROCM_WMMA_GEMM_OK && on_b.kernel.fn != nullptr)
     {
-        rc = launch_product(on_b, to_b, partials, stream);
+        rc = launch_product(p.type_idx, b_finish, on_b, to_b, on_b.scratch() != 0 ? scratch : nullptr, stream);
     }
     return rc;
 }
@@ -668,7 +791,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
     const float a = coefficients[0], b = coefficients[1], c = coefficients[2];
     const size_t cus     = compute_units();
     auto         product = [&](int types, int layout, int finish, const product_args& args) {
-        return launch_product(choose(types, layout, finish, args, cus), args, nullptr, stream);
+        return launch_product(types, finish, choose(types, layout, finish, args, cus), args, nullptr, stream);
     };
     product_args p{};
     p.kind   = product_kind::batch;

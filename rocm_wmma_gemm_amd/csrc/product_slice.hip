@@ -29,11 +29,11 @@ product_kernel made(int block_m, int block_n, int per_cu)
     return {&device::product_entry<Impl>, block_m, block_n, Impl::THREADS, nullptr, nullptr, per_cu};
 }
 
-template<int LAYOUT, int BM, int BN, class EPI>
+template<int LAYOUT, int BM, int BN, class EPI, bool NARROW = false>
 product_kernel tiled()
 {
     constexpr bool AK = LAYOUT != layout_mn, BK = LAYOUT == layout_kk;
-    using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, BM, BN, EPI>;
+    using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, BM, BN, EPI, NARROW>;
     product_fn finish = nullptr;
     if constexpr(!EPI::mirror)
     {
@@ -104,6 +104,25 @@ product_kernel tiled_finish(int finish)
     }
 }
 
+// (an epilogue that finds nothing to add leaves the plain one's result)
+template<int LAYOUT>
+product_kernel narrow(int finish)
+{
+    if constexpr(kSteps)
+    {
+        return kNone;
+    }
+    else if constexpr(LAYOUT == layout_mn)
+    {
+        return tiled<LAYOUT, 128, 128, device::epilogue_add, true>();
+    }
+    else
+    {
+        return finish == finish_logistic ? tiled<LAYOUT, 128, 128, device::epilogue_logistic, true>()
+                                         : tiled<LAYOUT, 128, 128, device::epilogue_layer, true>();
+    }
+}
+
 template<int LAYOUT, int BM, int BN>
 product_kernel skinny()
 {
@@ -161,6 +180,7 @@ product_kernel in_layout(int form, int finish)
                 return tiled_finish<LAYOUT, 192, 192>(finish);
             }
             return kNone;
+        case form_narrow_128: return narrow<LAYOUT>(finish);
         case form_skinny_16x32: return skinny<LAYOUT, 16, 32>();
         case form_skinny_16x64: return skinny<LAYOUT, 16, 64>();
         case form_skinny_32x32: return skinny<LAYOUT, 32, 32>();

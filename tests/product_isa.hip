@@ -23,3 +23,6 @@ CHECKED(f16, float, float, true, true, 128, epilogue_next_cols)
 CHECKED(f16, __bf16, float, true, true, 256, epilogue_last_cols)
 SHAPED(bf16, __bf16, __bf16, true, true, 128, 256, epilogue_logistic)
 CHECKED(f16, _Float16, _Float16, true, true, 192, epilogue_poly)
+// rows of C that do not start on 16 bytes
+template __global__ void device::tiled_product_entry<device::tiled_product<device::in_kind::bf16, float, float, true, true, 128, 128, device::epilogue_logistic, true>>(device::product_args);
+template __global__ void device::tiled_product_entry<device::tiled_product<device::in_kind::f16, _Float16, _Float16, false, false, 128, 128, device::epilogue_add, true>>(device::product_args);

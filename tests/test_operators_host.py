@@ -10,7 +10,7 @@ import pytest
 import rocm_wmma_gemm_amd as R
 from test_host import ROOT, _mfma_loops
 
-INSTANTIATED = 15
+INSTANTIATED = 17
 
 
 def test_tiled_products_keep_accumulators_in_place(tmp_path):
