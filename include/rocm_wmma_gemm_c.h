@@ -261,6 +261,23 @@ int rocm_wmma_gemm_grouped_backward(int type_idx, void* dA, void* dB, void* dbia
                                     const void* B, const void* preact, const int* offsets, size_t groups, size_t M,
                                     size_t N, size_t K, int layout_b, int activation, int accumulate, void* stream);
 
+/* How a layer's product would run (operands that start on 16 bytes assumed; groups 0: linear). */
+#define ROCM_WMMA_GEMM_PRODUCT_FORWARD 0
+#define ROCM_WMMA_GEMM_PRODUCT_GRADIENT_A 1
+#define ROCM_WMMA_GEMM_PRODUCT_GRADIENT_B 2
+typedef struct rocm_wmma_gemm_product_plan
+{
+    int form; /* kernel: 0, 1 general (any alignment), 2-4 persistent tiles, 6 the same with C of any
+                 alignment, 7-13 few rows against a weight */
+    int block_m, block_n; /* its tile */
+    int cut_tail; /* 1: tiles of the last round are cut along K and added up by a second kernel */
+    int k_slices; /* few rows: workgroups that share a tile */
+    int once; /* 1: the weight is loaded with the non-temporal hint */
+    int copies; /* bit 0: A, bit 1: B is first copied to rows that start on 16 bytes */
+} rocm_wmma_gemm_product_plan;
+int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N, size_t K, size_t groups, int layout_b,
+                                  int activation, rocm_wmma_gemm_product_plan* plan);
+
 /* Newton-Schulz steps that bring an update near the closest matrix with orthonormal rows or
  * columns (all singular values near 1): X = G / (|G|_F + epsilon), then `steps` times
  * X = a X + (b S + c S^2) X with S = X X^T, coefficients = {a, b, c}; O = X.  G and O: batch_count

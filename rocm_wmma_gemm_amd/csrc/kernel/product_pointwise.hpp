@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(256) column_sums(const slope_args args, OutT* 
 }
 
 // ---------------------------------------------------------------------------
-// Newton-Schulz steps: X is held twice, scaled by a power of two, with rows and columns padded with zeros
-// to multiples of 8: in fp32 (its linear term, see operators.hip) and in f16 (what is multiplied).
+// Newton-Schulz steps: X is held twice, scaled by a power of two, padded with zeros to rows of multiples
+// of 8 (and, where it is not tall, to a multiple of 8 of them): in fp32 (its linear term, see operators.hip) and in f16 (what is multiplied).
 // ---------------------------------------------------------------------------
 constexpr int square_parts = 1024; // the most workgroups that add up the squares of one matrix
 

@@ -119,6 +119,13 @@ int with_status(Body&& body)
     }
 }
 
+// (without a device, for a plan that is only asked for: an MI355X's)
+size_t compute_units()
+{
+    const size_t cus = compute_units_of_current_device();
+    return cus > 0 ? cus : 256;
+}
+
 // Which operands have rows (and groups) that all start on 16 bytes, as the kernels need them that
 // load 16 bytes at a time, straight to LDS, or store pieces of 16.
 struct starts_on_16
@@ -191,7 +198,7 @@ struct launch_choice
     bool           once = false; // B's loads carry the non-temporal hint
     bool           copy_a = false, copy_b = false; // work on padded copies
     size_t         copy_bytes = 0; // room for them
-    int            layout = 0;
+    int            layout = 0, form = 0;
     size_t         scratch() const
     {
         return copy_bytes + partial_bytes;
@@ -276,6 +283,7 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
     auto                 made = [&](int form) {
         launch_choice c;
         c.layout = layout;
+        c.form   = form;
         if(form != form_general_64 && form != form_general_128)
         {
             c.copy_a     = copy_a;
@@ -429,7 +437,7 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
         c.copy_bytes = 0;
         c.copy_a = c.copy_b = c.once = false;
         c.items      = tiles_of(args, 128, 128, false, true);
-        c.workgroups = std::min(c.items, c.kernel.per_cu * std::max<size_t>(compute_units_of_current_device(), 1));
+        c.workgroups = std::min(c.items, c.kernel.per_cu * compute_units());
     }
     if(c.kernel.fn == nullptr || c.items > most_extent)
     {
@@ -477,11 +485,6 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
     return ROCM_WMMA_GEMM_OK;
 }
 
-size_t compute_units()
-{
-    return std::max<size_t>(compute_units_of_current_device(), 1);
-}
-
 // A linear layer's problem, for one weight (groups = 1 and no offsets) or one per group of rows.
 struct layer
 {
@@ -516,6 +519,63 @@ product_args arguments(const layer& p)
     return a;
 }
 
+// The three products of a layer, without their pointers.
+struct layer_product
+{
+    product_args args;
+    int          layout, finish;
+};
+
+layer_product forward_product(const layer& p, bool extras)
+{
+    product_args a = arguments(p);
+    a.act          = p.act;
+    a.kind         = product_kind::rows;
+    a.M            = static_cast<int>(p.M);
+    a.N            = static_cast<int>(p.N);
+    a.K            = static_cast<int>(p.K);
+    a.lda          = p.K;
+    a.ldb          = p.layout_b == 1 ? p.K : p.N;
+    a.ldc          = p.N;
+    a.stride_b     = static_cast<long long>(p.N * p.K);
+    a.stride_bias  = p.N;
+    return {a, p.layout_b == 1 ? layout_kk : layout_kn,
+            p.act.kind == act_kind::logistic           ? finish_logistic
+            : p.act.kind == act_kind::relu || extras ? finish_layer
+                                                       : finish_plain};
+}
+
+// dA = dZ B^T; pitch: dZ's row length
+layer_product gradient_a(const layer& p, size_t pitch)
+{
+    product_args a = arguments(p);
+    a.kind         = product_kind::rows;
+    a.M            = static_cast<int>(p.M);
+    a.N            = static_cast<int>(p.K);
+    a.K            = static_cast<int>(p.N);
+    a.lda          = pitch;
+    a.ldb          = p.layout_b == 1 ? p.K : p.N;
+    a.ldc          = p.K;
+    a.stride_b     = static_cast<long long>(p.N * p.K);
+    return {a, p.layout_b == 1 ? layout_kn : layout_kk, finish_plain};
+}
+
+// dB, stored N x K: dZ^T A; stored K x N: A^T dZ
+layer_product gradient_b(const layer& p, size_t pitch, bool accumulate)
+{
+    const bool   nk = p.layout_b == 1;
+    product_args a  = arguments(p);
+    a.kind          = product_kind::sum;
+    a.M             = static_cast<int>(nk ? p.N : p.K);
+    a.N             = static_cast<int>(nk ? p.K : p.N);
+    a.K             = static_cast<int>(p.M);
+    a.lda           = nk ? pitch : p.K;
+    a.ldb           = nk ? p.K : pitch;
+    a.ldc           = a.N;
+    a.stride_c      = static_cast<long long>(p.N * p.K);
+    return {a, layout_mn, accumulate ? finish_add : finish_plain};
+}
+
 // C = act(A B + bias) + residual
 int forward(const layer& p, void* C, const void* A, const void* B, const rocm_wmma_gemm_epilogue& e,
             hipStream_t stream)
@@ -528,30 +588,17 @@ int forward(const layer& p, void* C, const void* A, const void* B, const rocm_wm
     {
         return ROCM_WMMA_GEMM_ERR_ARGUMENT;
     }
-    product_args a = arguments(p);
-    a.C            = C;
-    a.kept         = e.preact;
-    a.A            = A;
-    a.B            = B;
-    a.bias         = e.bias;
-    a.residual     = e.residual;
-    a.act          = p.act;
-    a.kind         = product_kind::rows;
-    a.M            = static_cast<int>(p.M);
-    a.N            = static_cast<int>(p.N);
-    a.K            = static_cast<int>(p.K);
-    a.lda          = p.K;
-    a.ldb          = p.layout_b == 1 ? p.K : p.N;
-    a.ldc          = p.N;
-    a.stride_b     = static_cast<long long>(p.N * p.K);
-    a.stride_bias  = p.N;
-    const int finish = p.act.kind == act_kind::logistic ? finish_logistic
-                       : p.act.kind == act_kind::relu || e.bias || e.residual || e.preact ? finish_layer
-                                                                                          : finish_plain;
-    const launch_choice c = choose(p.type_idx, p.layout_b == 1 ? layout_kk : layout_kn, finish, a, compute_units());
+    layer_product f = forward_product(p, e.bias || e.residual || e.preact);
+    f.args.C        = C;
+    f.args.kept     = e.preact;
+    f.args.A        = A;
+    f.args.B        = B;
+    f.args.bias     = e.bias;
+    f.args.residual = e.residual;
+    const launch_choice c = choose(p.type_idx, f.layout, f.finish, f.args, compute_units());
     workspace_lease     lease;
     char*               scratch = c.scratch() != 0 ? lease.acquire(c.scratch(), stream) : nullptr;
-    return launch_product(p.type_idx, finish, c, a, scratch, stream);
+    return launch_product(p.type_idx, f.finish, c, f.args, scratch, stream);
 }
 
 template<class InT>
@@ -586,7 +633,7 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     }
     const size_t       cus = compute_units();
     const void*        dz  = dC;
-    product_args       to_a = arguments(p), to_b = arguments(p);
+    layer_product      to_a, to_b;
     launch_choice      on_a, on_b;
     device::slope_args s{};
     // dZ and the sums of its columns live in the scratch buffer, and what the products ask for
@@ -601,49 +648,26 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     {
         return ROCM_WMMA_GEMM_ERR_LIMIT;
     }
+    to_a = gradient_a(p, pitch);
+    to_b = gradient_b(p, pitch, accumulate != 0);
     // (where the products find dZ is not known yet; the buffer is aligned for any kernel)
     auto placed = [&](const void* at) {
-        to_a.A = at;
-        (p.layout_b == 1 ? to_b.A : to_b.B) = at;
+        to_a.args.A                                   = at;
+        (p.layout_b == 1 ? to_b.args.A : to_b.args.B) = at;
     };
-    if(dA != nullptr)
-    {
-        to_a.C        = dA;
-        to_a.B        = B;
-        to_a.kind     = product_kind::rows;
-        to_a.M        = static_cast<int>(p.M);
-        to_a.N        = static_cast<int>(p.K);
-        to_a.K        = static_cast<int>(p.N);
-        to_a.lda      = pitch;
-        to_a.ldb      = p.layout_b == 1 ? p.K : p.N;
-        to_a.ldc      = p.K;
-        to_a.stride_b = static_cast<long long>(p.N * p.K);
-    }
-    if(dB != nullptr)
-    {
-        // stored N x K: dZ^T A; stored K x N: A^T dZ
-        const bool nk = p.layout_b == 1;
-        to_b.C        = dB;
-        (nk ? to_b.B : to_b.A) = A;
-        to_b.residual = accumulate ? dB : nullptr;
-        to_b.kind     = product_kind::sum;
-        to_b.M        = static_cast<int>(nk ? p.N : p.K);
-        to_b.N        = static_cast<int>(nk ? p.K : p.N);
-        to_b.K        = static_cast<int>(p.M);
-        to_b.lda      = nk ? pitch : p.K;
-        to_b.ldb      = nk ? p.K : pitch;
-        to_b.ldc      = to_b.N;
-        to_b.stride_c = static_cast<long long>(p.N * p.K);
-    }
+    to_a.args.C        = dA;
+    to_a.args.B        = B;
+    to_b.args.C        = dB;
+    to_b.args.residual = accumulate ? dB : nullptr;
+    (p.layout_b == 1 ? to_b.args.B : to_b.args.A) = A;
     placed(dz_bytes != 0 ? nullptr : dC);
-    const int a_layout = p.layout_b == 1 ? layout_kn : layout_kk, b_finish = accumulate ? finish_add : finish_plain;
     if(dA != nullptr && p.M != 0 && p.K != 0)
     {
-        on_a = choose(p.type_idx, a_layout, finish_plain, to_a, cus);
+        on_a = choose(p.type_idx, to_a.layout, to_a.finish, to_a.args, cus);
     }
     if(dB != nullptr && p.N != 0 && p.K != 0)
     {
-        on_b = choose(p.type_idx, layout_mn, b_finish, to_b, cus);
+        on_b = choose(p.type_idx, to_b.layout, to_b.finish, to_b.args, cus);
     }
     workspace_lease lease;
     const size_t    needed = dz_bytes + sums, cuts = std::max(on_a.scratch(), on_b.scratch());
@@ -691,11 +715,11 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     int rc = ROCM_WMMA_GEMM_OK;
     if(on_a.kernel.fn != nullptr)
     {
-        rc = launch_product(p.type_idx, finish_plain, on_a, to_a, on_a.scratch() != 0 ? scratch : nullptr, stream);
+        rc = launch_product(p.type_idx, to_a.finish, on_a, to_a.args, on_a.scratch() != 0 ? scratch : nullptr, stream);
     }
     if(rc == ROCM_WMMA_GEMM_OK && on_b.kernel.fn != nullptr)
     {
-        rc = launch_product(p.type_idx, b_finish, on_b, to_b, on_b.scratch() != 0 ? scratch : nullptr, stream);
+        rc = launch_product(p.type_idx, to_b.finish, on_b, to_b.args, on_b.scratch() != 0 ? scratch : nullptr, stream);
     }
     return rc;
 }
@@ -744,8 +768,10 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         return ROCM_WMMA_GEMM_OK;
     }
     const bool   tall = M > N;
-    const size_t mp = round_up8(M), np = round_up8(N), lp = std::min(mp, np);
+    // (the rows of a tall X are only summed over and written: they need no padding)
+    const size_t mp = tall ? M : round_up8(M), np = round_up8(N), lp = tall ? np : mp;
     const size_t each = mp * np, square = lp * lp;
+    // (whole pieces of 16 bytes a row: the last product writes the update itself)
     const bool   direct  = mp == M && np == N && aligned16(O);
     const size_t parts_b = whole_lines(batch * device::square_parts * sizeof(float)),
                  diag_b = whole_lines(batch * lp * sizeof(float)), x32_b = whole_lines(batch * each * 4),
@@ -933,6 +959,44 @@ int rocm_wmma_gemm_linear_backward(int type_idx, void* dA, void* dB, void* dbias
             return ROCM_WMMA_GEMM_ERR_ARGUMENT;
         }
         return backward(p, dA, dB, dbias, dC, A, B, preact, accumulate, stream_of(stream));
+    });
+}
+
+int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N, size_t K, size_t groups, int layout_b,
+                                  int activation, rocm_wmma_gemm_product_plan* plan)
+{
+    return with_status([&] {
+        // (offsets that nobody reads: groups of rows are told by their presence)
+        static const int somewhere = 0;
+        layer            p{type_idx, M, N, K, layout_b, groups != 0 ? &somewhere : nullptr, groups != 0 ? groups : 1, {}};
+        const int        rc = check_layer(p);
+        if(rc != ROCM_WMMA_GEMM_OK)
+        {
+            return rc;
+        }
+        if(!activation_of(activation, &p.act) || plan == nullptr || product < 0 || product > ROCM_WMMA_GEMM_PRODUCT_GRADIENT_B
+           || M == 0 || N == 0)
+        {
+            return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+        }
+        // dZ is written to rows that start on 16 bytes where dC's do not
+        const size_t        pitch = round_up8(p.N);
+        const layer_product f     = product == ROCM_WMMA_GEMM_PRODUCT_FORWARD      ? forward_product(p, true)
+                                    : product == ROCM_WMMA_GEMM_PRODUCT_GRADIENT_A ? gradient_a(p, pitch)
+                                                                                   : gradient_b(p, pitch, false);
+        if(f.args.M == 0 || f.args.N == 0)
+        {
+            return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+        }
+        const launch_choice c = choose(p.type_idx, f.layout, f.finish, f.args, compute_units());
+        plan->form            = c.form;
+        plan->block_m         = c.kernel.block_m;
+        plan->block_n         = c.kernel.block_n;
+        plan->cut_tail        = c.kernel.finish != nullptr && c.partial_bytes != 0;
+        plan->k_slices        = c.k_slices;
+        plan->once            = c.once;
+        plan->copies          = (c.copy_a ? 1 : 0) | (c.copy_b ? 2 : 0);
+        return ROCM_WMMA_GEMM_OK;
     });
 }
 

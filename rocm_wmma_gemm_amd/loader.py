@@ -57,6 +57,23 @@ class _EpilogueC(ctypes.Structure):
                 ("activation", ctypes.c_int)]
 
 
+class _ProductPlanC(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("form", "block_m", "block_n", "cut_tail", "k_slices", "once", "copies")]
+
+
+@dataclass(frozen=True)
+class ProductPlan:
+    """How a layer's product would run (the fields of rocm_wmma_gemm_product_plan)."""
+
+    form: int
+    block_m: int
+    block_n: int
+    cut_tail: int
+    k_slices: int
+    once: int
+    copies: int
+
+
 MAX_GROUPS = 512
 
 
@@ -217,6 +234,7 @@ class Loader:
                     ("linear_backward", [i] + [p] * 7 + [z] * 3 + [i] * 3 + [p]),
                     ("grouped", [i, p, p, p, p, z, z, z, z, i, p, p]),
                     ("grouped_backward", [i] + [p] * 8 + [z] * 4 + [i] * 3 + [p]),
+                    ("product_select", [i, i, z, z, z, z, i, i, p]),
                     ("orthogonalize", [i, i, p, p, z, z, z, i, p, ctypes.c_float, p])):
                 fn = getattr(L, "rocm_wmma_gemm_" + name)
                 fn.restype = ctypes.c_int
@@ -472,6 +490,16 @@ class Loader:
         """The gradients of grouped(); an empty group's are zero (unchanged with accumulate)."""
         self._backward(self._lib.rocm_wmma_gemm_grouped_backward, "grouped_backward", dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, activation,
                        accumulate, stream)
+
+    def product_select(self, product: str, M: int, N: int, K: int, groups: int = 0, type_idx: int = 2,
+                       layout_b=col_major, activation=activation.none) -> ProductPlan:
+        """Which kernel ``product`` ("forward", "gradient_a" or "gradient_b") of linear() (groups = 0)
+        or grouped() runs on, and how; operands that start on 16 bytes assumed."""
+        c = _ProductPlanC()
+        self._done("product_select", self._lib.rocm_wmma_gemm_product_select(
+            ("forward", "gradient_a", "gradient_b").index(product), type_idx, M, N, K, groups, int(layout_b),
+            int(activation), ctypes.byref(c)))
+        return ProductPlan(*[getattr(c, n) for n, _ in _ProductPlanC._fields_])
 
     def orthogonalize(self, O, G, M: int, N: int, batch_count: int = 1, steps: int = 5,
                       coefficients=(3.4445, -4.7750, 2.0315), epsilon: float = 1e-7, stream=None) -> None:

@@ -522,6 +522,78 @@ def test_captured_in_a_graph(loader):
 
 
 # ---------------------------------------------------------------------------------------------
+# every kernel form, at sizes that the library's own choice sends there
+# ---------------------------------------------------------------------------------------------
+COVERED = [  # (product, M, N, K, groups, layout of B, types)
+    ("forward", 2048, 4096, 512, 8, 1, 2), ("forward", 2048, 4096, 999, 8, 1, 0), ("forward", 512, 520, 512, 64, 0, 3),
+    ("forward", 384, 520, 16384, 0, 0, 1), ("forward", 100, 8192, 512, 8, 0, 2), ("forward", 384, 1024, 16384, 0, 1, 0),
+    ("forward", 1024, 1001, 512, 8, 0, 3), ("forward", 384, 1001, 16384, 0, 1, 2), ("forward", 1, 14336, 4096, 0, 1, 1),
+    ("forward", 48, 520, 16384, 0, 1, 2), ("forward", 1, 4096, 16384, 0, 0, 0), ("forward", 24, 1024, 16384, 0, 0, 3),
+    ("forward", 16, 8192, 1000, 8, 1, 2), ("forward", 64, 520, 8192, 0, 0, 0), ("forward", 24, 4096, 16384, 0, 0, 2),
+    ("forward", 256, 1001, 999, 8, 0, 1), ("forward", 48, 14336, 4096, 0, 1, 0), ("forward", 48, 4096, 16384, 0, 1, 3),
+    ("forward", 48, 8192, 1000, 8, 1, 0), ("forward", 384, 520, 16384, 0, 1, 2), ("forward", 1, 520, 16384, 0, 1, 1),
+    ("forward", 1, 520, 999, 0, 1, 2), ("forward", 32, 1001, 512, 64, 0, 0), ("forward", 1, 520, 999, 64, 1, 3),
+    ("forward", 4096, 5120, 5120, 0, 1, 2), ("forward", 1024, 1024, 999, 8, 0, 0),
+    ("gradient_a", 2048, 1001, 4096, 8, 1, 2), ("gradient_a", 384, 14336, 512, 0, 1, 0), ("gradient_a", 2048, 4096, 512, 8, 1, 1),
+    ("gradient_a", 384, 14336, 999, 0, 1, 2), ("gradient_a", 24, 14336, 1000, 0, 1, 3), ("gradient_a", 100, 14336, 999, 0, 0, 0),
+    ("gradient_b", 4096, 520, 999, 0, 1, 3), ("gradient_b", 2048, 520, 512, 0, 1, 2), ("gradient_b", 4096, 4096, 512, 0, 0, 0),
+    ("gradient_b", 777, 14336, 512, 0, 1, 1), ("gradient_b", 2048, 1024, 1000, 37, 0, 2), ("gradient_b", 3000, 2048, 1024, 11, 1, 3),
+]
+
+
+@pytest.mark.parametrize("case", range(len(COVERED)))
+def test_sizes_of_every_form(loader, case):
+    product, M, N, K, groups, layout, types = COVERED[case]
+    ab, out = PAIRS[types]
+    layout = R.m_layout(layout)
+    counts = routing(groups, M, case) if groups else [M]
+    ends, offsets = offsets_of(counts)
+    A, B = rnd((M, K), ab, 1), weights((K, N), layout, ab, 2, groups or None)
+    each = B if groups else B[None]
+    act = ACTS[case % 4] if product == "forward" else R.activation.none
+    if product == "forward":
+        bias = rnd((groups or 1, N), ab, 3)
+        residual = rnd((M, N), out, 4) if case % 2 else None
+        kept = torch.full((M, N), math.nan, dtype=ab, device="cuda") if case % 3 else None
+        C = torch.full((M, N), math.nan, dtype=out, device="cuda")
+        if groups:
+            loader.grouped(C, A, B, offsets, M, N, K, layout, bias=bias, residual=residual, preact=kept, activation=act)
+        else:
+            loader.linear(C, A, B, M, N, K, layout, bias=bias, residual=residual, preact=kept, activation=act)
+    else:
+        dC = rnd((M, N), ab, 3)
+        result = torch.full((M, K) if product == "gradient_a" else B.shape, math.nan, dtype=out, device="cuda")
+        wanted = (result, None, None) if product == "gradient_a" else (None, result, None)
+        if groups:
+            loader.grouped_backward(*wanted, dC, A, B, offsets, M, N, K, layout)
+        else:
+            loader.linear_backward(*wanted, dC, A, B, M, N, K, layout)
+    for e, count in enumerate(counts):
+        at, what = slice(ends[e], ends[e + 1]), f"{COVERED[case]} group {e}"
+        if product == "forward":
+            if count:
+                check_forward(C[at], None if kept is None else kept[at], A[at].double(), weight64(each[e], layout),
+                              bias[e], None if residual is None else residual[at], act, out, what)
+        elif product == "gradient_a":
+            if count:
+                check_backward(result[at], None, None, dC[at], None, None, each[e], layout, act, out, what)
+        else:
+            check_backward(None, result[e] if groups else result, None, dC[at], None, A[at], each[e], layout, act, out, what)
+
+
+def test_the_sizes_above_cover_the_forms(loader):
+    seen = {}
+    for product, M, N, K, groups, layout, types in COVERED:
+        p = loader.product_select(product, M, N, K, groups, types, R.m_layout(layout))
+        for what in (("form", p.form), ("cut", p.form if p.cut_tail else 0), ("slices", p.k_slices), ("once", p.once),
+                     ("copies", p.copies)):
+            seen.setdefault(what[0], set()).add(what[1])
+    assert seen["form"] >= {0, 1, 2, 3, 4, 6, 7, 8, 9, 10, 11, 12, 13}, seen
+    assert seen["cut"] >= {2, 3, 4, 6}, seen
+    assert seen["slices"] >= {1, 2, 4} and seen["once"] == {0, 1} and seen["copies"] >= {0, 1, 2, 3}, seen
+
+
+# ---------------------------------------------------------------------------------------------
 # Newton-Schulz steps
 # ---------------------------------------------------------------------------------------------
 def steps64(G, steps=5, coefficients=(3.4445, -4.7750, 2.0315), epsilon=1e-7):
@@ -627,3 +699,17 @@ def test_refusals(loader):
     with pytest.raises(ValueError, match="holds"):
         loader.orthogonalize(torch.zeros_like(A), A, 4, 8, 2)
     torch.cuda.synchronize()
+
+
+def test_the_example_runs():
+    """One training step and one decode step through the operators together."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, os.path.join(root, "examples", "expert_layer.py"), "--tokens", "300",
+                           "--experts", "5", "--hidden", "256", "--inner", "384"], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout + done.stderr
+    before, after = (float(x) for x in done.stdout.split("mean square of the output: ")[1].split("\n")[0].split(" -> "))
+    assert after < before

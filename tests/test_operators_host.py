@@ -62,3 +62,68 @@ def test_tiled_products_keep_accumulators_in_place(tmp_path):
                         break
                 n += 1
         assert checked >= 1, func
+
+
+@pytest.fixture(scope="module")
+def library():
+    return R.Loader(arch="gfx950")
+
+
+def test_entry_points_refuse_before_they_touch_the_device(library):
+    """Arguments out of range, missing operands and sizes beyond the limits are status codes, asked
+    of the C functions themselves, without a device."""
+    L, one = library._lib, ctypes.c_void_p(16)
+    epilogue = lambda act: ctypes.byref(loader_module()._EpilogueC(None, None, None, act))  # noqa: E731
+    ERR_ARGUMENT, ERR_LIMIT, OK = -2, -5, 0
+    linear = lambda *a: L.rocm_wmma_gemm_linear(*a, None)  # noqa: E731
+    assert linear(4, one, one, one, 8, 8, 8, 1, None) == ERR_ARGUMENT  # type pair
+    assert linear(0, one, one, one, 8, 8, 8, 2, None) == ERR_ARGUMENT  # layout
+    assert linear(0, one, one, one, 8, 8, 8, 1, epilogue(4)) == ERR_ARGUMENT  # activation
+    assert linear(0, one, one, one, 1 << 31, 8, 8, 1, None) == ERR_LIMIT
+    assert linear(0, None, one, one, 8, 8, 8, 1, None) == ERR_ARGUMENT
+    assert linear(0, one, one, None, 8, 8, 8, 1, None) == ERR_ARGUMENT
+    assert linear(0, None, None, None, 0, 8, 8, 1, None) == OK  # nothing to do
+    grouped = lambda *a: L.rocm_wmma_gemm_grouped(*a, None)  # noqa: E731
+    assert grouped(0, one, one, one, None, 4, 8, 8, 8, 1, None) == ERR_ARGUMENT  # no offsets
+    assert grouped(0, one, one, one, one, 513, 8, 8, 8, 1, None) == ERR_LIMIT
+    assert grouped(0, one, one, one, None, 0, 8, 8, 8, 1, None) == OK
+    backward = lambda *a: L.rocm_wmma_gemm_linear_backward(*a, None)  # noqa: E731
+    assert backward(0, one, None, None, None, one, one, None, 8, 8, 8, 1, 0, 0) == ERR_ARGUMENT  # no dC
+    assert backward(0, one, None, None, one, one, None, None, 8, 8, 8, 1, 0, 0) == ERR_ARGUMENT  # dA without B
+    assert backward(0, None, one, None, one, None, one, None, 8, 8, 8, 1, 0, 0) == ERR_ARGUMENT  # dB without A
+    assert backward(0, one, None, None, one, one, one, None, 8, 8, 8, 1, 2, 0) == ERR_ARGUMENT  # no preact
+    assert backward(0, one, None, None, one, one, one, None, 8, 8, 8, 1, 7, 0) == ERR_ARGUMENT
+    steps = (ctypes.c_float * 3)(1.5, -0.5, 0.0)
+    orth = lambda *a: L.rocm_wmma_gemm_orthogonalize(*a, None)  # noqa: E731
+    assert orth(3, 0, one, one, 8, 8, 1, 5, steps, 1e-7) == ERR_ARGUMENT  # G's type
+    assert orth(0, 2, one, one, 8, 8, 1, 5, steps, 1e-7) == ERR_ARGUMENT  # O's type
+    assert orth(0, 0, one, one, 8, 8, 1, 0, steps, 1e-7) == ERR_ARGUMENT  # no step
+    assert orth(0, 0, one, one, 8, 8, 1, 5, None, 1e-7) == ERR_ARGUMENT
+    assert orth(0, 0, None, one, 8, 8, 1, 5, steps, 1e-7) == ERR_ARGUMENT
+    assert orth(0, 0, one, one, (1 << 20) + 1, 8, 1, 5, steps, 1e-7) == ERR_LIMIT
+    assert orth(0, 0, None, None, 0, 8, 1, 5, steps, 1e-7) == OK
+
+
+def loader_module():
+    from rocm_wmma_gemm_amd import loader
+
+    return loader
+
+
+def test_product_plans(library):
+    """What the estimate picks follows the sizes: few rows stream a weight, many take large tiles,
+    a long K with few tiles is cut, and rows that do not start on 16 bytes are copied or staged."""
+    pick = library.product_select
+    assert pick("forward", 1, 4096, 4096).block_m <= 32
+    large = pick("forward", 8192, 8192, 4096)
+    assert (large.block_m, large.block_n, large.copies, large.cut_tail) == (256, 256, 0, 0)
+    assert pick("forward", 2048, 1024, 16384).cut_tail == 1
+    assert pick("forward", 16, 8192, 8192).once == 1 and pick("forward", 16, 4096, 4096).once == 0
+    assert pick("forward", 2048, 4096, 4001).copies == 3  # K-contiguous rows of 4001: A and B
+    assert pick("forward", 2048, 4096, 4001, layout_b=R.row_major).copies == 1
+    assert pick("gradient_b", 2048, 4001, 4096, layout_b=R.row_major).copies == 0  # dZ is written padded
+    assert pick("forward", 1, 520, 999, groups=64).form in (0, 1)
+    with pytest.raises(R.GemmLibraryError):
+        pick("forward", 0, 8, 8)
+    with pytest.raises(R.GemmLibraryError):
+        pick("forward", 8, 8, 8, groups=513)
