@@ -42,8 +42,7 @@ enum class diagonal_use
 {
     none  = 0,
     split = 1, // C is square: its diagonal goes there, and C gets zeros in its place
-    rows  = 2, // row i of R is multiplied by beta + alpha diagonal[i]
-    cols  = 3 // column i
+    rows  = 2 // row i of R is multiplied by beta + alpha diagonal[i]
 };
 
 struct act_args
@@ -77,6 +76,7 @@ struct product_args
     float*       diagonal; // stride_diagonal values from group to group
     long long    stride_diagonal;
     int          grid_m, grid_n; // tiles of a problem (rows: grid_m is not used)
+    int          wide; // few-row kernel: rows of C and of what is added start on 16 bytes
     float*       partials; // tiled kernels: nullptr, or room for a tile of fp32 per workgroup of the
                            // grid; the tiles of the last round may then be cut along K (cut_tail)
     int          workgroups; // of the grid that writes them
@@ -315,10 +315,9 @@ __device__ __forceinline__ void finish_element(const product_args& args, const p
     if(args.residual != nullptr)
     {
         float beta = args.beta;
-        if(args.diagonal_is == diagonal_use::rows || args.diagonal_is == diagonal_use::cols)
+        if(args.diagonal_is == diagonal_use::rows)
         {
-            beta += args.alpha * args.diagonal[x.group * args.stride_diagonal
-                                               + (args.diagonal_is == diagonal_use::rows ? row : col)];
+            beta += args.alpha * args.diagonal[x.group * args.stride_diagonal + row];
         }
         y += beta * (float)static_cast<const ResT*>(args.residual)[at];
     }
@@ -366,13 +365,25 @@ __device__ __forceinline__ void finish_piece(const product_args& args, const pro
     if(args.residual != nullptr)
     {
         const res8 r = *reinterpret_cast<const res8*>(static_cast<const ResT*>(args.residual) + at);
-        const bool rows = args.diagonal_is == diagonal_use::rows, cols = args.diagonal_is == diagonal_use::cols;
-        const float* d = args.diagonal + x.group * args.stride_diagonal;
-        const float  by_row = rows ? args.beta + args.alpha * d[row] : args.beta;
+        const float beta = args.diagonal_is == diagonal_use::rows
+                               ? args.beta + args.alpha * args.diagonal[x.group * args.stride_diagonal + row]
+                               : args.beta;
 #pragma unroll
         for(int e = 0; e < 8; ++e)
         {
-            y[e] += (cols ? args.beta + args.alpha * d[col + e] : by_row) * (float)r[e];
+            y[e] += beta * (float)r[e];
+        }
+    }
+    if(args.diagonal_is == diagonal_use::split && row >= col && row < col + 8)
+    {
+#pragma unroll
+        for(int e = 0; e < 8; ++e)
+        {
+            if(row == col + e)
+            {
+                args.diagonal[x.group * args.stride_diagonal + row] = y[e];
+                y[e]                                                = 0.0f;
+            }
         }
     }
     if(args.kept != nullptr)

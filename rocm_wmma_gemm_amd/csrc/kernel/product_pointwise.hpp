@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(256) column_sums(const slope_args args, OutT* 
 }
 
 // ---------------------------------------------------------------------------
-// Newton-Schulz steps: X is held twice, scaled by a power of two, padded with zeros to rows of multiples
-// of 8 (and, where it is not tall, to a multiple of 8 of them): in fp32 (its linear term, see operators.hip) and in f16 (what is multiplied).
+// Newton-Schulz steps: X has the smaller side as its rows (a tall G is transposed on the way in and
+// out) and is held twice, scaled by a power of two, padded with zeros to multiples of 8: in fp32
+// (its linear term, see operators.hip) and in f16 (what is multiplied).
 // ---------------------------------------------------------------------------
 constexpr int square_parts = 1024; // the most workgroups that add up the squares of one matrix
 
@@ -197,23 +198,10 @@ __global__ void __launch_bounds__(256) sum_squares(const GivenT* __restrict__ gi
     }
 }
 
-// X = G scale / (|G| + epsilon), padded.  A thread writes 8 elements of a row at a time; WIDE: G's
-// rows are whole pieces of 8 that start on 16 bytes.
-template<class GivenT, bool WIDE>
-__global__ void __launch_bounds__(256) orthogonal_start(const GivenT* __restrict__ given,
-                                                        const float* __restrict__ parts,
-                                                        float*    x32,
-                                                        _Float16* x16,
-                                                        int       rows,
-                                                        int       cols,
-                                                        int       rows_pad,
-                                                        int       cols_pad,
-                                                        float     scale,
-                                                        float     epsilon,
-                                                        int       used_parts)
+// The norm of a matrix from its partial sums, by every wave.
+__device__ __forceinline__ float norm_of(const float* parts, long long matrix, int used_parts)
 {
-    const long long matrix = blockIdx.y;
-    float           t      = 0.0f;
+    float t = 0.0f;
     for(int i = threadIdx.x & 63; i < used_parts; i += 64)
     {
         t += parts[matrix * square_parts + i];
@@ -223,10 +211,44 @@ __global__ void __launch_bounds__(256) orthogonal_start(const GivenT* __restrict
     {
         t += __shfl_xor(t, d);
     }
-    const float   f      = scale / (sqrtf(t) + epsilon);
-    const int     pieces = cols_pad / 8;
-    const GivenT* g      = given + matrix * rows * cols;
-    for(int row = blockIdx.x; row < rows_pad; row += gridDim.x)
+    return sqrtf(t);
+}
+
+struct start_args
+{
+    const void*  given;
+    const float* parts;
+    float*       x32;
+    _Float16*    x16;
+    int          rows, cols; // of G
+    int          rows_pad, cols_pad; // of X
+    float        scale, epsilon;
+    int          used_parts;
+};
+
+__device__ __forceinline__ void store_start(const start_args& args, long long at, const float (&y)[8])
+{
+    f16x8 h;
+#pragma unroll
+    for(int e = 0; e < 8; ++e)
+    {
+        h[e] = (_Float16)y[e];
+    }
+    *reinterpret_cast<f32x4*>(args.x32 + at)     = f32x4{y[0], y[1], y[2], y[3]};
+    *reinterpret_cast<f32x4*>(args.x32 + at + 4) = f32x4{y[4], y[5], y[6], y[7]};
+    *reinterpret_cast<f16x8*>(args.x16 + at)     = h;
+}
+
+// X = G scale / (|G| + epsilon), padded (blockIdx.y: the matrix).  A thread writes 8 elements of a row at a time;
+// WIDE: G needs no padding and its rows are whole pieces of 8 that start on 16 bytes.
+template<class GivenT, bool WIDE>
+__global__ void __launch_bounds__(256) orthogonal_start(const start_args args)
+{
+    const long long matrix = blockIdx.y;
+    const float     f      = args.scale / (norm_of(args.parts, matrix, args.used_parts) + args.epsilon);
+    const int       pieces = args.cols_pad / 8;
+    const GivenT*   g      = static_cast<const GivenT*>(args.given) + matrix * args.rows * args.cols;
+    for(int row = blockIdx.x; row < args.rows_pad; row += gridDim.x)
     {
         for(int piece = threadIdx.x; piece < pieces; piece += 256)
         {
@@ -235,7 +257,7 @@ __global__ void __launch_bounds__(256) orthogonal_start(const GivenT* __restrict
             float          y[8];
             if constexpr(WIDE)
             {
-                const given8 v = *reinterpret_cast<const given8*>(g + (long long)row * cols + col);
+                const given8 v = *reinterpret_cast<const given8*>(g + (long long)row * args.cols + col);
 #pragma unroll
                 for(int e = 0; e < 8; ++e)
                 {
@@ -247,28 +269,97 @@ __global__ void __launch_bounds__(256) orthogonal_start(const GivenT* __restrict
 #pragma unroll
                 for(int e = 0; e < 8; ++e)
                 {
-                    y[e] = row < rows && col + e < cols ? (float)g[(long long)row * cols + col + e] * f : 0.0f;
+                    y[e] = row < args.rows && col + e < args.cols ? (float)g[(long long)row * args.cols + col + e] * f : 0.0f;
                 }
             }
-            f16x8 h;
+            store_start(args, (matrix * args.rows_pad + row) * args.cols_pad + col, y);
+        }
+    }
+}
+
+// The same for a tall G: X is its transpose.  A workgroup turns 64 x 64 elements round in LDS
+// (blockIdx.x: tiles of X, row by row of tiles).
+template<class GivenT>
+__global__ void __launch_bounds__(256) orthogonal_start_tall(const start_args args)
+{
+    __shared__ float tile[64][65];
+    const long long  matrix = blockIdx.y;
+    const float      f      = args.scale / (norm_of(args.parts, matrix, args.used_parts) + args.epsilon);
+    const GivenT*    g      = static_cast<const GivenT*>(args.given) + matrix * args.rows * args.cols;
+    const int        across = (args.cols_pad + 63) / 64;
+    const int        x_row0 = blockIdx.x / across * 64, x_col0 = blockIdx.x % across * 64;
+    for(int i = threadIdx.x; i < 64 * 64; i += 256)
+    {
+        const int row = x_col0 + i / 64, col = x_row0 + i % 64; // of G
+        tile[i % 64][i / 64] = row < args.rows && col < args.cols ? (float)g[(long long)row * args.cols + col] * f : 0.0f;
+    }
+    __syncthreads();
+    for(int i = threadIdx.x; i < 64 * 8; i += 256)
+    {
+        const int row = i / 8, col = i % 8 * 8;
+        if(x_row0 + row < args.rows_pad && x_col0 + col < args.cols_pad)
+        {
+            float y[8];
 #pragma unroll
             for(int e = 0; e < 8; ++e)
             {
-                h[e] = (_Float16)y[e];
+                y[e] = tile[row][col + e];
             }
-            const long long at = (matrix * rows_pad + row) * cols_pad + col;
-            *reinterpret_cast<f32x4*>(x32 + at)     = f32x4{y[0], y[1], y[2], y[3]};
-            *reinterpret_cast<f32x4*>(x32 + at + 4) = f32x4{y[4], y[5], y[6], y[7]};
-            *reinterpret_cast<f16x8*>(x16 + at)     = h;
+            store_start(args, (matrix * args.rows_pad + x_row0 + row) * args.cols_pad + x_col0 + col, y);
+        }
+    }
+}
+
+// The finished update (rows x cols) from its padded form.
+template<class OutT>
+__global__ void __launch_bounds__(256) orthogonal_end(const OutT* __restrict__ padded, OutT* __restrict__ out, int rows,
+                                                      int cols, int rows_pad, int cols_pad)
+{
+    const long long matrix = blockIdx.y;
+    for(int row = blockIdx.x; row < rows; row += gridDim.x)
+    {
+        for(int col = threadIdx.x; col < cols; col += 256)
+        {
+            out[(matrix * rows + row) * cols + col] = padded[(matrix * rows_pad + row) * cols_pad + col];
+        }
+    }
+}
+
+// The same where the update is tall: out = X^T, X of cols rows padded to rows_pad x cols_pad.
+template<class OutT>
+__global__ void __launch_bounds__(256) orthogonal_end_tall(const OutT* __restrict__ padded, OutT* __restrict__ out,
+                                                           int rows, int cols, int rows_pad, int cols_pad)
+{
+    __shared__ OutT tile[64][66];
+    const long long matrix = blockIdx.y;
+    const int       across = (cols + 63) / 64, row0 = blockIdx.x / across * 64, col0 = blockIdx.x % across * 64; // of out
+    for(int i = threadIdx.x; i < 64 * 64; i += 256)
+    {
+        const int xr = col0 + i / 64, xc = row0 + i % 64;
+        if(xr < rows_pad && xc < cols_pad)
+        {
+            tile[i % 64][i / 64] = padded[(matrix * rows_pad + xr) * cols_pad + xc];
+        }
+    }
+    __syncthreads();
+    for(int i = threadIdx.x; i < 64 * 64; i += 256)
+    {
+        const int row = row0 + i / 64, col = col0 + i % 64;
+        if(row < rows && col < cols)
+        {
+            out[(matrix * rows + row) * cols + col] = tile[i / 64][i % 64];
         }
     }
 }
 
 // All steps of one small matrix (smaller side up to 64, larger up to 256) in one workgroup, in
-// fp32 from LDS: X with the smaller side as its rows, S and Q.  One launch instead of seventeen, and
-// nothing is rounded to f16: in a small matrix few roundings average out (8 x 8 with one strong
-// direction: 4.8e-3 off by the f16 products, 1e-6 here).  A thread of the S and Q products owns 4 x 4
-// elements, of the update whole columns of X, which depend on nothing but themselves and Q.
+// fp32 on the matrix cores (v_mfma_f32_16x16x4_f32), from LDS: X with the smaller side as its rows, and S,
+// then Q, in one buffer; rows and columns past the matrix are zeros throughout.  One launch instead of
+// seventeen, and nothing is rounded to f16: in a small matrix few roundings average out (8 x 8 with
+// one strong direction: 4.8e-3 off by the f16 products, 1e-6 here).  Wave w of sixteen owns tile
+// (w / 4, w mod 4) of S and Q, and of X the tiles (w mod 4, w / 4 + 4 i).  Pitches of 4 mod 64 floats spread the
+// 16 rows x 4 columns that a fragment read touches over all 64 banks.  Bound by the latency of LDS
+// and the matrix cores' fp32 rate; past 256 columns the seventeen launches are as fast.
 constexpr int small_side = 64, small_length = 256;
 
 struct steps_args
@@ -281,22 +372,28 @@ struct steps_args
 };
 
 template<class GivenT, class OutT>
-__global__ void __launch_bounds__(256) orthogonal_small(const steps_args args)
+__global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
 {
-    constexpr int XP = small_length + 1, SP = small_side + 4;
+    constexpr int XP = small_length + 4, SP = small_side + 4, THREADS = 1024, COLS = small_length / 16 / 4;
     __shared__ float x[small_side * XP];
-    __shared__ float s[small_side * SP], q[small_side * SP];
-    __shared__ float wave_sum[4];
-    const int       tid  = threadIdx.x;
+    __shared__ float s[small_side * SP];
+    __shared__ float wave_sum[16];
+    const int       tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, k4 = lane >> 4;
     const bool      tall = args.rows > args.cols;
     const int       l = tall ? args.cols : args.rows, h = tall ? args.rows : args.cols;
+    const int       l16 = (l + 15) / 16 * 16, h16 = (h + 15) / 16 * 16;
     const long long at = (long long)blockIdx.x * l * h;
     const GivenT*   g  = static_cast<const GivenT*>(args.given) + at;
     OutT*           o  = static_cast<OutT*>(args.out) + at;
     auto place = [&](int i) { return tall ? (i % l) * XP + i / l : (i / h) * XP + i % h; };
 
+    for(int i = tid; i < small_side * XP; i += THREADS)
+    {
+        x[i] = 0.0f;
+    }
+    __syncthreads();
     float t = 0.0f;
-    for(int i = tid; i < l * h; i += 256)
+    for(int i = tid; i < l * h; i += THREADS)
     {
         const float v = (float)g[i];
         x[place(i)]   = v;
@@ -307,122 +404,100 @@ __global__ void __launch_bounds__(256) orthogonal_small(const steps_args args)
     {
         t += __shfl_xor(t, d);
     }
-    if((tid & 63) == 0)
+    if(lane == 0)
     {
-        wave_sum[tid >> 6] = t;
+        wave_sum[wave] = t;
     }
     __syncthreads();
-    const float f = 1.0f / (sqrtf((wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3])) + args.epsilon);
-    for(int i = tid; i < l * h; i += 256)
+    t = 0.0f;
+#pragma unroll
+    for(int w = 0; w < 16; ++w)
+    {
+        t += wave_sum[w];
+    }
+    const float f = 1.0f / (sqrtf(t) + args.epsilon);
+    for(int i = tid; i < l * h; i += THREADS)
     {
         x[place(i)] *= f;
     }
-    const int ti = tid / 16 * 4, tj = tid % 16 * 4; // this thread's 4 x 4 elements of S and Q
+    const int ti = wave >> 2, tj = wave & 3;
+    float*    own = &s[(ti * 16 + 4 * k4) * SP + tj * 16 + r16]; // this lane's 4 rows of its tile of S
+    const bool used = ti * 16 < l16 && tj * 16 < l16; // (the others' tiles are zeros)
     for(int step = 0; step < args.steps; ++step)
     {
         __syncthreads();
-        if(ti < l && tj < l)
+        // S = X X^T
+        f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+        if(used)
         {
-            float acc[4][4] = {};
-            for(int k = 0; k < h; ++k)
+#pragma unroll 4
+            for(int k = 0; k < h16; k += 4)
             {
-                float u[4], v[4];
-#pragma unroll
-                for(int e = 0; e < 4; ++e)
-                {
-                    // (rows past l: read as row 0, their sums are not stored)
-                    u[e] = x[(ti + e < l ? ti + e : 0) * XP + k];
-                    v[e] = x[(tj + e < l ? tj + e : 0) * XP + k];
-                }
-#pragma unroll
-                for(int e = 0; e < 16; ++e)
-                {
-                    acc[e / 4][e % 4] += u[e / 4] * v[e % 4];
-                }
+                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[(ti * 16 + r16) * XP + k + k4], x[(tj * 16 + r16) * XP + k + k4],
+                                                           acc, 0, 0, 0);
             }
+        }
 #pragma unroll
-            for(int e = 0; e < 16; ++e)
+        for(int v = 0; v < 4; ++v)
+        {
+            own[v * SP] = acc[v];
+        }
+        __syncthreads();
+        // Q = b S + c S^2 (S is its own transpose: column j of it is row j)
+        f32x4 q{0.0f, 0.0f, 0.0f, 0.0f};
+        if(used)
+        {
+#pragma unroll 4
+            for(int k = 0; k < l16; k += 4)
             {
-                s[(ti + e / 4) * SP + tj + e % 4] = ti + e / 4 < l && tj + e % 4 < l ? acc[e / 4][e % 4] : 0.0f;
+                q = __builtin_amdgcn_mfma_f32_16x16x4f32(s[(ti * 16 + r16) * SP + k + k4], s[(tj * 16 + r16) * SP + k + k4], q,
+                                                         0, 0, 0);
             }
         }
         __syncthreads();
-        if(ti < l && tj < l)
+#pragma unroll
+        for(int v = 0; v < 4; ++v)
         {
-            float acc[4][4] = {};
-            for(int k = 0; k < l; ++k)
-            {
-                // (S is its own transpose: row k holds what column k does)
-                const f32x4 u = *reinterpret_cast<const f32x4*>(&s[k * SP + ti]);
-                const f32x4 v = *reinterpret_cast<const f32x4*>(&s[k * SP + tj]);
+            own[v * SP] = args.b * acc[v] + args.c * q[v];
+        }
+        __syncthreads();
+        // X = a X + Q X: every tile is read before any is written
+        f32x4 y[COLS];
 #pragma unroll
-                for(int e = 0; e < 16; ++e)
+        for(int i = 0; i < COLS; ++i)
+        {
+            y[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int rows = tj * 16;
+        if(rows < l16)
+        {
+#pragma unroll 2
+            for(int k = 0; k < l16; k += 4)
+            {
+                const float u = s[(rows + r16) * SP + k + k4];
+#pragma unroll
+                for(int i = 0; i < COLS; ++i)
                 {
-                    acc[e / 4][e % 4] += u[e / 4] * v[e % 4];
+                    y[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, x[(k + k4) * XP + (ti + 4 * i) * 16 + r16], y[i], 0, 0, 0);
                 }
-            }
-#pragma unroll
-            for(int e = 0; e < 16; ++e)
-            {
-                const int to = (ti + e / 4) * SP + tj + e % 4;
-                q[to]        = args.b * s[to] + args.c * acc[e / 4][e % 4];
             }
         }
         __syncthreads();
-        for(int col = tid; col < h; col += 256)
+#pragma unroll
+        for(int i = 0; i < COLS; ++i)
         {
-            float acc[small_side];
 #pragma unroll
-            for(int i = 0; i < small_side; ++i)
+            for(int v = 0; v < 4; ++v)
             {
-                acc[i] = 0.0f;
-            }
-            for(int k = 0; k < l; ++k)
-            {
-                const float v = x[k * XP + col];
-#pragma unroll
-                for(int i = 0; i < small_side; i += 4)
-                {
-                    if(i < l)
-                    {
-                        const f32x4 u = *reinterpret_cast<const f32x4*>(&q[k * SP + i]);
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-                            acc[i + e] += u[e] * v;
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for(int i = 0; i < small_side; ++i)
-            {
-                if(i < l)
-                {
-                    x[i * XP + col] = args.a * x[i * XP + col] + acc[i];
-                }
+                float& to = x[(rows + 4 * k4 + v) * XP + (ti + 4 * i) * 16 + r16];
+                to        = args.a * to + y[i][v];
             }
         }
     }
     __syncthreads();
-    for(int i = tid; i < l * h; i += 256)
+    for(int i = tid; i < l * h; i += THREADS)
     {
         o[i] = to_out<OutT>(x[place(i)]);
-    }
-}
-
-// The finished update from its padded form (where rows and columns are no multiples of 8).
-template<class OutT>
-__global__ void __launch_bounds__(256) orthogonal_end(const OutT* __restrict__ padded, OutT* __restrict__ out, int rows,
-                                                      int cols, int rows_pad, int cols_pad)
-{
-    const long long matrix = blockIdx.y;
-    for(int row = blockIdx.x; row < rows; row += gridDim.x)
-    {
-        for(int col = threadIdx.x; col < cols; col += 256)
-        {
-            out[(matrix * rows + row) * cols + col] = padded[(matrix * rows_pad + row) * cols_pad + col];
-        }
     }
 }
 

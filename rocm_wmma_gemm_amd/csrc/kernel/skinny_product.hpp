@@ -23,13 +23,12 @@ namespace device
 {
 
 // ONCE: the weight's loads carry the non-temporal hint (product_kernel::once).
-template<in_kind IN, class OutT, int BM, int BN, bool B_KMAJOR, bool ONCE>
+template<in_kind IN, class OutT, class ResT, int BM, int BN, bool B_KMAJOR, bool ONCE>
 struct skinny_product
 {
     using S   = stream_gemm<IN, OutT, BM, BN, true, B_KMAJOR>;
     using InT = typename S::InT;
     static constexpr int THREADS = S::THREADS, BK = S::BK, TM = S::TM, TN = S::TN, DEPTH = S::DEPTH;
-    static constexpr int MINE = (BM * BN + THREADS - 1) / THREADS; // elements of C of a thread
 
     __device__ __forceinline__ static void run(const product_args& args)
     {
@@ -47,8 +46,13 @@ struct skinny_product
             lds_int* off   = reinterpret_cast<lds_int*>(lds);
             lds_int* first = off + max_groups + 1;
             static_assert(2 * (max_groups + 1) * 4 <= S::LDS_BYTES, "the table fits the ring");
-            build_group_table(args.offsets, args.groups, args.M, BM, off, first);
-            const int total = __builtin_amdgcn_readfirstlane(first[args.groups]) * args.grid_n;
+            const bool batch = args.kind == product_kind::batch;
+            if(!batch)
+            {
+                build_group_table(args.offsets, args.groups, args.M, BM, off, first);
+            }
+            const int per_group = args.grid_m * args.grid_n;
+            const int total = batch ? args.groups * per_group : __builtin_amdgcn_readfirstlane(first[args.groups]) * args.grid_n;
             // (slices outermost over the grid's tiles, so that a tile's slices have one counter)
             const int most = gridDim.x / args.k_slices;
             slice          = blockIdx.x / most;
@@ -58,10 +62,19 @@ struct skinny_product
                 return; // (the grid covers the most tiles that this many rows can have)
             }
             const int item = xcd_remap(tile, total);
-            x.group        = group_of_tile(first, args.groups, item / args.grid_n);
-            const int f    = __builtin_amdgcn_readfirstlane(first[x.group]);
-            const int high = __builtin_amdgcn_readfirstlane(first[x.group + 1]) - f;
-            const int local = item - f * args.grid_n;
+            int       high = args.grid_m, local;
+            if(batch)
+            {
+                x.group = __builtin_amdgcn_readfirstlane(item / per_group);
+                local   = item - x.group * per_group;
+            }
+            else
+            {
+                x.group     = group_of_tile(first, args.groups, item / args.grid_n);
+                const int f = __builtin_amdgcn_readfirstlane(first[x.group]);
+                high        = __builtin_amdgcn_readfirstlane(first[x.group + 1]) - f;
+                local       = item - f * args.grid_n;
+            }
             tn              = local / high;
             tm              = local - tn * high;
             place_group(args, off, x);
@@ -198,24 +211,39 @@ struct skinny_product
         auto tile_sum = [&](int e) {
             return ((part[e] + part[BM * BN + e]) + part[2 * BM * BN + e]) + part[3 * BM * BN + e];
         };
-        auto finish = [&](int e, float sum) {
-            const int row = x.row0 + e / BN, col = x.col0 + e % BN;
-            if(row < x.m && col < args.N)
+        // Finishes the tile from sums that `sum_of` gives by element: 8 columns a thread where rows
+        // of C start on 16 bytes, else one.
+        auto finish = [&](auto sum_of) {
+            if(args.wide)
             {
-                finish_element<InT, OutT, OutT>(args, x, row, col, sum);
+                for(int piece = threadIdx.x; piece < BM * BN / 8; piece += THREADS)
+                {
+                    const int row = x.row0 + piece / (BN / 8), col = x.col0 + piece % (BN / 8) * 8;
+                    if(row < x.m && col < args.N)
+                    {
+                        float sum[8];
+#pragma unroll
+                        for(int e = 0; e < 8; ++e)
+                        {
+                            sum[e] = sum_of(piece * 8 + e);
+                        }
+                        finish_piece<InT, OutT, ResT>(args, x, row, col, sum);
+                    }
+                }
+                return;
+            }
+            for(int e = threadIdx.x; e < BM * BN; e += THREADS)
+            {
+                const int row = x.row0 + e / BN, col = x.col0 + e % BN;
+                if(row < x.m && col < args.N)
+                {
+                    finish_element<InT, OutT, ResT>(args, x, row, col, sum_of(e));
+                }
             }
         };
         if(args.k_slices == 1)
         {
-#pragma unroll 4
-            for(int m = 0; m < MINE; ++m)
-            {
-                const int e = threadIdx.x + m * THREADS;
-                if(e < BM * BN)
-                {
-                    finish(e, tile_sum(e));
-                }
-            }
+            finish(tile_sum);
             return;
         }
         // Parts travel at device scope, past the XCD's own L2; a workgroup counts itself in when its
@@ -252,8 +280,8 @@ struct skinny_product
         {
             return; // the last one to arrive finishes the tile
         }
-        for(int e = threadIdx.x; e < TILE; e += THREADS)
-        {
+        // (every slice's value of an element is on its way before the first is added)
+        finish([&](int e) {
             float v[MAX_SLICES];
 #pragma unroll
             for(int q = 0; q < MAX_SLICES; ++q)
@@ -268,8 +296,8 @@ struct skinny_product
             {
                 sum = q < args.k_slices ? sum + v[q] : sum;
             }
-            finish(e, sum);
-        }
+            return sum;
+        });
         if(threadIdx.x == 0)
         {
             // back to zero arrivals, for a replay of this launch (same epoch)

@@ -45,10 +45,8 @@ using epilogue_layer    = product_epilogue<true, false, true, false, false, fals
 using epilogue_logistic = product_epilogue<true, true, true, false, false, false, diagonal_use::none>;
 using epilogue_square   = product_epilogue<false, false, false, false, true, true, diagonal_use::none>;
 using epilogue_poly     = product_epilogue<false, false, true, false, true, true, diagonal_use::split>;
-using epilogue_next_rows = product_epilogue<false, false, true, true, true, false, diagonal_use::rows>;
-using epilogue_next_cols = product_epilogue<false, false, true, true, true, false, diagonal_use::cols>;
-using epilogue_last_rows = product_epilogue<false, false, true, false, true, false, diagonal_use::rows>;
-using epilogue_last_cols = product_epilogue<false, false, true, false, true, false, diagonal_use::cols>;
+using epilogue_next     = product_epilogue<false, false, true, true, true, false, diagonal_use::rows>;
+using epilogue_last     = product_epilogue<false, false, true, false, true, false, diagonal_use::rows>;
 
 // NARROW: rows of C, the residual, the second output or the bias do not start on 16 bytes: they go
 // element by element, a lane a column, so that a store instruction still writes runs of a row.
@@ -351,7 +349,7 @@ struct tiled_product
             = window(static_cast<const InT*>(args.bias) + w.x.group * args.stride_bias + col0,
                      EPI::layer && args.bias != nullptr);
         const __amdgpu_buffer_rsrc_t diagonal_from
-            = window(args.diagonal + w.x.group * args.stride_diagonal + (EPI::diagonal == diagonal_use::cols ? col0 : row0),
+            = window(args.diagonal + w.x.group * args.stride_diagonal + row0,
                      EPI::diagonal != diagonal_use::none);
 
         // this lane's pieces of a strip: row and column, place in the strip, offset in C in elements
@@ -378,7 +376,6 @@ struct tiled_product
         };
 
         float bias[PASSES][READS][EPI::layer ? PIECE : 1];
-        float by_col[PASSES][READS][EPI::diagonal == diagonal_use::cols ? PIECE : 1];
 #pragma unroll
         for(int p = 0; p < PASSES; ++p)
         {
@@ -405,21 +402,6 @@ struct tiled_product
                         {
                             const unsigned short b = (unsigned short)(v[e / 2] >> (16 * (e % 2)));
                             bias[p][q][4 * h + e]  = (float)__builtin_bit_cast(InT, b);
-                        }
-                    }
-                }
-                if constexpr(EPI::diagonal == diagonal_use::cols)
-                {
-                    const unsigned int from_at = col < cols ? (unsigned int)col * 4 : loop::STORE_RANGE;
-#pragma unroll
-                    for(int h = 0; h < PIECE / 4; ++h)
-                    {
-                        const f32x4 v = __builtin_bit_cast(
-                            f32x4, __builtin_amdgcn_raw_buffer_load_b128(diagonal_from, from_at + 16 * h, 0, 0));
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-                            by_col[p][q][4 * h + e] = args.beta + args.alpha * v[e];
                         }
                     }
                 }
@@ -535,10 +517,6 @@ struct tiled_product
                             if constexpr(EPI::diagonal == diagonal_use::rows)
                             {
                                 y[e] += (args.beta + args.alpha * by_row[block % AHEAD][q]) * r;
-                            }
-                            else if constexpr(EPI::diagonal == diagonal_use::cols)
-                            {
-                                y[e] += by_col[p][q][e] * r;
                             }
                             else
                             {

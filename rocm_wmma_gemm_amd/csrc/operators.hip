@@ -293,7 +293,8 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
         c.kernel = find_product(types, layout, form, finish);
         if(c.kernel.fn != nullptr)
         {
-            c.items      = tiles_of(args, c.kernel.block_m, c.kernel.block_n, symmetric, true);
+            // (the few-row kernel computes all of a symmetric product)
+            c.items      = tiles_of(args, c.kernel.block_m, c.kernel.block_n, symmetric && c.kernel.per_cu != 0, true);
             c.workgroups = c.kernel.per_cu == 0 ? c.items : std::min(c.items, c.kernel.per_cu * cus);
         }
         return c;
@@ -376,9 +377,10 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
         consider_tiled(narrow_cost);
     }
     // (the few-row kernel's offsets within a weight that is contiguous along N have 31 bits)
-    if(rows_kind && (layout == layout_kk || static_cast<long long>(args.K) * args.ldb < (1ll << 30)))
+    const bool batch = args.kind == product_kind::batch;
+    if((rows_kind || batch) && (layout == layout_kk || static_cast<long long>(args.K) * args.ldb < (1ll << 30)))
     {
-        const size_t rows = ceil_div(args.M, used);
+        const size_t rows = batch ? args.M : ceil_div(args.M, used);
         auto         consider = [&](const form_cost& f) {
             launch_choice c = made(f.form);
             if(c.kernel.fn == nullptr)
@@ -393,7 +395,7 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
             for(const size_t slices : {1, 2, 4})
             {
                 const launch_choice s = slices == 1 ? c : with_slices(c, slices);
-                if(slices > 1 && (s.k_slices == 1 || tiles * slices > slots))
+                if(slices > 1 && (batch || s.k_slices == 1 || tiles * slices > slots))
                 {
                     continue;
                 }
@@ -465,6 +467,7 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
     args.partials   = cuts ? reinterpret_cast<float*>(scratch) : nullptr;
     args.workgroups = static_cast<int>(c.workgroups);
     args.k_slices   = 1;
+    args.wide       = alignment_of(args).c;
     if(cuts && c.k_slices > 1)
     {
         args.arrivals = arrivals_of_current_device(false);
@@ -736,8 +739,8 @@ void by_element(int element, F&& f)
     }
 }
 
-// Newton-Schulz steps X <- a X + (b S + c S^2) X with S = X X^T (X^T X where X is tall, on the
-// other side), on X = G / (|G| + epsilon).
+// Newton-Schulz steps X <- a X + (b S + c S^2) X with S = X X^T on X = G / (|G| + epsilon), or on its
+// transpose where G is tall.
 //
 // What is rounded, and why: products take f16 operands.  Every singular value of X stays below
 // 1.3, so f16 holds X (scaled by about the root of its smaller side, a power of two, which
@@ -762,17 +765,15 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         auto run = [&](auto* typed) {
             using given_t = std::remove_pointer_t<decltype(typed)>;
             enqueue(f16 ? &device::orthogonal_small<given_t, _Float16> : &device::orthogonal_small<given_t, __bf16>,
-                    dim3(static_cast<unsigned>(batch)), dim3(256), stream, small);
+                    dim3(static_cast<unsigned>(batch)), dim3(1024), stream, small);
         };
         by_element(given_type, run);
         return ROCM_WMMA_GEMM_OK;
     }
     const bool   tall = M > N;
-    // (the rows of a tall X are only summed over and written: they need no padding)
-    const size_t mp = tall ? M : round_up8(M), np = round_up8(N), lp = tall ? np : mp;
-    const size_t each = mp * np, square = lp * lp;
-    // (whole pieces of 16 bytes a row: the last product writes the update itself)
-    const bool   direct  = mp == M && np == N && aligned16(O);
+    const size_t l = std::min(M, N), h = std::max(M, N), lp = round_up8(l), hp = round_up8(h);
+    const size_t each = lp * hp, square = lp * lp;
+    const bool   direct  = !tall && lp == l && hp == h && aligned16(O);
     const size_t parts_b = whole_lines(batch * device::square_parts * sizeof(float)),
                  diag_b = whole_lines(batch * lp * sizeof(float)), x32_b = whole_lines(batch * each * 4),
                  x16_b = whole_lines(batch * each * 2), sq_b = whole_lines(batch * square * 2);
@@ -793,7 +794,8 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
     _Float16* x16[2] = {reinterpret_cast<_Float16*>(rest), reinterpret_cast<_Float16*>(rest + x16_b)};
     char*     s = rest + 2 * x16_b;
     char*     q = s + sq_b;
-    const float scale = std::exp2(std::round(std::log2(std::sqrt(static_cast<float>(std::min(M, N))))));
+    const float scale = std::exp2(std::round(std::log2(std::sqrt(static_cast<float>(l)))));
+    const unsigned nb = static_cast<unsigned>(batch);
 
     auto start = [&](auto* typed) {
         using given_t = std::remove_pointer_t<decltype(typed)>;
@@ -804,14 +806,19 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         const size_t used = std::max<size_t>(
             1, std::min({ceil_div(M * N / (vector ? wide : 1), 4096), size_t{device::square_parts}, ceil_div(2048, batch)}));
         enqueue(vector ? &device::sum_squares<given_t, wide> : &device::sum_squares<given_t, 1>,
-                dim3(static_cast<unsigned>(used), static_cast<unsigned>(batch)), dim3(256), stream, given,
-                static_cast<long long>(M * N), parts);
-        const bool   whole = mp == M && np == N && aligned16(given);
-        const size_t row_groups = std::min<size_t>(mp, std::max<size_t>(1, 2048 / batch));
-        enqueue(whole ? &device::orthogonal_start<given_t, true> : &device::orthogonal_start<given_t, false>,
-                dim3(static_cast<unsigned>(row_groups), static_cast<unsigned>(batch)), dim3(256), stream, given,
-                parts, x32, x16[0], static_cast<int>(M), static_cast<int>(N), static_cast<int>(mp), static_cast<int>(np),
-                scale, epsilon, static_cast<int>(used));
+                dim3(static_cast<unsigned>(used), nb), dim3(256), stream, given, static_cast<long long>(M * N), parts);
+        const device::start_args args{given, parts, x32, x16[0], static_cast<int>(M), static_cast<int>(N),
+                                      static_cast<int>(lp), static_cast<int>(hp), scale, epsilon, static_cast<int>(used)};
+        if(tall)
+        {
+            enqueue(&device::orthogonal_start_tall<given_t>,
+                    dim3(static_cast<unsigned>(ceil_div(lp, 64) * ceil_div(hp, 64)), nb), dim3(256), stream, args);
+            return;
+        }
+        enqueue(lp == l && hp == h && aligned16(given) ? &device::orthogonal_start<given_t, true>
+                                                       : &device::orthogonal_start<given_t, false>,
+                dim3(static_cast<unsigned>(std::min<size_t>(lp, std::max<size_t>(1, 2048 / batch))), nb), dim3(256), stream,
+                args);
     };
     by_element(given_type, start);
     const float a = coefficients[0], b = coefficients[1], c = coefficients[2];
@@ -830,16 +837,16 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         const bool last = step + 1 == steps;
         // S = X X^T / scale^2
         p.C = s, p.A = x, p.B = x, p.residual = nullptr, p.kept = nullptr;
-        p.M = p.N = static_cast<int>(lp), p.K = static_cast<int>(tall ? mp : np);
-        p.lda = p.ldb = np, p.ldc = lp;
+        p.M = p.N = static_cast<int>(lp), p.K = static_cast<int>(hp);
+        p.lda = p.ldb = hp, p.ldc = lp;
         p.stride_a = p.stride_b = each, p.stride_c = square;
         p.alpha = 1.0f / (scale * scale), p.beta = 0.0f, p.diagonal_is = device::diagonal_use::none;
-        rc = product(types_steps_square, tall ? layout_mn : layout_kk, finish_square, p);
+        rc = product(types_steps_square, layout_kk, finish_square, p);
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             break;
         }
-        // Q = b S + c S^2 (S is its own transpose)
+        // Q = b S + c S^2 (S is its own transpose), its diagonal apart
         p.C = q, p.A = p.B = s, p.residual = s;
         p.K = static_cast<int>(lp), p.lda = p.ldb = lp, p.stride_a = p.stride_b = square;
         p.alpha = c, p.beta = b, p.diagonal_is = device::diagonal_use::split;
@@ -848,29 +855,27 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         {
             break;
         }
-        // X = (a + diagonal) X + Q X (tall: X (a + diagonal) + X Q, Q its own transpose)
-        p.A = tall ? static_cast<void*>(x) : q, p.B = tall ? q : static_cast<char*>(static_cast<void*>(x));
-        p.M = static_cast<int>(mp), p.N = static_cast<int>(np), p.K = static_cast<int>(lp);
-        p.lda = tall ? np : lp, p.ldb = tall ? lp : np, p.ldc = np;
-        p.stride_a = tall ? each : square, p.stride_b = tall ? square : each, p.stride_c = each;
+        // X = (a + diagonal) X + Q X
+        p.A = q, p.B = x;
+        p.M = static_cast<int>(lp), p.N = static_cast<int>(hp), p.K = static_cast<int>(lp);
+        p.lda = lp, p.ldb = hp, p.ldc = hp;
+        p.stride_a = square, p.stride_b = each, p.stride_c = each;
         p.residual = x32, p.alpha = last ? 1.0f / scale : 1.0f, p.beta = last ? a / scale : a;
-        p.diagonal_is = tall ? device::diagonal_use::cols : device::diagonal_use::rows;
+        p.diagonal_is = device::diagonal_use::rows;
         p.C = last ? (direct ? O : static_cast<void*>(x16[(step + 1) & 1])) : x32;
         p.kept = last ? nullptr : x16[(step + 1) & 1], p.keep_sum = 1;
-        rc = product(!last ? types_steps_next
-                            : out_type == ROCM_WMMA_GEMM_ELEMENT_F16 ? types_steps_f16 : types_steps_bf16,
-                            tall ? layout_kk : layout_kn,
-                            last ? (tall ? finish_last_cols : finish_last_rows) : tall ? finish_next_cols : finish_next_rows,
-                     p);
+        rc = product(!last ? types_steps_next : out_type == ROCM_WMMA_GEMM_ELEMENT_F16 ? types_steps_f16 : types_steps_bf16,
+                     layout_kn, last ? finish_last : finish_next, p);
         p.keep_sum = 0;
     }
     if(rc == ROCM_WMMA_GEMM_OK && !direct)
     {
         // (a 16-bit element is a 16-bit element)
-        enqueue(&device::orthogonal_end<unsigned short>,
-                dim3(static_cast<unsigned>(std::min<size_t>(M, 4096)), static_cast<unsigned>(batch)),
-                dim3(256), stream, reinterpret_cast<const unsigned short*>(x16[steps & 1]), static_cast<unsigned short*>(O),
-                static_cast<int>(M), static_cast<int>(N), static_cast<int>(mp), static_cast<int>(np));
+        const unsigned short* padded = reinterpret_cast<const unsigned short*>(x16[steps & 1]);
+        enqueue(tall ? &device::orthogonal_end_tall<unsigned short> : &device::orthogonal_end<unsigned short>,
+                dim3(static_cast<unsigned>(tall ? ceil_div(M, 64) * ceil_div(N, 64) : std::min<size_t>(M, 4096)), nb), dim3(256),
+                stream, padded, static_cast<unsigned short*>(O), static_cast<int>(M), static_cast<int>(N),
+                static_cast<int>(lp), static_cast<int>(hp));
     }
     return rc;
 }

@@ -65,38 +65,19 @@ product_kernel tiled_finish(int finish)
             default: return kNone;
         }
     }
-    else if constexpr(kTypes == types_steps_square)
+    else if constexpr(kTypes == types_steps_square && LAYOUT == layout_kk)
     {
-        if constexpr(LAYOUT != layout_kn)
+        switch(finish)
         {
-            if(finish == finish_square)
-            {
-                return tiled<LAYOUT, BM, BN, device::epilogue_square>();
-            }
+            case finish_square: return tiled<LAYOUT, BM, BN, device::epilogue_square>();
+            case finish_poly: return tiled<LAYOUT, BM, BN, device::epilogue_poly>();
+            default: return kNone;
         }
-        if constexpr(LAYOUT == layout_kk)
-        {
-            if(finish == finish_poly)
-            {
-                return tiled<LAYOUT, BM, BN, device::epilogue_poly>();
-            }
-        }
-        return kNone;
     }
-    else if constexpr(LAYOUT != layout_mn)
+    else if constexpr(kTypes != types_steps_square && LAYOUT == layout_kn)
     {
-        // Q X: rows of the residual meet the diagonal; X Q: columns
-        constexpr bool ROWS = LAYOUT == layout_kn;
-        if constexpr(kTypes == types_steps_next)
-        {
-            using epi = std::conditional_t<ROWS, device::epilogue_next_rows, device::epilogue_next_cols>;
-            return finish == (ROWS ? finish_next_rows : finish_next_cols) ? tiled<LAYOUT, BM, BN, epi>() : kNone;
-        }
-        else
-        {
-            using epi = std::conditional_t<ROWS, device::epilogue_last_rows, device::epilogue_last_cols>;
-            return finish == (ROWS ? finish_last_rows : finish_last_cols) ? tiled<LAYOUT, BM, BN, epi>() : kNone;
-        }
+        using epi = std::conditional_t<kTypes == types_steps_next, device::epilogue_next, device::epilogue_last>;
+        return tiled<LAYOUT, BM, BN, epi>();
     }
     else
     {
@@ -126,11 +107,15 @@ product_kernel narrow(int finish)
 template<int LAYOUT, int BM, int BN>
 product_kernel skinny()
 {
+    if constexpr(kSteps && LAYOUT == (kTypes == types_steps_square ? layout_kk : layout_kn) && BM >= 32 && BN >= 32)
+    {
+        return made<device::skinny_product<kIn, out_t, res_t, BM, BN, LAYOUT == layout_kk, false>>(BM, BN, 0);
+    }
     constexpr bool built = (BN == 64 && BM < 64) ? LAYOUT == layout_kn : BN == 16 ? LAYOUT == layout_kk : true;
     if constexpr(!kSteps && LAYOUT != layout_mn && built)
     {
-        using impl       = device::skinny_product<kIn, out_t, BM, BN, LAYOUT == layout_kk, false>;
-        using once       = device::skinny_product<kIn, out_t, BM, BN, LAYOUT == layout_kk, true>;
+        using impl       = device::skinny_product<kIn, out_t, res_t, BM, BN, LAYOUT == layout_kk, false>;
+        using once       = device::skinny_product<kIn, out_t, res_t, BM, BN, LAYOUT == layout_kk, true>;
         product_kernel k = made<impl>(BM, BN, 0);
         k.once           = &device::product_entry<once>;
         return k;
@@ -169,7 +154,7 @@ product_kernel in_layout(int form, int finish)
         case form_tiled_256: return tiled_finish<LAYOUT, 256, 256>(finish);
         case form_tiled_128: return tiled_finish<LAYOUT, 128, 128>(finish);
         case form_tiled_128x256:
-            if constexpr(!kSteps)
+            if constexpr(kTypes != types_steps_square) // (a mirrored tile is square)
             {
                 return tiled_finish<LAYOUT, 128, 256>(finish);
             }

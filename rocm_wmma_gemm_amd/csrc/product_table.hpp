@@ -66,10 +66,8 @@ enum product_finish
     finish_logistic, // the same with silu or gelu
     finish_square, // symmetric
     finish_poly, // symmetric, with a residual and the diagonal held apart
-    finish_next_rows, // + diagonal times residual, kept in A's type as well
-    finish_next_cols,
-    finish_last_rows, // the same without
-    finish_last_cols,
+    finish_next, // + diagonal times residual, by rows; kept in A's type as well
+    finish_last, // the same, not kept
     num_product_finishes
 };
 

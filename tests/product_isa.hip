@@ -16,11 +16,11 @@ CHECKED(bf16, __bf16, __bf16, true, true, 128, epilogue_logistic)
 CHECKED(f16, float, float, true, false, 128, epilogue_logistic)
 CHECKED(f16, _Float16, _Float16, false, false, 128, epilogue_add)
 CHECKED(f16, _Float16, _Float16, true, true, 256, epilogue_poly)
-CHECKED(f16, _Float16, _Float16, false, false, 256, epilogue_square)
+CHECKED(f16, _Float16, _Float16, true, true, 256, epilogue_square)
 CHECKED(f16, _Float16, _Float16, true, true, 128, epilogue_poly)
-CHECKED(f16, float, float, true, false, 256, epilogue_next_rows)
-CHECKED(f16, float, float, true, true, 128, epilogue_next_cols)
-CHECKED(f16, __bf16, float, true, true, 256, epilogue_last_cols)
+CHECKED(f16, float, float, true, false, 256, epilogue_next)
+CHECKED(f16, float, float, true, false, 128, epilogue_next)
+CHECKED(f16, __bf16, float, true, false, 256, epilogue_last)
 SHAPED(bf16, __bf16, __bf16, true, true, 128, 256, epilogue_logistic)
 CHECKED(f16, _Float16, _Float16, true, true, 192, epilogue_poly)
 // rows of C that do not start on 16 bytes
