@@ -193,6 +193,70 @@ __device__ __forceinline__ void order_groups(int groups, IntPtr off, IntPtr orde
     __syncthreads();
 }
 
+// Where a group's tiles fit the grid several times, the workgroups form that many teams of `tiles`, and a
+// team takes whole groups: each group, in order_groups' order, goes to the team with the least to do
+// so far.  A group costs its K tiles and what a tile's start and end take, about 5 more.
+constexpr int most_teamed_groups = 64, most_teams = 64, tile_overhead = 5;
+
+RWG_HD inline int teams_of(int groups, int tiles, int workgroups)
+{
+    const int teams = workgroups / tiles;
+    // (left-over workgroups stay idle: not more than one in eight)
+    return groups <= most_teamed_groups && groups > teams && teams >= 2 && teams <= most_teams && teams * tiles * 8 >= workgroups * 7 ? teams
+                                                                                                                  : 0;
+}
+
+// The least of a wave's 64 values, in every lane: four shifts within rows of 16 lanes, two broadcasts
+// across them (a few cycles each, where a shuffle through LDS takes sixty).
+__device__ __forceinline__ int least_of_wave(int v)
+{
+    constexpr int most = 0x7fffffff;
+    auto          least = [](int a, int b) { return a < b ? a : b; };
+    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x111, 0xf, 0xf, false)); // row_shr:1
+    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x112, 0xf, 0xf, false));
+    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x114, 0xf, 0xf, false));
+    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x118, 0xf, 0xf, false));
+    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x142, 0xa, 0xf, false)); // row_bcast:15
+    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x143, 0xc, 0xf, false)); // row_bcast:31
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The groups of team `team`, into mine[0 ..]; returns how many.  Called by all threads of a workgroup;
+// ready behind its barrier.
+template<class IntPtr>
+__device__ __forceinline__ int deal_groups(int groups, int teams, int team, int BK, IntPtr off, IntPtr order, IntPtr mine,
+                                           IntPtr count)
+{
+    if(threadIdx.x < 64)
+    {
+        const int lane  = threadIdx.x;
+        const int group = order[lane < groups ? lane : 0]; // the lane-th in order, and its cost
+        const int cost  = (off[group + 1] - off[group] + BK - 1) / BK + tile_overhead;
+        int       load = lane < teams ? 0 : 1 << 24, taken = 0;
+        for(int i = 0; i < groups; ++i)
+        {
+            // the least load, of those the first team
+            const int to = least_of_wave(load * 64 + lane) & 63;
+            load += lane == to ? __builtin_amdgcn_readlane(cost, i) : 0;
+            if(to == team)
+            {
+                const int e = __builtin_amdgcn_readlane(group, i);
+                if(lane == 0)
+                {
+                    mine[taken] = e;
+                }
+                ++taken;
+            }
+        }
+        if(lane == 0)
+        {
+            *count = taken;
+        }
+    }
+    __syncthreads();
+    return *count;
+}
+
 // The group that row tile number `tile` belongs to: the last e with first[e] <= tile (groups
 // without rows share their successor's number and are passed over).  Asked by whole waves, 64
 // groups at a time.

@@ -63,7 +63,7 @@ struct tiled_product
     // a wave's strip: 16 rows of a part of the columns of its tile in fp32, 16 bytes of padding a row
     static constexpr int PASSES = RING == 3 ? 4 : 2;
     static constexpr int HALF = TN / PASSES, ROW_BYTES = HALF * 64, PITCH = ROW_BYTES + 16, STRIP = 16 * PITCH;
-    static constexpr int TABLE = 3 * (max_groups + 1) * 4;
+    static constexpr int TABLE = (3 * (max_groups + 1) + most_teamed_groups + 1) * 4;
     static constexpr int LDS_BYTES = RING_BYTES + 4 * STRIP + TABLE;
     // workgroups per compute unit: what the LDS holds
     static constexpr int PER_CU = LDS_BYTES <= 80 * 1024 ? 2 : 1;
@@ -89,6 +89,8 @@ struct tiled_product
     {
         const lds_int *off, *first, *order;
         tail_cut       cut;
+        int            teams; // groups go to teams of workgroups (order then lists this team's); 0: tiles are dealt one by one
+        int            positions, begin, hop; // of this workgroup: begin, begin + hop, ... < positions
     };
 
     __device__ __forceinline__ static int tiles_per_group(const product_args& args)
@@ -111,6 +113,16 @@ struct tiled_product
             else if(args.groups > 1)
             {
                 order_groups(args.groups, off, order);
+                const int each = tiles_per_group(args), teams = teams_of(args.groups, each, workgroups);
+                if(teams != 0)
+                {
+                    lds_int*  mine = order + max_groups + 1;
+                    const int team = (int)blockIdx.x / each;
+                    // (a workgroup beyond the last team has no group)
+                    const int n = deal_groups(args.groups, teams, team, BK, off, order, mine, mine + most_teamed_groups);
+                    return {off, first, mine, {tiles, 0, 1, 1}, teams,
+                            __builtin_amdgcn_readfirstlane(team < teams ? n : 0), 0, 1};
+                }
             }
         }
         // (where groups differ in K the slices would too: those launches are not cut)
@@ -120,7 +132,7 @@ struct tiled_product
         cut.cut            = __builtin_amdgcn_readfirstlane(cut.cut);
         cut.slices         = __builtin_amdgcn_readfirstlane(cut.slices);
         cut.each           = __builtin_amdgcn_readfirstlane(cut.each);
-        return {off, first, order, cut};
+        return {off, first, order, cut, 0, cut.positions(), (int)blockIdx.x, workgroups};
     }
 
     // Tile number `tile` of the launch: its group and place.
@@ -140,7 +152,13 @@ struct tiled_product
             const int tiles = tiles_per_group(args);
             x.group         = tile / tiles;
             local           = tile - x.group * tiles;
-            if(args.kind == product_kind::sum && args.groups > 1)
+            if(pl.teams != 0)
+            {
+                // position `tile` of the team's list; the workgroup's place in the team is its tile
+                x.group = pl.order[tile];
+                local   = xcd_remap((int)blockIdx.x % tiles, tiles);
+            }
+            else if(args.kind == product_kind::sum && args.groups > 1)
             {
                 // (one group after the other over the whole GPU, an XCD on neighbouring tiles)
                 x.group = pl.order[x.group];
@@ -605,7 +623,7 @@ struct tiled_product
     static constexpr int FINISH_ROWS = THREADS * 8 / BN, FINISH_PARTS = BM / FINISH_ROWS;
     __device__ __forceinline__ static void finish_cut(const product_args& args)
     {
-        __shared__ int table_raw[3 * (max_groups + 1)];
+        __shared__ int table_raw[TABLE / 4];
         lds_int*       table = (lds_int*)table_raw;
         const plan     pl = make_plan(args, table, args.workgroups);
         const int      parts = pl.cut.cut * FINISH_PARTS;
@@ -656,8 +674,8 @@ struct tiled_product
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wave_m = wave / 2, wave_n = wave % 2;
         const plan pl = make_plan(args, reinterpret_cast<lds_int*>(lds + RING_BYTES + 4 * STRIP), (int)gridDim.x);
-        const int  total = pl.cut.positions(), hop = (int)gridDim.x;
-        int        pos = (int)blockIdx.x;
+        const int  total = pl.positions, hop = pl.hop;
+        int        pos = pl.begin;
         if(pos >= total)
         {
             return;
@@ -692,7 +710,7 @@ struct tiled_product
             if(--stream_left == 0)
             {
                 // (past its last item the stream starts over: the loads go where nobody reads)
-                const work nx = decode(args, pl, stream_pos < total ? stream_pos : (int)blockIdx.x);
+                const work nx = decode(args, pl, stream_pos < total ? stream_pos : pl.begin);
                 a_src         = nx.a;
                 b_src         = nx.b;
                 a_end         = nx.a_end;
