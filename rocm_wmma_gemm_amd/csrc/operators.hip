@@ -461,6 +461,12 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
         args = on;
         scratch += c.copy_bytes;
     }
+    if(args.offsets == nullptr && args.kind != product_kind::batch)
+    {
+        // (one group of all rows: nothing to look up, 1 us less of a small call)
+        args.kind     = product_kind::batch;
+        args.stride_a = args.stride_b = args.stride_c = 0;
+    }
     const bool cuts = c.partial_bytes != 0 && scratch != nullptr;
     args.grid_m     = static_cast<int>(ceil_div(args.M, c.kernel.block_m));
     args.grid_n     = static_cast<int>(ceil_div(args.N, c.kernel.block_n));
