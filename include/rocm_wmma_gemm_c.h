@@ -217,7 +217,7 @@ int rocm_wmma_gemm_noalloc(int type_idx, void* C, void* A, void* B, size_t M, si
  * stored N x K).  type_idx names the types of C and of A and B as above; bias has A's type,
  * residual and dbias C's, preact (the sum before the activation, M x N) A's, as dC.  Everything is added up
  * and activated in fp32, each output rounded once.  `stream` is the address of a hipStream_t;
- * the calls enqueue and return.  M, N, K below 2^31; a size of 0 leaves the sums empty.
+ * the calls enqueue and return.  M, N, K up to 2^31 - 256; a size of 0 leaves the sums empty.
  * --------------------------------------------------------------------------------------- */
 #define ROCM_WMMA_GEMM_ACT_NONE 0
 #define ROCM_WMMA_GEMM_ACT_RELU 1

@@ -208,17 +208,17 @@ RWG_HD inline int teams_of(int groups, int tiles, int workgroups)
 
 // The least of a wave's 64 values, in every lane: four shifts within rows of 16 lanes, two broadcasts
 // across them (a few cycles each, where a shuffle through LDS takes sixty).
-__device__ __forceinline__ int least_of_wave(int v)
+__device__ __forceinline__ unsigned int least_of_wave(unsigned int v)
 {
-    constexpr int most = 0x7fffffff;
-    auto          least = [](int a, int b) { return a < b ? a : b; };
-    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x111, 0xf, 0xf, false)); // row_shr:1
-    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x112, 0xf, 0xf, false));
-    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x114, 0xf, 0xf, false));
-    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x118, 0xf, 0xf, false));
-    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x142, 0xa, 0xf, false)); // row_bcast:15
-    v = least(v, __builtin_amdgcn_update_dpp(most, v, 0x143, 0xc, 0xf, false)); // row_bcast:31
-    return __builtin_amdgcn_readlane(v, 63);
+    constexpr int most = -1; // (all ones: no lane's value is more)
+    auto least = [&](int other) { v = v < (unsigned int)other ? v : (unsigned int)other; };
+    least(__builtin_amdgcn_update_dpp(most, (int)v, 0x111, 0xf, 0xf, false)); // row_shr:1
+    least(__builtin_amdgcn_update_dpp(most, (int)v, 0x112, 0xf, 0xf, false));
+    least(__builtin_amdgcn_update_dpp(most, (int)v, 0x114, 0xf, 0xf, false));
+    least(__builtin_amdgcn_update_dpp(most, (int)v, 0x118, 0xf, 0xf, false));
+    least(__builtin_amdgcn_update_dpp(most, (int)v, 0x142, 0xa, 0xf, false)); // row_bcast:15
+    least(__builtin_amdgcn_update_dpp(most, (int)v, 0x143, 0xc, 0xf, false)); // row_bcast:31
+    return (unsigned int)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // The groups of team `team`, into mine[0 ..]; returns how many.  Called by all threads of a workgroup;
@@ -232,11 +232,11 @@ __device__ __forceinline__ int deal_groups(int groups, int teams, int team, int 
         const int lane  = threadIdx.x;
         const int group = order[lane < groups ? lane : 0]; // the lane-th in order, and its cost
         const int cost  = (off[group + 1] - off[group] + BK - 1) / BK + tile_overhead;
-        int       load = lane < teams ? 0 : 1 << 24, taken = 0;
+        int       load = 0, taken = 0;
         for(int i = 0; i < groups; ++i)
         {
-            // the least load, of those the first team
-            const int to = least_of_wave(load * 64 + lane) & 63;
+            // the least load, of those the first team (all K tiles of 2^31 rows, times 64, fit 32 bits unsigned)
+            const int to = (int)(least_of_wave(lane < teams ? (unsigned int)load * 64 + lane : ~0u) & 63u);
             load += lane == to ? __builtin_amdgcn_readlane(cost, i) : 0;
             if(to == team)
             {

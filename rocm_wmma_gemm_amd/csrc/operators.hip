@@ -54,7 +54,8 @@ using device::act_kind;
 using device::product_args;
 using device::product_kind;
 
-constexpr size_t most_extent = 0x7fffffff;
+// (an extent rounded up to any tile still fits an int)
+constexpr size_t most_extent = 0x7fffff00;
 
 constexpr size_t ceil_div(size_t a, size_t b)
 {

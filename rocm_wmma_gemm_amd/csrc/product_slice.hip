@@ -35,7 +35,7 @@ product_kernel tiled()
     constexpr bool AK = LAYOUT != layout_mn, BK = LAYOUT == layout_kk;
     using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, BM, BN, EPI, NARROW>;
     product_fn finish = nullptr;
-    if constexpr(!EPI::mirror)
+    if constexpr(!kSteps) // (the steps' products are not cut: their scratch memory holds matrices)
     {
         finish = &device::tiled_finish_entry<impl>;
     }

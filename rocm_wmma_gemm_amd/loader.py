@@ -387,9 +387,13 @@ class Loader:
 
     @staticmethod
     def _device_of(name, t):
+        import torch
+
         device = t.get_device()
         if device < 0:
             raise ValueError(f"{name} must be a device tensor")
+        if device != torch.cuda.current_device():  # (whose scratch buffer and streams the library uses)
+            raise ValueError(f"{name} is on device {device}, the current one is {torch.cuda.current_device()}")
         return device
 
     @staticmethod

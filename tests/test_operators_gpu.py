@@ -713,3 +713,14 @@ def test_the_example_runs():
     assert done.returncode == 0, done.stdout + done.stderr
     before, after = (float(x) for x in done.stdout.split("mean square of the output: ")[1].split("\n")[0].split(" -> "))
     assert after < before
+
+
+def test_operands_on_another_device_than_the_current_one(loader, monkeypatch):
+    A, B, C = (torch.zeros(s, dtype=BF16, device="cuda") for s in ((4, 8), (16, 8), (4, 16)))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(ValueError, match="the current one is 1"):
+        loader.linear(C, A, B, 4, 16, 8)
+    with pytest.raises(ValueError, match="the current one is 1"):
+        loader.linear_backward(torch.zeros_like(A), None, None, C, A, B, 4, 16, 8)
+    with pytest.raises(ValueError, match="the current one is 1"):
+        loader.orthogonalize(C, C, 4, 16)

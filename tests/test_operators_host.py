@@ -80,6 +80,7 @@ def test_entry_points_refuse_before_they_touch_the_device(library):
     assert linear(0, one, one, one, 8, 8, 8, 2, None) == ERR_ARGUMENT  # layout
     assert linear(0, one, one, one, 8, 8, 8, 1, epilogue(4)) == ERR_ARGUMENT  # activation
     assert linear(0, one, one, one, 1 << 31, 8, 8, 1, None) == ERR_LIMIT
+    assert linear(0, one, one, one, 8, 8, (1 << 31) - 255, 1, None) == ERR_LIMIT  # (its tiles' end leaves an int)
     assert linear(0, None, one, one, 8, 8, 8, 1, None) == ERR_ARGUMENT
     assert linear(0, one, one, None, 8, 8, 8, 1, None) == ERR_ARGUMENT
     assert linear(0, None, None, None, 0, 8, 8, 1, None) == OK  # nothing to do
