@@ -3,7 +3,9 @@
 //
 // C tile of 128 x 128 (64 x 64 for small problems) per workgroup, 4 waves, 32x32x16 MFMA, two
 // stages of BK in LDS.  It serves what the direct-to-LDS kernels cannot: rows that do not start
-// on 16 bytes.  Bound by the 2-byte gathers of operands that are contiguous along M or N.
+// on 16 bytes.  Bound by the 2-byte gathers of operands that are contiguous along M or N:
+// 1999 x 1001 x 999 takes 115 us here and 32 on padded copies, so it is left with what is too
+// small for copies to pay and with calls that get no scratch memory.
 #ifndef ROCM_WMMA_GEMM_GENERAL_PRODUCT_HPP
 #define ROCM_WMMA_GEMM_GENERAL_PRODUCT_HPP
 

@@ -11,7 +11,9 @@ namespace rocm_wmma_gemm
 namespace device
 {
 
-// dZ = dC * act'(Z), and the sums of its columns over runs of slope_rows rows of a group.
+// dZ = dC * act'(Z), and the sums of its columns over runs of slope_rows rows of a group.  4096 x 5120
+// bf16: 29 us, 4.35 TB/s; 8192 x 4096 in 16 groups 52 us, 3.9 TB/s.  Runs of 16 or 64 rows and non-temporal
+// loads change a backward pass by less than 2 %, up for some sizes and down for others.
 constexpr int slope_rows = 32; // rows of a run (a workgroup's); a group's last run is shorter
 
 struct slope_args
@@ -356,7 +358,8 @@ __global__ void __launch_bounds__(256) orthogonal_end_tall(const OutT* __restric
 // fp32 on the matrix cores (v_mfma_f32_16x16x4_f32), from LDS: X with the smaller side as its rows, and S,
 // then Q, in one buffer; rows and columns past the matrix are zeros throughout.  One launch instead of
 // seventeen, and nothing is rounded to f16: in a small matrix few roundings average out (8 x 8 with
-// one strong direction: 4.8e-3 off by the f16 products, 1e-6 here).  Wave w of sixteen owns tile
+// one strong direction: 4.8e-3 off by the f16 products, 1e-6 here).  Five steps of 64 x 64 take 29 us,
+// of 64 x 256 63 us (16 of them; 512 136).  Wave w of sixteen owns tile
 // (w / 4, w mod 4) of S and Q, and of X the tiles (w mod 4, w / 4 + 4 i).  Pitches of 4 mod 64 floats spread the
 // 16 rows x 4 columns that a fragment read touches over all 64 banks.  Bound by the latency of LDS
 // and the matrix cores' fp32 rate; past 256 columns the seventeen launches are as fast.
@@ -378,7 +381,8 @@ __global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
     __shared__ float x[small_side * XP];
     __shared__ float s[small_side * SP];
     __shared__ float wave_sum[16];
-    const int       tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, k4 = lane >> 4;
+    const int       tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, k4 = lane >> 4;
+    const int       wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool      tall = args.rows > args.cols;
     const int       l = tall ? args.cols : args.rows, h = tall ? args.rows : args.cols;
     const int       l16 = (l + 15) / 16 * 16, h16 = (h + 15) / 16 * 16;
@@ -430,11 +434,14 @@ __global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
         f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
         if(used)
         {
-#pragma unroll 4
-            for(int k = 0; k < h16; k += 4)
+            for(int k0 = 0; k0 < h16; k0 += 16)
             {
-                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[(ti * 16 + r16) * XP + k + k4], x[(tj * 16 + r16) * XP + k + k4],
-                                                           acc, 0, 0, 0);
+#pragma unroll
+                for(int k = k0; k < k0 + 16; k += 4)
+                {
+                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[(ti * 16 + r16) * XP + k + k4],
+                                                               x[(tj * 16 + r16) * XP + k + k4], acc, 0, 0, 0);
+                }
             }
         }
 #pragma unroll
@@ -447,11 +454,14 @@ __global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
         f32x4 q{0.0f, 0.0f, 0.0f, 0.0f};
         if(used)
         {
-#pragma unroll 4
-            for(int k = 0; k < l16; k += 4)
+            for(int k0 = 0; k0 < l16; k0 += 16)
             {
-                q = __builtin_amdgcn_mfma_f32_16x16x4f32(s[(ti * 16 + r16) * SP + k + k4], s[(tj * 16 + r16) * SP + k + k4], q,
-                                                         0, 0, 0);
+#pragma unroll
+                for(int k = k0; k < k0 + 16; k += 4)
+                {
+                    q = __builtin_amdgcn_mfma_f32_16x16x4f32(s[(ti * 16 + r16) * SP + k + k4],
+                                                             s[(tj * 16 + r16) * SP + k + k4], q, 0, 0, 0);
+                }
             }
         }
         __syncthreads();
@@ -471,14 +481,27 @@ __global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
         const int rows = tj * 16;
         if(rows < l16)
         {
-#pragma unroll 2
-            for(int k = 0; k < l16; k += 4)
+            for(int k0 = 0; k0 < l16; k0 += 16)
             {
-                const float u = s[(rows + r16) * SP + k + k4];
+                float u[4];
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                {
+                    u[k] = s[(rows + r16) * SP + k0 + 4 * k + k4];
+                }
 #pragma unroll
                 for(int i = 0; i < COLS; ++i)
                 {
-                    y[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u, x[(k + k4) * XP + (ti + 4 * i) * 16 + r16], y[i], 0, 0, 0);
+                    const int cols = (ti + 4 * i) * 16;
+                    if(cols < h16)
+                    {
+#pragma unroll
+                        for(int k = 0; k < 4; ++k)
+                        {
+                            y[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[k], x[(k0 + 4 * k + k4) * XP + cols + r16], y[i], 0,
+                                                                        0, 0);
+                        }
+                    }
                 }
             }
         }

@@ -3,8 +3,9 @@
 //
 // A workgroup owns BM rows x BN columns of a group's C and the whole sum: it streams its BN rows
 // of the weight from memory exactly once, BM rows of A come out of L2.  Bound by the weights'
-// bytes; experts without rows have no tiles, so their weights are never read.  Ring, swizzles and
-// waits are the streaming kernel's; the four waves split K and their partial tiles meet in LDS,
+// bytes: 16 rows on 14 of 64 weights of 2048 x 4096 take 41 us, 5.75 TB/s; 32 x 4096 x 14336 on 32 x 16 tiles
+// 29.4 us, 4.0 TB/s (16 x 32 tiles 33.8, two slices of K 39).  Experts without rows have no tiles, so their
+// weights are never read.  Ring, swizzles and waits are the streaming kernel's; the four waves split K and their partial tiles meet in LDS,
 // where bias, activation and residual join them.  The row tiles that share a slice of a weight are
 // neighbours on one XCD.
 //
