@@ -258,6 +258,16 @@ constexpr form_cost skinny_costs_kn[] = {
     {form_skinny_32x32, 3.5f, 0.16f, 0.24f, 3.0e6f}, {form_skinny_32x64, 4.0f, 0.19f, 0.30f, 4.2e6f},
     {form_skinny_64x32, 4.0f, 0.21f, 0.34f, 2.8e6f}, {form_skinny_64x64, 4.5f, 0.25f, 0.28f, 4.0e6f},
 };
+// What the end of a tile of a Newton-Schulz step takes beyond a layer's, in us per 128 x 128 elements: it is
+// written twice, or reads and writes fp32.  (Against none over 19 sizes from 192 x 3328 to 4096 x 4096: 0.98 of
+// their time, 11 x 320 x 768 206 -> 178 us, 1336 x 1064 313 -> 268, none slower by more than 1 %.)
+constexpr float steps_finish_us(int finish)
+{
+    return finish == finish_square                              ? 2.5f
+           : finish == finish_poly                              ? 5.0f
+           : finish == finish_next || finish == finish_last ? 3.0f
+                                                                : 0.0f;
+}
 constexpr float bytes_per_us = 4.5e6f; // of partial tiles, written and read once each
 constexpr float join_us      = 9.0f; // the scratch buffer's lease and a second launch, or the exchange in one
 // A weight of this many bytes is not in the 256 MB memory-side cache when it is read again, behind
@@ -347,12 +357,13 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
         const float flops = 2.0f * tiles_of(args, 64, 64, false, false) * 4096 * k64 * 64;
         offer(made(general), 5.0f + std::max(flops / general_flops[layout], k64 * general_k64));
     }
-    auto consider_tiled = [&](const form_cost& f) {
+    auto consider_tiled = [&](form_cost f) {
         const launch_choice c = made(f.form);
         if(c.kernel.fn == nullptr)
         {
             return;
         }
+        f.fixed += steps_finish_us(finish) * c.kernel.block_m * c.kernel.block_n / (128 * 128);
         const size_t tiles = tiles_of(args, c.kernel.block_m, c.kernel.block_n, symmetric, false);
         const size_t slots = c.kernel.per_cu * cus, rounds = tiles / slots, rest = tiles % slots;
         const float  whole = rounds * round_us(f, slots, cus, c.kernel.per_cu, k64), least_us = weight / f.stream;
