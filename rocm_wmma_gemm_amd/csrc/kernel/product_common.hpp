@@ -15,18 +15,12 @@
 #define ROCM_WMMA_GEMM_PRODUCT_COMMON_HPP
 
 #include "gemm_kernel.hpp"
+#include "product_cut.hpp"
 
 namespace rocm_wmma_gemm
 {
 namespace device
 {
-
-enum class product_kind
-{
-    batch = 0,
-    rows  = 1,
-    sum   = 2
-};
 
 // y = x s(u) with s the logistic function covers silu (u = x) and the tanh form of gelu
 // (0.5 (1 + tanh t) = s(2 t), so u = 2 sqrt(2/pi) (x + 0.044715 x^3)): u = k1 x + k3 x^3.
@@ -84,37 +78,6 @@ struct product_args
     unsigned int* arrivals; // with k_slices > 1: a counter per tile, and this launch's tag in them
     unsigned int  arrival_epoch;
 };
-
-// How the tiles of a launch are dealt to its persistent workgroups: whole tiles round by round, and
-// where the last round has tiles for at most half of them, each of those in `slices` runs of `each` K
-// tiles that another kernel adds up.
-struct tail_cut
-{
-    int whole; // tiles before the cut ones
-    int cut; // tiles that are cut
-    int slices, each;
-    RWG_HD int positions() const
-    {
-        return whole + cut * slices;
-    }
-};
-
-// A slice shorter than this many K tiles costs more to write and add up than it saves.
-constexpr int least_slice = 4, most_slices = 16;
-
-RWG_HD inline tail_cut cut_tail(int tiles, int workgroups, int k_tiles, bool may_cut)
-{
-    const int rest   = tiles % workgroups;
-    int       slices = may_cut && rest > 0 ? workgroups / rest : 1;
-    slices           = slices < most_slices ? slices : most_slices;
-    slices           = slices < k_tiles / least_slice ? slices : k_tiles / least_slice;
-    if(slices < 2)
-    {
-        return {tiles, 0, 1, k_tiles};
-    }
-    const int each = (k_tiles + slices - 1) / slices;
-    return {tiles - rest, rest, (k_tiles + each - 1) / each, each};
-}
 
 __device__ __forceinline__ int clamped_offset(int v, int rows)
 {

@@ -128,9 +128,11 @@ struct tiled_product
                 }
             }
         }
-        // (where groups differ in K the slices would too: those launches are not cut)
+        // (where groups differ in K the slices would too: those launches are not cut; a single group's sum is
+        // cut by the rows it has, which its offsets say)
         const bool may_cut = args.partials != nullptr && !EPI::mirror && (args.kind != product_kind::sum || args.groups == 1);
-        tail_cut   cut     = cut_tail(tiles, workgroups, (args.K + BK - 1) / BK, may_cut);
+        const int  rows    = args.kind == product_kind::sum ? off[1] - off[0] : 0;
+        tail_cut   cut     = cut_tail(tiles, workgroups, summed_tiles(args.kind, args.K, rows, BK), may_cut);
         cut.whole          = __builtin_amdgcn_readfirstlane(cut.whole);
         cut.cut            = __builtin_amdgcn_readfirstlane(cut.cut);
         cut.slices         = __builtin_amdgcn_readfirstlane(cut.slices);
@@ -193,7 +195,7 @@ struct tiled_product
     __device__ __forceinline__ static work decode(const product_args& args, const plan& pl, int pos)
     {
         work w;
-        int  tile, k0 = 0;
+        int  tile, slice = 0, k0 = 0;
         w.partial = nullptr;
         if(pos < pl.cut.whole)
         {
@@ -201,7 +203,8 @@ struct tiled_product
         }
         else
         {
-            const int p = xcd_remap(pos - pl.cut.whole, pl.cut.cut * pl.cut.slices), slice = p / pl.cut.cut;
+            const int p = xcd_remap(pos - pl.cut.whole, pl.cut.cut * pl.cut.slices);
+            slice       = p / pl.cut.cut;
             const int t = p - slice * pl.cut.cut;
             tile        = pl.cut.whole + t;
             k0          = slice * pl.cut.each;
@@ -209,7 +212,7 @@ struct tiled_product
         }
         w.x         = locate(args, pl, tile);
         const int k = w.x.k > BK ? (w.x.k + BK - 1) / BK : 1;
-        w.nk        = w.partial == nullptr ? k : (k - k0 < pl.cut.each ? k - k0 : pl.cut.each);
+        w.nk        = w.partial == nullptr ? k : run_of_slice(pl.cut, slice, k).count;
         w.nk        = __builtin_amdgcn_readfirstlane(w.nk);
         w.ends_k    = k0 + w.nk == k;
 

@@ -724,3 +724,25 @@ def test_operands_on_another_device_than_the_current_one(loader, monkeypatch):
         loader.linear_backward(torch.zeros_like(A), None, None, C, A, B, 4, 16, 8)
     with pytest.raises(ValueError, match="the current one is 1"):
         loader.orthogonalize(C, C, 4, 16)
+
+
+@pytest.mark.parametrize("rows", [0, 1, 100, 3840, 3841, 3904], ids=_id)
+def test_one_group_of_fewer_rows_than_the_call(loader, rows):
+    """The gradient of a single group's weight, whose tiles are cut along the rows: those that its offsets
+    leave out are not read."""
+    M, N, K = 3904, 512, 512
+    assert loader.product_select("gradient_b", M, N, K, 1, 3).cut_tail == 1
+    for layout, before, add in ((R.col_major, 0, False), (R.row_major, (M - rows) // 2, True)):
+        _, offsets = offsets_of([rows], before)
+        at = slice(before, before + rows)
+        A, B, dC = rnd((M, K), BF16, 1), weights((K, N), layout, BF16, 2, 1), rnd((M, N), BF16, 3)
+        for t in (A, dC):
+            t[:at.start] = math.nan
+            t[at.stop:] = math.nan
+        dA = torch.full((M, K), -7.0, dtype=F32, device="cuda")
+        dB, dbias = rnd(B.shape, F32, 5), rnd((1, N), F32, 6)
+        old = (dB[0].clone(), dbias[0].clone())
+        loader.grouped_backward(dA, dB, dbias, dC, A, B, offsets, M, N, K, layout, accumulate=add)
+        assert (dA[:at.start] == -7).all() and (dA[at.stop:] == -7).all()
+        check_backward(dA[at] if rows else None, dB[0], dbias[0], dC[at], None, A[at], B[0], layout, R.activation.none, F32,
+                       f"{rows} rows {layout.name}", old if add else None)

@@ -128,3 +128,16 @@ def test_product_plans(library):
         pick("forward", 0, 8, 8)
     with pytest.raises(R.GemmLibraryError):
         pick("forward", 8, 8, 8, groups=513)
+
+
+@pytest.fixture(scope="module")
+def product_checks(tmp_path_factory):
+    out = tmp_path_factory.mktemp("products") / "product_checks"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", os.path.join(ROOT, "rocm_wmma_gemm_amd", "csrc"),
+                    os.path.join(ROOT, "tests", "product_checks.cpp"), "-o", str(out)], check=True)
+    return str(out)
+
+
+def test_every_slice_of_a_cut_tile_lies_in_its_sum(product_checks):
+    r = subprocess.run([product_checks, "cuts"], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
