@@ -26,9 +26,10 @@ struct slope_args
     const int*  offsets; // groups + 1, or nullptr: one group
     int         groups, rows, cols;
     act_args    act;
+    int         run0, block0; // the launch's first run and block of columns: a grid holds fewer than there can be
 };
 
-// A wave takes 64 * WIDTH columns, the four waves of a workgroup every fourth row of a run
+// A wave takes 64 * WIDTH columns (blockIdx.y), the four waves of a workgroup every fourth row of a run
 // (blockIdx.x); WIDTH = 8 where rows start on 16 bytes, else 1.  The sums of a run are added in
 // the order of its rows within a wave, then in wave order: the same in every call.
 template<class InT, int WIDTH>
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
     __shared__ int   off[max_groups + 1], first[max_groups + 1];
     __shared__ float part[4][64 * WIDTH];
     build_group_table(args.offsets, args.groups, args.rows, slope_rows, &off[0], &first[0]);
-    const int run = blockIdx.x;
+    const int run = args.run0 + blockIdx.x;
     if(run >= first[args.groups])
     {
         return;
@@ -46,7 +47,7 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
     const int row0  = off[group] + (run - first[group]) * slope_rows;
     const int row1  = row0 + slope_rows < off[group + 1] ? row0 + slope_rows : off[group + 1];
     const int lane  = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col   = (blockIdx.y * 64 + lane) * WIDTH;
+    const int block = args.block0 + blockIdx.y, col = (block * 64 + lane) * WIDTH;
     typedef InT in_t __attribute__((ext_vector_type(WIDTH)));
     float       sum[WIDTH];
 #pragma unroll
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
     __syncthreads();
     for(int i = threadIdx.x; i < 64 * WIDTH; i += 256)
     {
-        const int c = (blockIdx.y * 64 + i % 64) * WIDTH + i / 64;
+        const int c = (block * 64 + i % 64) * WIDTH + i / 64;
         if(c < args.cols)
         {
             args.sums[(long long)run * args.cols + c] = ((part[0][i] + part[1][i]) + part[2][i]) + part[3][i];
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(256) activation_slope(const slope_args args)
     }
 }
 
-// The sums of a group's runs: the gradient of its bias (blockIdx.y: the group).  Each of four waves
+// The sums of a group's runs: the gradient of its bias (blockIdx.y: the group, blockIdx.x: 64 columns).  Each of four waves
 // adds up a quarter of the runs in their order, then the quarters are added in theirs.
 template<class OutT>
 __global__ void __launch_bounds__(256) column_sums(const slope_args args, OutT* __restrict__ dbias, int accumulate)
@@ -123,7 +124,8 @@ __global__ void __launch_bounds__(256) column_sums(const slope_args args, OutT* 
     __shared__ int   off[max_groups + 1], first[max_groups + 1];
     __shared__ float part[4][64];
     build_group_table(args.offsets, args.groups, args.rows, slope_rows, &off[0], &first[0]);
-    const int group = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+    const int group = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = (args.block0 + blockIdx.x) * 64 + lane;
     const int run0 = first[group], runs = first[group + 1] - run0, each = (runs + 3) / 4;
     const int begin = run0 + wave * each, end = run0 + ((wave + 1) * each < runs ? (wave + 1) * each : runs);
     float     s = 0.0f;

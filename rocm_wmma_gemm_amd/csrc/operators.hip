@@ -57,6 +57,10 @@ using device::product_kind;
 // (an extent rounded up to any tile still fits an int)
 constexpr size_t most_extent = 0x7fffff00;
 
+// What a launch may have: its threads along x are counted in 32 bits (a kernel with a workgroup for every
+// tile may ask for more), its workgroups along y in 16.  most_groups_x: of 256 threads, where they come in parts.
+constexpr size_t most_threads_x = 0xffffffff, most_groups_x = size_t{1} << 20, most_groups_y = 65535;
+
 constexpr size_t ceil_div(size_t a, size_t b)
 {
     return (a + b - 1) / b;
@@ -395,7 +399,7 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
         const size_t rows = batch ? args.M : ceil_div(args.M, used);
         auto         consider = [&](const form_cost& f) {
             launch_choice c = made(f.form);
-            if(c.kernel.fn == nullptr)
+            if(c.kernel.fn == nullptr || c.items * c.kernel.threads > most_threads_x)
             {
                 return;
             }
@@ -468,8 +472,8 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
         const device::pack_job ja = job(am, args.A, on.A), jb = job(bm, args.B, on.B);
         const size_t pieces = std::max(c.copy_a ? am.rows * am.padded() / 8 : 0, c.copy_b ? bm.rows * bm.padded() / 8 : 0);
         enqueue(&device::pack_padded<unsigned short>,
-                dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(pieces, 256), 8192)), c.copy_a && c.copy_b ? 2 : 1),
-                dim3(256), stream, c.copy_a ? ja : jb, c.copy_b ? jb : ja);
+               dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(pieces, 256), 8192)), c.copy_a && c.copy_b ? 2 : 1),
+               dim3(256), stream, c.copy_a ? ja : jb, c.copy_b ? jb : ja);
         args = on;
         scratch += c.copy_bytes;
     }
@@ -497,11 +501,11 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
         args.k_slices      = c.k_slices;
     }
     enqueue(c.once && c.kernel.once != nullptr ? c.kernel.once : c.kernel.fn,
-            dim3(static_cast<unsigned>(c.workgroups * args.k_slices)), dim3(c.kernel.threads), stream, args);
+           dim3(static_cast<unsigned>(c.workgroups * args.k_slices)), dim3(c.kernel.threads), stream, args);
     if(cuts && c.kernel.finish != nullptr)
     {
         enqueue(c.kernel.finish, dim3(static_cast<unsigned>(std::min<size_t>(2048, c.workgroups * 8))),
-                dim3(c.kernel.threads), stream, args);
+               dim3(c.kernel.threads), stream, args);
     }
     return ROCM_WMMA_GEMM_OK;
 }
@@ -622,19 +626,37 @@ int forward(const layer& p, void* C, const void* A, const void* B, const rocm_wm
     return launch_product(p.type_idx, f.finish, c, f.args, scratch, stream);
 }
 
-template<class InT>
-void launch_slope(const device::slope_args& s, size_t runs, bool wide, hipStream_t stream)
+// Calls f(first, count) for the parts of `all` workgroups that a launch may have along one dimension.
+template<class F>
+void in_parts(size_t all, size_t most, F&& f)
 {
-    const unsigned columns = wide ? 512 : 64;
-    enqueue(wide ? &device::activation_slope<InT, 8> : &device::activation_slope<InT, 1>,
-            dim3(static_cast<unsigned>(runs), static_cast<unsigned>(ceil_div(s.cols, columns))), dim3(256), stream, s);
+    for(size_t first = 0; first < all; first += most)
+    {
+        f(static_cast<int>(first), static_cast<unsigned>(std::min(all - first, most)));
+    }
+}
+
+template<class InT>
+void launch_slope(device::slope_args s, size_t runs, bool wide, hipStream_t stream)
+{
+    in_parts(runs, most_groups_x, [&](int run0, unsigned some_runs) {
+        in_parts(ceil_div(s.cols, wide ? 512 : 64), most_groups_y, [&](int block0, unsigned some_blocks) {
+            s.run0   = run0;
+            s.block0 = block0;
+            enqueue(wide ? &device::activation_slope<InT, 8> : &device::activation_slope<InT, 1>, dim3(some_runs, some_blocks),
+                   dim3(256), stream, s);
+        });
+    });
 }
 
 template<class OutT>
-void launch_column_sums(const device::slope_args& s, void* dbias, int accumulate, hipStream_t stream)
+void launch_column_sums(device::slope_args s, void* dbias, int accumulate, hipStream_t stream)
 {
-    enqueue(&device::column_sums<OutT>, dim3(static_cast<unsigned>(ceil_div(s.cols, 64)), static_cast<unsigned>(s.groups)),
-            dim3(256), stream, s, static_cast<OutT*>(dbias), accumulate);
+    in_parts(ceil_div(s.cols, 64), most_groups_x, [&](int block0, unsigned some_blocks) {
+        s.block0 = block0;
+        enqueue(&device::column_sums<OutT>, dim3(some_blocks, static_cast<unsigned>(s.groups)), dim3(256), stream, s,
+               static_cast<OutT*>(dbias), accumulate);
+    });
 }
 
 // dZ = dC act'(Z); dA = dZ B^T, dB = A^T dZ, dbias = sum of dZ's rows, group by group
@@ -665,10 +687,6 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     const size_t runs   = p.M / device::slope_rows + std::min(p.groups, p.M);
     const size_t dz_bytes = passes && pitched ? whole_lines(p.M * pitch * 2) : 0;
     const size_t sums     = passes && dbias != nullptr ? whole_lines(runs * p.N * sizeof(float)) : 0;
-    if(runs > most_extent || ceil_div(p.N, 64) > 65535)
-    {
-        return ROCM_WMMA_GEMM_ERR_LIMIT;
-    }
     to_a = gradient_a(p, pitch);
     to_b = gradient_b(p, pitch, accumulate != 0);
     // (where the products find dZ is not known yet; the buffer is aligned for any kernel)
@@ -783,7 +801,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         auto run = [&](auto* typed) {
             using given_t = std::remove_pointer_t<decltype(typed)>;
             enqueue(f16 ? &device::orthogonal_small<given_t, _Float16> : &device::orthogonal_small<given_t, __bf16>,
-                    dim3(static_cast<unsigned>(batch)), dim3(1024), stream, small);
+                   dim3(static_cast<unsigned>(batch)), dim3(1024), stream, small);
         };
         by_element(given_type, run);
         return ROCM_WMMA_GEMM_OK;
@@ -824,19 +842,19 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         const size_t used = std::max<size_t>(
             1, std::min({ceil_div(M * N / (vector ? wide : 1), 4096), size_t{device::square_parts}, ceil_div(2048, batch)}));
         enqueue(vector ? &device::sum_squares<given_t, wide> : &device::sum_squares<given_t, 1>,
-                dim3(static_cast<unsigned>(used), nb), dim3(256), stream, given, static_cast<long long>(M * N), parts);
+               dim3(static_cast<unsigned>(used), nb), dim3(256), stream, given, static_cast<long long>(M * N), parts);
         const device::start_args args{given, parts, x32, x16[0], static_cast<int>(M), static_cast<int>(N),
                                       static_cast<int>(lp), static_cast<int>(hp), scale, epsilon, static_cast<int>(used)};
         if(tall)
         {
             enqueue(&device::orthogonal_start_tall<given_t>,
-                    dim3(static_cast<unsigned>(ceil_div(lp, 64) * ceil_div(hp, 64)), nb), dim3(256), stream, args);
+                   dim3(static_cast<unsigned>(ceil_div(lp, 64) * ceil_div(hp, 64)), nb), dim3(256), stream, args);
             return;
         }
         enqueue(lp == l && hp == h && aligned16(given) ? &device::orthogonal_start<given_t, true>
-                                                       : &device::orthogonal_start<given_t, false>,
-                dim3(static_cast<unsigned>(std::min<size_t>(lp, std::max<size_t>(1, 2048 / batch))), nb), dim3(256), stream,
-                args);
+                                                      : &device::orthogonal_start<given_t, false>,
+               dim3(static_cast<unsigned>(std::min<size_t>(lp, std::max<size_t>(1, 2048 / batch))), nb), dim3(256), stream,
+               args);
     };
     by_element(given_type, start);
     const float a = coefficients[0], b = coefficients[1], c = coefficients[2];
@@ -891,9 +909,9 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         // (a 16-bit element is a 16-bit element)
         const unsigned short* padded = reinterpret_cast<const unsigned short*>(x16[steps & 1]);
         enqueue(tall ? &device::orthogonal_end_tall<unsigned short> : &device::orthogonal_end<unsigned short>,
-                dim3(static_cast<unsigned>(tall ? ceil_div(M, 64) * ceil_div(N, 64) : std::min<size_t>(M, 4096)), nb), dim3(256),
-                stream, padded, static_cast<unsigned short*>(O), static_cast<int>(M), static_cast<int>(N),
-                static_cast<int>(lp), static_cast<int>(hp));
+               dim3(static_cast<unsigned>(tall ? ceil_div(M, 64) * ceil_div(N, 64) : std::min<size_t>(M, 4096)), nb), dim3(256),
+               stream, padded, static_cast<unsigned short*>(O), static_cast<int>(M), static_cast<int>(N),
+               static_cast<int>(lp), static_cast<int>(hp));
     }
     return rc;
 }

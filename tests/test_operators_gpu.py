@@ -746,3 +746,21 @@ def test_one_group_of_fewer_rows_than_the_call(loader, rows):
         assert (dA[:at.start] == -7).all() and (dA[at.stop:] == -7).all()
         check_backward(dA[at] if rows else None, dB[0], dbias[0], dC[at], None, A[at], B[0], layout, R.activation.none, F32,
                        f"{rows} rows {layout.name}", old if add else None)
+
+
+@pytest.mark.parametrize("size", [((1 << 25) + 1000, 8), (3, (1 << 22) + 64), (5, (1 << 22) + 65)], ids=_id)
+def test_backward_of_more_runs_and_columns_than_the_grid_has(loader, size):
+    """Rows past 2^25 (more than a million runs) and more than 65535 blocks of 64 columns."""
+    M, N = size
+    dC, Z = torch.zeros((M, N), dtype=F16, device="cuda"), torch.zeros((M, N), dtype=F16, device="cuda")
+    rows = [r for r in (0, 1, 31, 32, 4095, (1 << 25) - 1, 1 << 25, (1 << 25) + 31, M - 33, M - 1) if 0 <= r < M]
+    for i, r in enumerate(rows):
+        dC[r], Z[r] = rnd((N,), F16, i), rnd((N,), F16, 100 + i)
+    B = weights((4, N), R.col_major, F16, 2)
+    dA, dbias = (torch.full(s, math.nan, dtype=F16, device="cuda") for s in ((M, 4), (N,)))
+    loader.linear_backward(dA, None, dbias, dC, None, B, M, N, 4, preact=Z, activation=R.activation.silu)
+    at = sorted(set(rows))
+    check_backward(dA[at], None, dbias, dC[at], Z[at], None, B, R.col_major, R.activation.silu, F16, f"{size}")
+    others = torch.ones(M, dtype=torch.bool, device="cuda")
+    others[at] = False
+    assert (dA[others] == 0).all()

@@ -1,9 +1,11 @@
 """The layer products without a GPU: what the compiler made of the hand-placed loop, and what the
 C entry points refuse before they touch the device."""
 import ctypes
+import json
 import os
 import re
 import subprocess
+import sys
 
 import pytest
 
@@ -141,3 +143,44 @@ def product_checks(tmp_path_factory):
 def test_every_slice_of_a_cut_tile_lies_in_its_sum(product_checks):
     r = subprocess.run([product_checks, "cuts"], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.fixture(scope="module")
+def recorded(tmp_path_factory):
+    """What calls would launch: a function of [entry point, arguments] pairs (recorded_launches.py)."""
+    so = tmp_path_factory.mktemp("recorder") / "recorder.so"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", os.path.join(ROOT, "tests", "hip_recorder.cpp"), "-o",
+                    str(so)], check=True)
+
+    def ask(*calls):
+        r = subprocess.run([sys.executable, os.path.join(ROOT, "tests", "recorded_launches.py"), str(so), json.dumps(calls)],
+                           capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0, r.stdout + r.stderr
+        return json.loads(r.stdout.strip().split("\n")[-1])
+
+    return ask
+
+
+MOST = (1 << 31) - 256  # the largest extent that the entry points take
+
+
+def test_every_launch_fits_the_grid(recorded):
+    """Sizes up to the documented limits launch what HIP takes: fewer than 2^32 threads along x, at most 65535
+    workgroups along y."""
+    calls = []
+    for m, n, k in ((1, 1, 1), (1 << 29, 8, 8), (MOST, 8, 8), (MOST, 4, 8), (3, MOST, 8), (3, MOST - 1, 1), (8, 8, MOST),
+                    (1 << 24, 64, 64), (MOST, 1, 1)):
+        calls.append(["linear", [2, "p", "p", "p", m, n, k, 1, None, None]])
+        calls.append(["linear", [0, "p", "p", "p", m, n, k, 0, None, None]])
+        calls.append(["grouped", [2, "p", "p", "p", "p", 512, m, n, k, 1, None, None]])
+    for m, n, k in ((1 << 24, 8, 8), (1 << 29, 8, 8), (MOST, 8, 8), (3, 5 << 20, 8), (3, 1 << 28, 8)):
+        for act in (0, 2):
+            for wanted in (("p", None, None), (None, "p", None), (None, None, "p"), ("p", "p", "p")):
+                calls.append(["linear_backward", [3, *wanted, "p", "p", "p", "p", m, n, k, 1, act, 0, None]])
+                calls.append(["grouped_backward", [3, *wanted, "p", "p", "p", "p", "p", 4, m, n, k, 0, act, 1, None]])
+    for m, n, batch in ((1, 1, 65535), (64, 256, 65535), (100, 70, 65535), (1 << 20, 8, 3), (1 << 20, 65, 1), (65, 1 << 20, 1)):
+        calls.append(["orthogonalize", [2, 1, "p", "p", m, n, batch, 5, "s", 1e-7, None]])
+    for call, (status, launches) in zip(calls, recorded(*calls)):
+        # (-3: more scratch memory than there may be; nothing is launched then)
+        assert status == 0 and launches or status == -3 and not launches, (call, status, launches)
+        assert not any(failed for *_, failed in launches), (call, launches)
