@@ -61,6 +61,16 @@ constexpr size_t most_extent = 0x7fffff00;
 // tile may ask for more), its workgroups along y in 16.  most_groups_x: of 256 threads, where they come in parts.
 constexpr size_t most_threads_x = 0xffffffff, most_groups_x = size_t{1} << 20, most_groups_y = 65535;
 
+// enqueue(), unless a launch of this call before it was rejected: it would read what that one was to write.
+template<class... A>
+void follow(A&&... a)
+{
+    if(launch_failure == hipSuccess)
+    {
+        enqueue(std::forward<A>(a)...);
+    }
+}
+
 constexpr size_t ceil_div(size_t a, size_t b)
 {
     return (a + b - 1) / b;
@@ -471,7 +481,7 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
         const matrix_of_rows   am = rows_of_a(args, c.layout), bm = rows_of_b(args, c.layout);
         const device::pack_job ja = job(am, args.A, on.A), jb = job(bm, args.B, on.B);
         const size_t pieces = std::max(c.copy_a ? am.rows * am.padded() / 8 : 0, c.copy_b ? bm.rows * bm.padded() / 8 : 0);
-        enqueue(&device::pack_padded<unsigned short>,
+        follow(&device::pack_padded<unsigned short>,
                dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(pieces, 256), 8192)), c.copy_a && c.copy_b ? 2 : 1),
                dim3(256), stream, c.copy_a ? ja : jb, c.copy_b ? jb : ja);
         args = on;
@@ -500,11 +510,11 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
         args.arrival_epoch = next_arrival_epoch();
         args.k_slices      = c.k_slices;
     }
-    enqueue(c.once && c.kernel.once != nullptr ? c.kernel.once : c.kernel.fn,
+    follow(c.once && c.kernel.once != nullptr ? c.kernel.once : c.kernel.fn,
            dim3(static_cast<unsigned>(c.workgroups * args.k_slices)), dim3(c.kernel.threads), stream, args);
     if(cuts && c.kernel.finish != nullptr)
     {
-        enqueue(c.kernel.finish, dim3(static_cast<unsigned>(std::min<size_t>(2048, c.workgroups * 8))),
+        follow(c.kernel.finish, dim3(static_cast<unsigned>(std::min<size_t>(2048, c.workgroups * 8))),
                dim3(c.kernel.threads), stream, args);
     }
     return ROCM_WMMA_GEMM_OK;
@@ -643,7 +653,7 @@ void launch_slope(device::slope_args s, size_t runs, bool wide, hipStream_t stre
         in_parts(ceil_div(s.cols, wide ? 512 : 64), most_groups_y, [&](int block0, unsigned some_blocks) {
             s.run0   = run0;
             s.block0 = block0;
-            enqueue(wide ? &device::activation_slope<InT, 8> : &device::activation_slope<InT, 1>, dim3(some_runs, some_blocks),
+            follow(wide ? &device::activation_slope<InT, 8> : &device::activation_slope<InT, 1>, dim3(some_runs, some_blocks),
                    dim3(256), stream, s);
         });
     });
@@ -654,7 +664,7 @@ void launch_column_sums(device::slope_args s, void* dbias, int accumulate, hipSt
 {
     in_parts(ceil_div(s.cols, 64), most_groups_x, [&](int block0, unsigned some_blocks) {
         s.block0 = block0;
-        enqueue(&device::column_sums<OutT>, dim3(some_blocks, static_cast<unsigned>(s.groups)), dim3(256), stream, s,
+        follow(&device::column_sums<OutT>, dim3(some_blocks, static_cast<unsigned>(s.groups)), dim3(256), stream, s,
                static_cast<OutT*>(dbias), accumulate);
     });
 }
@@ -800,7 +810,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         const bool               f16 = out_type == ROCM_WMMA_GEMM_ELEMENT_F16;
         auto run = [&](auto* typed) {
             using given_t = std::remove_pointer_t<decltype(typed)>;
-            enqueue(f16 ? &device::orthogonal_small<given_t, _Float16> : &device::orthogonal_small<given_t, __bf16>,
+            follow(f16 ? &device::orthogonal_small<given_t, _Float16> : &device::orthogonal_small<given_t, __bf16>,
                    dim3(static_cast<unsigned>(batch)), dim3(1024), stream, small);
         };
         by_element(given_type, run);
@@ -841,17 +851,17 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
         // (a workgroup for every 4096 pieces, but at most eight to a compute unit over the batch)
         const size_t used = std::max<size_t>(
             1, std::min({ceil_div(M * N / (vector ? wide : 1), 4096), size_t{device::square_parts}, ceil_div(2048, batch)}));
-        enqueue(vector ? &device::sum_squares<given_t, wide> : &device::sum_squares<given_t, 1>,
+        follow(vector ? &device::sum_squares<given_t, wide> : &device::sum_squares<given_t, 1>,
                dim3(static_cast<unsigned>(used), nb), dim3(256), stream, given, static_cast<long long>(M * N), parts);
         const device::start_args args{given, parts, x32, x16[0], static_cast<int>(M), static_cast<int>(N),
                                       static_cast<int>(lp), static_cast<int>(hp), scale, epsilon, static_cast<int>(used)};
         if(tall)
         {
-            enqueue(&device::orthogonal_start_tall<given_t>,
+            follow(&device::orthogonal_start_tall<given_t>,
                    dim3(static_cast<unsigned>(ceil_div(lp, 64) * ceil_div(hp, 64)), nb), dim3(256), stream, args);
             return;
         }
-        enqueue(lp == l && hp == h && aligned16(given) ? &device::orthogonal_start<given_t, true>
+        follow(lp == l && hp == h && aligned16(given) ? &device::orthogonal_start<given_t, true>
                                                       : &device::orthogonal_start<given_t, false>,
                dim3(static_cast<unsigned>(std::min<size_t>(lp, std::max<size_t>(1, 2048 / batch))), nb), dim3(256), stream,
                args);
@@ -908,7 +918,7 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
     {
         // (a 16-bit element is a 16-bit element)
         const unsigned short* padded = reinterpret_cast<const unsigned short*>(x16[steps & 1]);
-        enqueue(tall ? &device::orthogonal_end_tall<unsigned short> : &device::orthogonal_end<unsigned short>,
+        follow(tall ? &device::orthogonal_end_tall<unsigned short> : &device::orthogonal_end<unsigned short>,
                dim3(static_cast<unsigned>(tall ? ceil_div(M, 64) * ceil_div(N, 64) : std::min<size_t>(M, 4096)), nb), dim3(256),
                stream, padded, static_cast<unsigned short*>(O), static_cast<int>(M), static_cast<int>(N),
                static_cast<int>(lp), static_cast<int>(hp));

@@ -184,3 +184,16 @@ def test_every_launch_fits_the_grid(recorded):
         # (-3: more scratch memory than there may be; nothing is launched then)
         assert status == 0 and launches or status == -3 and not launches, (call, status, launches)
         assert not any(failed for *_, failed in launches), (call, launches)
+
+
+def test_nothing_follows_a_launch_that_failed(recorded):
+    """A kernel that reads what a rejected one was to write is not launched: the results stay as they were."""
+    for call in (["linear_backward", [2, "p", "p", "p", "p", "p", "p", "p", 300, 512, 256, 1, 2, 0, None]],
+                 ["grouped_backward", [2, "p", "p", "p", "p", "p", "p", "p", "p", 4, 300, 512, 256, 1, 2, 1, None]],
+                 ["linear", [2, "p", "p", "p", 2048, 4096, 4001, 1, None, None]],  # copies of A and B first
+                 ["orthogonalize", [2, 1, "p", "p", 300, 200, 2, 2, "s", 1e-7, None]]):
+        (status, whole), = recorded(call)
+        assert status == 0 and len(whole) >= 2
+        for n in range(len(whole)):
+            (status, launches), = recorded(["fail", n], call)
+            assert status == -4 and len(launches) == n + 1, (call, n, launches)
