@@ -1,6 +1,7 @@
 // How the tiles of a layer product's launch are dealt to its persistent workgroups: whole tiles round by
 // round, and where the last round has tiles for at most half of them, each of those in slices along K that
-// another kernel adds up.  Integer arithmetic alone, so that the host can check it.
+// another kernel adds up; and which tiles a symmetric product has.  Integer arithmetic alone, so that the host
+// can check it.
 #ifndef ROCM_WMMA_GEMM_PRODUCT_CUT_HPP
 #define ROCM_WMMA_GEMM_PRODUCT_CUT_HPP
 
@@ -64,6 +65,22 @@ RWG_HD inline tile_run run_of_slice(const tail_cut& cut, int slice, int k_tiles)
 {
     const int from = slice * cut.each;
     return {from, k_tiles - from < cut.each ? k_tiles - from : cut.each};
+}
+
+// Tile `local` of the tiles on and above the diagonal of g x g: rows r and g - 1 - r of the triangle
+// together have g + 1 tiles.
+RWG_HD inline tile_coord triangle_tile(int local, int g)
+{
+    const int r = local / (g + 1), c = local - r * (g + 1), m = c < g - r ? r : g - 1 - r;
+    return {m, c < g - r ? r + c : m + c - (g - r)};
+}
+
+// Whether a tile of the triangle, corner (row0, col0), is written a second time, transposed, below the
+// diagonal.  A tile on the diagonal is not: it holds both halves, and two waves would store each of its
+// elements in no order (the matrix cores' sums for (i, j) and (j, i) may differ in their last bits).
+RWG_HD inline bool has_mirror(int row0, int col0)
+{
+    return row0 != col0;
 }
 
 } // namespace device

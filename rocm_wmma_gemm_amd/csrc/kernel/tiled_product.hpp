@@ -173,10 +173,7 @@ struct tiled_product
         tile_coord t;
         if constexpr(EPI::mirror)
         {
-            // rows r and g - 1 - r of the triangle together have g + 1 tiles
-            const int g = args.grid_n, r = local / (g + 1), c = local - r * (g + 1);
-            t.m = c < g - r ? r : g - 1 - r;
-            t.n = c < g - r ? r + c : t.m + c - (g - r);
+            t = triangle_tile(local, args.grid_n);
         }
         else
         {
@@ -344,7 +341,7 @@ struct tiled_product
     }
 
     // The wave's part of a finished tile, corner (row_w, col_w) in the workgroup's; MIRRORED: its
-    // transpose, to the mirrored place.
+    // transpose, to the mirrored place (see has_mirror).
     template<bool MIRRORED>
     __device__ __forceinline__ static void write(const product_args& args, const work& w, f32x4 (&acc)[TM][TN],
                                                  int row_w, int col_w, int lane, lds_char_ptr strip)
@@ -366,7 +363,9 @@ struct tiled_product
         }
         const bool has_kept = (EPI::layer || EPI::kept) && args.kept != nullptr;
         const bool has_residual = EPI::residual && args.residual != nullptr;
-        const __amdgpu_buffer_rsrc_t to = window(static_cast<OutT*>(args.C) + at, true);
+        // (a tile without a mirror has no transposed place: its stores are dropped)
+        const __amdgpu_buffer_rsrc_t to
+            = window(static_cast<OutT*>(args.C) + at, !MIRRORED || has_mirror(w.x.row0, w.x.col0));
         const __amdgpu_buffer_rsrc_t kept_to
             = window(static_cast<InT*>(args.kept) + at, has_kept);
         const __amdgpu_buffer_rsrc_t from

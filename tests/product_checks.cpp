@@ -1,6 +1,7 @@
 // Host-only checks of how the layer products deal their tiles (compiled here for the CPU).
 #include <cstdio>
 #include <cstring>
+#include <vector>
 
 #include "kernel/product_cut.hpp"
 
@@ -56,9 +57,33 @@ static int check_cuts()
     return 0;
 }
 
+// A symmetric product of g x g tiles: every tile of the square is written once, by itself or as the mirror of
+// the one above the diagonal.
+static int check_triangle()
+{
+    for(int g = 1; g <= 60; ++g)
+    {
+        std::vector<int> written(g * g, 0);
+        for(int local = 0; local < g * (g + 1) / 2; ++local)
+        {
+            const tile_coord t = triangle_tile(local, g);
+            if(t.m < 0 || t.n < t.m || t.n >= g)
+                return fail("a tile outside the triangle", g, t.m, t.n, local, -1);
+            ++written[t.m * g + t.n];
+            written[t.n * g + t.m] += has_mirror(t.m * 128, t.n * 128);
+        }
+        for(int i = 0; i < g * g; ++i)
+            if(written[i] != 1)
+                return fail("a tile not written once", g, i / g, i % g, written[i], -1);
+    }
+    return 0;
+}
+
 int main(int argc, char** argv)
 {
     if(argc == 2 && !std::strcmp(argv[1], "cuts"))
         return check_cuts();
+    if(argc == 2 && !std::strcmp(argv[1], "triangle"))
+        return check_triangle();
     return 2;
 }

@@ -764,3 +764,16 @@ def test_backward_of_more_runs_and_columns_than_the_grid_has(loader, size):
     others = torch.ones(M, dtype=torch.bool, device="cuda")
     others[at] = False
     assert (dA[others] == 0).all()
+
+
+@pytest.mark.parametrize("shape", [(4, 1000, 520), (1, 1024, 2048), (8, 640, 1024), (1, 2304, 2304)], ids=_id)
+def test_large_updates_repeat_bit_for_bit(loader, shape):
+    """Sizes whose symmetric products run on tiles that are written twice, mirrored."""
+    batch, M, N = shape
+    G = rnd(shape, F32, 4)
+    seen = []
+    for _ in range(6):
+        O = torch.empty(G.shape, dtype=F16, device="cuda")
+        loader.orthogonalize(O, G, M, N, batch)
+        seen.append(O)
+    assert all(torch.equal(seen[0], other) for other in seen[1:])

@@ -145,6 +145,11 @@ def test_every_slice_of_a_cut_tile_lies_in_its_sum(product_checks):
     assert r.returncode == 0, r.stdout + r.stderr
 
 
+def test_every_tile_of_a_symmetric_product_is_written_once(product_checks):
+    r = subprocess.run([product_checks, "triangle"], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 @pytest.fixture(scope="module")
 def recorded(tmp_path_factory):
     """What calls would launch: a function of [entry point, arguments] pairs (recorded_launches.py)."""
