@@ -243,7 +243,9 @@ int rocm_wmma_gemm_linear(int type_idx, void* C, const void* A, const void* B, s
  * dA = dZ B^T (M x K), dB = A^T dZ (in B's layout), dbias = sum of dZ's rows (N); a NULL result is not
  * computed.  accumulate 1: dB and dbias are added to.  dZ is rounded to A's type before it is
  * multiplied (not in dbias); it and the partial sums of dbias live in the library's scratch buffer, so a call
- * on a capturing stream for which that buffer is too small returns ROCM_WMMA_GEMM_ERR_SCRATCH.
+ * on a capturing stream for which that buffer is too small returns ROCM_WMMA_GEMM_ERR_SCRATCH, and so does
+ * any call for which they take more than 16 GiB (2 bytes an element of dZ, where there is an activation or dC's rows
+ * do not start on 16 bytes, and N / 8 bytes a row for dbias).
  * (The gradient of the residual is dC.) */
 int rocm_wmma_gemm_linear_backward(int type_idx, void* dA, void* dB, void* dbias, const void* dC, const void* A,
                                    const void* B, const void* preact, size_t M, size_t N, size_t K, int layout_b,
@@ -282,7 +284,8 @@ int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N,
  * columns (all singular values near 1): X = G / (|G|_F + epsilon), then `steps` times
  * X = a X + (b S + c S^2) X with S = X X^T, coefficients = {a, b, c}; O = X.  G and O: batch_count
  * row-major M x N matrices; G of type F16, BF16 or F32, O of type F16 or BF16.  M and N up to 2^20.
- * Works in the library's scratch buffer (8 bytes an element and 4 min(M, N)^2 per matrix). */
+ * Works in the library's scratch buffer (8 bytes an element and 4 min(M, N)^2 per matrix, 16 GiB at most: a
+ * batch that needs more goes in parts, a single matrix that does returns ROCM_WMMA_GEMM_ERR_SCRATCH). */
 #define ROCM_WMMA_GEMM_ELEMENT_F16 0
 #define ROCM_WMMA_GEMM_ELEMENT_BF16 1
 #define ROCM_WMMA_GEMM_ELEMENT_F32 2

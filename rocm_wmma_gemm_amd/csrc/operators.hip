@@ -785,6 +785,36 @@ void by_element(int element, F&& f)
     }
 }
 
+struct update
+{
+    int          given_type, out_type;
+    void*        O;
+    const void*  G;
+    size_t       M, N, batch;
+    int          steps;
+    const float* coefficients;
+    float        epsilon;
+    hipStream_t  stream;
+};
+
+// The scratch memory of an update's matrices, `batch` of them: where each part starts, and its end.
+struct steps_scratch
+{
+    size_t l, h, lp, hp, each, square; // smaller and larger side, padded to multiples of 8; elements of X and S
+    size_t diagonal, x32, x16, x16_bytes, s, q, bytes; // (the partial sums of squares come first)
+    steps_scratch(size_t M, size_t N, size_t batch)
+        : l(std::min(M, N)), h(std::max(M, N)), lp(round_up8(l)), hp(round_up8(h)), each(lp * hp), square(lp * lp)
+    {
+        diagonal  = whole_lines(batch * device::square_parts * sizeof(float));
+        x32       = diagonal + whole_lines(batch * lp * sizeof(float));
+        x16       = x32 + whole_lines(batch * each * 4);
+        x16_bytes = whole_lines(batch * each * 2);
+        s         = x16 + 2 * x16_bytes;
+        q         = s + whole_lines(batch * square * 2);
+        bytes     = q + whole_lines(batch * square * 2);
+    }
+};
+
 // Newton-Schulz steps X <- a X + (b S + c S^2) X with S = X X^T on X = G / (|G| + epsilon), or on its
 // transpose where G is tall.
 //
@@ -800,46 +830,25 @@ void by_element(int element, F&& f)
 //     fp32 X in the epilogue: X = (a + diagonal) X + Q X.
 // Against 64 bits, 512 x 1024: 7.5e-4 for noise, 2.4e-4 for a momentum of 16 strong directions (2.1e-2
 // with all of it from f16, 1.6e-1 from bf16); 1 x 40: 7.2e-4 (3.7e-3 with the diagonal in f16).
-int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M, size_t N, size_t batch, int steps,
-                  const float* coefficients, float epsilon, hipStream_t stream)
+int steps_in(char* ws, const update& u)
 {
-    if(std::min(M, N) <= device::small_side && std::max(M, N) <= device::small_length)
-    {
-        const device::steps_args small{G, O, static_cast<int>(M), static_cast<int>(N), steps, coefficients[0],
-                                       coefficients[1], coefficients[2], epsilon};
-        const bool               f16 = out_type == ROCM_WMMA_GEMM_ELEMENT_F16;
-        auto run = [&](auto* typed) {
-            using given_t = std::remove_pointer_t<decltype(typed)>;
-            follow(f16 ? &device::orthogonal_small<given_t, _Float16> : &device::orthogonal_small<given_t, __bf16>,
-                   dim3(static_cast<unsigned>(batch)), dim3(1024), stream, small);
-        };
-        by_element(given_type, run);
-        return ROCM_WMMA_GEMM_OK;
-    }
-    const bool   tall = M > N;
-    const size_t l = std::min(M, N), h = std::max(M, N), lp = round_up8(l), hp = round_up8(h);
-    const size_t each = lp * hp, square = lp * lp;
-    const bool   direct  = !tall && lp == l && hp == h && aligned16(O);
-    const size_t parts_b = whole_lines(batch * device::square_parts * sizeof(float)),
-                 diag_b = whole_lines(batch * lp * sizeof(float)), x32_b = whole_lines(batch * each * 4),
-                 x16_b = whole_lines(batch * each * 2), sq_b = whole_lines(batch * square * 2);
-    if(batch * each > (size_t{1} << 36))
-    {
-        return ROCM_WMMA_GEMM_ERR_LIMIT;
-    }
-    workspace_lease lease;
-    char*           ws = lease.acquire(parts_b + diag_b + x32_b + 2 * x16_b + 2 * sq_b, stream);
-    if(ws == nullptr)
-    {
-        return ROCM_WMMA_GEMM_ERR_SCRATCH;
-    }
-    float*    parts = reinterpret_cast<float*>(ws);
-    float*    diagonal = reinterpret_cast<float*>(ws + parts_b);
-    float*    x32   = reinterpret_cast<float*>(ws + parts_b + diag_b);
-    char*     rest  = ws + parts_b + diag_b + x32_b;
-    _Float16* x16[2] = {reinterpret_cast<_Float16*>(rest), reinterpret_cast<_Float16*>(rest + x16_b)};
-    char*     s = rest + 2 * x16_b;
-    char*     q = s + sq_b;
+    const size_t        M = u.M, N = u.N, batch = u.batch;
+    const steps_scratch at(M, N, batch);
+    const size_t        l = at.l, h = at.h, lp = at.lp, hp = at.hp, each = at.each, square = at.square;
+    const int           given_type = u.given_type, out_type = u.out_type, steps = u.steps;
+    const void*         G = u.G;
+    void*               O = u.O;
+    const float*        coefficients = u.coefficients;
+    const float         epsilon = u.epsilon;
+    const hipStream_t   stream = u.stream;
+    const bool          tall   = M > N;
+    const bool          direct = !tall && lp == l && hp == h && aligned16(O);
+    float*    parts    = reinterpret_cast<float*>(ws);
+    float*    diagonal = reinterpret_cast<float*>(ws + at.diagonal);
+    float*    x32      = reinterpret_cast<float*>(ws + at.x32);
+    _Float16* x16[2]   = {reinterpret_cast<_Float16*>(ws + at.x16), reinterpret_cast<_Float16*>(ws + at.x16 + at.x16_bytes)};
+    char*     s        = ws + at.s;
+    char*     q        = ws + at.q;
     const float scale = std::exp2(std::round(std::log2(std::sqrt(static_cast<float>(l)))));
     const unsigned nb = static_cast<unsigned>(batch);
 
@@ -922,6 +931,43 @@ int orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M
                dim3(static_cast<unsigned>(tall ? ceil_div(M, 64) * ceil_div(N, 64) : std::min<size_t>(M, 4096)), nb), dim3(256),
                stream, padded, static_cast<unsigned short*>(O), static_cast<int>(M), static_cast<int>(N),
                static_cast<int>(lp), static_cast<int>(hp));
+    }
+    return rc;
+}
+
+int orthogonalize(const update& u)
+{
+    if(std::min(u.M, u.N) <= device::small_side && std::max(u.M, u.N) <= device::small_length)
+    {
+        const device::steps_args small{u.G, u.O, static_cast<int>(u.M), static_cast<int>(u.N), u.steps, u.coefficients[0],
+                                       u.coefficients[1], u.coefficients[2], u.epsilon};
+        const bool               f16 = u.out_type == ROCM_WMMA_GEMM_ELEMENT_F16;
+        auto run = [&](auto* typed) {
+            using given_t = std::remove_pointer_t<decltype(typed)>;
+            follow(f16 ? &device::orthogonal_small<given_t, _Float16> : &device::orthogonal_small<given_t, __bf16>,
+                   dim3(static_cast<unsigned>(u.batch)), dim3(1024), u.stream, small);
+        };
+        by_element(u.given_type, run);
+        return ROCM_WMMA_GEMM_OK;
+    }
+    // (more matrices than the scratch buffer may hold the state of go in parts, of equal size)
+    const size_t fit  = std::max<size_t>(1, workspace_limit_bytes / steps_scratch(u.M, u.N, 1).bytes);
+    const size_t some = ceil_div(u.batch, ceil_div(u.batch, fit));
+    workspace_lease lease;
+    char*           ws = lease.acquire(steps_scratch(u.M, u.N, some).bytes, u.stream);
+    if(ws == nullptr)
+    {
+        return ROCM_WMMA_GEMM_ERR_SCRATCH;
+    }
+    const size_t given_bytes = u.given_type == ROCM_WMMA_GEMM_ELEMENT_F32 ? 4 : 2;
+    int          rc          = ROCM_WMMA_GEMM_OK;
+    for(size_t first = 0; first < u.batch && rc == ROCM_WMMA_GEMM_OK; first += some)
+    {
+        update part = u;
+        part.batch  = std::min(some, u.batch - first);
+        part.G      = static_cast<const char*>(u.G) + first * u.M * u.N * given_bytes;
+        part.O      = static_cast<char*>(u.O) + first * u.M * u.N * 2;
+        rc          = steps_in(ws, part);
     }
     return rc;
 }
@@ -1073,8 +1119,7 @@ int rocm_wmma_gemm_orthogonalize(int given_type, int out_type, void* O, const vo
         {
             return ROCM_WMMA_GEMM_ERR_LIMIT;
         }
-        return orthogonalize(given_type, out_type, O, G, M, N, batch_count, steps, coefficients, epsilon,
-                             stream_of(stream));
+        return orthogonalize({given_type, out_type, O, G, M, N, batch_count, steps, coefficients, epsilon, stream_of(stream)});
     });
 }
 

@@ -777,3 +777,17 @@ def test_large_updates_repeat_bit_for_bit(loader, shape):
         loader.orthogonalize(O, G, M, N, batch)
         seen.append(O)
     assert all(torch.equal(seen[0], other) for other in seen[1:])
+
+
+def test_more_updates_than_the_scratch_buffer_holds(loader):
+    batch, M, N = 31, 72, 1 << 20  # 18.9 GB of state
+    G = torch.empty((batch, M, N), dtype=BF16, device="cuda")
+    for i in range(batch):
+        G[i] = rnd((M, N), BF16, i)
+    O = torch.full(G.shape, math.nan, dtype=BF16, device="cuda")
+    loader.orthogonalize(O, G, M, N, batch)
+    for i in (0, 14, 15, 16, 30):
+        want = steps64(G[i:i + 1])[0]
+        off = (O[i].double() - want).norm() / want.norm()
+        assert off <= STEPS_TOLERANCE[BF16], (i, off)
+    loader.workspace_release()

@@ -202,3 +202,14 @@ def test_nothing_follows_a_launch_that_failed(recorded):
         for n in range(len(whole)):
             (status, launches), = recorded(["fail", n], call)
             assert status == -4 and len(launches) == n + 1, (call, n, launches)
+
+
+def test_a_large_batch_of_updates_goes_in_parts(recorded):
+    """More matrices than the scratch buffer may hold (16 GiB) go in parts of one size, each the launches of a
+    batch; one matrix past it is refused."""
+    one = lambda batch, m=4096, n=8192: ["orthogonalize", [2, 1, "p", "p", m, n, batch, 2, "s", 1e-7, None]]  # noqa: E731
+    (rc, alone), (rc64, all64), (rc65, all65), (refused, none) = recorded(one(32), one(64), one(65), one(1, 1 << 18, 1 << 14))
+    assert (rc, rc64, rc65) == (0, 0, 0)
+    assert len(all64) == 2 * len(alone) and len(all65) == 2 * len(alone)
+    assert [x[1] for x in all64[:2]] == [32, 32] and [x[1] for x in all65[:1] + all65[len(alone):len(alone) + 1]] == [33, 32]
+    assert (refused, none) == (-3, [])
