@@ -155,19 +155,20 @@ __global__ void __launch_bounds__(256) column_sums(const slope_args args, OutT* 
 constexpr int square_parts = 1024; // the most workgroups that add up the squares of one matrix
 
 // blockIdx.y: the matrix, blockIdx.x: one of `parts` runs of it.  One partial sum per workgroup, in a
-// fixed order.  WIDTH elements at a time (16 bytes where the matrices are aligned, else one).
+// fixed order.  WIDTH elements at a time (16 bytes where the matrices are aligned, else one).  In fp64, as the
+// norm and the factor made of it: the square of an fp32 or bf16 element may lie outside fp32's range.
 template<class GivenT, int WIDTH>
 __global__ void __launch_bounds__(256) sum_squares(const GivenT* __restrict__ given, long long count,
-                                                   float* __restrict__ parts)
+                                                   double* __restrict__ parts)
 {
     typedef GivenT given_t __attribute__((ext_vector_type(WIDTH)));
     const given_t* g    = reinterpret_cast<const given_t*>(given + blockIdx.y * count);
     const long long n   = count / WIDTH, hop = 256ll * gridDim.x;
-    float           s[WIDTH];
+    double          s[WIDTH];
 #pragma unroll
     for(int v = 0; v < WIDTH; ++v)
     {
-        s[v] = 0.0f;
+        s[v] = 0.0;
     }
 #pragma unroll 4
     for(long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += hop)
@@ -176,10 +177,10 @@ __global__ void __launch_bounds__(256) sum_squares(const GivenT* __restrict__ gi
 #pragma unroll
         for(int v = 0; v < WIDTH; ++v)
         {
-            s[v] += (float)x[v] * (float)x[v];
+            s[v] += (double)x[v] * (double)x[v];
         }
     }
-    float t = 0.0f;
+    double t = 0.0;
 #pragma unroll
     for(int v = 0; v < WIDTH; ++v)
     {
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(256) sum_squares(const GivenT* __restrict__ gi
     {
         t += __shfl_xor(t, d);
     }
-    __shared__ float wave_sum[4];
+    __shared__ double wave_sum[4];
     if((threadIdx.x & 63) == 0)
     {
         wave_sum[threadIdx.x >> 6] = t;
@@ -203,9 +204,9 @@ __global__ void __launch_bounds__(256) sum_squares(const GivenT* __restrict__ gi
 }
 
 // The norm of a matrix from its partial sums, by every wave.
-__device__ __forceinline__ float norm_of(const float* parts, long long matrix, int used_parts)
+__device__ __forceinline__ double norm_of(const double* parts, long long matrix, int used_parts)
 {
-    float t = 0.0f;
+    double t = 0.0;
     for(int i = threadIdx.x & 63; i < used_parts; i += 64)
     {
         t += parts[matrix * square_parts + i];
@@ -215,13 +216,13 @@ __device__ __forceinline__ float norm_of(const float* parts, long long matrix, i
     {
         t += __shfl_xor(t, d);
     }
-    return sqrtf(t);
+    return sqrt(t);
 }
 
 struct start_args
 {
-    const void*  given;
-    const float* parts;
+    const void*   given;
+    const double* parts;
     float*       x32;
     _Float16*    x16;
     int          rows, cols; // of G
@@ -249,7 +250,7 @@ template<class GivenT, bool WIDE>
 __global__ void __launch_bounds__(256) orthogonal_start(const start_args args)
 {
     const long long matrix = blockIdx.y;
-    const float     f      = args.scale / (norm_of(args.parts, matrix, args.used_parts) + args.epsilon);
+    const double    f      = args.scale / (norm_of(args.parts, matrix, args.used_parts) + args.epsilon);
     const int       pieces = args.cols_pad / 8;
     const GivenT*   g      = static_cast<const GivenT*>(args.given) + matrix * args.rows * args.cols;
     for(int row = blockIdx.x; row < args.rows_pad; row += gridDim.x)
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(256) orthogonal_start(const start_args args)
 #pragma unroll
                 for(int e = 0; e < 8; ++e)
                 {
-                    y[e] = (float)v[e] * f;
+                    y[e] = (float)((double)v[e] * f);
                 }
             }
             else
@@ -273,7 +274,8 @@ __global__ void __launch_bounds__(256) orthogonal_start(const start_args args)
 #pragma unroll
                 for(int e = 0; e < 8; ++e)
                 {
-                    y[e] = row < args.rows && col + e < args.cols ? (float)g[(long long)row * args.cols + col + e] * f : 0.0f;
+                    y[e] = row < args.rows && col + e < args.cols ? (float)((double)g[(long long)row * args.cols + col + e] * f)
+                                                                        : 0.0f;
                 }
             }
             store_start(args, (matrix * args.rows_pad + row) * args.cols_pad + col, y);
@@ -288,14 +290,14 @@ __global__ void __launch_bounds__(256) orthogonal_start_tall(const start_args ar
 {
     __shared__ float tile[64][65];
     const long long  matrix = blockIdx.y;
-    const float      f      = args.scale / (norm_of(args.parts, matrix, args.used_parts) + args.epsilon);
+    const double     f      = args.scale / (norm_of(args.parts, matrix, args.used_parts) + args.epsilon);
     const GivenT*    g      = static_cast<const GivenT*>(args.given) + matrix * args.rows * args.cols;
     const int        across = (args.cols_pad + 63) / 64;
     const int        x_row0 = blockIdx.x / across * 64, x_col0 = blockIdx.x % across * 64;
     for(int i = threadIdx.x; i < 64 * 64; i += 256)
     {
         const int row = x_col0 + i / 64, col = x_row0 + i % 64; // of G
-        tile[i % 64][i / 64] = row < args.rows && col < args.cols ? (float)g[(long long)row * args.cols + col] * f : 0.0f;
+        tile[i % 64][i / 64] = row < args.rows && col < args.cols ? (float)((double)g[(long long)row * args.cols + col] * f) : 0.0f;
     }
     __syncthreads();
     for(int i = threadIdx.x; i < 64 * 8; i += 256)
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
     constexpr int XP = small_length + 4, SP = small_side + 4, THREADS = 1024, COLS = small_length / 16 / 4;
     __shared__ float x[small_side * XP];
     __shared__ float s[small_side * SP];
-    __shared__ float wave_sum[16];
+    __shared__ double wave_sum[16];
     const int       tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, k4 = lane >> 4;
     const int       wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool      tall = args.rows > args.cols;
@@ -398,12 +400,12 @@ __global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
         x[i] = 0.0f;
     }
     __syncthreads();
-    float t = 0.0f;
+    double t = 0.0;
     for(int i = tid; i < l * h; i += THREADS)
     {
         const float v = (float)g[i];
         x[place(i)]   = v;
-        t += v * v;
+        t += (double)v * (double)v;
     }
 #pragma unroll
     for(int d = 32; d > 0; d /= 2)
@@ -415,16 +417,17 @@ __global__ void __launch_bounds__(1024) orthogonal_small(const steps_args args)
         wave_sum[wave] = t;
     }
     __syncthreads();
-    t = 0.0f;
+    t = 0.0;
 #pragma unroll
     for(int w = 0; w < 16; ++w)
     {
         t += wave_sum[w];
     }
-    const float f = 1.0f / (sqrtf(t) + args.epsilon);
+    const double f = 1.0 / (sqrt(t) + args.epsilon);
     for(int i = tid; i < l * h; i += THREADS)
     {
-        x[place(i)] *= f;
+        float& to = x[place(i)];
+        to        = (float)((double)to * f);
     }
     const int ti = wave >> 2, tj = wave & 3;
     float*    own = &s[(ti * 16 + 4 * k4) * SP + tj * 16 + r16]; // this lane's 4 rows of its tile of S

@@ -805,7 +805,7 @@ struct steps_scratch
     steps_scratch(size_t M, size_t N, size_t batch)
         : l(std::min(M, N)), h(std::max(M, N)), lp(round_up8(l)), hp(round_up8(h)), each(lp * hp), square(lp * lp)
     {
-        diagonal  = whole_lines(batch * device::square_parts * sizeof(float));
+        diagonal  = whole_lines(batch * device::square_parts * sizeof(double));
         x32       = diagonal + whole_lines(batch * lp * sizeof(float));
         x16       = x32 + whole_lines(batch * each * 4);
         x16_bytes = whole_lines(batch * each * 2);
@@ -843,7 +843,7 @@ int steps_in(char* ws, const update& u)
     const hipStream_t   stream = u.stream;
     const bool          tall   = M > N;
     const bool          direct = !tall && lp == l && hp == h && aligned16(O);
-    float*    parts    = reinterpret_cast<float*>(ws);
+    double*   parts    = reinterpret_cast<double*>(ws);
     float*    diagonal = reinterpret_cast<float*>(ws + at.diagonal);
     float*    x32      = reinterpret_cast<float*>(ws + at.x32);
     _Float16* x16[2]   = {reinterpret_cast<_Float16*>(ws + at.x16), reinterpret_cast<_Float16*>(ws + at.x16 + at.x16_bytes)};

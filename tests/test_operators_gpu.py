@@ -791,3 +791,21 @@ def test_more_updates_than_the_scratch_buffer_holds(loader):
         off = (O[i].double() - want).norm() / want.norm()
         assert off <= STEPS_TOLERANCE[BF16], (i, off)
     loader.workspace_release()
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 56), (2, 96, 160), (1, 300, 201), (1, 640, 1024)], ids=_id)
+@pytest.mark.parametrize("given", [F32, BF16], ids=_id)
+def test_updates_of_any_scale(loader, shape, given):
+    """The square of an element may leave fp32 where the element does not: a power of two that all of G is
+    multiplied by changes no bit of the update."""
+    batch, M, N = shape
+    G = rnd(shape, F32, 1).to(given)
+    G = torch.where(G.abs() < 2.0 ** -10, torch.zeros_like(G), G)  # (nothing turns subnormal below)
+    want = torch.empty(shape, dtype=F16, device="cuda")
+    loader.orthogonalize(want, G, M, N, batch, epsilon=0.0)
+    off = (want.double() - steps64(G, epsilon=0.0)).norm() / want.double().norm()
+    assert off <= STEPS_TOLERANCE[F16], off
+    for power in (-110, -75, 70, 120):
+        O = torch.full(shape, math.nan, dtype=F16, device="cuda")
+        loader.orthogonalize(O, G * 2.0 ** power, M, N, batch, epsilon=0.0)
+        assert torch.equal(O, want), power
