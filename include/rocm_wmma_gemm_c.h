@@ -263,14 +263,20 @@ int rocm_wmma_gemm_grouped_backward(int type_idx, void* dA, void* dB, void* dbia
                                     const void* B, const void* preact, const int* offsets, size_t groups, size_t M,
                                     size_t N, size_t K, int layout_b, int activation, int accumulate, void* stream);
 
-/* How a layer's product would run (operands that start on 16 bytes assumed; groups 0: linear). */
+/* How a layer's product would run (operands that start on 16 bytes assumed; groups 0: linear), or one of the
+ * products of an update's steps (rocm_wmma_gemm_orthogonalize): of M x N matrices, `groups` of them, type_idx
+ * one of those whose A has O's type; K, layout_b and activation are not looked at. */
 #define ROCM_WMMA_GEMM_PRODUCT_FORWARD 0
 #define ROCM_WMMA_GEMM_PRODUCT_GRADIENT_A 1
 #define ROCM_WMMA_GEMM_PRODUCT_GRADIENT_B 2
+#define ROCM_WMMA_GEMM_PRODUCT_STEPS_S 3    /* S = X X^T */
+#define ROCM_WMMA_GEMM_PRODUCT_STEPS_Q 4    /* Q = b S + c S^2 */
+#define ROCM_WMMA_GEMM_PRODUCT_STEPS_X 5    /* X = a X + Q X, but for the last step's */
+#define ROCM_WMMA_GEMM_PRODUCT_STEPS_LAST 6 /* the last step's */
 typedef struct rocm_wmma_gemm_product_plan
 {
-    int form; /* kernel: 0, 1 general (any alignment), 2-4 persistent tiles, 6 the same with C of any
-                 alignment, 7-13 few rows against a weight */
+    int form; /* kernel: 0, 1 general (any alignment), 2-5 persistent tiles, 6 the same with C of any
+                 alignment, 7-13 few rows against a weight, 14 all steps of a matrix in one workgroup */
     int block_m, block_n; /* its tile */
     int cut_tail; /* 1: tiles of the last round are cut along K and added up by a second kernel */
     int k_slices; /* few rows: workgroups that share a tile */

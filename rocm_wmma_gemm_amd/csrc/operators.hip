@@ -815,6 +815,66 @@ struct steps_scratch
     }
 };
 
+// The products of a step, without their pointers and factors: S = X X^T, Q = b S + c S^2, X = (a + diagonal) X + Q X.
+enum class step_part
+{
+    square,
+    poly,
+    next,
+    last
+};
+
+struct step_product
+{
+    product_args args;
+    int          types, layout, finish;
+};
+
+step_product product_of_step(step_part part, int out_type, const steps_scratch& at, size_t batch)
+{
+    product_args p{};
+    p.kind            = product_kind::batch;
+    p.groups          = static_cast<int>(batch);
+    p.stride_diagonal = static_cast<long long>(at.lp);
+    p.M               = static_cast<int>(at.lp);
+    if(part == step_part::square || part == step_part::poly)
+    {
+        const bool of_x = part == step_part::square;
+        p.N             = p.M;
+        p.K             = static_cast<int>(of_x ? at.hp : at.lp);
+        p.lda = p.ldb = p.K, p.ldc = at.lp;
+        p.stride_a = p.stride_b = static_cast<long long>(of_x ? at.each : at.square);
+        p.stride_c              = static_cast<long long>(at.square);
+        p.diagonal_is           = of_x ? device::diagonal_use::none : device::diagonal_use::split;
+        return {p, types_steps_square, layout_kk, of_x ? finish_square : finish_poly};
+    }
+    p.N = static_cast<int>(at.hp), p.K = static_cast<int>(at.lp);
+    p.lda = at.lp, p.ldb = p.ldc = at.hp;
+    p.stride_a = static_cast<long long>(at.square);
+    p.stride_b = p.stride_c = static_cast<long long>(at.each);
+    p.diagonal_is           = device::diagonal_use::rows;
+    if(part == step_part::next)
+    {
+        return {p, types_steps_next, layout_kn, finish_next};
+    }
+    return {p, out_type == ROCM_WMMA_GEMM_ELEMENT_F16 ? types_steps_f16 : types_steps_bf16, layout_kn, finish_last};
+}
+
+constexpr size_t most_update = size_t{1} << 20, most_updates = most_groups_y; // sides of a matrix, matrices
+
+// How many of a batch's matrices work at the same time: those whose state the scratch buffer may hold, in parts of
+// equal size.
+size_t updates_at_once(size_t M, size_t N, size_t batch)
+{
+    const size_t fit = std::max<size_t>(1, workspace_limit_bytes / steps_scratch(M, N, 1).bytes);
+    return ceil_div(batch, ceil_div(batch, fit));
+}
+
+bool fits_one_workgroup(size_t M, size_t N)
+{
+    return std::min(M, N) <= device::small_side && std::max(M, N) <= device::small_length;
+}
+
 // Newton-Schulz steps X <- a X + (b S + c S^2) X with S = X X^T on X = G / (|G| + epsilon), or on its
 // transpose where G is tall.
 //
@@ -877,51 +937,42 @@ int steps_in(char* ws, const update& u)
     };
     by_element(given_type, start);
     const float a = coefficients[0], b = coefficients[1], c = coefficients[2];
-    const size_t cus     = compute_units();
-    auto         product = [&](int types, int layout, int finish, const product_args& args) {
-        return launch_product(types, finish, choose(types, layout, finish, args, cus), args, nullptr, stream);
+    const size_t cus = compute_units();
+    auto         run = [&](const step_product& f) {
+        return launch_product(f.types, f.finish, choose(f.types, f.layout, f.finish, f.args, cus), f.args, nullptr, stream);
     };
-    product_args p{};
-    p.kind   = product_kind::batch;
-    p.groups = static_cast<int>(batch);
-    p.diagonal = diagonal, p.stride_diagonal = lp;
-    int rc   = ROCM_WMMA_GEMM_OK;
+    auto part = [&](step_part which, void* to, const void* left, const void* right, const void* added, float alpha, float beta) {
+        step_product f = product_of_step(which, out_type, at, batch);
+        f.args.diagonal = diagonal;
+        f.args.C = to, f.args.A = left, f.args.B = right, f.args.residual = added;
+        f.args.alpha = alpha, f.args.beta = beta;
+        return f;
+    };
+    int rc = ROCM_WMMA_GEMM_OK;
     for(int step = 0; step < steps && rc == ROCM_WMMA_GEMM_OK; ++step)
     {
-        _Float16* x    = x16[step & 1];
+        _Float16 * x = x16[step & 1], *next_x = x16[(step + 1) & 1];
         const bool last = step + 1 == steps;
-        // S = X X^T / scale^2
-        p.C = s, p.A = x, p.B = x, p.residual = nullptr, p.kept = nullptr;
-        p.M = p.N = static_cast<int>(lp), p.K = static_cast<int>(hp);
-        p.lda = p.ldb = hp, p.ldc = lp;
-        p.stride_a = p.stride_b = each, p.stride_c = square;
-        p.alpha = 1.0f / (scale * scale), p.beta = 0.0f, p.diagonal_is = device::diagonal_use::none;
-        rc = product(types_steps_square, layout_kk, finish_square, p);
+        rc = run(part(step_part::square, s, x, x, nullptr, 1.0f / (scale * scale), 0.0f));
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             break;
         }
-        // Q = b S + c S^2 (S is its own transpose), its diagonal apart
-        p.C = q, p.A = p.B = s, p.residual = s;
-        p.K = static_cast<int>(lp), p.lda = p.ldb = lp, p.stride_a = p.stride_b = square;
-        p.alpha = c, p.beta = b, p.diagonal_is = device::diagonal_use::split;
-        rc = product(types_steps_square, layout_kk, finish_poly, p);
+        // (S is its own transpose; Q's diagonal apart)
+        rc = run(part(step_part::poly, q, s, s, s, c, b));
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             break;
         }
-        // X = (a + diagonal) X + Q X
-        p.A = q, p.B = x;
-        p.M = static_cast<int>(lp), p.N = static_cast<int>(hp), p.K = static_cast<int>(lp);
-        p.lda = lp, p.ldb = hp, p.ldc = hp;
-        p.stride_a = square, p.stride_b = each, p.stride_c = each;
-        p.residual = x32, p.alpha = last ? 1.0f / scale : 1.0f, p.beta = last ? a / scale : a;
-        p.diagonal_is = device::diagonal_use::rows;
-        p.C = last ? (direct ? O : static_cast<void*>(x16[(step + 1) & 1])) : x32;
-        p.kept = last ? nullptr : x16[(step + 1) & 1], p.keep_sum = 1;
-        rc = product(!last ? types_steps_next : out_type == ROCM_WMMA_GEMM_ELEMENT_F16 ? types_steps_f16 : types_steps_bf16,
-                     layout_kn, last ? finish_last : finish_next, p);
-        p.keep_sum = 0;
+        if(last)
+        {
+            rc = run(part(step_part::last, direct ? O : static_cast<void*>(next_x), q, x, x32, 1.0f / scale, a / scale));
+            break;
+        }
+        step_product f  = part(step_part::next, x32, q, x, x32, 1.0f, a);
+        f.args.kept     = next_x;
+        f.args.keep_sum = 1;
+        rc              = run(f);
     }
     if(rc == ROCM_WMMA_GEMM_OK && !direct)
     {
@@ -937,7 +988,7 @@ int steps_in(char* ws, const update& u)
 
 int orthogonalize(const update& u)
 {
-    if(std::min(u.M, u.N) <= device::small_side && std::max(u.M, u.N) <= device::small_length)
+    if(fits_one_workgroup(u.M, u.N))
     {
         const device::steps_args small{u.G, u.O, static_cast<int>(u.M), static_cast<int>(u.N), u.steps, u.coefficients[0],
                                        u.coefficients[1], u.coefficients[2], u.epsilon};
@@ -950,9 +1001,7 @@ int orthogonalize(const update& u)
         by_element(u.given_type, run);
         return ROCM_WMMA_GEMM_OK;
     }
-    // (more matrices than the scratch buffer may hold the state of go in parts, of equal size)
-    const size_t fit  = std::max<size_t>(1, workspace_limit_bytes / steps_scratch(u.M, u.N, 1).bytes);
-    const size_t some = ceil_div(u.batch, ceil_div(u.batch, fit));
+    const size_t    some = updates_at_once(u.M, u.N, u.batch);
     workspace_lease lease;
     char*           ws = lease.acquire(steps_scratch(u.M, u.N, some).bytes, u.stream);
     if(ws == nullptr)
@@ -1063,6 +1112,41 @@ int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N,
                                   int activation, rocm_wmma_gemm_product_plan* plan)
 {
     return with_status([&] {
+        if(plan == nullptr || product < 0 || product > ROCM_WMMA_GEMM_PRODUCT_STEPS_LAST)
+        {
+            return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+        }
+        const auto answer = [&](const launch_choice& c) {
+            plan->form     = c.form;
+            plan->block_m  = c.kernel.block_m;
+            plan->block_n  = c.kernel.block_n;
+            plan->cut_tail = c.kernel.finish != nullptr && c.partial_bytes != 0;
+            plan->k_slices = c.k_slices;
+            plan->once     = c.once;
+            plan->copies   = (c.copy_a ? 1 : 0) | (c.copy_b ? 2 : 0);
+            return ROCM_WMMA_GEMM_OK;
+        };
+        if(product >= ROCM_WMMA_GEMM_PRODUCT_STEPS_S)
+        {
+            if(type_idx < 0 || type_idx > ROCM_WMMA_GEMM_TYPE_F32_BF16 || M == 0 || N == 0 || groups == 0)
+            {
+                return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+            }
+            if(M > most_update || N > most_update || groups > most_updates)
+            {
+                return ROCM_WMMA_GEMM_ERR_LIMIT;
+            }
+            if(fits_one_workgroup(M, N))
+            {
+                *plan = {num_product_forms, rocm_wmma_gemm::device::small_side, rocm_wmma_gemm::device::small_length, 0, 1, 0, 0};
+                return ROCM_WMMA_GEMM_OK;
+            }
+            const size_t       some = updates_at_once(M, N, groups);
+            const step_product f = product_of_step(static_cast<step_part>(product - ROCM_WMMA_GEMM_PRODUCT_STEPS_S),
+                                                   is_bf16(type_idx) ? ROCM_WMMA_GEMM_ELEMENT_BF16 : ROCM_WMMA_GEMM_ELEMENT_F16,
+                                                   steps_scratch(M, N, some), some);
+            return answer(choose(f.types, f.layout, f.finish, f.args, compute_units()));
+        }
         // (offsets that nobody reads: groups of rows are told by their presence)
         static const int somewhere = 0;
         layer            p{type_idx, M, N, K, layout_b, groups != 0 ? &somewhere : nullptr, groups != 0 ? groups : 1, {}};
@@ -1071,8 +1155,7 @@ int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N,
         {
             return rc;
         }
-        if(!activation_of(activation, &p.act) || plan == nullptr || product < 0 || product > ROCM_WMMA_GEMM_PRODUCT_GRADIENT_B
-           || M == 0 || N == 0)
+        if(!activation_of(activation, &p.act) || M == 0 || N == 0)
         {
             return ROCM_WMMA_GEMM_ERR_ARGUMENT;
         }
@@ -1085,15 +1168,7 @@ int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N,
         {
             return ROCM_WMMA_GEMM_ERR_ARGUMENT;
         }
-        const launch_choice c = choose(p.type_idx, f.layout, f.finish, f.args, compute_units());
-        plan->form            = c.form;
-        plan->block_m         = c.kernel.block_m;
-        plan->block_n         = c.kernel.block_n;
-        plan->cut_tail        = c.kernel.finish != nullptr && c.partial_bytes != 0;
-        plan->k_slices        = c.k_slices;
-        plan->once            = c.once;
-        plan->copies          = (c.copy_a ? 1 : 0) | (c.copy_b ? 2 : 0);
-        return ROCM_WMMA_GEMM_OK;
+        return answer(choose(p.type_idx, f.layout, f.finish, f.args, compute_units()));
     });
 }
 
@@ -1115,7 +1190,7 @@ int rocm_wmma_gemm_orthogonalize(int given_type, int out_type, void* O, const vo
         {
             return ROCM_WMMA_GEMM_ERR_ARGUMENT;
         }
-        if(M > (1u << 20) || N > (1u << 20) || batch_count > 65535)
+        if(M > most_update || N > most_update || batch_count > most_updates)
         {
             return ROCM_WMMA_GEMM_ERR_LIMIT;
         }

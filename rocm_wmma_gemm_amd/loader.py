@@ -495,13 +495,17 @@ class Loader:
         self._backward(self._lib.rocm_wmma_gemm_grouped_backward, "grouped_backward", dA, dB, dbias, dC, A, B, offsets, M, N, K, layout_b, preact, activation,
                        accumulate, stream)
 
+    _PRODUCTS = ("forward", "gradient_a", "gradient_b", "steps_s", "steps_q", "steps_x", "steps_last")
+
     def product_select(self, product: str, M: int, N: int, K: int, groups: int = 0, type_idx: int = 2,
                        layout_b=col_major, activation=activation.none) -> ProductPlan:
         """Which kernel ``product`` ("forward", "gradient_a" or "gradient_b") of linear() (groups = 0)
-        or grouped() runs on, and how; operands that start on 16 bytes assumed."""
+        or grouped() runs on, and how; operands that start on 16 bytes assumed.  Or a product of
+        orthogonalize() for ``groups`` M x N matrices: "steps_s" (X X^T), "steps_q" (b S + c S^2), "steps_x"
+        (a X + Q X) or "steps_last" (the last step's; type_idx one whose A has the type of O)."""
         c = _ProductPlanC()
         self._done("product_select", self._lib.rocm_wmma_gemm_product_select(
-            ("forward", "gradient_a", "gradient_b").index(product), type_idx, M, N, K, groups, int(layout_b),
+            self._PRODUCTS.index(product), type_idx, M, N, K, groups, int(layout_b),
             int(activation), ctypes.byref(c)))
         return ProductPlan(*[getattr(c, n) for n, _ in _ProductPlanC._fields_])
 

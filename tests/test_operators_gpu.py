@@ -809,3 +809,48 @@ def test_updates_of_any_scale(loader, shape, given):
         O = torch.full(shape, math.nan, dtype=F16, device="cuda")
         loader.orthogonalize(O, G * 2.0 ** power, M, N, batch, epsilon=0.0)
         assert torch.equal(O, want), power
+
+
+# Updates whose products run on each kernel form, with odd and even numbers of tile rows (128: 5, 9, 18; 192: 5, 22;
+# 256: 4, 5), odd sides, tall and wide, alone and in a batch.
+STEPS_COVERED = [(1, 8, 8), (1, 8, 300), (2, 65, 130), (3, 70, 900), (32, 8, 520), (64, 65, 65), (64, 900, 65), (1, 1024, 2048),
+                 (4, 1000, 520), (16, 1001, 520), (4, 1100, 1101), (1, 2304, 2304), (16, 900, 900), (1, 4096, 4096),
+                 (16, 1024, 1024), (16, 1275, 1280), (8, 768, 2304), (1, 1536, 4096), (1, 3000, 1100), (1, 4090, 1530)]
+
+
+def check_update(O, G, what):
+    """By norm, and element by element.  Where the norm of the error is within its bound, its root mean square is;
+    an element's error is a sum of many roundings, which pass eight times that in fewer than one of 10^14."""
+    want = steps64(G)
+    tol = STEPS_TOLERANCE[O.dtype]
+    for i in range(G.shape[0]):
+        err = O[i].double() - want[i]
+        size = want[i].norm() / math.sqrt(want[i].numel())
+        off = err.norm() / want[i].norm()
+        assert off <= tol, (what, i, off)
+        worst = (err.abs() - UNIT[O.dtype] * want[i].abs()).max() / size
+        assert worst <= 8 * tol, (what, i, worst, int((err.abs() - UNIT[O.dtype] * want[i].abs()).argmax()))
+
+
+@pytest.mark.parametrize("shape", STEPS_COVERED, ids=_id)
+@pytest.mark.parametrize("spectrum", ["noise", "few strong directions"])
+def test_updates_on_every_form(loader, shape, spectrum):
+    batch, M, N = shape
+    G = rnd(shape, F32, 1)
+    if spectrum != "noise":
+        rank = max(1, min(M, N) // 32)
+        G = 0.1 * G + torch.matmul(rnd((batch, M, rank), F32, 2), rnd((batch, rank, N), F32, 3))
+    for given, out in ((F32, BF16), (BF16, F16)):
+        O = torch.full(shape, math.nan, dtype=out, device="cuda")
+        loader.orthogonalize(O, G.to(given), M, N, batch)
+        check_update(O, G.to(given), f"{shape} {given} {out}")
+
+
+def test_the_updates_above_cover_the_forms(loader):
+    seen = {}
+    for batch, M, N in STEPS_COVERED:
+        for product in ("steps_s", "steps_q", "steps_x", "steps_last"):
+            for types in (0, 2):
+                seen.setdefault(product, set()).add(loader.product_select(product, M, N, 0, batch, types).form)
+    assert seen["steps_s"] >= {2, 3, 5, 9, 11, 12, 14} and seen["steps_q"] >= {2, 3, 5, 9, 11, 12, 14}, seen
+    assert seen["steps_x"] >= {2, 3, 4, 9, 10, 14} and seen["steps_last"] >= {2, 3, 4, 9, 10, 14}, seen

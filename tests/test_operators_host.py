@@ -213,3 +213,17 @@ def test_a_large_batch_of_updates_goes_in_parts(recorded):
     assert len(all64) == 2 * len(alone) and len(all65) == 2 * len(alone)
     assert [x[1] for x in all64[:2]] == [32, 32] and [x[1] for x in all65[:1] + all65[len(alone):len(alone) + 1]] == [33, 32]
     assert (refused, none) == (-3, [])
+
+
+def test_plans_of_an_update(library):
+    """The products of an update's steps are described like a layer's; small matrices stay in one workgroup."""
+    pick = lambda part, m, n, batch: library.product_select(part, m, n, 0, batch)  # noqa: E731
+    for part in ("steps_s", "steps_q", "steps_x", "steps_last"):
+        assert pick(part, 64, 256, 7).form == 14 and pick(part, 256, 64, 1).form == 14
+        assert pick(part, 64, 257, 1).form != 14
+        assert pick(part, 300, 200, 2) == pick(part, 200, 300, 2)  # a tall matrix is transposed
+        for m, n, batch in ((0, 8, 1), (8, 0, 1), (8, 8, 0), ((1 << 20) + 1, 8, 1), (8, 8, 65536)):
+            with pytest.raises(R.GemmLibraryError):
+                pick(part, m, n, batch)
+    large = pick("steps_s", 4096, 4096, 1)
+    assert (large.block_m, large.block_n) == (192, 192) and pick("steps_x", 4096, 4096, 1).block_m == 256
