@@ -813,8 +813,8 @@ def test_updates_of_any_scale(loader, shape, given):
 
 # Updates whose products run on each kernel form, with odd and even numbers of tile rows (128: 5, 9, 18; 192: 5, 22;
 # 256: 4, 5), odd sides, tall and wide, alone and in a batch.
-STEPS_COVERED = [(1, 8, 8), (1, 8, 300), (2, 65, 130), (3, 70, 900), (32, 8, 520), (64, 65, 65), (64, 900, 65), (1, 1024, 2048),
-                 (4, 1000, 520), (16, 1001, 520), (4, 1100, 1101), (1, 2304, 2304), (16, 900, 900), (1, 4096, 4096),
+STEPS_COVERED = [(1, 8, 8), (1, 8, 300), (32, 33, 262), (2, 65, 130), (3, 70, 900), (32, 8, 520), (64, 65, 65), (64, 900, 65),
+                 (1, 1024, 2048), (4, 1000, 520), (16, 1001, 520), (4, 1100, 1101), (1, 2304, 2304), (16, 900, 900), (1, 4096, 4096),
                  (16, 1024, 1024), (16, 1275, 1280), (8, 768, 2304), (1, 1536, 4096), (1, 3000, 1100), (1, 4090, 1530)]
 
 
@@ -853,4 +853,53 @@ def test_the_updates_above_cover_the_forms(loader):
             for types in (0, 2):
                 seen.setdefault(product, set()).add(loader.product_select(product, M, N, 0, batch, types).form)
     assert seen["steps_s"] >= {2, 3, 5, 9, 11, 12, 14} and seen["steps_q"] >= {2, 3, 5, 9, 11, 12, 14}, seen
-    assert seen["steps_x"] >= {2, 3, 4, 9, 10, 14} and seen["steps_last"] >= {2, 3, 4, 9, 10, 14}, seen
+    assert seen["steps_x"] >= {2, 3, 4, 9, 10, 11, 14} and seen["steps_last"] >= {2, 3, 4, 9, 10, 11, 14}, seen
+
+
+ACCUMULATED = [  # (M, N, K, groups, layout of B, types): gradients of weights
+    (40, 100, 77, 0, 1, 2), (300, 64, 64, 0, 1, 2), (4096, 520, 999, 0, 1, 3), (2048, 520, 512, 0, 1, 2), (3904, 512, 512, 1, 1, 3),
+    (4096, 4096, 512, 0, 0, 0), (777, 14336, 512, 0, 1, 1), (8192, 1024, 1024, 0, 0, 1), (1024, 4096, 4096, 0, 0, 3),
+    (4096, 5120, 5120, 0, 1, 2), (8192, 4352, 4608, 0, 1, 3), (2000, 2048, 4096, 4, 1, 1), (2048, 2048, 2048, 16, 1, 2),
+    (2048, 1024, 1000, 37, 0, 2), (3000, 2048, 1024, 11, 1, 3), (999, 1001, 999, 24, 1, 0),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ACCUMULATED)))
+def test_accumulated_gradients_on_every_form(loader, case):
+    """dB and dbias added to what is there, at the sizes of an accumulating training step: on each kernel form,
+    on tiles that are cut along the rows, on groups that are dealt to teams of workgroups."""
+    M, N, K, groups, layout, types = ACCUMULATED[case]
+    ab, out = PAIRS[types]
+    layout = R.m_layout(layout)
+    counts = routing(groups, M, case) if groups else [M]
+    if groups > 2:
+        counts[1] += counts[2]  # (a group without rows keeps what it has)
+        counts[2] = 0
+    ends, offsets = offsets_of(counts)
+    act = ACTS[case % 4]
+    A, dC, Z = rnd((M, K), ab, 1), rnd((M, N), ab, 3), rnd((M, N), ab, 4, 2.0)
+    shape = (N, K) if layout == R.col_major else (K, N)
+    lead = (groups,) if groups else ()
+    dB, dbias = rnd(lead + shape, out, 5), rnd(lead + (N,), out, 6)
+    old = (dB.clone(), dbias.clone())
+    for twice in range(2):
+        if groups:
+            loader.grouped_backward(None, dB, dbias, dC, A, None, offsets, M, N, K, layout, preact=Z, activation=act,
+                                    accumulate=True)
+        else:
+            loader.linear_backward(None, dB, dbias, dC, A, None, M, N, K, layout, preact=Z, activation=act, accumulate=True)
+        for e in range(len(counts)):
+            at, what = slice(ends[e], ends[e + 1]), f"{ACCUMULATED[case]} group {e}, call {twice}"
+            mine = (lambda t: t[e]) if groups else (lambda t: t)
+            shape_only = torch.zeros(shape, dtype=ab, device="cuda")
+            check_backward(None, mine(dB), mine(dbias), dC[at], Z[at], A[at], shape_only, layout, act, out, what,
+                           (mine(old[0]), mine(old[1])))
+            if counts[e] == 0:
+                assert torch.equal(mine(dB), mine(old[0])) and torch.equal(mine(dbias), mine(old[1])), what
+        old = (dB.clone(), dbias.clone())
+
+
+def test_the_accumulated_sizes_cover_the_forms(loader):
+    plans = [loader.product_select("gradient_b", M, N, K, groups, types, R.m_layout(layout))
+             for M, N, K, groups, layout, types in ACCUMULATED]
+    assert {p.form for p in plans} >= {1, 2, 3, 4, 6} and {p.form for p in plans if p.cut_tail} >= {2, 3, 4, 6}, plans
