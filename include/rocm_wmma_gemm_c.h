@@ -242,7 +242,7 @@ int rocm_wmma_gemm_linear(int type_idx, void* C, const void* A, const void* B, s
 /* With dZ = dC act'(preact) (preact may be NULL for ROCM_WMMA_GEMM_ACT_NONE):
  * dA = dZ B^T (M x K), dB = A^T dZ (in B's layout), dbias = sum of dZ's rows (N); a NULL result is not
  * computed.  accumulate 1: dB and dbias are added to.  dZ is rounded to A's type before it is
- * multiplied (not in dbias); it and the partial sums of dbias live in the library's scratch buffer, so a call
+ * multiplied (not in dbias), so that behind an activation gradients of type F32 hold dZ's 8 (bf16) or 11 (f16) bits; it and the partial sums of dbias live in the library's scratch buffer, so a call
  * on a capturing stream for which that buffer is too small returns ROCM_WMMA_GEMM_ERR_SCRATCH, and so does
  * any call for which they take more than 16 GiB (2 bytes an element of dZ, where there is an activation or dC's rows
  * do not start on 16 bytes, and N / 8 bytes a row for dbias).
@@ -290,6 +290,11 @@ int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N,
  * columns (all singular values near 1): X = G / (|G|_F + epsilon), then `steps` times
  * X = a X + (b S + c S^2) X with S = X X^T, coefficients = {a, b, c}; O = X.  G and O: batch_count
  * row-major M x N matrices; G of type F16, BF16 or F32, O of type F16 or BF16.  M and N up to 2^20.
+ * Matrices of up to 64 x 256 (either way up) are worked on in fp32.  The products of larger ones take f16
+ * operands (X, S and b S + c S^2 rounded to 11 bits; a X and the diagonal of b S + c S^2 stay in fp32), which leaves
+ * 6e-4 to 8e-4 of an update's norm after five steps with the usual coefficients (3.4445, -4.7750, 2.0315), and
+ * needs singular values s of the iterates with |b| s^2 + |c| s^4 and 2 s sqrt(min(M, N)) below 65504: with other
+ * coefficients that let them grow past that, O is infinite or no number.
  * Works in the library's scratch buffer (8 bytes an element and 4 min(M, N)^2 per matrix, 16 GiB at most: a
  * batch that needs more goes in parts, a single matrix that does returns ROCM_WMMA_GEMM_ERR_SCRATCH). */
 #define ROCM_WMMA_GEMM_ELEMENT_F16 0

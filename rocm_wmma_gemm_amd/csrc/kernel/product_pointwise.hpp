@@ -11,9 +11,12 @@ namespace rocm_wmma_gemm
 namespace device
 {
 
-// dZ = dC * act'(Z), and the sums of its columns over runs of slope_rows rows of a group.  4096 x 5120
-// bf16: 29 us, 4.35 TB/s; 8192 x 4096 in 16 groups 52 us, 3.9 TB/s.  Runs of 16 or 64 rows and non-temporal
-// loads change a backward pass by less than 2 %, up for some sizes and down for others.
+// dZ = dC * act'(Z), and the sums of its columns over runs of slope_rows rows of a group.  dZ is rounded to A's
+// type, as both products need it: the matrix cores' 16-bit rate takes 16-bit operands, and one for its upper
+// and one for its lower half would double the products.  It costs 2.3e-3 of a bf16 gradient's norm against 1.7e-3
+// for the rounding of the result alone.  The sums are of the values before that rounding.  4096 x 5120 bf16: 29 us,
+// 4.35 TB/s; 8192 x 4096 in 16 groups 52 us, 3.9 TB/s.  Runs of 16 or 64 rows and non-temporal loads change
+// a backward pass by less than 2 %, up for some sizes and down for others.
 constexpr int slope_rows = 32; // rows of a run (a workgroup's); a group's last run is shorter
 
 struct slope_args

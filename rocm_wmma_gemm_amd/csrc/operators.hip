@@ -878,10 +878,13 @@ bool fits_one_workgroup(size_t M, size_t N)
 // Newton-Schulz steps X <- a X + (b S + c S^2) X with S = X X^T on X = G / (|G| + epsilon), or on its
 // transpose where G is tall.
 //
-// What is rounded, and why: products take f16 operands.  Every singular value of X stays below
-// 1.3, so f16 holds X (scaled by about the root of its smaller side, a power of two, which
-// keeps its elements near 1), S and Q = b S + c S^2 with 11 bits; bf16 would leave 8.  Two terms
-// are kept from that rounding, because it is the largest part of the error there:
+// What is rounded, and why: products of matrices past small_side x small_length take f16 operands.  With the
+// coefficients that are the Python default every singular value of X stays below 1.3, so f16 holds X (scaled by
+// about the root of its smaller side, a power of two, which keeps its elements near 1), S and Q = b S + c S^2
+// with 11 bits; bf16 would leave 8.  Coefficients whose iterates grow are right as long as f16 holds those three:
+// |b| s^2 + |c| s^4 and s times twice the root of the smaller side below 65504 for the largest singular value s of an
+// iterate.  Past it Q or X turns infinite, and the update is no number.  Two terms are kept from the rounding,
+// because it is the largest part of the error there:
 //   - a X: small singular directions grow 3.4 times a step, and a rounding of the large ones
 //     (white noise in all directions) with them, so X is also kept in fp32 and only the products
 //     see the f16 copy;

@@ -513,7 +513,9 @@ class Loader:
                       coefficients=(3.4445, -4.7750, 2.0315), epsilon: float = 1e-7, stream=None) -> None:
         """O = G / (|G| + epsilon) after ``steps`` Newton-Schulz steps x -> a x + b x^3 + c x^5 on
         its singular values, for a batch of row-major M x N matrices: an update with singular
-        values near 1.  G: f16, bf16 or f32; O: f16 or bf16."""
+        values near 1.  G: f16, bf16 or f32; O: f16 or bf16.  Matrices past 64 x 256 are multiplied with f16
+        operands: coefficients may not let the singular values s of an iterate grow past |b| s^2 + |c| s^4 or
+        2 s sqrt(min(M, N)) of 65504 (with the default they stay below 1.3); smaller ones are worked on in fp32."""
         import torch
 
         self._sizes(M, N, batch_count)

@@ -903,3 +903,38 @@ def test_the_accumulated_sizes_cover_the_forms(loader):
     plans = [loader.product_select("gradient_b", M, N, K, groups, types, R.m_layout(layout))
              for M, N, K, groups, layout, types in ACCUMULATED]
     assert {p.form for p in plans} >= {1, 2, 3, 4, 6} and {p.form for p in plans if p.cut_tail} >= {2, 3, 4, 6}, plans
+
+
+def steps_bound(G, steps, coefficients, out, epsilon=1e-7):
+    """What f16 operands may leave of an update, to first order, in the Frobenius norm: every operand is off by
+    2^-11 of itself, and a step passes on what came before times the largest slope of its polynomial."""
+    a, b, c = coefficients
+    u, X = 2.0 ** -11, G.double()
+    X = X / (X.norm() + epsilon)
+    X = X.t().contiguous() if X.shape[0] > X.shape[1] else X
+    norm2 = lambda t: torch.linalg.matrix_norm(t, 2).item()  # noqa: E731
+    normf = lambda t: t.norm().item()  # noqa: E731
+    E = 0.0
+    for _ in range(steps):
+        S = X @ X.t()
+        Q = b * S + c * (S @ S)
+        x2, s2 = norm2(X), norm2(S)
+        dS = 2 * u * x2 * normf(X) + u * normf(S)
+        dQ = abs(b) * dS + abs(c) * (2 * s2 * dS + 2 * u * s2 * normf(S)) + u * normf(Q)
+        E = E * (abs(a) + 3 * abs(b) * x2 ** 2 + 5 * abs(c) * x2 ** 4) + dQ * x2 + u * norm2(Q) * normf(X)
+        X = a * X + Q @ X
+    return 1.1 * E / normf(X) + UNIT[out]
+
+
+@pytest.mark.parametrize("shape", [(64, 256), (256, 64), (64, 257), (65, 256), (300, 200), (520, 1001)], ids=_id)
+@pytest.mark.parametrize("steps, coefficients", [(2, (3.0, -1.0, 0.0)), (1, (4.0, -2.0, 0.0)), (2, (2.0, 1.0, 1.0))], ids=_id)
+def test_updates_whose_singular_values_grow(loader, shape, steps, coefficients):
+    """Coefficients whose iterates reach 2 (and back), 2 and several hundred, on both sides of the size from which
+    operands are rounded to f16."""
+    M, N = shape
+    G = 0.02 * rnd((M, N), F32, 1) / math.sqrt(M + N) + torch.outer(rnd((M,), F32, 2), rnd((N,), F32, 3)) / math.sqrt(M * N)
+    O = torch.full((M, N), math.nan, dtype=BF16, device="cuda")
+    loader.orthogonalize(O, G, M, N, steps=steps, coefficients=coefficients)
+    want = steps64(G[None], steps, coefficients)[0]
+    off = ((O.double() - want).norm() / want.norm()).item()
+    assert off <= steps_bound(G, steps, coefficients, BF16), off
