@@ -690,8 +690,10 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     launch_choice      on_a, on_b;
     device::slope_args s{};
     // dZ and the sums of its columns live in the scratch buffer, and what the products ask for
-    // (a dC whose rows do not start on 16 bytes is copied to rows that do, as dZ is written)
-    const bool   pitched = sloped || p.N % 8 != 0 || !aligned16(dC);
+    // (a dC whose rows do not start on 16 bytes is copied to rows that do, as dZ is written; for the bias alone
+    // there is nobody to read either)
+    const bool   wants_a = dA != nullptr && p.M != 0 && p.K != 0, wants_b = dB != nullptr && p.N != 0 && p.K != 0;
+    const bool   pitched = (wants_a || wants_b) && (sloped || p.N % 8 != 0 || !aligned16(dC));
     const bool   passes  = (pitched || dbias != nullptr) && p.N != 0;
     const size_t pitch   = pitched ? round_up8(p.N) : p.N;
     const size_t runs   = p.M / device::slope_rows + std::min(p.groups, p.M);
@@ -710,11 +712,11 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
     to_b.args.residual = accumulate ? dB : nullptr;
     (p.layout_b == 1 ? to_b.args.B : to_b.args.A) = A;
     placed(dz_bytes != 0 ? nullptr : dC);
-    if(dA != nullptr && p.M != 0 && p.K != 0)
+    if(wants_a)
     {
         on_a = choose(p.type_idx, to_a.layout, to_a.finish, to_a.args, cus);
     }
-    if(dB != nullptr && p.N != 0 && p.K != 0)
+    if(wants_b)
     {
         on_b = choose(p.type_idx, to_b.layout, to_b.finish, to_b.args, cus);
     }

@@ -227,3 +227,10 @@ def test_plans_of_an_update(library):
                 pick(part, m, n, batch)
     large = pick("steps_s", 4096, 4096, 1)
     assert (large.block_m, large.block_n) == (192, 192) and pick("steps_x", 4096, 4096, 1).block_m == 256
+
+
+def test_the_bias_alone_needs_no_dz(recorded):
+    """dbias without dA and dB is answered where dZ itself (34 GB here) would pass the scratch buffer."""
+    bias_only = lambda n, act: ["linear_backward", [2, None, None, "p", "p", None, None, "p", 1 << 28, n, 8, 1, act, 0, None]]  # noqa: E731
+    for status, launches in recorded(bias_only(64, 2), bias_only(63, 0)):
+        assert status == 0 and len(launches) >= 2, (status, launches)
