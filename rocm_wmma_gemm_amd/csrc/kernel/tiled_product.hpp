@@ -131,12 +131,16 @@ struct tiled_product
         // (where groups differ in K the slices would too: those launches are not cut; a single group's sum is
         // cut by the rows it has, which its offsets say)
         const bool may_cut = args.partials != nullptr && !EPI::mirror && (args.kind != product_kind::sum || args.groups == 1);
-        const int  rows    = args.kind == product_kind::sum ? off[1] - off[0] : 0;
-        tail_cut   cut     = cut_tail(tiles, workgroups, summed_tiles(args.kind, args.K, rows, BK), may_cut);
-        cut.whole          = __builtin_amdgcn_readfirstlane(cut.whole);
-        cut.cut            = __builtin_amdgcn_readfirstlane(cut.cut);
-        cut.slices         = __builtin_amdgcn_readfirstlane(cut.slices);
-        cut.each           = __builtin_amdgcn_readfirstlane(cut.each);
+        tail_cut   cut{tiles, 0, 1, 0};
+        if(may_cut)
+        {
+            const int rows = args.kind == product_kind::sum ? off[1] - off[0] : 0;
+            cut            = cut_tail(tiles, workgroups, summed_tiles(args.kind, args.K, rows, BK), true);
+            cut.whole      = __builtin_amdgcn_readfirstlane(cut.whole);
+            cut.cut        = __builtin_amdgcn_readfirstlane(cut.cut);
+            cut.slices     = __builtin_amdgcn_readfirstlane(cut.slices);
+            cut.each       = __builtin_amdgcn_readfirstlane(cut.each);
+        }
         return {off, first, order, cut, 0, cut.positions(), (int)blockIdx.x, workgroups};
     }
 
