@@ -292,7 +292,7 @@ int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N,
  * row-major M x N matrices; G of type F16, BF16 or F32, O of type F16 or BF16.  M and N up to 2^20.
  * Matrices of up to 64 x 256 (either way up) are worked on in fp32.  The products of larger ones take f16
  * operands (X, S and b S + c S^2 rounded to 11 bits; a X and the diagonal of b S + c S^2 stay in fp32), which leaves
- * 6e-4 to 8e-4 of an update's norm after five steps with the usual coefficients (3.4445, -4.7750, 2.0315), and
+ * up to 8e-4 of an update's norm after five steps with the usual coefficients (3.4445, -4.7750, 2.0315), and
  * needs singular values s of the iterates with |b| s^2 + |c| s^4 and 2 s sqrt(min(M, N)) below 65504: with other
  * coefficients that let them grow past that, O is infinite or no number.
  * Works in the library's scratch buffer (8 bytes an element and 4 min(M, N)^2 per matrix, 16 GiB at most: a

@@ -893,8 +893,9 @@ bool fits_one_workgroup(size_t M, size_t N)
 //   - Q's diagonal: near the end Q is about -2.7 I, and rounding that moves whole rows of X by
 //     four times as much.  The diagonal stays in fp32 beside Q, whose own is zero, and meets the
 //     fp32 X in the epilogue: X = (a + diagonal) X + Q X.
-// Against 64 bits, 512 x 1024: 7.5e-4 for noise, 2.4e-4 for a momentum of 16 strong directions (2.1e-2
-// with all of it from f16, 1.6e-1 from bf16); 1 x 40: 7.2e-4 (3.7e-3 with the diagonal in f16).
+// Against 64 bits, an f16 update of 512 x 1024 is 7.8e-4 off for noise and 3.2e-4 for a momentum of 16 strong
+// directions, where the rounding of the result leaves 2.1e-4 (simulated for the latter: 2.1e-2 with all of it from
+// f16, 1.6e-1 from bf16); 1 x 300: 3.7e-4.
 int steps_in(char* ws, const update& u)
 {
     const size_t        M = u.M, N = u.N, batch = u.batch;
