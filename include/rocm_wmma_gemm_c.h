@@ -303,6 +303,67 @@ int rocm_wmma_gemm_product_select(int product, int type_idx, size_t M, size_t N,
 int rocm_wmma_gemm_orthogonalize(int given_type, int out_type, void* O, const void* G, size_t M, size_t N,
                                  size_t batch_count, int steps, const float* coefficients, float epsilon, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * From a router to the experts and back: additions with no counterpart in the reference.
+ *
+ * M tokens choose k of E experts each.  route picks them from the router's logits (M x E), dispatch sorts the
+ * tokens' rows by expert and writes the row offsets that rocm_wmma_gemm_grouped reads, combine sums the experts' rows
+ * by token.  All matrices are row-major and packed and may start on any element; element types are
+ * ROCM_WMMA_GEMM_ELEMENT_* as above.  E up to 512, k up to 32, M k up to 2^31 - 256.  A size of 0 is no error.  The
+ * calls enqueue on *stream and return; none but dispatch (past 4096 choices) uses the library's scratch buffer.
+ * --------------------------------------------------------------------------------------- */
+#define ROCM_WMMA_GEMM_SCORE_SOFTMAX 0 /* e^x over the sum of all e^x */
+#define ROCM_WMMA_GEMM_SCORE_SIGMOID 1 /* 1 / (1 + e^-x) */
+
+#define ROCM_WMMA_GEMM_MAX_EXPERTS 512
+#define ROCM_WMMA_GEMM_MAX_CHOICES 32
+#define ROCM_WMMA_GEMM_MAX_EXPERT_GROUPS 16
+
+typedef struct rocm_wmma_gemm_routing
+{
+    int                  score; /* ROCM_WMMA_GEMM_SCORE_* */
+    const float*         bias; /* E values added to the scores for the choice alone, or NULL */
+    const unsigned char* mask; /* M values, 0: the token goes nowhere; or NULL */
+    int                  groups; /* the experts form this many groups of neighbours (1: no groups); divides E */
+    int                  kept_groups; /* a token chooses from this many of them */
+    int                  group_best; /* 1 or 2: the sum of so many of a group's best biased scores decides which are kept */
+    int                  renormalize; /* 1: a token's weights are divided by the sum of their scores */
+    float                scale; /* and multiplied by this */
+} rocm_wmma_gemm_routing;
+
+/* chosen (M x k): the experts of the largest biased score, of the largest logit where there is no bias, the best
+ * first; of equal ones the lower expert.  weights (M x k): their scores, without the bias.  What decides is worked out in
+ * fp64.  A masked token's experts are -1, its weights 0.  A logit of -infinity has the score 0; a token whose chosen
+ * scores are all 0 has weights 0.  A logit that is no number is chosen last, and its token's weights may be no numbers. */
+int rocm_wmma_gemm_route(int logits_type, int* chosen, float* weights, const void* logits,
+                         const rocm_wmma_gemm_routing* routing, size_t M, size_t E, size_t k, void* stream);
+
+/* dlogits (M x E, the logits' type) from dweights (M x k): the gradient of the weights; the choice has none, nor has
+ * the bias.  chosen: route's; an expert outside 0 .. E - 1 has no gradient. */
+int rocm_wmma_gemm_route_backward(int logits_type, void* dlogits, const float* dweights, const int* chosen,
+                                  const void* logits, size_t M, size_t E, size_t k, int score, int renormalize, float scale,
+                                  void* stream);
+
+/* offsets (E + 1): where every expert's rows start when the choices are sorted by expert, within an expert in
+ * their order; places (M x k): the row of every choice, -1 for one outside 0 .. E - 1 (it has no row); rows (M k x N of
+ * rows_type): row places[t k + j] is row t of X (M x N).  rows may be NULL: then X is not read.  Rows from
+ * offsets[E] on are left as they were.  The gradient of X is combine without weights of rows'. */
+int rocm_wmma_gemm_dispatch(int rows_type, void* rows, int* offsets, int* places, const void* X, const int* chosen,
+                            size_t E, size_t M, size_t N, size_t k, void* stream);
+
+/* C (M x N): the sum over a token's choices of weights[t k + j] (NULL: 1) times row places[t k + j] of rows (M k x
+ * N), plus residual (M x N of C's type, or NULL; may be C itself).  A place outside 0 .. M k - 1 adds nothing.  Summed
+ * in fp32 in the order of the choices, rounded once.  out_type: rows_type or F32. */
+int rocm_wmma_gemm_combine(int rows_type, int out_type, void* C, const void* rows, const int* places, const float* weights,
+                           const void* residual, size_t M, size_t N, size_t k, void* stream);
+
+/* drows (M k x N of rows_type, or NULL): weight times dC's row, for the rows that places name (each once); the others
+ * are left as they were.  dweights (M x k, or NULL): the product of dC's row with the choice's, 0 for a
+ * place outside 0 .. M k - 1.  dC: M x N of out_type; rows may be NULL where dweights is. */
+int rocm_wmma_gemm_combine_backward(int rows_type, int out_type, void* drows, float* dweights, const void* dC,
+                                    const void* rows, const int* places, const float* weights, size_t M, size_t N, size_t k,
+                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,8 +16,9 @@ from .loader import (  # noqa: F401
     library_path,
     m_layout,
     row_major,
+    score,
     source_stamp,
 )
 
-__all__ = ["Loader", "GemmLibraryError", "VariantInfo", "m_layout", "row_major", "col_major", "activation",
+__all__ = ["Loader", "GemmLibraryError", "VariantInfo", "m_layout", "row_major", "col_major", "activation", "score",
            "library_path", "build_library", "source_stamp"]

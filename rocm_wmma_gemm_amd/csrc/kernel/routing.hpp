@@ -1,0 +1,754 @@
+// The kernels from a router's logits to rows sorted by expert and back: the choice of the experts with its
+// gradient, the sort of the choices with the copy of their rows, the weighted sum of the experts' rows with its
+// gradients.  All are bound by memory, or by the latency of a launch where there are few tokens.
+#ifndef ROCM_WMMA_GEMM_ROUTING_HPP
+#define ROCM_WMMA_GEMM_ROUTING_HPP
+
+#include "product_common.hpp"
+
+namespace rocm_wmma_gemm
+{
+namespace device
+{
+
+constexpr int route_lanes   = 16; // of a token
+constexpr int most_choices  = 32; // experts of a token
+constexpr int most_parts    = 16; // groups of experts
+constexpr int most_dispatch = max_groups; // experts
+
+// ------------------------------------------------------------------ sixteen lanes together
+
+// The value of the lane that `control` names within the row of 16 lanes.
+template<int CONTROL, class T>
+__device__ __forceinline__ T from_row(T v)
+{
+    if constexpr(sizeof(T) == 8)
+    {
+        const unsigned long long b  = __builtin_bit_cast(unsigned long long, v);
+        const unsigned int       lo = __builtin_amdgcn_update_dpp(0, (int)b, CONTROL, 0xf, 0xf, false);
+        const unsigned int       hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CONTROL, 0xf, 0xf, false);
+        return __builtin_bit_cast(T, (unsigned long long)hi << 32 | lo);
+    }
+    else
+    {
+        const int b = __builtin_bit_cast(int, v);
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, b, CONTROL, 0xf, 0xf, false));
+    }
+}
+
+// Joins the values of 1, 2, 4, 8 or 16 neighbouring lanes, in every one of them: neighbours, pairs, then the mirror
+// images in 8 and in 16 lanes (whose values are equal within 4 and 8 by then).
+template<class T, class Join>
+__device__ __forceinline__ T join_row(T v, int lanes, Join join)
+{
+    v = lanes > 1 ? join(v, from_row<0xb1>(v)) : v; // quad_perm 1 0 3 2
+    v = lanes > 2 ? join(v, from_row<0x4e>(v)) : v; // quad_perm 2 3 0 1
+    v = lanes > 4 ? join(v, from_row<0x141>(v)) : v; // row_half_mirror
+    v = lanes > 8 ? join(v, from_row<0x140>(v)) : v; // row_mirror
+    return v;
+}
+
+template<class T>
+__device__ __forceinline__ T sum_of_row(T v)
+{
+    return join_row(v, route_lanes, [](T a, T b) { return a + b; });
+}
+
+// The value of lane `from` of the token's sixteen.
+template<class T>
+__device__ __forceinline__ T of_lane(T v, int from)
+{
+    const int lane = (int)(threadIdx.x & 48) | from;
+    if constexpr(sizeof(T) == 8)
+    {
+        const unsigned long long b  = __builtin_bit_cast(unsigned long long, v);
+        const unsigned int       lo = __shfl((int)b, lane), hi = __shfl((int)(b >> 32), lane);
+        return __builtin_bit_cast(T, (unsigned long long)hi << 32 | lo);
+    }
+    else
+    {
+        return __builtin_bit_cast(T, __shfl(__builtin_bit_cast(int, v), lane));
+    }
+}
+
+// ------------------------------------------------------------------ the choice
+
+struct route_args
+{
+    int*         chosen; // tokens x k
+    float*       weights; // tokens x k
+    const void*  logits; // tokens x experts
+    const float* bias; // nullptr, or one an expert: added for the choice alone
+    const unsigned char* mask; // nullptr, or one a token: 0 goes nowhere
+    long long    tokens;
+    int          experts, k;
+    int          groups, size; // of experts: experts = groups * size
+    int          kept, best; // groups that a token may choose from; how many of its best make a group's score
+    int          spread, chunk; // lanes of a group, and experts of a lane (spread * chunk >= size, spread * groups <= 16)
+    int          renormalize;
+    float        scale;
+};
+
+// A choice as one number that v_max_f64 orders: the value, whose last 9 bits tell the expert, so that of equal
+// values the lower expert is more.  (The values that the bits can confuse differ by 2^-44 of themselves; logits, which
+// have 24 bits, none.)  No number counts as the lowest value.
+constexpr unsigned long long choice_bits = 511;
+__device__ __forceinline__ double choice_key(double value, int expert)
+{
+    constexpr double most = 1.7976931348623157e308;
+    value = value >= -most ? value : -most;
+    value = (value <= most ? value : most) + 0.0;
+    unsigned long long b = __builtin_bit_cast(unsigned long long, value);
+    b = (b & ~choice_bits) | (unsigned long long)((b >> 63) != 0 ? expert : (int)choice_bits - expert);
+    return __builtin_bit_cast(double, b);
+}
+__device__ __forceinline__ int expert_of_key(double key)
+{
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, key);
+    return (b >> 63) != 0 ? (int)(b & choice_bits) : (int)(choice_bits - (b & choice_bits));
+}
+
+// Sixteen lanes a token, CHUNK experts a lane (args.chunk of them used).  Mathematics: scores s = softmax(x) or
+// 1 / (1 + e^-x); the k experts of the largest s + bias (of the largest x where there is no bias: the same order)
+// among the experts of the `kept` groups whose `best` largest s + bias sum to most; weights scale s, or scale s over the
+// sum of the chosen s.  Everything that decides is held in fp64, so that the choice is the definition's and not that of
+// a rounding: fp64 runs at the fp32 rate here.
+template<class InT, int CHUNK, bool SIGMOID>
+__device__ __forceinline__ void route_token(const route_args& args, long long token, int lane)
+{
+    const InT* const x     = static_cast<const InT*>(args.logits) + token * args.experts;
+    const int        group = lane / args.spread, within = lane % args.spread * args.chunk;
+    const int        first = group * args.size + within; // this lane's experts: first .. first + count - 1
+    int              count = args.size - within;
+    count                  = count < args.chunk ? count : args.chunk;
+    count                  = group < args.groups && count > 0 ? count : 0;
+    const double least = -__builtin_inf();
+    float        logit[CHUNK];
+#pragma unroll
+    for(int i = 0; i < CHUNK; ++i)
+    {
+        logit[i] = i < count ? (float)x[first + i] : -__builtin_inff();
+    }
+    const bool by_score = args.bias != nullptr || args.groups > 1;
+    // softmax: its largest logit and sum, where the scores need them
+    double top = 0.0, total = 1.0;
+    if constexpr(!SIGMOID)
+    {
+        float most = -__builtin_inff();
+#pragma unroll
+        for(int i = 0; i < CHUNK; ++i)
+        {
+            most = __builtin_fmaxf(most, logit[i]);
+        }
+        most = join_row(most, route_lanes, [](float a, float b) { return __builtin_fmaxf(a, b); });
+        top  = most > -__builtin_inff() ? (double)most : 0.0; // (no finite logit: all scores are 0)
+        if(by_score || !args.renormalize)
+        {
+            double sum = 0.0;
+#pragma unroll
+            for(int i = 0; i < CHUNK; ++i)
+            {
+                sum += i < count ? exp((double)logit[i] - top) : 0.0;
+            }
+            sum   = sum_of_row(sum);
+            total = sum == 0.0 ? 1.0 : sum;
+        }
+    }
+    auto score = [&](float l) {
+        return SIGMOID ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - top) / total;
+    };
+    double key[CHUNK];
+    double high = least, second = least; // the lane's two best values
+#pragma unroll
+    for(int i = 0; i < CHUNK; ++i)
+    {
+        double value = (double)logit[i];
+        if(by_score)
+        {
+            const double s = i < count ? score(logit[i]) + (args.bias != nullptr ? (double)args.bias[first + i] : 0.0) : least;
+            const double v = s >= least ? s : least; // (no number: the lowest)
+            second         = __builtin_fmax(second, __builtin_fmin(high, v));
+            high           = __builtin_fmax(high, v);
+            value          = args.bias != nullptr ? s : value;
+        }
+        key[i] = i < count ? choice_key(value, first + i) : least;
+    }
+    if(args.groups > 1)
+    {
+        // the group's two best, over its lanes
+        const int spread = args.spread;
+        auto      meet   = [&](double h, double s) {
+            second = __builtin_fmax(__builtin_fmin(high, h), __builtin_fmax(second, s));
+            high   = __builtin_fmax(high, h);
+        };
+        if(spread > 1)
+        {
+            meet(from_row<0xb1>(high), from_row<0xb1>(second));
+        }
+        if(spread > 2)
+        {
+            meet(from_row<0x4e>(high), from_row<0x4e>(second));
+        }
+        if(spread > 4)
+        {
+            meet(from_row<0x141>(high), from_row<0x141>(second));
+        }
+        const double of_group = args.best > 1 && args.size > 1 ? high + second : high;
+        int          better   = 0;
+        for(int g = 0; g < args.groups; ++g)
+        {
+            const double other = of_lane(of_group, g * spread);
+            better += other > of_group || (other == of_group && g < group);
+        }
+        if(better >= args.kept)
+        {
+#pragma unroll
+            for(int i = 0; i < CHUNK; ++i)
+            {
+                key[i] = least;
+            }
+        }
+    }
+    // k times the largest of all lanes' keys
+    int mine[2] = {0, 0};
+    for(int j = 0; j < args.k; ++j)
+    {
+        double most = key[0];
+#pragma unroll
+        for(int i = 1; i < CHUNK; ++i)
+        {
+            most = __builtin_fmax(most, key[i]);
+        }
+        most = join_row(most, route_lanes, [](double a, double b) { return __builtin_fmax(a, b); });
+#pragma unroll
+        for(int i = 0; i < CHUNK; ++i)
+        {
+            key[i] = key[i] == most ? least : key[i];
+        }
+        const int e = expert_of_key(most);
+        mine[0]     = lane == j ? e : mine[0];
+        mine[1]     = lane + route_lanes == j ? e : mine[1];
+    }
+    // lane j: the j-th and the (16 + j)-th choice
+    const bool real = args.mask == nullptr || args.mask[token] != 0;
+    double     s[2];
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+    {
+        s[h] = lane + h * route_lanes < args.k ? score((float)x[mine[h]]) : 0.0;
+    }
+    double factor = args.scale;
+    if(args.renormalize)
+    {
+        const double sum = sum_of_row(s[0] + s[1]);
+        factor           = sum == 0.0 ? 0.0 : factor / sum;
+    }
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+    {
+        const int j = lane + h * route_lanes;
+        if(j < args.k)
+        {
+            args.chosen[token * args.k + j]  = real ? mine[h] : -1;
+            args.weights[token * args.k + j] = real ? (float)(factor * s[h]) : 0.0f;
+        }
+    }
+}
+
+// (all lanes of a token leave the loop together)
+template<class InT, int CHUNK, bool SIGMOID>
+__global__ void __launch_bounds__(256) route(const route_args args)
+{
+    constexpr int each = 256 / route_lanes; // tokens of a workgroup
+    for(long long token = (long long)blockIdx.x * each + threadIdx.x / route_lanes; token < args.tokens;
+        token += (long long)gridDim.x * each)
+    {
+        route_token<InT, CHUNK, SIGMOID>(args, token, threadIdx.x % route_lanes);
+    }
+}
+
+struct route_back_args
+{
+    void*        dlogits; // tokens x experts, of the logits' type
+    const float* dweights; // tokens x k
+    const int*   chosen; // tokens x k
+    const void*  logits;
+    long long    tokens;
+    int          experts, k, renormalize;
+    float        scale;
+};
+
+// The gradient of the weights by the logits; the choice itself has none.  With ds_j = scale (dw_j - D) / sum, D = sum_i dw_i
+// w_i / scale, (renormalised; else scale dw_j): sigmoid dx_j = ds_j s_j (1 - s_j) for the chosen, 0 for the others; softmax
+// dx_e = s_e (ds_e - sum_j s_j ds_j), where the sum is 0 if the weights are renormalised, so that the logits
+// that were not chosen are not even read.  Sixteen lanes a token; a choice outside the experts has no gradient, one
+// that is listed twice has both.
+template<class InT, bool SIGMOID>
+__device__ __forceinline__ void route_back_token(const route_back_args& args, long long token, int lane)
+{
+    const InT* const x  = static_cast<const InT*>(args.logits) + token * args.experts;
+    InT* const       dx = static_cast<InT*>(args.dlogits) + token * args.experts;
+    int              e[2];
+    float            dw[2], logit[2];
+    float            most = -__builtin_inff();
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+    {
+        const int j = lane + h * route_lanes;
+        e[h]        = j < args.k ? args.chosen[token * args.k + j] : -1;
+        e[h]        = e[h] >= 0 && e[h] < args.experts ? e[h] : -1;
+        dw[h]       = e[h] >= 0 ? args.dweights[token * args.k + j] : 0.0f;
+        logit[h]    = e[h] >= 0 ? (float)x[e[h]] : -__builtin_inff();
+        most        = __builtin_fmaxf(most, logit[h]);
+    }
+    const bool none  = sum_of_row((e[0] >= 0 ? 1 : 0) + (e[1] >= 0 ? 1 : 0)) == 0; // (a token that went nowhere)
+    const bool dense = !SIGMOID && !args.renormalize && !none;
+    float      top = 0.0f, total = 1.0f;
+    if constexpr(!SIGMOID)
+    {
+        if(dense)
+        {
+            for(int i = lane; i < args.experts; i += route_lanes)
+            {
+                most = __builtin_fmaxf(most, (float)x[i]);
+            }
+        }
+        top = join_row(most, route_lanes, [](float a, float b) { return __builtin_fmaxf(a, b); });
+        top = top > -__builtin_inff() ? top : 0.0f;
+        if(dense)
+        {
+            float sum = 0.0f;
+            for(int i = lane; i < args.experts; i += route_lanes)
+            {
+                sum += expf((float)x[i] - top);
+            }
+            sum   = sum_of_row(sum);
+            total = sum == 0.0f ? 1.0f : sum;
+        }
+    }
+    float s[2], ds[2];
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+    {
+        s[h]  = e[h] < 0 ? 0.0f : SIGMOID ? 1.0f / (1.0f + expf(-logit[h])) : expf(logit[h] - top) / total;
+        ds[h] = args.scale * dw[h];
+    }
+    if(args.renormalize)
+    {
+        const float sum  = sum_of_row(s[0] + s[1]);
+        const float rest = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float dot  = sum_of_row(ds[0] * s[0] * rest + ds[1] * s[1] * rest);
+        ds[0]            = (ds[0] - dot) * rest;
+        ds[1]            = (ds[1] - dot) * rest;
+    }
+    // what every chosen logit gets, and what all get
+    float       own[2];
+    const float all = dense ? sum_of_row(s[0] * ds[0] + s[1] * ds[1]) : 0.0f;
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+    {
+        // (1 - s of a sigmoid: e^-x s, which keeps its digits where s is near 1)
+        own[h] = SIGMOID ? ds[h] * s[h] * (logit[h] > 0.0f ? expf(-logit[h]) * s[h] : 1.0f - s[h]) : s[h] * ds[h];
+        own[h] = e[h] < 0 ? 0.0f : own[h];
+    }
+    for(int base = 0; base < args.experts; base += route_lanes)
+    {
+        const int i = base + lane;
+        float     d = 0.0f;
+        if(dense && i < args.experts)
+        {
+            d = -all * (expf((float)x[i] - top) / total);
+        }
+        for(int j = 0; j < args.k; ++j)
+        {
+            const int   at  = of_lane(j < route_lanes ? e[0] : e[1], j % route_lanes);
+            const float add = of_lane(j < route_lanes ? own[0] : own[1], j % route_lanes);
+            d += at == i ? add : 0.0f;
+        }
+        if(i < args.experts)
+        {
+            dx[i] = to_out<InT>(d);
+        }
+    }
+}
+
+template<class InT, bool SIGMOID>
+__global__ void __launch_bounds__(256) route_backward(const route_back_args args)
+{
+    constexpr int each = 256 / route_lanes;
+    for(long long token = (long long)blockIdx.x * each + threadIdx.x / route_lanes; token < args.tokens;
+        token += (long long)gridDim.x * each)
+    {
+        route_back_token<InT, SIGMOID>(args, token, threadIdx.x % route_lanes);
+    }
+}
+
+// ------------------------------------------------------------------ the sort
+
+// A stable counting sort of the choices by expert, 1024 threads a block, 64 choices a wave at a time: the lanes
+// with one expert find each other by nine ballots, one for each bit of its number, and their leader counts them in its
+// wave's row of the histogram.  Nothing depends on the order in which waves or blocks run.
+constexpr int sort_waves = 16, sort_rounds = 4, sort_block = sort_waves * 64 * sort_rounds; // choices of a block
+
+struct sort_tables
+{
+    int counts[sort_waves][max_groups]; // of a wave, then what lies before it in its block
+    int first[max_groups + 1]; // of an expert, over the block
+};
+
+// The ranks of a block's choices within their expert and block, in rank[]; the block's counts by expert in
+// tables.first[0 .. experts - 1].  Choices outside the experts have rank -1.
+__device__ __forceinline__ void rank_choices(const int* chosen, long long begin, long long end, int experts, sort_tables& tables,
+                                             int (&expert)[sort_rounds], int (&rank)[sort_rounds])
+{
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for(int e = threadIdx.x; e < sort_waves * max_groups; e += 1024)
+    {
+        (&tables.counts[0][0])[e] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for(int r = 0; r < sort_rounds; ++r)
+    {
+        const long long at = begin + (wave * sort_rounds + r) * 64 + lane;
+        int             e  = at < end ? chosen[at] : -1;
+        const bool      is = e >= 0 && e < experts;
+        unsigned long long same = __ballot(is);
+#pragma unroll
+        for(int bit = 0; bit < 9; ++bit)
+        {
+            const bool               set = (e >> bit & 1) != 0;
+            const unsigned long long b   = __ballot(set);
+            same &= set ? b : ~b;
+        }
+        expert[r] = is ? e : -1;
+        rank[r]   = -1;
+        if(is)
+        {
+            // (every lane reads its expert's count before the leader adds: one wave, LDS in order)
+            volatile int* const count  = &tables.counts[wave][e];
+            const int           before = __popcll(same & ((1ull << lane) - 1ull));
+            const int           sofar  = *count;
+            rank[r]                    = sofar + before;
+            if(before == 0)
+            {
+                *count = sofar + __popcll(same);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    for(int e = threadIdx.x; e < experts; e += 1024)
+    {
+        int sum = 0;
+#pragma unroll
+        for(int w = 0; w < sort_waves; ++w)
+        {
+            const int c         = tables.counts[w][e];
+            tables.counts[w][e] = sum;
+            sum += c;
+        }
+        tables.first[e] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for(int r = 0; r < sort_rounds; ++r)
+    {
+        rank[r] += expert[r] >= 0 ? tables.counts[wave][expert[r]] : 0;
+    }
+}
+
+// first[0 .. experts - 1]: counts, then their exclusive sums, and the sum of all in first[experts].  One wave.
+__device__ __forceinline__ void scan_experts(int* first, int experts)
+{
+    if(threadIdx.x < 64)
+    {
+        const int lane  = threadIdx.x;
+        int       carry = 0;
+        for(int base = 0; base < experts; base += 64)
+        {
+            const int e   = base + lane;
+            const int own = e < experts ? first[e] : 0;
+            int       sum = own;
+#pragma unroll
+            for(int d = 1; d < 64; d *= 2)
+            {
+                const int u = __shfl_up(sum, d);
+                sum += lane >= d ? u : 0;
+            }
+            if(e < experts)
+            {
+                first[e] = carry + sum - own;
+            }
+            carry += __shfl(sum, 63);
+        }
+        if(lane == 0)
+        {
+            first[experts] = carry;
+        }
+    }
+    __syncthreads();
+}
+
+struct dispatch_args
+{
+    void*       rows; // tokens * k x row_bytes
+    int*        offsets; // experts + 1
+    int*        places; // tokens x k
+    const void* x; // tokens x row_bytes
+    const int*  chosen; // tokens x k
+    int*        counts; // blocks x experts: of a block, then where its first choice of an expert goes
+    long long   slots; // tokens * k
+    long long   tokens;
+    long long   row_bytes;
+    int         experts, k, blocks;
+    int         copy; // 0: rows are not wanted
+};
+
+// The counts of every block and the ranks within it (in places, until the bases are known).  A single block knows
+// all: it writes places and offsets.
+__global__ void __launch_bounds__(1024) dispatch_rank(const dispatch_args args)
+{
+    __shared__ sort_tables tables;
+    int                    expert[sort_rounds], rank[sort_rounds];
+    const long long        begin = (long long)blockIdx.x * sort_block;
+    rank_choices(args.chosen, begin, args.slots, args.experts, tables, expert, rank);
+    const bool alone = args.blocks == 1;
+    if(alone)
+    {
+        scan_experts(tables.first, args.experts);
+        for(int e = threadIdx.x; e <= args.experts; e += 1024)
+        {
+            args.offsets[e] = tables.first[e];
+        }
+    }
+    else
+    {
+        for(int e = threadIdx.x; e < args.experts; e += 1024)
+        {
+            args.counts[(long long)blockIdx.x * args.experts + e] = tables.first[e];
+        }
+    }
+#pragma unroll
+    for(int r = 0; r < sort_rounds; ++r)
+    {
+        const long long at = begin + ((threadIdx.x >> 6) * sort_rounds + r) * 64 + (threadIdx.x & 63);
+        if(at < args.slots)
+        {
+            args.places[at] = expert[r] < 0 ? -1 : alone ? tables.first[expert[r]] + rank[r] : rank[r];
+        }
+    }
+}
+
+// Where every block's choices of every expert begin, and the offsets.  One workgroup.
+__global__ void __launch_bounds__(1024) dispatch_scan(const dispatch_args args)
+{
+    __shared__ int first[max_groups + 1];
+    for(int e = threadIdx.x; e < args.experts; e += 1024)
+    {
+        int sum = 0;
+#pragma unroll 8
+        for(int b = 0; b < args.blocks; ++b)
+        {
+            sum += args.counts[(long long)b * args.experts + e];
+        }
+        first[e] = sum;
+    }
+    __syncthreads();
+    scan_experts(first, args.experts);
+    for(int e = threadIdx.x; e <= args.experts; e += 1024)
+    {
+        args.offsets[e] = first[e];
+    }
+    for(int e = threadIdx.x; e < args.experts; e += 1024)
+    {
+        int at = first[e];
+#pragma unroll 8
+        for(int b = 0; b < args.blocks; ++b)
+        {
+            int* const here  = args.counts + (long long)b * args.experts + e;
+            const int  count = *here;
+            *here            = at;
+            at += count;
+        }
+    }
+}
+
+// A token's row to the places of its choices; a wave a token, PIECE bytes a lane.  With counts (several blocks) the
+// places are still ranks: their bases are added first.
+template<class Piece>
+__global__ void __launch_bounds__(256) dispatch_rows(const dispatch_args args)
+{
+    const int lane = threadIdx.x & 63;
+    for(long long token = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); token < args.tokens; token += (long long)gridDim.x * 4)
+    {
+        const long long slot  = token * args.k + lane;
+        int             place = -1;
+        if(lane < args.k)
+        {
+            place = args.places[slot];
+            if(args.counts != nullptr && place >= 0)
+            {
+                place += args.counts[slot / sort_block * args.experts + args.chosen[slot]];
+                args.places[slot] = place;
+            }
+        }
+        if(!args.copy)
+        {
+            continue;
+        }
+        const long long    pieces = args.row_bytes / (long long)sizeof(Piece);
+        const Piece* const from   = static_cast<const Piece*>(args.x) + token * pieces;
+        Piece* const       to     = static_cast<Piece*>(args.rows);
+        for(long long at = lane; at < pieces; at += 64)
+        {
+            const Piece v = from[at];
+            for(int j = 0; j < args.k; ++j)
+            {
+                const int p = __builtin_amdgcn_readlane(place, j);
+                if(p >= 0)
+                {
+                    to[p * pieces + at] = v;
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ the sum
+
+struct combine_args
+{
+    void*        out; // tokens x cols
+    const void*  rows; // tokens * k x cols
+    const int*   places; // tokens x k
+    const float* weights; // nullptr: 1
+    const void*  residual; // nullptr, or tokens x cols of out's type
+    long long    tokens, cols, slots;
+    int          k;
+    // backward
+    void*        drows; // nullptr: not wanted
+    float*       dweights; // nullptr: not wanted
+    const void*  dout;
+};
+
+template<class T, int WIDTH>
+using vec_of = T __attribute__((ext_vector_type(WIDTH)));
+
+// out = sum over the choices of weight * row (+ residual), in fp32 in the order of the choices, rounded once.  WIDTH
+// elements a thread; blockIdx.x: the token, blockIdx.y: 256 pieces of its row.
+template<class InT, class OutT, int WIDTH>
+__global__ void __launch_bounds__(256) combine(const combine_args args, int block0)
+{
+    for(long long token = blockIdx.x; token < args.tokens; token += gridDim.x)
+    {
+        const long long col = ((long long)(block0 + blockIdx.y) * 256 + threadIdx.x) * WIDTH;
+        if(col >= args.cols)
+        {
+            return;
+        }
+        float sum[WIDTH];
+#pragma unroll
+        for(int v = 0; v < WIDTH; ++v)
+        {
+            sum[v] = 0.0f;
+        }
+        const int*   places  = args.places + token * args.k;
+        const float* weights = args.weights != nullptr ? args.weights + token * args.k : nullptr;
+#pragma unroll 8
+        for(int j = 0; j < args.k; ++j)
+        {
+            const int p = places[j];
+            if(p >= 0 && p < args.slots)
+            {
+                const float            w = weights != nullptr ? weights[j] : 1.0f;
+                const vec_of<InT, WIDTH> y
+                    = *reinterpret_cast<const vec_of<InT, WIDTH>*>(static_cast<const InT*>(args.rows) + p * args.cols + col);
+#pragma unroll
+                for(int v = 0; v < WIDTH; ++v)
+                {
+                    sum[v] += w * (float)y[v];
+                }
+            }
+        }
+        const long long at = token * args.cols + col;
+        if(args.residual != nullptr)
+        {
+            const vec_of<OutT, WIDTH> r = *reinterpret_cast<const vec_of<OutT, WIDTH>*>(static_cast<const OutT*>(args.residual) + at);
+#pragma unroll
+            for(int v = 0; v < WIDTH; ++v)
+            {
+                sum[v] += (float)r[v];
+            }
+        }
+        vec_of<OutT, WIDTH> o;
+#pragma unroll
+        for(int v = 0; v < WIDTH; ++v)
+        {
+            o[v] = to_out<OutT>(sum[v]);
+        }
+        *reinterpret_cast<vec_of<OutT, WIDTH>*>(static_cast<OutT*>(args.out) + at) = o;
+    }
+}
+
+// The gradients: of a row, weight * dout; of a weight, the product of dout with its row.  A wave a choice: the k waves
+// of a token share dout in the caches.
+template<class InT, class OutT, int WIDTH>
+__global__ void __launch_bounds__(256) combine_backward(const combine_args args)
+{
+    const int lane = threadIdx.x & 63;
+    for(long long slot = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); slot < args.slots; slot += (long long)gridDim.x * 4)
+    {
+        const int  p  = args.places[slot];
+        const bool is = p >= 0 && p < args.slots;
+        float      dot = 0.0f;
+        if(is)
+        {
+            const float       w    = args.weights != nullptr ? args.weights[slot] : 1.0f;
+            const OutT* const d0   = static_cast<const OutT*>(args.dout) + slot / args.k * args.cols;
+            const InT* const  y0   = static_cast<const InT*>(args.rows) + p * args.cols;
+            InT* const        to   = static_cast<InT*>(args.drows) + p * args.cols;
+#pragma unroll 4
+            for(long long col = lane * WIDTH; col < args.cols; col += 64 * WIDTH)
+            {
+                const vec_of<OutT, WIDTH> d = *reinterpret_cast<const vec_of<OutT, WIDTH>*>(d0 + col);
+                if(args.dweights != nullptr)
+                {
+                    const vec_of<InT, WIDTH> y = *reinterpret_cast<const vec_of<InT, WIDTH>*>(y0 + col);
+#pragma unroll
+                    for(int v = 0; v < WIDTH; ++v)
+                    {
+                        dot += (float)d[v] * (float)y[v];
+                    }
+                }
+                if(args.drows != nullptr)
+                {
+                    vec_of<InT, WIDTH> o;
+#pragma unroll
+                    for(int v = 0; v < WIDTH; ++v)
+                    {
+                        o[v] = to_out<InT>(w * (float)d[v]);
+                    }
+                    *reinterpret_cast<vec_of<InT, WIDTH>*>(to + col) = o;
+                }
+            }
+        }
+        if(args.dweights != nullptr)
+        {
+#pragma unroll
+            for(int d = 1; d < 64; d *= 2)
+            {
+                dot += __shfl_xor(dot, d);
+            }
+            if(lane == 0)
+            {
+                args.dweights[slot] = dot;
+            }
+        }
+    }
+}
+
+} // namespace device
+} // namespace rocm_wmma_gemm
+
+#endif // ROCM_WMMA_GEMM_ROUTING_HPP

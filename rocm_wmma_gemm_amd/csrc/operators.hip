@@ -3,13 +3,10 @@
 // are additions with no counterpart in the reference.
 #include <rocm_wmma_gemm_c.h>
 
-#include <algorithm>
 #include <cmath>
-#include <exception>
 
-#include "host_services.hpp"
 #include "kernel/product_pointwise.hpp"
-#include "product_table.hpp"
+#include "product_host.hpp"
 
 namespace rocm_wmma_gemm
 {
@@ -54,53 +51,6 @@ using device::act_kind;
 using device::product_args;
 using device::product_kind;
 
-// (an extent rounded up to any tile still fits an int)
-constexpr size_t most_extent = 0x7fffff00;
-
-// What a launch may have: its threads along x are counted in 32 bits (a kernel with a workgroup for every
-// tile may ask for more), its workgroups along y in 16.  most_groups_x: of 256 threads, where they come in parts.
-constexpr size_t most_threads_x = 0xffffffff, most_groups_x = size_t{1} << 20, most_groups_y = 65535;
-
-// enqueue(), unless a launch of this call before it was rejected: it would read what that one was to write.
-template<class... A>
-void follow(A&&... a)
-{
-    if(launch_failure == hipSuccess)
-    {
-        enqueue(std::forward<A>(a)...);
-    }
-}
-
-constexpr size_t ceil_div(size_t a, size_t b)
-{
-    return (a + b - 1) / b;
-}
-
-constexpr size_t round_up8(size_t x)
-{
-    return (x + 7) / 8 * 8;
-}
-
-constexpr size_t whole_lines(size_t bytes)
-{
-    return (bytes + 255) / 256 * 256;
-}
-
-hipStream_t stream_of(void* stream)
-{
-    return stream ? *static_cast<hipStream_t*>(stream) : nullptr;
-}
-
-size_t out_size(int type_idx)
-{
-    return type_idx == ROCM_WMMA_GEMM_TYPE_F32_F16 || type_idx == ROCM_WMMA_GEMM_TYPE_F32_BF16 ? 4 : 2;
-}
-
-bool is_bf16(int type_idx)
-{
-    return type_idx == ROCM_WMMA_GEMM_TYPE_BF16_BF16 || type_idx == ROCM_WMMA_GEMM_TYPE_F32_BF16;
-}
-
 // The constants of an activation; false for a code that is none.
 bool activation_of(int code, act_args* act)
 {
@@ -115,30 +65,6 @@ bool activation_of(int code, act_args* act)
             return true;
         default: return false;
     }
-}
-
-// Runs `body`, a function that returns a status, for an entry point with C linkage: no exception
-// leaves it, and a launch that the runtime rejected becomes a status.
-template<class Body>
-int with_status(Body&& body)
-{
-    launch_failure = hipSuccess;
-    try
-    {
-        const int rc = body();
-        return rc == ROCM_WMMA_GEMM_OK && launch_failure != hipSuccess ? ROCM_WMMA_GEMM_ERR_RUNTIME : rc;
-    }
-    catch(const std::exception&)
-    {
-        return ROCM_WMMA_GEMM_ERR_RUNTIME;
-    }
-}
-
-// (without a device, for a plan that is only asked for: an MI355X's)
-size_t compute_units()
-{
-    const size_t cus = compute_units_of_current_device();
-    return cus > 0 ? cus : 256;
 }
 
 // Which operands have rows (and groups) that all start on 16 bytes, as the kernels need them that
@@ -201,24 +127,6 @@ product_args on_copies(product_args x, int layout, bool copy_a, bool copy_b, cha
     }
     return x;
 }
-
-// A product's kernel, and how the tiles that would leave compute units idle are cut along K.
-struct launch_choice
-{
-    product_kernel kernel{nullptr, 0, 0, 0, nullptr, nullptr, 0};
-    size_t         items = 0; // tiles, or the most there can be (rows: the device knows how many)
-    size_t         workgroups = 0;
-    size_t         partial_bytes = 0; // room that cutting needs; 0: nothing is cut
-    int            k_slices = 1; // workgroups that share a tile of the few-row kernel
-    bool           once = false; // B's loads carry the non-temporal hint
-    bool           copy_a = false, copy_b = false; // work on padded copies
-    size_t         copy_bytes = 0; // room for them
-    int            layout = 0, form = 0;
-    size_t         scratch() const
-    {
-        return copy_bytes + partial_bytes;
-    }
-};
 
 // Tiles of a product: at most (`most`), and about (rows of several groups end inside a tile, half
 // full on average).
@@ -297,7 +205,8 @@ float round_us(const form_cost& f, size_t tiles, size_t cus, int per_cu, float k
     return f.fixed + k64 * (f.alone + (f.full - f.alone) * busy);
 }
 
-// Which kernel a product runs on: the least estimated time of the forms that can take it.
+} // namespace
+
 launch_choice choose(int types, int layout, int finish, const product_args& given, size_t cus)
 {
     const bool         symmetric = finish == finish_square || finish == finish_poly;
@@ -451,8 +360,6 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
     return best;
 }
 
-// One product on the kernel chosen for it.  scratch: the room that the choice asked for.  Without it (a
-// capture forbids to allocate) nothing is cut, and the general kernel stands in for one that needs copies.
 int launch_product(int types, int finish, launch_choice c, product_args args, char* scratch, hipStream_t stream)
 {
     if(args.N == 0 || args.M == 0 || args.groups == 0)
@@ -519,6 +426,9 @@ int launch_product(int types, int finish, launch_choice c, product_args args, ch
     }
     return ROCM_WMMA_GEMM_OK;
 }
+
+namespace
+{
 
 // A linear layer's problem, for one weight (groups = 1 and no offsets) or one per group of rows.
 struct layer
@@ -634,16 +544,6 @@ int forward(const layer& p, void* C, const void* A, const void* B, const rocm_wm
     workspace_lease     lease;
     char*               scratch = c.scratch() != 0 ? lease.acquire(c.scratch(), stream) : nullptr;
     return launch_product(p.type_idx, f.finish, c, f.args, scratch, stream);
-}
-
-// Calls f(first, count) for the parts of `all` workgroups that a launch may have along one dimension.
-template<class F>
-void in_parts(size_t all, size_t most, F&& f)
-{
-    for(size_t first = 0; first < all; first += most)
-    {
-        f(static_cast<int>(first), static_cast<unsigned>(std::min(all - first, most)));
-    }
 }
 
 template<class InT>
@@ -773,18 +673,6 @@ int backward(const layer& p, void* dA, void* dB, void* dbias, const void* dC, co
         rc = launch_product(p.type_idx, to_b.finish, on_b, to_b.args, on_b.scratch() != 0 ? scratch : nullptr, stream);
     }
     return rc;
-}
-
-// Calls f with a null pointer of an element type.
-template<class F>
-void by_element(int element, F&& f)
-{
-    switch(element)
-    {
-        case ROCM_WMMA_GEMM_ELEMENT_F16: f(static_cast<_Float16*>(nullptr)); break;
-        case ROCM_WMMA_GEMM_ELEMENT_BF16: f(static_cast<__bf16*>(nullptr)); break;
-        default: f(static_cast<float*>(nullptr)); break;
-    }
 }
 
 struct update

@@ -1,0 +1,303 @@
+// Host side of what stands around a layer of experts: the choice of the experts, the rows sorted by expert, the
+// weighted sum of their rows, and the gradients of these.  They are additions with no counterpart in the reference.
+#include <cmath>
+
+#include "kernel/routing.hpp"
+#include "product_host.hpp"
+
+namespace rocm_wmma_gemm
+{
+namespace host
+{
+namespace
+{
+
+// Tokens of a call, and choices (their places are ints).
+constexpr size_t most_tokens = most_extent, most_slots = most_extent;
+
+bool is_element(int code)
+{
+    return code >= ROCM_WMMA_GEMM_ELEMENT_F16 && code <= ROCM_WMMA_GEMM_ELEMENT_F32;
+}
+
+size_t element_size(int code)
+{
+    return code == ROCM_WMMA_GEMM_ELEMENT_F32 ? 4 : 2;
+}
+
+bool is_score(int code)
+{
+    return code == ROCM_WMMA_GEMM_SCORE_SOFTMAX || code == ROCM_WMMA_GEMM_SCORE_SIGMOID;
+}
+
+template<class InT, bool SIGMOID>
+void launch_route(const device::route_args& a, hipStream_t stream)
+{
+    const dim3 grid(static_cast<unsigned>(std::min(ceil_div(a.tokens, 256 / device::route_lanes), most_groups_x)));
+    auto       with = [&](auto kernel) { follow(kernel, grid, dim3(256), stream, a); };
+    a.chunk <= 1    ? with(&device::route<InT, 1, SIGMOID>)
+    : a.chunk <= 2  ? with(&device::route<InT, 2, SIGMOID>)
+    : a.chunk <= 4  ? with(&device::route<InT, 4, SIGMOID>)
+    : a.chunk <= 8  ? with(&device::route<InT, 8, SIGMOID>)
+    : a.chunk <= 16 ? with(&device::route<InT, 16, SIGMOID>)
+    : a.chunk <= 32 ? with(&device::route<InT, 32, SIGMOID>)
+                    : with(&device::route<InT, 64, SIGMOID>);
+}
+
+int route(int type, int* chosen, float* weights, const void* logits, const rocm_wmma_gemm_routing& r, size_t M, size_t E,
+          size_t k, hipStream_t stream)
+{
+    if(!is_element(type) || !is_score(r.score) || r.groups < 1 || r.kept_groups < 1 || r.kept_groups > r.groups
+       || r.group_best < 1 || r.group_best > 2 || (r.renormalize & ~1) || !std::isfinite(r.scale))
+    {
+        return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+    }
+    if(M > most_tokens || E > device::max_groups || k > device::most_choices || r.groups > device::most_parts || M * k > most_slots)
+    {
+        return ROCM_WMMA_GEMM_ERR_LIMIT;
+    }
+    if(M == 0 || k == 0)
+    {
+        return ROCM_WMMA_GEMM_OK;
+    }
+    const size_t groups = r.groups;
+    if(E == 0 || E % groups != 0 || k > E / groups * r.kept_groups || chosen == nullptr || weights == nullptr || logits == nullptr)
+    {
+        return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+    }
+    device::route_args a{chosen, weights, logits, r.bias, r.mask, static_cast<long long>(M), static_cast<int>(E),
+                         static_cast<int>(k), r.groups, static_cast<int>(E / groups), r.kept_groups, r.group_best, 1, 0,
+                         r.renormalize, r.scale};
+    // (as many lanes a group as there are, a power of two)
+    while(2 * a.spread * a.groups <= device::route_lanes)
+    {
+        a.spread *= 2;
+    }
+    a.chunk = static_cast<int>(ceil_div(a.size, a.spread));
+    by_element(type, [&](auto* typed) {
+        using in_t = std::remove_pointer_t<decltype(typed)>;
+        r.score == ROCM_WMMA_GEMM_SCORE_SIGMOID ? launch_route<in_t, true>(a, stream) : launch_route<in_t, false>(a, stream);
+    });
+    return ROCM_WMMA_GEMM_OK;
+}
+
+int route_backward(int type, void* dlogits, const float* dweights, const int* chosen, const void* logits, size_t M, size_t E,
+                   size_t k, int score, int renormalize, float scale, hipStream_t stream)
+{
+    if(!is_element(type) || !is_score(score) || (renormalize & ~1) || !std::isfinite(scale))
+    {
+        return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+    }
+    if(M > most_tokens || E > device::max_groups || k > device::most_choices || M * k > most_slots)
+    {
+        return ROCM_WMMA_GEMM_ERR_LIMIT;
+    }
+    if(M == 0 || E == 0)
+    {
+        return ROCM_WMMA_GEMM_OK;
+    }
+    if(dlogits == nullptr || logits == nullptr || (k != 0 && (dweights == nullptr || chosen == nullptr)))
+    {
+        return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+    }
+    const device::route_back_args a{dlogits, dweights, chosen, logits, static_cast<long long>(M), static_cast<int>(E),
+                                    static_cast<int>(k), renormalize, scale};
+    by_element(type, [&](auto* typed) {
+        using in_t = std::remove_pointer_t<decltype(typed)>;
+        follow(score == ROCM_WMMA_GEMM_SCORE_SIGMOID ? &device::route_backward<in_t, true> : &device::route_backward<in_t, false>,
+               dim3(static_cast<unsigned>(std::min(ceil_div(M, 256 / device::route_lanes), most_groups_x))), dim3(256), stream, a);
+    });
+    return ROCM_WMMA_GEMM_OK;
+}
+
+// Whether an address may be read in pieces of that many bytes (a power of two).
+bool starts_on(const void* p, size_t bytes)
+{
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+int dispatch(int type, void* rows, int* offsets, int* places, const void* x, const int* chosen, size_t E, size_t M, size_t N,
+             size_t k, hipStream_t stream)
+{
+    if(!is_element(type))
+    {
+        return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+    }
+    if(E > device::most_dispatch || M > most_tokens || N > most_extent || k > device::most_choices || M * k > most_slots)
+    {
+        return ROCM_WMMA_GEMM_ERR_LIMIT;
+    }
+    const size_t slots = M * k;
+    const bool   copy  = rows != nullptr && N != 0 && slots != 0;
+    if(offsets == nullptr || (slots != 0 && (places == nullptr || chosen == nullptr)) || (copy && x == nullptr))
+    {
+        return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+    }
+    device::dispatch_args a{rows, offsets, places, x, chosen, nullptr, static_cast<long long>(slots), static_cast<long long>(M),
+                            static_cast<long long>(N * element_size(type)), static_cast<int>(E), static_cast<int>(k), 1, copy};
+    const size_t blocks = std::max<size_t>(1, ceil_div(slots, device::sort_block));
+    a.blocks            = static_cast<int>(blocks);
+    workspace_lease lease;
+    if(blocks > 1)
+    {
+        a.counts = reinterpret_cast<int*>(lease.acquire(blocks * std::max<size_t>(1, E) * sizeof(int), stream));
+        if(a.counts == nullptr)
+        {
+            return ROCM_WMMA_GEMM_ERR_SCRATCH;
+        }
+    }
+    follow(&device::dispatch_rank, dim3(static_cast<unsigned>(blocks)), dim3(1024), stream, a);
+    if(blocks > 1)
+    {
+        follow(&device::dispatch_scan, dim3(1), dim3(1024), stream, a);
+    }
+    if(copy || blocks > 1)
+    {
+        size_t piece = 16;
+        while(piece > 1 && (a.row_bytes % piece != 0 || !starts_on(x, piece) || !starts_on(rows, piece)))
+        {
+            piece /= 2;
+        }
+        const dim3 grid(static_cast<unsigned>(std::min<size_t>(ceil_div(M, 4), size_t{1} << 16)));
+        follow(piece == 16  ? &device::dispatch_rows<device::u32x4>
+               : piece == 8 ? &device::dispatch_rows<unsigned long long>
+               : piece == 4 ? &device::dispatch_rows<unsigned int>
+                            : &device::dispatch_rows<unsigned short>,
+               grid, dim3(256), stream, a);
+    }
+    return ROCM_WMMA_GEMM_OK;
+}
+
+// Calls f with null pointers of the rows' and the output's types; false if the two do not go together.
+template<class F>
+bool by_pair(int rows_type, int out_type, F&& f)
+{
+    if(!is_element(rows_type) || (out_type != rows_type && out_type != ROCM_WMMA_GEMM_ELEMENT_F32))
+    {
+        return false;
+    }
+    by_element(rows_type, [&](auto* in) {
+        out_type == rows_type ? f(in, in) : f(in, static_cast<float*>(nullptr));
+    });
+    return true;
+}
+
+int check_rows(size_t M, size_t N, size_t k)
+{
+    return M > most_tokens || N > most_extent || k > device::most_choices || M * k > most_slots ? ROCM_WMMA_GEMM_ERR_LIMIT
+                                                                                                : ROCM_WMMA_GEMM_OK;
+}
+
+int combine(int rows_type, int out_type, const device::combine_args& a, hipStream_t stream)
+{
+    // (elements of a piece: 16 bytes of a 16-bit type, or one)
+    const size_t in = element_size(rows_type), out = element_size(out_type);
+    const bool   eight = a.cols % 8 == 0 && starts_on(a.rows, 8 * in) && starts_on(a.out, 8 * out) && starts_on(a.residual, 8 * out);
+    by_pair(rows_type, out_type, [&](auto* in_typed, auto* out_typed) {
+        using in_t  = std::remove_pointer_t<decltype(in_typed)>;
+        using out_t = std::remove_pointer_t<decltype(out_typed)>;
+        in_parts(ceil_div(a.cols, eight ? 2048 : 256), most_groups_y, [&](int block0, unsigned blocks) {
+            follow(eight ? &device::combine<in_t, out_t, 8> : &device::combine<in_t, out_t, 1>,
+                   dim3(static_cast<unsigned>(std::min<long long>(a.tokens, most_groups_x)), blocks), dim3(256), stream, a, block0);
+        });
+    });
+    return ROCM_WMMA_GEMM_OK;
+}
+
+int combine_backward(int rows_type, int out_type, const device::combine_args& a, hipStream_t stream)
+{
+    const size_t in = element_size(rows_type), out = element_size(out_type);
+    const bool   eight = a.cols % 8 == 0 && starts_on(a.rows, 8 * in) && starts_on(a.drows, 8 * in) && starts_on(a.dout, 8 * out);
+    by_pair(rows_type, out_type, [&](auto* in_typed, auto* out_typed) {
+        using in_t  = std::remove_pointer_t<decltype(in_typed)>;
+        using out_t = std::remove_pointer_t<decltype(out_typed)>;
+        follow(eight ? &device::combine_backward<in_t, out_t, 8> : &device::combine_backward<in_t, out_t, 1>,
+               dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(a.slots, 4), most_groups_x))), dim3(256), stream, a);
+    });
+    return ROCM_WMMA_GEMM_OK;
+}
+
+} // namespace
+} // namespace host
+} // namespace rocm_wmma_gemm
+
+extern "C" {
+
+using namespace rocm_wmma_gemm::host;
+namespace device = rocm_wmma_gemm::device;
+
+int rocm_wmma_gemm_route(int logits_type, int* chosen, float* weights, const void* logits,
+                         const rocm_wmma_gemm_routing* routing, size_t M, size_t E, size_t k, void* stream)
+{
+    return with_status([&] {
+        return routing == nullptr ? ROCM_WMMA_GEMM_ERR_ARGUMENT
+                                  : route(logits_type, chosen, weights, logits, *routing, M, E, k, stream_of(stream));
+    });
+}
+
+int rocm_wmma_gemm_route_backward(int logits_type, void* dlogits, const float* dweights, const int* chosen,
+                                  const void* logits, size_t M, size_t E, size_t k, int score, int renormalize, float scale,
+                                  void* stream)
+{
+    return with_status([&] {
+        return route_backward(logits_type, dlogits, dweights, chosen, logits, M, E, k, score, renormalize, scale,
+                              stream_of(stream));
+    });
+}
+
+int rocm_wmma_gemm_dispatch(int rows_type, void* rows, int* offsets, int* places, const void* X, const int* chosen,
+                            size_t E, size_t M, size_t N, size_t k, void* stream)
+{
+    return with_status([&] { return dispatch(rows_type, rows, offsets, places, X, chosen, E, M, N, k, stream_of(stream)); });
+}
+
+int rocm_wmma_gemm_combine(int rows_type, int out_type, void* C, const void* rows, const int* places, const float* weights,
+                           const void* residual, size_t M, size_t N, size_t k, void* stream)
+{
+    return with_status([&] {
+        if(!by_pair(rows_type, out_type, [](auto*, auto*) {}))
+        {
+            return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+        }
+        const int rc = check_rows(M, N, k);
+        if(rc != ROCM_WMMA_GEMM_OK || M == 0 || N == 0)
+        {
+            return rc;
+        }
+        if(C == nullptr || (k != 0 && (rows == nullptr || places == nullptr)))
+        {
+            return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+        }
+        return combine(rows_type, out_type,
+                       {C, rows, places, weights, residual, static_cast<long long>(M), static_cast<long long>(N),
+                        static_cast<long long>(M * k), static_cast<int>(k), nullptr, nullptr, nullptr},
+                       stream_of(stream));
+    });
+}
+
+int rocm_wmma_gemm_combine_backward(int rows_type, int out_type, void* drows, float* dweights, const void* dC,
+                                    const void* rows, const int* places, const float* weights, size_t M, size_t N, size_t k,
+                                    void* stream)
+{
+    return with_status([&] {
+        if(!by_pair(rows_type, out_type, [](auto*, auto*) {}))
+        {
+            return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+        }
+        const int rc = check_rows(M, N, k);
+        if(rc != ROCM_WMMA_GEMM_OK || M == 0 || k == 0 || (drows == nullptr && dweights == nullptr))
+        {
+            return rc;
+        }
+        if(places == nullptr || (N != 0 && (dC == nullptr || (dweights != nullptr && rows == nullptr))))
+        {
+            return ROCM_WMMA_GEMM_ERR_ARGUMENT;
+        }
+        return combine_backward(rows_type, out_type,
+                                {nullptr, rows, places, weights, nullptr, static_cast<long long>(M), static_cast<long long>(N),
+                                 static_cast<long long>(M * k), static_cast<int>(k), drows, dweights, dC},
+                                stream_of(stream));
+    });
+}
+
+} // extern "C"

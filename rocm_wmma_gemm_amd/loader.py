@@ -52,6 +52,22 @@ class activation(enum.IntEnum):
     gelu = 3  # the tanh form
 
 
+class score(enum.IntEnum):
+    """What a router makes of its logits (the codes of include/rocm_wmma_gemm_c.h)."""
+
+    softmax = 0
+    sigmoid = 1
+
+
+def _score(code):
+    return code if type(code) is score else score(code)
+
+
+class _RoutingC(ctypes.Structure):
+    _fields_ = [("score", ctypes.c_int), ("bias", ctypes.c_void_p), ("mask", ctypes.c_void_p)] + [
+        (n, ctypes.c_int) for n in ("groups", "kept_groups", "group_best", "renormalize")] + [("scale", ctypes.c_float)]
+
+
 class _EpilogueC(ctypes.Structure):
     _fields_ = [("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("preact", ctypes.c_void_p),
                 ("activation", ctypes.c_int)]
@@ -75,6 +91,7 @@ class ProductPlan:
 
 
 MAX_GROUPS = 512
+MAX_EXPERTS, MAX_CHOICES, MAX_EXPERT_GROUPS = 512, 32, 16
 
 
 class _VariantInfoC(ctypes.Structure):
@@ -235,7 +252,12 @@ class Loader:
                     ("grouped", [i, p, p, p, p, z, z, z, z, i, p, p]),
                     ("grouped_backward", [i] + [p] * 8 + [z] * 4 + [i] * 3 + [p]),
                     ("product_select", [i, i, z, z, z, z, i, i, p]),
-                    ("orthogonalize", [i, i, p, p, z, z, z, i, p, ctypes.c_float, p])):
+                    ("orthogonalize", [i, i, p, p, z, z, z, i, p, ctypes.c_float, p]),
+                    ("route", [i, p, p, p, p, z, z, z, p]),
+                    ("route_backward", [i, p, p, p, p, z, z, z, i, i, ctypes.c_float, p]),
+                    ("dispatch", [i] + [p] * 5 + [z] * 4 + [p]),
+                    ("combine", [i, i] + [p] * 5 + [z] * 3 + [p]),
+                    ("combine_backward", [i, i] + [p] * 6 + [z] * 3 + [p])):
                 fn = getattr(L, "rocm_wmma_gemm_" + name)
                 fn.restype = ctypes.c_int
                 fn.argtypes = args
@@ -531,3 +553,129 @@ class Loader:
         self._done("orthogonalize", self._lib.rocm_wmma_gemm_orthogonalize(
             codes[G.dtype], codes[O.dtype], o, g, M, N, batch_count, steps, (ctypes.c_float * 3)(*coefficients),
             epsilon, ctypes.byref(handle)))
+
+    # ------------------------------------------------------------------ from a router to the experts and back
+    _ELEMENTS = {}
+
+    @classmethod
+    def _element(cls, name, t):
+        """Code of a tensor's element type."""
+        code = cls._ELEMENTS.get(t.dtype)
+        if code is None:
+            import torch
+
+            cls._ELEMENTS.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+            code = cls._ELEMENTS.get(t.dtype)
+            if code is None:
+                raise TypeError(f"{name} must be f16, bf16 or f32, got {t.dtype}")
+        return code
+
+    @staticmethod
+    def _plain_types():
+        import torch
+
+        return torch.int32, torch.float32
+
+    def _handle_on(self, stream, device):
+        return ctypes.byref(ctypes.c_void_p(self._stream_on(stream, device)))
+
+    def route(self, chosen, weights, logits, M: int, E: int, k: int, score=score.softmax, bias=None, mask=None,
+              groups: int = 1, kept_groups: int | None = None, group_best: int = 2, renormalize: bool = True,
+              scale: float = 1.0, stream=None) -> None:
+        """The k experts of every token, the best first, and their weights, from a router's logits (M x E: f16, bf16
+        or f32).  chosen: M x k int32; weights: M x k f32.
+
+        score: softmax over the experts, or sigmoid.  bias (E, f32) is added to the scores for the choice alone; the experts
+        of the largest sums are chosen, of the largest logits where there is no bias; of equal ones the lower.  groups: the
+        experts form so many groups of neighbours, of which those ``kept_groups`` (all) take part whose
+        ``group_best`` (1 or 2) best biased scores sum to most.  renormalize: a token's weights are divided by their sum; then
+        multiplied by ``scale``.  mask (M, bool or uint8): tokens where it is 0 go nowhere: experts -1, weights 0."""
+        import torch
+
+        self._sizes(M, E, k)
+        int32, f32 = self._plain_types()
+        held, device = self._held, self._device_of("logits", logits)
+        if mask is not None and mask.dtype is not torch.bool:
+            mask_type = torch.uint8
+        else:
+            mask_type = torch.bool
+        r = _RoutingC(_score(score), None if bias is None else held("bias", bias, E, f32, device),
+                      None if mask is None else held("mask", mask, M, mask_type, device), groups,
+                      groups if kept_groups is None else kept_groups, group_best, 1 if renormalize else 0, scale)
+        self._done("route", self._lib.rocm_wmma_gemm_route(
+            self._element("logits", logits), held("chosen", chosen, M * k, int32, device),
+            held("weights", weights, M * k, f32, device), held("logits", logits, M * E, logits.dtype, device),
+            ctypes.byref(r), M, E, k, self._handle_on(stream, device)))
+
+    def route_backward(self, dlogits, dweights, chosen, logits, M: int, E: int, k: int, score=score.softmax,
+                       renormalize: bool = True, scale: float = 1.0, stream=None) -> None:
+        """The gradient of route()'s weights by the logits: dlogits (M x E, the logits' type) from dweights (M x k, f32)
+        and the experts that were chosen.  The choice itself has no gradient, nor has the bias."""
+        self._sizes(M, E, k)
+        int32, f32 = self._plain_types()
+        held, device = self._held, self._device_of("dlogits", dlogits)
+        self._done("route_backward", self._lib.rocm_wmma_gemm_route_backward(
+            self._element("logits", logits), held("dlogits", dlogits, M * E, logits.dtype, device),
+            held("dweights", dweights, M * k, f32, device), held("chosen", chosen, M * k, int32, device),
+            held("logits", logits, M * E, logits.dtype, device), M, E, k, _score(score), 1 if renormalize else 0, scale,
+            self._handle_on(stream, device)))
+
+    def dispatch(self, rows, offsets, places, X, chosen, M: int, N: int, k: int, stream=None) -> None:
+        """Sorts the choices of M tokens by expert, in their order within one.  offsets (E + 1 int32): where every expert's
+        rows start, as grouped() reads them; places (M x k int32): the row of every choice, -1 for a choice outside 0 .. E - 1;
+        rows (M k x N): the tokens' rows of X (M x N: f16, bf16 or f32) in that order.  rows None: the offsets and
+        places alone.  Rows from offsets[E] on are left as they were.  The gradient of X is
+        combine() of rows' without weights."""
+        self._sizes(M, N, k)
+        int32, _ = self._plain_types()
+        held, device = self._held, self._device_of("offsets", offsets)
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets must hold experts + 1 row offsets")
+        E = offsets.numel() - 1
+        code, to, x = 2, None, None
+        if rows is not None:
+            if X is None:
+                raise ValueError("rows needs X")
+            code, to = self._element("X", X), held("rows", rows, M * k * N, X.dtype, device)
+            x = held("X", X, M * N, X.dtype, device)
+        self._done("dispatch", self._lib.rocm_wmma_gemm_dispatch(
+            code, to, held("offsets", offsets, E + 1, int32, device), held("places", places, M * k, int32, device), x,
+            held("chosen", chosen, M * k, int32, device), E, M, N, k, self._handle_on(stream, device)))
+
+    def combine(self, C, rows, places, M: int, N: int, k: int, weights=None, residual=None, stream=None) -> None:
+        """C (M x N) = the sum over a token's k choices of weights (M x k, f32; None: 1) times the row of ``rows`` (M k x N)
+        that ``places`` names, plus residual (M x N of C's type; may be C itself).  A place of -1 adds nothing.  C: the type
+        of rows, or f32; summed in f32, rounded once."""
+        self._sizes(M, N, k)
+        int32, f32 = self._plain_types()
+        held, device = self._held, self._device_of("C", C)
+        out = self._element("C", C)
+        self._done("combine", self._lib.rocm_wmma_gemm_combine(
+            self._element("rows", rows), out, held("C", C, M * N, C.dtype, device),
+            held("rows", rows, M * k * N, rows.dtype, device), held("places", places, M * k, int32, device),
+            None if weights is None else held("weights", weights, M * k, f32, device),
+            None if residual is None else held("residual", residual, M * N, C.dtype, device), M, N, k,
+            self._handle_on(stream, device)))
+
+    def combine_backward(self, drows, dweights, dC, rows, places, M: int, N: int, k: int, weights=None,
+                         stream=None) -> None:
+        """The gradients of combine() from dC (M x N, C's type): drows (M k x N, the type of rows) = weight times dC's row,
+        for the rows that ``places`` names, each once (others are left as they were); dweights (M x k, f32) = the product of
+        dC's row with the choice's.  A result that is None is not computed.  (The gradient of the residual is dC.)"""
+        self._sizes(M, N, k)
+        if drows is None and dweights is None:
+            raise ValueError("none of drows and dweights is wanted")
+        if dweights is not None and rows is None:
+            raise ValueError("dweights needs rows")
+        int32, f32 = self._plain_types()
+        held, device = self._held, self._device_of("dC", dC)
+        kind = rows if rows is not None else drows
+        self._done("combine_backward", self._lib.rocm_wmma_gemm_combine_backward(
+            self._element("rows", kind), self._element("dC", dC),
+            None if drows is None else held("drows", drows, M * k * N, kind.dtype, device),
+            None if dweights is None else held("dweights", dweights, M * k, f32, device),
+            held("dC", dC, M * N, dC.dtype, device),
+            None if rows is None else held("rows", rows, M * k * N, kind.dtype, device),
+            held("places", places, M * k, int32, device),
+            None if weights is None else held("weights", weights, M * k, f32, device), M, N, k,
+            self._handle_on(stream, device)))
