@@ -364,6 +364,48 @@ int rocm_wmma_gemm_combine_backward(int rows_type, int out_type, void* drows, fl
                                     const void* rows, const int* places, const float* weights, size_t M, size_t N, size_t k,
                                     void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * A projection onto a vocabulary with its loss: additions with no counterpart in the reference.
+ *
+ * Logits z = A B of M states (A: M x K, row-major) over N entries (B: K x N, layout_b as for a linear layer: 1, weights stored
+ * N x K, or 0), which are never kept: they are worked out piece by piece, and again for the gradient.  A and B have the
+ * element F16 or BF16, loss, lse and dloss are fp32 and have one value a row.  lse: log sum_v e^(z_v / temperature)
+ * (temperature 1 for cross entropy), which the backward pass reads.  Softmax, sums and losses are worked out in fp32.  M up to
+ * 2^20, N and K up to 2^31 - 256; a size of 0 is no error.  Rows of A that are left out must hold numbers all the same (they are
+ * multiplied by 0).  The calls enqueue on *stream and return; they work in the library's scratch buffer and return
+ * ROCM_WMMA_GEMM_ERR_SCRATCH where it cannot be had (on a capturing stream: make one eager call first).
+ * --------------------------------------------------------------------------------------- */
+
+/* loss_t = lse_t - z_t,target; 0 for a row whose target lies outside 0 .. N - 1 (it is left out).  targets: M values of 32 bits, or
+ * of 64 with wide_targets 1. */
+int rocm_wmma_gemm_linear_cross_entropy(int element, float* loss, float* lse, const void* A, const void* B,
+                                        const void* targets, int wide_targets, size_t M, size_t N, size_t K, int layout_b,
+                                        void* stream);
+
+/* dz = dloss (softmax(z) - [v = target]), 0 in rows that are left out; dA = dz B^T (M x K), dB = A^T dz in B's layout; a NULL result is
+ * not computed.  accumulate 1: dB is added to.  type_idx: the types of dA and dB, and of A and B.  dz is rounded to A's
+ * type before it is multiplied, in f16 times a power of two that brings the largest dloss near 2^14. */
+int rocm_wmma_gemm_linear_cross_entropy_backward(int type_idx, void* dA, void* dB, const float* dloss, const float* lse,
+                                                 const void* A, const void* B, const void* targets, int wide_targets, size_t M,
+                                                 size_t N, size_t K, int layout_b, int accumulate, void* stream);
+
+/* Most entries of a row's list. */
+#define ROCM_WMMA_GEMM_MAX_ENTRIES 256
+
+/* Distillation from the k entries of every row that a teacher lists, with its logits (teacher: M x k, fp32): q = softmax(teacher /
+ * temperature) over the row's list, p = softmax(z / temperature) over all N, loss = temperature^2 sum_j q_j (log q_j - log p_entry j).
+ * entries: M x k of 32 or (wide_entries 1) 64 bits; one outside 0 .. N - 1 is not in the list; a row with an empty list is left
+ * out: its loss is 0.  picked (M x k, fp32) receives the logits z of the entries, which the backward pass reads. */
+int rocm_wmma_gemm_linear_distillation(int element, float* loss, float* lse, float* picked, const void* A, const void* B,
+                                       const void* entries, int wide_entries, const float* teacher, size_t M, size_t N,
+                                       size_t K, size_t k, float temperature, int layout_b, void* stream);
+
+/* dz = dloss temperature (p - q), with the shares of an entry that is listed more than once added up; the rest as above. */
+int rocm_wmma_gemm_linear_distillation_backward(int type_idx, void* dA, void* dB, const float* dloss, const float* lse,
+                                                const float* picked, const void* A, const void* B, const void* entries,
+                                                int wide_entries, const float* teacher, size_t M, size_t N, size_t K, size_t k,
+                                                float temperature, int layout_b, int accumulate, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -61,6 +61,8 @@ struct product_args
     int          groups;
     int          M, N, K; // of every problem; rows: M counts the rows of all groups, sum: K does
     long long    lda, ldb, ldc; // of the contiguous rows in memory
+    long long    b_skip; // B is a block of a wider matrix: elements of its last row in memory that lie past the matrix' end
+    int          padded_c; // rows of C have room for whole pieces of 8, and nobody reads past N
     long long    stride_a, stride_b, stride_c, stride_bias; // elements from group to group (batch)
     float        alpha, beta;
     act_args     act;

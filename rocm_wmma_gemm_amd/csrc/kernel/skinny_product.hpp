@@ -88,7 +88,8 @@ struct skinny_product
         const InT*      a0 = static_cast<const InT*>(args.A) + x.a_at + x.row0 * lda;
         const InT*      b0 = static_cast<const InT*>(args.B) + x.b_at + (B_KMAJOR ? x.col0 * ldb : (long long)x.col0);
         const u32x4     rsrc_a = S::descriptor(a0, (x.m - x.row0) * lda * 2);
-        const u32x4     rsrc_b = S::descriptor(b0, B_KMAJOR ? (args.N - x.col0) * ldb * 2 : (args.K * ldb - x.col0) * 2);
+        const u32x4     rsrc_b = S::descriptor(
+            b0, ((B_KMAJOR ? (args.N - x.col0) * ldb : args.K * ldb - x.col0) - args.b_skip) * 2);
         const int          sub    = lane >> 4, slot = lane & 15;
         const int          chunk  = slot ^ ((4 * wave + sub) & 15);
         const unsigned int voff_a = (unsigned int)(((4 * wave + sub) * lda + chunk * 8) * 2);

@@ -229,8 +229,9 @@ struct tiled_product
         w.a_end = loop::scalar_pointer(A_KMAJOR ? A + last * args.stride_a + args.M * args.lda
                                                 : A + w.x.a_at + w.x.k * args.lda);
         w.b_end = loop::scalar_pointer(
-            B_KMAJOR ? B + (args.kind == product_kind::sum ? 0 : (args.groups - 1) * args.stride_b) + args.N * args.ldb
-                     : B + w.x.b_at + w.x.k * args.ldb);
+            (B_KMAJOR ? B + (args.kind == product_kind::sum ? 0 : (args.groups - 1) * args.stride_b) + args.N * args.ldb
+                      : B + w.x.b_at + w.x.k * args.ldb)
+            - args.b_skip);
         // (a group without rows to add up: its one K tile is all zeros)
         w.a_end = w.a_end < w.a ? w.a : w.a_end;
         w.b_end = w.b_end < w.b ? w.b : w.b_end;

@@ -77,7 +77,7 @@ struct starts_on_16
 starts_on_16 alignment_of(const product_args& x)
 {
     return {x.lda % 8 == 0 && x.stride_a % 8 == 0 && aligned16(x.A), x.ldb % 8 == 0 && x.stride_b % 8 == 0 && aligned16(x.B),
-            x.ldc % 8 == 0 && x.N % 8 == 0 && x.stride_c % 8 == 0 && aligned16(x.C) && aligned16(x.kept)
+            x.ldc % 8 == 0 && (x.N % 8 == 0 || x.padded_c) && x.stride_c % 8 == 0 && aligned16(x.C) && aligned16(x.kept)
                 && aligned16(x.residual) && aligned16(x.bias)};
 }
 

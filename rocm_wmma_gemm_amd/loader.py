@@ -91,7 +91,7 @@ class ProductPlan:
 
 
 MAX_GROUPS = 512
-MAX_EXPERTS, MAX_CHOICES, MAX_EXPERT_GROUPS = 512, 32, 16
+MAX_EXPERTS, MAX_CHOICES, MAX_EXPERT_GROUPS, MAX_ENTRIES = 512, 32, 16, 256
 
 
 class _VariantInfoC(ctypes.Structure):
@@ -257,7 +257,11 @@ class Loader:
                     ("route_backward", [i, p, p, p, p, z, z, z, i, i, ctypes.c_float, p]),
                     ("dispatch", [i] + [p] * 5 + [z] * 4 + [p]),
                     ("combine", [i, i] + [p] * 5 + [z] * 3 + [p]),
-                    ("combine_backward", [i, i] + [p] * 6 + [z] * 3 + [p])):
+                    ("combine_backward", [i, i] + [p] * 6 + [z] * 3 + [p]),
+                    ("linear_cross_entropy", [i] + [p] * 5 + [i, z, z, z, i, p]),
+                    ("linear_cross_entropy_backward", [i] + [p] * 7 + [i, z, z, z, i, i, p]),
+                    ("linear_distillation", [i] + [p] * 6 + [i, p, z, z, z, z, ctypes.c_float, i, p]),
+                    ("linear_distillation_backward", [i] + [p] * 8 + [i, p, z, z, z, z, ctypes.c_float, i, i, p])):
                 fn = getattr(L, "rocm_wmma_gemm_" + name)
                 fn.restype = ctypes.c_int
                 fn.argtypes = args
@@ -679,3 +683,95 @@ class Loader:
             held("places", places, M * k, int32, device),
             None if weights is None else held("weights", weights, M * k, f32, device), M, N, k,
             self._handle_on(stream, device)))
+
+    # ------------------------------------------------------------------ a projection onto a vocabulary and its loss
+    def _indices(self, name, t, need, device):
+        """(address, 1 for 64 bits) of a tensor of indices."""
+        import torch
+
+        if t.dtype is not torch.int64 and t.dtype is not torch.int32:
+            raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+        return self._held(name, t, need, t.dtype, device), 1 if t.dtype is torch.int64 else 0
+
+    def _list(self, entries, teacher, M, device):
+        if entries.dim() != 2 or entries.shape[0] != M:
+            raise ValueError(f"entries must be {M} lists of one length, got {tuple(entries.shape)}")
+        k = entries.shape[1]
+        if k > MAX_ENTRIES:
+            raise ValueError(f"{k} entries a row: at most {MAX_ENTRIES}")
+        _, f32 = self._plain_types()
+        return (*self._indices("entries", entries, M * k, device), self._held("teacher", teacher, M * k, f32, device), k)
+
+    def _operands(self, A, B, M, N, K, device):
+        """Element code and addresses of the states and the weights."""
+        code = self._element("A", A)
+        if code == 2:
+            raise TypeError("A and B must be f16 or bf16")
+        return code, self._held("A", A, M * K, A.dtype, device), self._held("B", B, K * N, A.dtype, device)
+
+    def _gradients(self, dA, dB, A, M, N, K, device):
+        """Type pair and addresses of the gradients that are wanted."""
+        wanted = [t for t in (dA, dB) if t is not None]
+        if not wanted:
+            raise ValueError("none of dA and dB is wanted")
+        out = wanted[0].dtype
+        if any(t.dtype is not out for t in wanted):
+            raise TypeError("dA and dB must share an element type")
+        return (_type_slot(out, A.dtype), None if dA is None else self._held("dA", dA, M * K, out, device),
+                None if dB is None else self._held("dB", dB, K * N, out, device))
+
+    def linear_cross_entropy(self, loss, lse, A, B, targets, M: int, N: int, K: int, layout_b=col_major, stream=None) -> None:
+        """The cross entropy of every row of the logits A B (A: M x K, B: K x N as in linear(), f16 or bf16) against its
+        target, without keeping the logits: loss (M, f32) = log sum_v e^z_v - z_target; 0 for a target outside 0 .. N - 1,
+        whose row is left out.  lse (M, f32) receives the logarithms, for the backward pass.  targets: M int32 or int64."""
+        self._sizes(M, N, K)
+        _, f32 = self._plain_types()
+        held, device = self._held, self._device_of("A", A)
+        code, a, b = self._operands(A, B, M, N, K, device)
+        self._done("linear_cross_entropy", self._lib.rocm_wmma_gemm_linear_cross_entropy(
+            code, held("loss", loss, M, f32, device), held("lse", lse, M, f32, device), a, b,
+            *self._indices("targets", targets, M, device), M, N, K, m_layout(layout_b), self._handle_on(stream, device)))
+
+    def linear_cross_entropy_backward(self, dA, dB, dloss, lse, A, B, targets, M: int, N: int, K: int, layout_b=col_major,
+                                      accumulate: bool = False, stream=None) -> None:
+        """The gradients of linear_cross_entropy() from dloss (M, f32) and its lse: dz = dloss (softmax(z) - 1 at the
+        target), dA = dz B^T (M x K) and dB = A^T dz in B's layout, of A's type or f32.  A result that is None is not
+        computed.  accumulate: dB is added to."""
+        self._sizes(M, N, K)
+        _, f32 = self._plain_types()
+        held, device = self._held, self._device_of("A", A)
+        _, a, b = self._operands(A, B, M, N, K, device)
+        self._done("linear_cross_entropy_backward", self._lib.rocm_wmma_gemm_linear_cross_entropy_backward(
+            *self._gradients(dA, dB, A, M, N, K, device), held("dloss", dloss, M, f32, device), held("lse", lse, M, f32, device),
+            a, b, *self._indices("targets", targets, M, device), M, N, K, m_layout(layout_b), 1 if accumulate else 0,
+            self._handle_on(stream, device)))
+
+    def linear_distillation(self, loss, lse, picked, A, B, entries, teacher, M: int, N: int, K: int, layout_b=col_major,
+                            temperature: float = 1.0, stream=None) -> None:
+        """How far every row of the logits A B is from the entries that a teacher lists for it (entries: M x k int32 or int64,
+        teacher: M x k f32, its logits): loss (M, f32) = temperature^2 sum_j q_j (log q_j - log p_j) with q the
+        softmax of the row's teacher over the temperature and p that of the logits over all N.  An entry outside 0 .. N - 1 is not
+        in the list; a row with an empty list is left out, its loss is 0.  lse (M, f32) and picked (M x k, f32: the logits of
+        the entries) are for the backward pass."""
+        self._sizes(M, N, K)
+        _, f32 = self._plain_types()
+        held, device = self._held, self._device_of("A", A)
+        code, a, b = self._operands(A, B, M, N, K, device)
+        at, wide, given, k = self._list(entries, teacher, M, device)
+        self._done("linear_distillation", self._lib.rocm_wmma_gemm_linear_distillation(
+            code, held("loss", loss, M, f32, device), held("lse", lse, M, f32, device), held("picked", picked, M * k, f32, device),
+            a, b, at, wide, given, M, N, K, k, temperature, m_layout(layout_b), self._handle_on(stream, device)))
+
+    def linear_distillation_backward(self, dA, dB, dloss, lse, picked, A, B, entries, teacher, M: int, N: int, K: int,
+                                     layout_b=col_major, temperature: float = 1.0, accumulate: bool = False, stream=None) -> None:
+        """The gradients of linear_distillation() by the states and the weights, as linear_cross_entropy_backward()'s, from
+        its lse and picked.  (The teacher's logits have none.)"""
+        self._sizes(M, N, K)
+        _, f32 = self._plain_types()
+        held, device = self._held, self._device_of("A", A)
+        _, a, b = self._operands(A, B, M, N, K, device)
+        at, wide, given, k = self._list(entries, teacher, M, device)
+        self._done("linear_distillation_backward", self._lib.rocm_wmma_gemm_linear_distillation_backward(
+            *self._gradients(dA, dB, A, M, N, K, device), held("dloss", dloss, M, f32, device), held("lse", lse, M, f32, device),
+            held("picked", picked, M * k, f32, device), a, b, at, wide, given, M, N, K, k, temperature, m_layout(layout_b),
+            1 if accumulate else 0, self._handle_on(stream, device)))
