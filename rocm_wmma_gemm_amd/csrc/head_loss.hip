@@ -20,7 +20,13 @@ constexpr size_t most_rows = size_t{1} << 20; // (a piece of 1024 columns of the
 
 // A piece of the logits in fp32 is read back from the memory-side cache where it is not larger than this.
 constexpr size_t piece_bytes = size_t{128} << 20;
+// A piece of their gradient in 16 bits.
+constexpr size_t slope_bytes = size_t{512} << 20;
+// The statistics of rows that go together.
+constexpr size_t parts_bytes = size_t{256} << 20;
 constexpr size_t least_piece = 1024, piece_grain = 256; // columns
+// Fewer rows stream the weights through the few-row kernels, which write their logits.
+constexpr size_t least_fused_rows = 192;
 
 // An operand's rows in memory.
 struct operand
@@ -154,10 +160,12 @@ const void* block_of_b(const head& h, const operand& b, size_t v0)
     return b.at == nullptr ? nullptr : static_cast<const char*>(b.at) + v0 * (h.layout_b == 1 ? b.ld : 1) * 2;
 }
 
-// z = A B for a piece of the vocabulary, in fp32, rows `pitch` apart
-step logits_of(const head& h, const operand& a, const operand& b, size_t v0, size_t cols, float* z, size_t pitch)
+// z = A B for a piece of the vocabulary: in fp32, rows `pitch` apart (finish_plain), or their gradient in 16 bits
+// (finish_slope), or their statistics alone (finish_parts)
+step logits_of(const head& h, int finish, const operand& a, const operand& b, size_t v0, size_t cols, void* z, size_t pitch)
 {
-    step s{h.to_f32(), h.layout_b == 1 ? layout_kk : layout_kn, finish_plain, one_problem(product_kind::rows, h.M, cols, h.K)};
+    step s{finish == finish_plain ? h.to_f32() : h.to_16(), h.layout_b == 1 ? layout_kk : layout_kn, finish,
+           one_problem(product_kind::rows, h.M, cols, h.K)};
     s.args.A      = a.at;
     s.args.B      = block_of_b(h, b, v0);
     s.args.C      = z;
@@ -166,10 +174,20 @@ step logits_of(const head& h, const operand& a, const operand& b, size_t v0, siz
     s.args.ldc    = pitch;
     s.args.b_skip = h.layout_b == 1 ? 0 : v0;
     s.args.padded_c = 1;
+    s.args.alpha    = finish == finish_plain ? 1.0f : h.want.scale2;
+    s.args.col_base = static_cast<int>(v0);
     return s;
 }
 
-// dA += dz B^T for a piece: to fp32 rows `pitch` apart, or (whole) to where they belong
+// Whether the logits' products end in a tile's statistics or gradients, or write the logits for a pass of their own: few
+// rows, and rows too long for the tiles' offsets.
+bool fuses(const head& h, const operand& a, const operand& b)
+{
+    return h.M >= least_fused_rows && h.N != 0
+           && logits_of(h, finish_slope, a, b, 0, h.N, nullptr, round_up8(h.N)).plan(compute_units()).kernel.fn != nullptr;
+}
+
+// dA += dz B^T for a piece, rows `pitch` apart
 step states_of(const head& h, const void* dz, size_t dz_pitch, const operand& b, size_t v0, size_t cols, int types, void* to, size_t pitch,
                bool add)
 {
@@ -187,12 +205,12 @@ step states_of(const head& h, const void* dz, size_t dz_pitch, const operand& b,
     return s;
 }
 
-// the piece's part of dB, in B's layout: dz^T A, or A^T dz
+// the piece's part of dB, in B's layout: unit dz^T A, or unit A^T dz
 step weights_of(const head& h, const operand& a, const void* dz, size_t dz_pitch, size_t cols, int types, void* to, size_t pitch, bool add,
-                bool padded)
+                const float* unit)
 {
     const bool nk = h.layout_b == 1;
-    step       s{types, layout_mn, add ? finish_add : finish_plain, one_problem(product_kind::sum, nk ? cols : h.K, nk ? h.K : cols, h.M)};
+    step       s{types, layout_mn, finish_back, one_problem(product_kind::sum, nk ? cols : h.K, nk ? h.K : cols, h.M)};
     s.args.A        = nk ? dz : a.at;
     s.args.B        = nk ? a.at : dz;
     s.args.lda      = nk ? dz_pitch : a.ld;
@@ -200,7 +218,7 @@ step weights_of(const head& h, const operand& a, const void* dz, size_t dz_pitch
     s.args.C        = to;
     s.args.residual = add ? to : nullptr;
     s.args.ldc      = pitch;
-    s.args.padded_c = padded;
+    s.args.alpha_at = unit;
     return s;
 }
 
@@ -246,7 +264,124 @@ unsigned row_groups(size_t rows)
     return static_cast<unsigned>(std::min<size_t>(ceil_div(rows, 4), 8192));
 }
 
-// loss, lse and (a list) the listed logits
+// The rows row0 .. row0 + rows - 1 of a problem.
+head rows_of(const head& h, size_t row0, size_t rows)
+{
+    head   p    = h;
+    const size_t first = row0 * h.want.k;
+    p.M         = rows;
+    p.A         = static_cast<const char*>(h.A) + row0 * h.K * 2;
+    p.want.rows = static_cast<int>(rows);
+    p.want.entries = static_cast<const char*>(h.want.entries) + first * (h.want.wide ? 8 : 4);
+    p.want.teacher = h.want.teacher != nullptr ? h.want.teacher + first : nullptr;
+    return p;
+}
+
+// The listed logits where no logits are written.
+void pick(const head& h, const operand& a, const operand& b, float* picked, hipStream_t stream)
+{
+    const bool     nk = h.layout_b == 1;
+    const bool     eight = nk && h.K % 8 == 0 && a.ld % 8 == 0 && b.ld % 8 == 0 && aligned16(a.at) && aligned16(b.at);
+    const unsigned groups = static_cast<unsigned>(std::min<size_t>(ceil_div(h.M * h.want.k, 4), size_t{1} << 16));
+    const device::pick_args args{h.want, a.at, b.at, static_cast<long long>(a.ld), nk ? static_cast<long long>(b.ld) : 1,
+                                 nk ? 1 : static_cast<long long>(b.ld), static_cast<int>(h.K), picked};
+    if(h.bf16())
+    {
+        follow(eight ? &device::pick_products<__bf16, 8> : &device::pick_products<__bf16, 1>, dim3(groups), dim3(256), stream, args);
+    }
+    else
+    {
+        follow(eight ? &device::pick_products<_Float16, 8> : &device::pick_products<_Float16, 1>, dim3(groups), dim3(256), stream, args);
+    }
+}
+
+// loss, lse and (a list) the listed logits of some rows, from operands whose copies are made
+struct loss_plan
+{
+    bool   fused;
+    pieces p;
+    size_t each, all; // parts of a piece, of a row
+    size_t z_at, parts_at, picked_at, product_at, product;
+    launch_choice tiles; // fused
+    loss_plan(const head& h, const operand& a, const operand& b, bool own_picked, room r)
+        // (a column of weights that are stored K x N is gathered element by element: a list of them is picked from the logits)
+        : fused((h.layout_b == 1 || h.want.teacher == nullptr) && fuses(h, a, b)), p(h.N, fused ? h.N : piece_bytes / (4 * h.M))
+    {
+        product = 0;
+        if(fused)
+        {
+            tiles   = logits_of(h, finish_parts, a, b, 0, h.N, nullptr, round_up8(h.N)).plan(compute_units());
+            each    = ceil_div(h.N, tiles.kernel.block_n / 2); // (a wave's columns)
+            all     = each;
+            product = tiles.scratch();
+        }
+        else
+        {
+            each = ceil_div(p.cols, device::part_cols);
+            all  = h.N != 0 ? each * p.count : 0;
+            for(size_t v0 = 0; v0 < h.N; v0 += p.cols)
+            {
+                product = std::max(product, logits_of(h, finish_plain, a, b, v0, std::min(p.cols, h.N - v0), nullptr, p.pitch())
+                                                .plan(compute_units())
+                                                .scratch());
+                v0 = v0 == 0 && p.count > 2 ? (p.count - 2) * p.cols : v0; // (the first and the last are all there are)
+            }
+        }
+        z_at       = fused ? 0 : r.take(h.M * p.pitch() * 4);
+        parts_at   = r.take(h.M * all * sizeof(device::softmax_part));
+        picked_at  = own_picked ? r.take(h.M * sizeof(float)) : 0;
+        product_at = r.bytes;
+    }
+    size_t bytes() const
+    {
+        return product_at + product;
+    }
+};
+
+int loss_of_rows(const head& h, const loss_plan& plan, const operand& a, const operand& b, float* loss, float* lse, float* picked, char* ws,
+                 hipStream_t stream)
+{
+    using device::softmax_part;
+    float* const        of_targets = picked == nullptr ? reinterpret_cast<float*>(ws + plan.picked_at) : picked;
+    softmax_part* const parts      = reinterpret_cast<softmax_part*>(ws + plan.parts_at);
+    char* const         scratch    = ws + plan.product_at;
+    if(plan.fused)
+    {
+        step s              = logits_of(h, finish_parts, a, b, 0, h.N, nullptr, round_up8(h.N));
+        s.args.parts        = parts;
+        s.args.parts_of_row = static_cast<int>(plan.all);
+        const int rc        = launch_product(s.types, s.finish, plan.tiles, s.args, plan.product != 0 ? scratch : nullptr, stream);
+        if(rc != ROCM_WMMA_GEMM_OK)
+        {
+            return rc;
+        }
+        pick(h, a, b, of_targets, stream);
+    }
+    const unsigned pick_groups = static_cast<unsigned>(std::min<size_t>(ceil_div(h.M * h.want.k, 256), 4096));
+    for(size_t v0 = 0; !plan.fused && v0 < std::max<size_t>(h.N, 1); v0 += plan.p.cols)
+    {
+        const size_t cols  = std::min(plan.p.cols, h.N - v0), pitch = plan.p.pitch();
+        float* const z     = reinterpret_cast<float*>(ws + plan.z_at);
+        const int    rc    = logits_of(h, finish_plain, a, b, v0, cols, z, pitch).run(scratch, stream);
+        if(rc != ROCM_WMMA_GEMM_OK)
+        {
+            return rc;
+        }
+        follow(&device::pick_entries, dim3(pick_groups), dim3(256), stream, h.want, static_cast<const float*>(z),
+               static_cast<long long>(pitch), static_cast<long long>(v0), static_cast<int>(cols), of_targets);
+        if(cols != 0)
+        {
+            // (the last piece may have fewer parts than the others: its rest has none)
+            const device::part_args args{z, parts, static_cast<long long>(pitch), static_cast<int>(cols),
+                                         static_cast<int>(v0 / plan.p.cols * plan.each), static_cast<int>(plan.all), h.want.scale2};
+            follow(&device::softmax_parts, dim3(static_cast<unsigned>(h.M), static_cast<unsigned>(plan.each)), dim3(256), stream, args);
+        }
+    }
+    follow(&device::join_rows, dim3(row_groups(h.M)), dim3(256), stream,
+           device::join_args{h.want, parts, of_targets, loss, lse, static_cast<int>(plan.all)});
+    return ROCM_WMMA_GEMM_OK;
+}
+
 int loss_of(const head& h, float* loss, float* lse, float* picked, hipStream_t stream)
 {
     if(h.M == 0)
@@ -257,85 +392,52 @@ int loss_of(const head& h, float* loss, float* lse, float* picked, hipStream_t s
     {
         return ROCM_WMMA_GEMM_ERR_ARGUMENT;
     }
-    const pieces  p(h.N, piece_bytes / (4 * h.M));
-    const size_t  each = ceil_div(p.cols, device::part_cols), all = h.N != 0 ? each * p.count : 0;
-    room          r;
-    const copies  c(h, p.count, r);
-    const operand plan_a = c.plan_a(h), plan_b = c.plan_b(h);
-    const size_t  z_at = r.take(h.M * p.pitch() * 4), parts_at = r.take(h.M * all * sizeof(float2)),
-                 picked_at = picked == nullptr ? r.take(h.M * sizeof(float)) : 0, product_at = r.bytes;
-    size_t product = 0;
-    for(size_t v0 = 0; v0 < h.N; v0 += p.cols)
-    {
-        product = std::max(product, logits_of(h, plan_a, plan_b, v0, std::min(p.cols, h.N - v0), nullptr, p.pitch()).plan(compute_units()).scratch());
-        v0 = v0 == 0 && p.count > 2 ? (p.count - 2) * p.cols : v0; // (the first and the last are all there are)
-    }
+    // rows have nothing to do with each other: as many go together as leave the statistics their room (64 columns a part)
+    const size_t some = std::min(h.M, std::max<size_t>(4096, parts_bytes / sizeof(device::softmax_part) / (h.N / 64 + 1)));
+    room         r;
+    const copies c(h, pieces(h.N, piece_bytes / (4 * some)).count, r);
+    const loss_plan first(rows_of(h, 0, some), c.plan_a(h), c.plan_b(h), picked == nullptr, r);
+    const size_t    rest = h.M % some;
+    const loss_plan last  = rest != 0 ? loss_plan(rows_of(h, 0, rest), c.plan_a(h), c.plan_b(h), picked == nullptr, r) : first;
     workspace_lease lease;
-    char*           ws = lease.acquire(product_at + product, stream);
+    char*           ws = lease.acquire(std::max(first.bytes(), last.bytes()), stream);
     if(ws == nullptr)
     {
         return ROCM_WMMA_GEMM_ERR_SCRATCH;
     }
     const operand a = c.run_a(h, ws, stream), b = c.run_b(h, ws, stream);
-    float* const  z    = reinterpret_cast<float*>(ws + z_at);
-    float* const  of_targets = picked == nullptr ? reinterpret_cast<float*>(ws + picked_at) : picked;
-    float2* const parts = reinterpret_cast<float2*>(ws + parts_at);
-    const unsigned pick_groups = static_cast<unsigned>(std::min<size_t>(ceil_div(h.M * h.want.k, 256), 4096));
-    for(size_t v0 = 0; v0 < std::max<size_t>(h.N, 1); v0 += p.cols)
+    for(size_t row = 0; row < h.M; row += some)
     {
-        const size_t cols = std::min(p.cols, h.N - v0);
-        const int    rc   = logits_of(h, a, b, v0, cols, z, p.pitch()).run(ws + product_at, stream);
+        const size_t  rows = std::min(some, h.M - row);
+        const operand from{static_cast<const char*>(a.at) + row * a.ld * 2, a.ld};
+        const int     rc = loss_of_rows(rows_of(h, row, rows), rows == some ? first : last, from, b, loss + row, lse + row,
+                                        picked != nullptr ? picked + row * h.want.k : nullptr, ws, stream);
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             return rc;
         }
-        follow(&device::pick_entries, dim3(pick_groups), dim3(256), stream, h.want, static_cast<const float*>(z),
-               static_cast<long long>(p.pitch()), static_cast<long long>(v0), static_cast<int>(cols), of_targets);
-        if(cols != 0)
-        {
-            // (the last piece may have fewer parts than the others: its rest has none)
-            const device::part_args args{z, parts, static_cast<long long>(p.pitch()), static_cast<int>(cols),
-                                         static_cast<int>(v0 / p.cols * each), static_cast<int>(all), h.want.scale};
-            follow(&device::softmax_parts, dim3(static_cast<unsigned>(h.M), static_cast<unsigned>(each)), dim3(256), stream, args);
-        }
     }
-    follow(&device::join_rows, dim3(row_groups(h.M)), dim3(256), stream,
-           device::join_args{h.want, parts, of_targets, loss, lse, static_cast<int>(all)});
     return ROCM_WMMA_GEMM_OK;
 }
 
 template<class InT>
-void launch_slope(const device::softmax_slope_args& s, hipStream_t stream)
+void launch_slope(const device::softmax_slope_args& s, bool fused, hipStream_t stream)
 {
-    follow(&device::softmax_slope<InT>, dim3(static_cast<unsigned>(s.want.rows), static_cast<unsigned>(ceil_div(s.pitch, 2048))), dim3(256),
-           stream, s);
+    if(!fused)
+    {
+        follow(&device::softmax_slope<InT>, dim3(static_cast<unsigned>(s.want.rows), static_cast<unsigned>(ceil_div(s.pitch, 2048))),
+               dim3(256), stream, s);
+    }
     if(s.want.teacher != nullptr)
     {
         follow(&device::listed_slope<InT>, dim3(row_groups(s.want.rows)), dim3(256), stream, s);
     }
 }
 
-void launch_scaled(int out_type, const float* from, size_t pitch, void* to, size_t to_pitch, size_t rows, size_t cols, const float* unit,
-                   bool add, hipStream_t stream)
-{
-    if(rows == 0 || cols == 0)
-    {
-        return;
-    }
-    by_element(out_type, [&](auto* typed) {
-        using out_t = std::remove_pointer_t<decltype(typed)>;
-        follow(&device::scaled_rows<out_t>, dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(rows * ceil_div(cols, 4), 256), 8192))),
-               dim3(256), stream, from, static_cast<long long>(pitch), static_cast<out_t*>(to), static_cast<long long>(to_pitch),
-               static_cast<long long>(rows), static_cast<long long>(cols), unit, add ? 1 : 0);
-    });
-}
-
 // dA and dB (either may be missing) from the loss's gradient by row.
 //
-// What is rounded, and why: dz = dloss T (p - q) to A's type, as both products need it.  In bf16 it costs 2.4e-3 of a
-// gradient's norm where the result's own rounding leaves 1.7e-3.  f16 would lose what lies below 6e-8: there dz is held
-// times a power of two that depends on the largest dloss, and the products come out in fp32 and are brought
-// back as they are rounded.
+// What is rounded, and why: dz to A's type, as both products need it, in the units of record_args.  dA's parts are added up in
+// fp32 over the pieces.
 int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss, const float* lse, const float* picked, bool accumulate,
                  hipStream_t stream)
 {
@@ -348,43 +450,39 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     {
         return ROCM_WMMA_GEMM_ERR_ARGUMENT;
     }
-    const bool   scaled = !h.bf16(), f32 = out == ROCM_WMMA_GEMM_ELEMENT_F32;
-    const size_t size = f32 ? 4 : 2, cus = compute_units();
-    const int    direct_types = f32 ? h.to_f32() : h.to_16();
-    const pieces p(h.N, piece_bytes / (4 * std::max<size_t>(h.M, 1)));
-    const size_t pitch = p.pitch(), k_pitch = round_up8(h.K);
-    // dA is added up in fp32 over the pieces, in its own place if that is fp32
-    const bool own_place = !scaled && h.K % 8 == 0 && aligned16(dA) && (f32 || p.count == 1);
-    // where the weights' part of a piece goes in fp32 first: as dB's rows
-    const size_t part_rows = h.layout_b == 1 ? p.cols : h.K, part_pitch = h.layout_b == 1 ? k_pitch : pitch;
+    const bool   f32 = out == ROCM_WMMA_GEMM_ELEMENT_F32;
+    const size_t size = f32 ? 4 : 2, cus = compute_units(), rows = std::max<size_t>(h.M, 1);
+    const int    types = f32 ? h.to_f32() : h.to_16();
     room         r;
-    const copies c(h, p.count, r);
+    const copies c(h, pieces(h.N, slope_bytes / (2 * rows)).count, r);
     const operand plan_a = c.plan_a(h), plan_b = c.plan_b(h);
-    const size_t z_at = r.take(h.M * pitch * 4), dz_at = r.take(h.M * pitch * 2), factor_at = r.take(h.M * 4), unit_at = r.take(8),
-                 sum_at = wants_a && !own_place ? r.take(h.M * k_pitch * 4) : 0,
-                 part_at = wants_b && scaled ? r.take(part_rows * part_pitch * 4) : 0, product_at = r.bytes;
-    auto logits = [&](const operand& a, const operand& b, size_t v0, size_t cols, float* z) {
-        return logits_of(h, a, b, v0, cols, z, pitch);
+    const bool   fused = fuses(h, plan_a, plan_b);
+    const pieces p(h.N, fused ? slope_bytes / (2 * rows) : piece_bytes / (4 * rows));
+    const size_t pitch = p.pitch(), k_pitch = round_up8(h.K);
+    const size_t z_at = fused ? 0 : r.take(h.M * pitch * 4), dz_at = r.take(h.M * pitch * 2),
+                 records_at = r.take(h.M * sizeof(device::loss_record)), unit_at = r.take(8),
+                 sum_at = wants_a ? r.take(h.M * k_pitch * 4) : 0, product_at = r.bytes;
+    auto logits = [&](const operand& a, const operand& b, size_t v0, size_t cols, char* ws) {
+        step s = logits_of(h, fused ? finish_slope : finish_plain, a, b, v0, cols, ws != nullptr ? ws + (fused ? dz_at : z_at) : nullptr, pitch);
+        s.args.records = ws != nullptr ? reinterpret_cast<const device::loss_record*>(ws + records_at) : nullptr;
+        return s;
     };
-    auto states = [&](const operand& b, size_t v0, size_t cols, const void* dz, void* sum) {
-        return states_of(h, dz, pitch, b, v0, cols, own_place ? direct_types : h.to_f32(), own_place ? dA : sum, own_place ? h.K : k_pitch,
-                         v0 != 0);
+    auto states = [&](const operand& b, size_t v0, size_t cols, char* ws) {
+        return states_of(h, ws != nullptr ? ws + dz_at : nullptr, pitch, b, v0, cols, h.to_f32(), ws != nullptr ? ws + sum_at : nullptr,
+                         k_pitch, v0 != 0);
     };
-    auto weights = [&](const operand& a, size_t v0, size_t cols, const void* dz, void* part) {
-        if(scaled)
-        {
-            return weights_of(h, a, dz, pitch, cols, h.to_f32(), part, part_pitch, false, true);
-        }
-        void* to = static_cast<char*>(dB) + v0 * (h.layout_b == 1 ? h.K : 1) * size;
-        return weights_of(h, a, dz, pitch, cols, direct_types, to, h.b_length(), accumulate, false);
+    auto weights = [&](const operand& a, size_t v0, size_t cols, char* ws) {
+        return weights_of(h, a, ws != nullptr ? ws + dz_at : nullptr, pitch, cols, types,
+                          static_cast<char*>(dB) + v0 * (h.layout_b == 1 ? h.K : 1) * size, h.b_length(), accumulate,
+                          ws != nullptr ? reinterpret_cast<const float*>(ws + unit_at) : nullptr);
     };
     size_t product = 0;
     for(size_t v0 = 0; v0 < std::max<size_t>(h.N, 1); v0 += p.cols)
     {
         const size_t cols = std::min(p.cols, h.N - v0);
         product = std::max(product, logits(plan_a, plan_b, v0, cols, nullptr).plan(cus).scratch());
-        product = std::max(product, wants_a ? states(plan_b, v0, cols, nullptr, nullptr).plan(cus).scratch() : 0);
-        product = std::max(product, wants_b ? weights(plan_a, v0, cols, nullptr, nullptr).plan(cus).scratch() : 0);
+        product = std::max(product, wants_a ? states(plan_b, v0, cols, nullptr).plan(cus).scratch() : 0);
+        product = std::max(product, wants_b ? weights(plan_a, v0, cols, nullptr).plan(cus).scratch() : 0);
         v0 = v0 == p.cols && p.count > 3 ? (p.count - 2) * p.cols : v0; // (the first, one behind it, the last)
     }
     workspace_lease lease;
@@ -395,53 +493,45 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     }
     const operand a = c.run_a(h, ws, stream), b = c.run_b(h, ws, stream);
     char* const   scratch = ws + product_at;
-    float* const  factor  = reinterpret_cast<float*>(ws + factor_at);
-    float* const  unit    = reinterpret_cast<float*>(ws + unit_at);
-    const device::factor_args f{h.want, dloss, factor, unit, scaled ? 1 : 0};
+    const device::record_args f{h.want, dloss, lse, reinterpret_cast<device::loss_record*>(ws + records_at),
+                                reinterpret_cast<float*>(ws + unit_at)};
+    follow(&device::gradient_unit, dim3(1), dim3(1024), stream, f);
     if(h.M != 0)
     {
-        if(scaled)
-        {
-            follow(&device::gradient_unit, dim3(1), dim3(1024), stream, f);
-        }
-        follow(&device::gradient_factors, dim3(row_groups(h.M)), dim3(256), stream, f);
+        follow(&device::gradient_records, dim3(row_groups(h.M)), dim3(256), stream, f);
     }
-    const float* back = scaled && h.M != 0 ? unit + 1 : nullptr;
-    int          rc   = ROCM_WMMA_GEMM_OK;
+    int rc = ROCM_WMMA_GEMM_OK;
     for(size_t v0 = 0; v0 < std::max<size_t>(h.N, 1) && rc == ROCM_WMMA_GEMM_OK; v0 += p.cols)
     {
         const size_t cols = std::min(p.cols, h.N - v0);
         if(h.M != 0 && cols != 0)
         {
-            float* const z = reinterpret_cast<float*>(ws + z_at);
-            rc             = logits(a, b, v0, cols, z).run(scratch, stream);
+            rc = logits(a, b, v0, cols, ws).run(scratch, stream);
             if(rc != ROCM_WMMA_GEMM_OK)
             {
                 return rc;
             }
-            const device::softmax_slope_args s{h.want, z, ws + dz_at, static_cast<long long>(pitch), static_cast<long long>(v0),
-                                               static_cast<int>(cols), lse, factor, picked};
-            h.bf16() ? launch_slope<__bf16>(s, stream) : launch_slope<_Float16>(s, stream);
+            const device::softmax_slope_args s{h.want, reinterpret_cast<const float*>(ws + z_at), ws + dz_at, static_cast<long long>(pitch),
+                                               static_cast<long long>(v0), static_cast<int>(cols), f.records, picked};
+            h.bf16() ? launch_slope<__bf16>(s, fused, stream) : launch_slope<_Float16>(s, fused, stream);
         }
         if(wants_a)
         {
-            rc = states(b, v0, cols, ws + dz_at, ws + sum_at).run(scratch, stream);
+            rc = states(b, v0, cols, ws).run(scratch, stream);
         }
         if(wants_b && rc == ROCM_WMMA_GEMM_OK)
         {
-            rc = weights(a, v0, cols, ws + dz_at, ws + part_at).run(scratch, stream);
-            if(scaled)
-            {
-                const bool nk = h.layout_b == 1;
-                launch_scaled(out, reinterpret_cast<const float*>(ws + part_at), part_pitch,
-                              static_cast<char*>(dB) + v0 * (nk ? h.K : 1) * size, h.b_length(), nk ? cols : h.K, nk ? h.K : cols, back,
-                              accumulate, stream);
-            }
+            rc = weights(a, v0, cols, ws).run(scratch, stream);
         }
     }
-    if(rc == ROCM_WMMA_GEMM_OK && wants_a && !own_place)
+    if(rc == ROCM_WMMA_GEMM_OK && wants_a)
     {
-        launch_scaled(out, reinterpret_cast<const float*>(ws + sum_at), k_pitch, dA, h.K, h.M, h.K, back, false, stream);
+        by_element(out, [&](auto* typed) {
+            using out_t = std::remove_pointer_t<decltype(typed)>;
+            follow(&device::scaled_rows<out_t>, dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(h.M * k_pitch, 1024), 8192))), dim3(256),
+                   stream, reinterpret_cast<const float*>(ws + sum_at), static_cast<long long>(k_pitch), static_cast<out_t*>(dA),
+                   static_cast<long long>(h.M), static_cast<long long>(h.K), f.unit);
+        });
     }
     return rc;
 }
@@ -464,7 +554,7 @@ head head_of(int in, size_t M, size_t N, size_t K, int layout_b, const void* A, 
 {
     return {in, M, N, K, layout_b, A, B,
             {entries, wide, teacher, static_cast<long long>(N), static_cast<int>(std::min(M, most_rows + 1)),
-             static_cast<int>(std::min<size_t>(k, device::most_entries + 1)), 1.0f / temperature}};
+             static_cast<int>(std::min<size_t>(k, device::most_entries + 1)), 1.0f / temperature, device::log2_of_e / temperature}};
 }
 
 } // namespace

@@ -4,8 +4,8 @@
 // Mathematics, for a row with logits x = z / T (T: the temperature, 1 for cross entropy), lse = log sum_v e^x_v and a
 // wanted distribution q (of the target alone, or the softmax of a teacher's listed logits over T):
 //   loss = T^2 sum_v q_v (log q_v - x_v + lse), d loss / d z_v = T (e^(x_v - lse) - q_v).
-// A part of a row leaves its largest x and its sum of e^(x - largest); the parts of a row are joined by one wave in
-// a fixed order, in fp32.
+// Powers are of 2, which the hardware has: x log2(e) = scale2 z.  A part of a row leaves its largest such number and the sum of
+// 2^(number - largest) (softmax_part); the parts of a row are joined by one wave in a fixed order, in fp32.
 #ifndef ROCM_WMMA_GEMM_HEAD_LOSS_HPP
 #define ROCM_WMMA_GEMM_HEAD_LOSS_HPP
 
@@ -27,8 +27,10 @@ struct wanted_args
     const float* teacher; // rows x k, nullptr: a target (k = 1)
     long long    vocabulary;
     int          rows, k;
-    float        scale; // 1 / T
+    float        scale, scale2; // 1 / T, log2(e) / T
 };
+
+constexpr float log2_of_e = 1.4426950408889634f, log_of_2 = 0.6931471805599453f;
 
 // Entry j of a row, -1 where it lies outside the vocabulary.
 __device__ __forceinline__ long long entry_of(const wanted_args& w, long long at)
@@ -37,13 +39,13 @@ __device__ __forceinline__ long long entry_of(const wanted_args& w, long long at
     return v >= 0 && v < w.vocabulary ? v : -1;
 }
 
-// Joins two parts' (largest, sum).
-__device__ __forceinline__ void join_part(float& top, float& sum, float other_top, float other_sum)
+// Joins two parts.
+__device__ __forceinline__ softmax_part joined(softmax_part a, softmax_part b)
 {
-    const float most = __builtin_fmaxf(top, other_top);
-    // (a part without a finite value: e^(-inf - -inf) would be no number)
-    sum = (top == most ? sum : sum * expf(top - most)) + (other_top == most ? other_sum : other_sum * expf(other_top - most));
-    top = most;
+    const float most = __builtin_fmaxf(a.top, b.top);
+    // (a part without a finite value: 2^(-inf - -inf) would be no number)
+    return {most, (a.top == most ? a.sum : a.sum * __builtin_amdgcn_exp2f(a.top - most))
+                      + (b.top == most ? b.sum : b.sum * __builtin_amdgcn_exp2f(b.top - most))};
 }
 
 template<int LANES>
@@ -60,16 +62,16 @@ __device__ __forceinline__ float sum_of_lanes(float v)
 // The statistics of part blockIdx.y of row blockIdx.x: 256 threads, four columns at a time.
 struct part_args
 {
-    const float* z; // rows x pitch
-    float2*      parts; // rows x all
-    long long    pitch;
-    int          cols, part0, all;
-    float        scale;
+    const float*  z; // rows x pitch
+    softmax_part* parts; // rows x all
+    long long     pitch;
+    int           cols, part0, all;
+    float         scale2;
 };
 
 __global__ void __launch_bounds__(256) softmax_parts(const part_args args)
 {
-    __shared__ float2  of_wave[4];
+    __shared__ softmax_part of_wave[4];
     const long long    row   = blockIdx.x;
     const int          begin = blockIdx.y * part_cols, end = args.cols - begin < part_cols ? args.cols : begin + part_cols;
     const float* const z     = args.z + row * args.pitch;
@@ -87,7 +89,7 @@ __global__ void __launch_bounds__(256) softmax_parts(const part_args args)
 #pragma unroll
         for(int e = 0; e < 4; ++e)
         {
-            x[4 * i + e] = col + e < end ? v[e] * args.scale : -__builtin_inff();
+            x[4 * i + e] = col + e < end ? v[e] * args.scale2 : -__builtin_inff();
             top          = __builtin_fmaxf(top, x[4 * i + e]);
         }
     }
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(256) softmax_parts(const part_args args)
 #pragma unroll
     for(int i = 0; i < part_cols / 256; ++i)
     {
-        sum += expf(x[i] - from);
+        sum += __builtin_amdgcn_exp2f(x[i] - from);
     }
     sum = sum_of_lanes<64>(sum);
     if((threadIdx.x & 63) == 0)
@@ -111,12 +113,8 @@ __global__ void __launch_bounds__(256) softmax_parts(const part_args args)
     __syncthreads();
     if(threadIdx.x == 0)
     {
-#pragma unroll
-        for(int w = 1; w < 4; ++w)
-        {
-            join_part(top, sum, of_wave[w].x, of_wave[w].y);
-        }
-        args.parts[row * args.all + args.part0 + blockIdx.y] = {top, sum};
+        args.parts[row * args.all + args.part0 + blockIdx.y]
+            = joined(joined(of_wave[0], of_wave[1]), joined(of_wave[2], of_wave[3]));
     }
 }
 
@@ -135,6 +133,52 @@ __global__ void __launch_bounds__(256)
         else if(v < 0 && col0 == 0)
         {
             picked[at] = 0.0f;
+        }
+    }
+}
+
+// The listed logits worked out on their own, where no logits are written: a wave an entry, the product of the row's state with
+// the entry's weights.  Bound by the gather of the weights' rows (2048 rows of 32 entries and a K of 2048: see pick_products'
+// figures in the tables of times).  STEP: elements of a load; step_b: from one element of an entry's weights to the next.
+struct pick_args
+{
+    wanted_args want;
+    const void* A; // rows, lda apart
+    const void* B;
+    long long   lda, entry_b, step_b; // elements from an entry to the next, and within one
+    int         K;
+    float*      picked;
+};
+
+template<class InT, int STEP>
+__global__ void __launch_bounds__(256) pick_products(const pick_args args)
+{
+    typedef InT     in_t __attribute__((ext_vector_type(STEP)));
+    const int       lane  = threadIdx.x & 63;
+    const long long total = (long long)args.want.rows * args.want.k;
+    for(long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); at < total; at += (long long)gridDim.x * 4)
+    {
+        const long long v   = entry_of(args.want, at);
+        float           sum = 0.0f;
+        if(v >= 0)
+        {
+            const InT* const a = static_cast<const InT*>(args.A) + at / args.want.k * args.lda;
+            const InT* const b = static_cast<const InT*>(args.B) + v * args.entry_b;
+#pragma unroll 4
+            for(int i = lane * STEP; i < args.K; i += 64 * STEP)
+            {
+                const in_t x = *reinterpret_cast<const in_t*>(a + i), y = *reinterpret_cast<const in_t*>(b + i * args.step_b);
+#pragma unroll
+                for(int e = 0; e < STEP; ++e)
+                {
+                    sum += (float)x[e] * (float)y[e];
+                }
+            }
+            sum = sum_of_lanes<64>(sum);
+        }
+        if(lane == 0)
+        {
+            args.picked[at] = sum;
         }
     }
 }
@@ -183,12 +227,12 @@ __device__ __forceinline__ listed_row read_list(const wanted_args& w, long long 
 
 struct join_args
 {
-    wanted_args   want;
-    const float2* parts; // rows x all
-    const float*  picked; // rows x k
-    float*        loss;
-    float*        lse;
-    int           all;
+    wanted_args         want;
+    const softmax_part* parts; // rows x all
+    const float*        picked; // rows x k
+    float*              loss;
+    float*              lse;
+    int                 all;
 };
 
 // The loss of a row from its parts: a wave a row.
@@ -197,24 +241,25 @@ __global__ void __launch_bounds__(256) join_rows(const join_args args)
     const int lane = threadIdx.x & 63;
     for(long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < args.want.rows; row += (long long)gridDim.x * 4)
     {
-        float top = -__builtin_inff(), sum = 0.0f;
+        softmax_part all{-__builtin_inff(), 0.0f};
+#pragma unroll 4
         for(int p = lane; p < args.all; p += 64)
         {
-            const float2 part = args.parts[row * args.all + p];
-            join_part(top, sum, part.x, part.y);
+            all = joined(all, args.parts[row * args.all + p]);
         }
 #pragma unroll
         for(int d = 1; d < 64; d *= 2)
         {
-            const float t = __shfl_xor(top, d), s = __shfl_xor(sum, d);
-            join_part(top, sum, t, s);
+            const softmax_part other{__shfl_xor(all.top, d), __shfl_xor(all.sum, d)};
+            all = joined(all, other);
         }
-        const float rest = logf(sum), lse = top + rest;
+        // (what lies between the largest logit and a listed one first: it is exact where the two are near)
+        const float rest = log2f(all.sum);
+        auto        less_log_p = [&](float z) { return ((all.top - z * args.want.scale2) + rest) * log_of_2; };
         float       loss = 0.0f;
         if(args.want.teacher == nullptr)
         {
-            // (what lies between the largest logit and the target first: it is exact where the two are near)
-            loss = entry_of(args.want, row) >= 0 ? (top - args.picked[row]) + rest : 0.0f;
+            loss = entry_of(args.want, row) >= 0 ? less_log_p(args.picked[row]) : 0.0f;
         }
         else
         {
@@ -223,18 +268,17 @@ __global__ void __launch_bounds__(256) join_rows(const join_args args)
 #pragma unroll
             for(int r = 0; r < list_rounds; ++r)
             {
-                const int   j = r * 64 + lane;
                 const float q = l.e[r] * norm;
                 if(q > 0.0f || q != q)
                 {
-                    loss += q * ((l.x[r] - log_norm) + ((top - args.picked[row * args.want.k + j] * args.want.scale) + rest));
+                    loss += q * ((l.x[r] - log_norm) + less_log_p(args.picked[row * args.want.k + r * 64 + lane]));
                 }
             }
             loss = sum_of_lanes<64>(loss) / (args.want.scale * args.want.scale);
         }
         if(lane == 0)
         {
-            args.lse[row]  = lse;
+            args.lse[row]  = (all.top + rest) * log_of_2;
             args.loss[row] = loss;
         }
     }
@@ -242,20 +286,22 @@ __global__ void __launch_bounds__(256) join_rows(const join_args args)
 
 // ------------------------------------------------------------------ the gradient
 
-// What every row's gradient is multiplied by: the loss's gradient times T, times a power of two that brings the largest to
-// 2^13 .. 2^14 where the logits' gradient is held in f16 (whose range ends at 6e-5 below and at 65504 above; p - q is at most 1),
-// 0 for a row that is compared with nothing.  unit[0]: that power of two, unit[1]: 1 over it.
-struct factor_args
+// The gradient of a row's logits is worked out as T dloss / most 2^14 (p - q), with `most` the largest T |dloss| of all
+// rows, and 0 for a row that is compared with nothing; the products' sums are brought back by unit = most 2^-14 as they are
+// rounded.  It is held in 16 bits, whose smallest number in f16 is 6e-8 (p - q is at most 1, so 2^14 stays in range), and where
+// all rows have one dloss, as under a mean, its rounding leaves p - q of a target with a small p as it is: against 64 bits a bf16
+// gradient is 2.0e-3 off instead of 2.6e-3 with dloss itself in it.
+struct record_args
 {
     wanted_args  want;
     const float* dloss;
-    float*       factor;
-    float*       unit;
-    int          scaled; // 0: the power of two is 1
+    const float* lse;
+    loss_record* records;
+    float*       unit; // [0]: unit, [1]: most
 };
 
 // (one workgroup: the largest of all rows)
-__global__ void __launch_bounds__(1024) gradient_unit(const factor_args args)
+__global__ void __launch_bounds__(1024) gradient_unit(const record_args args)
 {
     __shared__ float of_wave[16];
     float            most = 0.0f;
@@ -281,24 +327,25 @@ __global__ void __launch_bounds__(1024) gradient_unit(const factor_args args)
         {
             most = __builtin_fmaxf(most, of_wave[w]);
         }
-        // (both the power and 1 over it are fp32 numbers)
-        int up = most > 0.0f ? 13 - ilogbf(most) : 0;
-        up     = up > 120 ? 120 : up < -120 ? -120 : up;
-        args.unit[0] = args.scaled ? ldexpf(1.0f, up) : 1.0f;
-        args.unit[1] = args.scaled ? ldexpf(1.0f, -up) : 1.0f;
+        most         = most > 0.0f ? most : 1.0f;
+        args.unit[0] = most * 0x1p-14f;
+        args.unit[1] = most;
     }
 }
 
 // A wave a row (a list has to be looked through for an entry).
-__global__ void __launch_bounds__(256) gradient_factors(const factor_args args)
+__global__ void __launch_bounds__(256) gradient_records(const record_args args)
 {
-    const int lane = threadIdx.x & 63;
+    const int   lane = threadIdx.x & 63;
+    const float most = args.unit[1];
     for(long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < args.want.rows; row += (long long)gridDim.x * 4)
     {
-        bool is;
+        bool      is;
+        long long target = -1;
         if(args.want.teacher == nullptr)
         {
-            is = entry_of(args.want, row) >= 0;
+            target = entry_of(args.want, row);
+            is     = target >= 0;
         }
         else
         {
@@ -307,7 +354,7 @@ __global__ void __launch_bounds__(256) gradient_factors(const factor_args args)
         }
         if(lane == 0)
         {
-            args.factor[row] = is ? args.dloss[row] / args.want.scale * (args.scaled ? args.unit[0] : 1.0f) : 0.0f;
+            args.records[row] = {args.lse[row] * log2_of_e, is ? args.dloss[row] / args.want.scale / most * 0x1p14f : 0.0f, (int)target, 0};
         }
     }
 }
@@ -320,12 +367,11 @@ struct softmax_slope_args
     long long    pitch; // a multiple of 8
     long long    col0; // of the piece in the vocabulary
     int          cols; // columns past them are written as zeros
-    const float* lse;
-    const float* factor;
+    const loss_record* records;
     const float* picked; // rows x k (a list)
 };
 
-// dz = factor (e^(x - lse) - q), 8 columns a thread; q of a target alone (a list's entries are put right by listed_slope).
+// dz = factor (2^(scale2 z - lse) - q), 8 columns a thread; q of a target alone (a list's entries are put right by listed_slope).
 template<class InT>
 __global__ void __launch_bounds__(256) softmax_slope(const softmax_slope_args args)
 {
@@ -336,26 +382,22 @@ __global__ void __launch_bounds__(256) softmax_slope(const softmax_slope_args ar
     {
         return;
     }
-    const float  factor = args.factor[row], lse = args.lse[row];
-    const float* z      = args.z + row * args.pitch + col;
+    const loss_record own    = args.records[row];
+    const long long   target = own.target - args.col0;
+    const float*      z      = args.z + row * args.pitch + col;
     const f32x4  lo = *reinterpret_cast<const f32x4*>(z), hi = *reinterpret_cast<const f32x4*>(z + 4);
-    long long    target = -1;
-    if(args.want.teacher == nullptr)
-    {
-        target = entry_of(args.want, row) - args.col0;
-    }
     in8 o;
 #pragma unroll
     for(int e = 0; e < 8; ++e)
     {
-        const float p = expf((e < 4 ? lo[e & 3] : hi[e & 3]) * args.want.scale - lse);
-        const float d = factor * (p - (target == col + e ? 1.0f : 0.0f));
-        o[e]          = to_out<InT>(factor == 0.0f || col + e >= args.cols ? 0.0f : d);
+        const float p = __builtin_amdgcn_exp2f((e < 4 ? lo[e & 3] : hi[e & 3]) * args.want.scale2 - own.lse);
+        const float d = own.factor * (p - (target == col + e ? 1.0f : 0.0f));
+        o[e]          = to_out<InT>(own.factor == 0.0f || col + e >= args.cols ? 0.0f : d);
     }
     *reinterpret_cast<in8*>(static_cast<InT*>(args.dz) + row * args.pitch + col) = o;
 }
 
-// The listed entries of a piece: factor (e^(x - lse) - q), from the logits that the loss picked; q of an entry that is
+// The listed entries of a piece: factor (2^(scale2 z - lse) - q), from the logits that the loss picked; q of an entry that is
 // listed more than once is the sum of its q, in the order of the list, and each of them writes the same.  A wave a row.
 template<class InT>
 __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args args)
@@ -370,7 +412,8 @@ __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args arg
     {
         const long long row    = first + wave;
         const bool      is     = row < args.want.rows;
-        const float     factor = is ? args.factor[row] : 0.0f;
+        const loss_record own = is ? args.records[row] : loss_record{};
+        const float     factor = own.factor;
         if(is)
         {
             const listed_row l    = read_list(args.want, row);
@@ -385,7 +428,6 @@ __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args arg
         __syncthreads();
         if(factor != 0.0f)
         {
-            const float lse = args.lse[row];
             for(int j = lane; j < k; j += 64)
             {
                 const long long v = entries[wave][j];
@@ -396,7 +438,7 @@ __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args arg
                     {
                         q += entries[wave][i] == v ? shares[wave][i] : 0.0f;
                     }
-                    const float p = expf(args.picked[row * k + j] * args.want.scale - lse);
+                    const float p = __builtin_amdgcn_exp2f(args.picked[row * k + j] * args.want.scale2 - own.lse);
                     static_cast<InT*>(args.dz)[row * args.pitch + (v - args.col0)] = to_out<InT>(factor * (p - q));
                 }
             }
@@ -405,28 +447,28 @@ __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args arg
     }
 }
 
-// out (rows of `cols` elements, `out_pitch` apart) = from (pitch apart) * unit, added to what is there or not.
+// out (rows of `cols` elements) = from (pitch apart) * unit.
 template<class OutT>
 __global__ void __launch_bounds__(256)
-    scaled_rows(const float* __restrict__ from, long long pitch, OutT* out, long long out_pitch, long long rows, long long cols,
-                const float* __restrict__ unit, int add)
+    scaled_rows(const float* __restrict__ from, long long pitch, OutT* __restrict__ out, long long rows, long long cols,
+                const float* __restrict__ unit)
 {
-    const float     by     = unit != nullptr ? *unit : 1.0f;
+    const float     by     = *unit;
     const long long pieces = (cols + 3) / 4, total = rows * pieces; // (from's rows are padded to whole pieces)
-    const bool      whole  = cols % 4 == 0 && out_pitch % 4 == 0 && reinterpret_cast<unsigned long long>(out) % (4 * sizeof(OutT)) == 0;
+    const bool      whole  = cols % 4 == 0 && reinterpret_cast<unsigned long long>(out) % (4 * sizeof(OutT)) == 0;
     typedef OutT    out4 __attribute__((ext_vector_type(4)));
     for(long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long long)gridDim.x * 256)
     {
         const long long row = at / pieces, col = (at - row * pieces) * 4;
         const f32x4     v   = *reinterpret_cast<const f32x4*>(from + row * pitch + col);
-        OutT* const     to  = out + row * out_pitch + col;
+        OutT* const     to  = out + row * cols + col;
         if(whole)
         {
-            out4 o = add ? *reinterpret_cast<const out4*>(to) : out4{};
+            out4 o;
 #pragma unroll
             for(int e = 0; e < 4; ++e)
             {
-                o[e] = to_out<OutT>(add ? (float)o[e] + v[e] * by : v[e] * by);
+                o[e] = to_out<OutT>(v[e] * by);
             }
             *reinterpret_cast<out4*>(to) = o;
             continue;
@@ -436,7 +478,7 @@ __global__ void __launch_bounds__(256)
         {
             if(col + e < cols)
             {
-                to[e] = to_out<OutT>(add ? (float)to[e] + v[e] * by : v[e] * by);
+                to[e] = to_out<OutT>(v[e] * by);
             }
         }
     }

@@ -39,6 +39,28 @@ enum class diagonal_use
     rows  = 2 // row i of R is multiplied by beta + alpha diagonal[i]
 };
 
+// What a tile of logits leaves instead of itself (see head_loss.hpp).
+enum class loss_use
+{
+    none  = 0,
+    parts = 1, // of each of its rows, the statistics of every 16 TN columns: see softmax_part
+    slope = 2 // the gradient: factor (2^(alpha z - lse) - [target]), from the rows' loss_records
+};
+
+// The largest of some logits of a row, times alpha (so that powers are of 2), and the sum of 2^(alpha z - largest).
+struct softmax_part
+{
+    float top, sum;
+};
+
+struct loss_record
+{
+    float lse; // log2 of the sum of 2^(alpha z)
+    float factor; // 0: the row's gradient is 0, whatever its logits are
+    int   target; // a column (of the matrix that B is a block of), or -1
+    int   unused; // (16 bytes)
+};
+
 struct act_args
 {
     act_kind kind;
@@ -65,6 +87,11 @@ struct product_args
     int          padded_c; // rows of C have room for whole pieces of 8, and nobody reads past N
     long long    stride_a, stride_b, stride_c, stride_bias; // elements from group to group (batch)
     float        alpha, beta;
+    const float* alpha_at; // nullptr, or where on the device alpha is (finish_back)
+    const loss_record* records; // one a row
+    softmax_part* parts; // rows x parts_of_row
+    int          parts_of_row, part0; // the launch's first part
+    int          col_base; // the first column's number in the matrix that B is a block of
     act_args     act;
     int          keep_sum; // kept holds 0: alpha A B + bias, before the activation (A's type);
                            // 1: the finished value, C's, in A's type
@@ -334,7 +361,8 @@ template<class InT, class OutT, class ResT>
 __device__ __forceinline__ void finish_element(const product_args& args, const product_item& x, int row, int col,
                                                float sum)
 {
-    float z = args.alpha * sum;
+    const float alpha = args.alpha_at != nullptr ? *args.alpha_at : args.alpha;
+    float       z     = alpha * sum;
     if(args.bias != nullptr)
     {
         z += (float)static_cast<const InT*>(args.bias)[x.group * args.stride_bias + col];
@@ -346,7 +374,7 @@ __device__ __forceinline__ void finish_element(const product_args& args, const p
         float beta = args.beta;
         if(args.diagonal_is == diagonal_use::rows)
         {
-            beta += args.alpha * args.diagonal[x.group * args.stride_diagonal + row];
+            beta += alpha * args.diagonal[x.group * args.stride_diagonal + row];
         }
         y += beta * (float)static_cast<const ResT*>(args.residual)[at];
     }
@@ -370,12 +398,13 @@ __device__ __forceinline__ void finish_piece(const product_args& args, const pro
     typedef InT     in8 __attribute__((ext_vector_type(8)));
     typedef OutT    out8 __attribute__((ext_vector_type(8)));
     typedef ResT    res8 __attribute__((ext_vector_type(8)));
-    const long long at = x.c_at + row * args.ldc + col;
+    const long long at    = x.c_at + row * args.ldc + col;
+    const float     alpha = args.alpha_at != nullptr ? *args.alpha_at : args.alpha;
     float           z[8], y[8];
 #pragma unroll
     for(int e = 0; e < 8; ++e)
     {
-        z[e] = args.alpha * sum[e];
+        z[e] = alpha * sum[e];
     }
     if(args.bias != nullptr)
     {
@@ -395,7 +424,7 @@ __device__ __forceinline__ void finish_piece(const product_args& args, const pro
     {
         const res8 r = *reinterpret_cast<const res8*>(static_cast<const ResT*>(args.residual) + at);
         const float beta = args.diagonal_is == diagonal_use::rows
-                               ? args.beta + args.alpha * args.diagonal[x.group * args.stride_diagonal + row]
+                               ? args.beta + alpha * args.diagonal[x.group * args.stride_diagonal + row]
                                : args.beta;
 #pragma unroll
         for(int e = 0; e < 8; ++e)

@@ -31,9 +31,12 @@ namespace device
 {
 
 // What a kernel does to its tiles, at compile time.
-template<bool LAYER, bool LOGISTIC, bool RESIDUAL, bool KEPT, bool SCALED, bool MIRROR, diagonal_use DIAGONAL>
+template<bool LAYER, bool LOGISTIC, bool RESIDUAL, bool KEPT, bool SCALED, bool MIRROR, diagonal_use DIAGONAL,
+         bool BACK = false, loss_use LOSS = loss_use::none>
 struct product_epilogue
 {
+    static constexpr bool back = BACK; // alpha lies on the device
+    static constexpr loss_use loss = LOSS;
     static constexpr bool layer = LAYER; // bias, and relu or nothing; the sum before it is kept
     static constexpr bool logistic = LOGISTIC; // the activation is x s(u)
     static constexpr bool residual = RESIDUAL;
@@ -50,6 +53,10 @@ using epilogue_square   = product_epilogue<false, false, false, false, true, tru
 using epilogue_poly     = product_epilogue<false, false, true, false, true, true, diagonal_use::split>;
 using epilogue_next     = product_epilogue<false, false, true, true, true, false, diagonal_use::rows>;
 using epilogue_last     = product_epilogue<false, false, true, false, true, false, diagonal_use::rows>;
+
+using epilogue_back     = product_epilogue<false, false, true, false, true, false, diagonal_use::none, true>;
+using epilogue_parts    = product_epilogue<false, false, false, false, false, false, diagonal_use::none, false, loss_use::parts>;
+using epilogue_slope    = product_epilogue<false, false, false, false, false, false, diagonal_use::none, false, loss_use::slope>;
 
 // NARROW: rows of C, the residual, the second output or the bias do not start on 16 bytes: they go
 // element by element, a lane a column, so that a store instruction still writes runs of a row.
@@ -309,7 +316,7 @@ struct tiled_product
         // (a layer's C is not read again here, and its stores make the loop's operands no room in the
         // caches: 2 % of a backward pass of experts, 392 us against 400.  What a Newton-Schulz step
         // leaves the next one reads.)
-        constexpr int NT = EPI::scaled ? 0 : 2;
+        constexpr int NT = (EPI::scaled && !EPI::back) || EPI::loss == loss_use::slope ? 0 : 2;
         if constexpr(PIECE == 1 && sizeof(T) == 4)
         {
             __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, y[0]), to, at, wave_at, NT);
@@ -366,6 +373,8 @@ struct tiled_product
             row_w       = col_w;
             col_w       = t;
         }
+        constexpr bool SLOPE = EPI::loss == loss_use::slope;
+        const float    alpha = EPI::back ? *args.alpha_at : args.alpha;
         const bool has_kept = (EPI::layer || EPI::kept) && args.kept != nullptr;
         const bool has_residual = EPI::residual && args.residual != nullptr;
         // (a tile without a mirror has no transposed place: its stores are dropped)
@@ -437,12 +446,43 @@ struct tiled_product
                 }
             }
         }
+        // what a column past the edge adds to its logit (-infinity: its power is 0), and the columns' numbers
+        float past_edge[SLOPE ? PASSES : 1][READS][SLOPE ? PIECE : 1];
+        const __amdgpu_buffer_rsrc_t records_from = window(args.records + row0, SLOPE);
+        const int                    number0      = args.col_base + col0 + col_w;
+        if constexpr(SLOPE)
+        {
+#pragma unroll
+            for(int p = 0; p < PASSES; ++p)
+            {
+#pragma unroll
+                for(int q = 0; q < READS; ++q)
+                {
+#pragma unroll
+                    for(int e = 0; e < PIECE; ++e)
+                    {
+                        past_edge[p][q][e] = col_w + p * HALF * 16 + piece_col[q] + e < cols ? 0.0f : -__builtin_inff();
+                    }
+                }
+            }
+        }
         // residual pieces (and, by rows, what they are multiplied by) of AHEAD blocks are on their way
         constexpr int WANT = sizeof(OutT) == 4 || sizeof(ResT) == 4 || PER_CU > 1 || EPI::mirror ? 2 : 4;
         constexpr int AHEAD = NARROW ? 1 : BLOCKS < WANT ? BLOCKS : WANT;
         piece<ResT, PIECE> residual[EPI::residual ? AHEAD : 1][PASSES][READS];
         float              by_row[EPI::diagonal == diagonal_use::rows ? AHEAD : 1][READS];
+        u32x4              record[SLOPE ? AHEAD : 1][READS];
         auto fetch = [&](int block) {
+            if constexpr(SLOPE)
+            {
+#pragma unroll
+                for(int q = 0; q < READS; ++q)
+                {
+                    const int row = row_w + 16 * block + piece_row[q];
+                    record[block % AHEAD][q] = __builtin_amdgcn_raw_buffer_load_b128(
+                        records_from, row < rows ? row * (unsigned int)sizeof(loss_record) : loop::STORE_RANGE, 0, 0);
+                }
+            }
             if constexpr(EPI::residual)
             {
 #pragma unroll
@@ -511,7 +551,7 @@ struct tiled_product
                     if constexpr(NARROW)
                     {
                         const float v = *reinterpret_cast<const lds_float*>(strip + strip_at[q]);
-                        z[0]          = EPI::scaled ? args.alpha * v : v;
+                        z[0]          = EPI::scaled ? alpha * v : v;
                     }
 #pragma unroll
                     for(int h = 0; h < PIECE / 4; ++h)
@@ -520,7 +560,7 @@ struct tiled_product
 #pragma unroll
                         for(int e = 0; e < 4; ++e)
                         {
-                            z[4 * h + e] = EPI::scaled ? args.alpha * v[e] : v[e];
+                            z[4 * h + e] = EPI::scaled ? alpha * v[e] : v[e];
                         }
                     }
                     const unsigned int off = offset(block, p, q, sizeof(OutT));
@@ -532,6 +572,18 @@ struct tiled_product
                             z[e] += bias[p][q][e];
                         }
                         y[e] = z[e];
+                        if constexpr(SLOPE)
+                        {
+                            // (the power is the hardware's, 1 ulp; below 2^-126 it gives 0)
+                            const u32x4        r = record[block % AHEAD][q];
+                            const unsigned int lse_bits = r[0], factor_bits = r[1];
+                            const float        lse = __builtin_bit_cast(float, lse_bits);
+                            const float        factor = __builtin_bit_cast(float, factor_bits);
+                            const int          hit = (int)r[2] - (number0 + p * HALF * 16 + piece_col[q]);
+                            const float        power
+                                = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], args.alpha, past_edge[p][q][e]) - lse);
+                            y[e] = factor == 0.0f ? 0.0f : factor * (power - (hit == e ? 1.0f : 0.0f));
+                        }
                         if constexpr(EPI::logistic)
                         {
                             const float c = __builtin_amdgcn_fmed3f(z[e], -1.0e4f, 1.0e4f); // (see activate)
@@ -546,7 +598,7 @@ struct tiled_product
                             const float r = residual[block % AHEAD][p][q].get(e);
                             if constexpr(EPI::diagonal == diagonal_use::rows)
                             {
-                                y[e] += (args.beta + args.alpha * by_row[block % AHEAD][q]) * r;
+                                y[e] += (args.beta + alpha * by_row[block % AHEAD][q]) * r;
                             }
                             else
                             {
@@ -589,6 +641,70 @@ struct tiled_product
             if(block + AHEAD < BLOCKS)
             {
                 fetch(block + AHEAD);
+            }
+        }
+    }
+
+    // The statistics of the wave's rows over its columns, straight from the accumulators: a lane has 4 TN of a row's 16 TN
+    // columns, four lanes meet.  What lies past the edge counts as -infinity.
+    __device__ __forceinline__ static void write_parts(const product_args& args, const work& w, f32x4 (&acc)[TM][TN], int row_w,
+                                                       int col_w, int lane)
+    {
+        const int r16 = lane & 15, g = lane >> 4;
+        const int rows = w.x.m - w.x.row0 - row_w, cols = args.N - w.x.col0 - col_w;
+        float     past_edge[TN][4], top[TM], sum[TM];
+#pragma unroll
+        for(int j = 0; j < TN; ++j)
+        {
+#pragma unroll
+            for(int e = 0; e < 4; ++e)
+            {
+                past_edge[j][e] = 16 * j + 4 * g + e < cols ? 0.0f : -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for(int block = 0; block < TM; ++block)
+        {
+            loop::pin_row(acc[block]);
+            float x[TN][4], most = -__builtin_inff();
+#pragma unroll
+            for(int j = 0; j < TN; ++j)
+            {
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                {
+                    x[j][e] = __builtin_fmaf(acc[block][j][e], args.alpha, past_edge[j][e]);
+                    most    = __builtin_fmaxf(most, x[j][e]);
+                }
+            }
+            const float from = most > -__builtin_inff() ? most : 0.0f;
+            float       s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for(int j = 0; j < TN; ++j)
+            {
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                {
+                    s[e] += __builtin_amdgcn_exp2f(x[j][e] - from);
+                }
+            }
+            top[block] = most;
+            sum[block] = (s[0] + s[1]) + (s[2] + s[3]);
+        }
+#pragma unroll
+        for(int block = 0; block < TM; ++block)
+        {
+            const float most = top[block];
+            float       all  = __builtin_fmaxf(most, __shfl_xor(most, 16));
+            all              = __builtin_fmaxf(all, __shfl_xor(all, 32));
+            float s          = sum[block] * (most == all ? 1.0f : __builtin_amdgcn_exp2f(most - all));
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            const int row = 16 * block + r16;
+            if(g == 0 && row < rows && cols > 0)
+            {
+                args.parts[(long long)(w.x.row0 + row_w + row) * args.parts_of_row + args.part0 + (w.x.col0 + col_w) / (16 * TN)]
+                    = {all, s};
             }
         }
     }
@@ -817,7 +933,15 @@ struct tiled_product
             }
             // (the MFMAs are invisible to the compiler: their result latency is covered by hand)
             asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-            if constexpr(!EPI::mirror)
+            if constexpr(EPI::loss == loss_use::parts)
+            {
+                write_parts(args, cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane);
+            }
+            else if constexpr(EPI::loss == loss_use::slope)
+            {
+                write<false>(args, cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
+            }
+            else if constexpr(!EPI::mirror)
             {
                 if(cur.partial != nullptr)
                 {

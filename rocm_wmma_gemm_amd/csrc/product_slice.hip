@@ -35,7 +35,8 @@ product_kernel tiled()
     constexpr bool AK = LAYOUT != layout_mn, BK = LAYOUT == layout_kk;
     using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, BM, BN, EPI, NARROW>;
     product_fn finish = nullptr;
-    if constexpr(!kSteps) // (the steps' products are not cut: their scratch memory holds matrices)
+    // (the steps' products are not cut: their scratch memory holds matrices; logits leave whole tiles)
+    if constexpr(!kSteps && EPI::loss == device::loss_use::none)
     {
         finish = &device::tiled_finish_entry<impl>;
     }
@@ -52,6 +53,7 @@ product_kernel tiled_finish(int finish)
         {
             case finish_plain: return tiled<LAYOUT, BM, BN, device::epilogue_plain>();
             case finish_add: return tiled<LAYOUT, BM, BN, device::epilogue_add>();
+            case finish_back: return tiled<LAYOUT, BM, BN, device::epilogue_back>();
             default: return kNone;
         }
     }
@@ -62,8 +64,18 @@ product_kernel tiled_finish(int finish)
             case finish_plain: return tiled<LAYOUT, BM, BN, device::epilogue_plain>();
             case finish_layer: return tiled<LAYOUT, BM, BN, device::epilogue_layer>();
             case finish_logistic: return tiled<LAYOUT, BM, BN, device::epilogue_logistic>();
-            default: return kNone;
+            default: break;
         }
+        if constexpr(kTypes == types_f16_f16 || kTypes == types_bf16_bf16) // logits: C has the operands' type, or there is none
+        {
+            switch(finish)
+            {
+                case finish_parts: return tiled<LAYOUT, BM, BN, device::epilogue_parts>();
+                case finish_slope: return tiled<LAYOUT, BM, BN, device::epilogue_slope>();
+                default: break;
+            }
+        }
+        return kNone;
     }
     else if constexpr(kTypes == types_steps_square && LAYOUT == layout_kk)
     {
@@ -95,7 +107,8 @@ product_kernel narrow(int finish)
     }
     else if constexpr(LAYOUT == layout_mn)
     {
-        return tiled<LAYOUT, 128, 128, device::epilogue_add, true>();
+        return finish == finish_back ? tiled<LAYOUT, 128, 128, device::epilogue_back, true>()
+                                     : tiled<LAYOUT, 128, 128, device::epilogue_add, true>();
     }
     else
     {
@@ -147,6 +160,10 @@ product_kernel general(int form)
 template<int LAYOUT>
 product_kernel in_layout(int form, int finish)
 {
+    if((finish == finish_parts || finish == finish_slope) && (form < form_tiled_256 || form > form_tiled_192))
+    {
+        return kNone;
+    }
     switch(form)
     {
         case form_general_128:

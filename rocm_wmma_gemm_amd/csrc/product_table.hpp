@@ -68,6 +68,9 @@ enum product_finish
     finish_poly, // symmetric, with a residual and the diagonal held apart
     finish_next, // + diagonal times residual, by rows; kept in A's type as well
     finish_last, // the same, not kept
+    finish_back, // gradients of weights: alpha from the device, a residual is added
+    finish_parts, // logits of 16-bit operands that leave their statistics (whole tiles of any extent, never cut)
+    finish_slope, // or their gradient, in the operands' type
     num_product_finishes
 };
 

@@ -1,10 +1,14 @@
 """The losses of a projection without a GPU: what the C entry points refuse before they touch the device, and what calls
 would launch."""
 import ctypes
+import os
+import re
+import subprocess
 
 import pytest
 
 import rocm_wmma_gemm_amd as R
+from test_host import ROOT, _mfma_loops
 from test_operators_host import recorded  # noqa: F401  (a fixture)
 
 ARGUMENT, SCRATCH, LIMIT, OK = -2, -3, -5, 0
@@ -85,7 +89,55 @@ def test_nothing_of_a_loss_follows_a_launch_that_failed(recorded):  # noqa: F811
 
 
 def test_the_logits_of_a_large_vocabulary_are_not_kept(recorded):  # noqa: F811
-    """2^19 rows over 2^17 entries (137 GB of logits in 16 bits) go in pieces that the scratch buffer holds."""
+    """2^19 rows over 2^17 entries (137 GB of logits in 16 bits) go in pieces that the scratch buffer holds: the loss in
+    33 blocks of rows (256 MB of statistics, 8 bytes for 64 columns, hold 16376 rows) of three launches each, the
+    gradient in at least as many pieces of columns as 512 MB hold 1024 of them, 128, of three."""
     for call in calls_of(1, 1 << 19, 1 << 17, 64, 1):
         (status, launches), = recorded(call)
-        assert status == 0 and len(launches) > 100
+        assert status == 0 and len(launches) >= (128 * 2 if "backward" in call[0] else 3 * 33)
+
+
+def test_tiled_products_behind_a_loss_keep_accumulators_in_place(tmp_path):
+    """As for the layers' (test_operators_host.py): no accumulator copies and no spills in the MFMA loops, and behind every MFMA
+    that a path leaves the loop from two s_nop 15 before anything names an accumulator."""
+    hipcc = "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not found")
+    asm = tmp_path / "loss_isa.s"
+    subprocess.run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                    "-I" + os.path.join(ROOT, "rocm_wmma_gemm_amd", "csrc"), "-S", "--cuda-device-only", "-o", str(asm),
+                    os.path.join(ROOT, "tests", "loss_isa.hip")], check=True, capture_output=True, timeout=900)
+    text = asm.read_text()
+    loops = {}
+    for f, body in _mfma_loops(text):
+        if "tiled_product" in f and (f not in loops or len(body) < len(loops[f])):
+            loops[f] = body
+    assert len(loops) == 10
+    for func, body in loops.items():
+        whole = text[text.index(func + ":"):]
+        whole = whole[:whole.index(".Lfunc_end")]
+        expected = 32 if "Li128ELi128E" in func else 64 if "Li128ELi256E" in func else 128
+        assert sum("v_mfma_f32_16x16x32" in b for b in body) == whole.count("v_mfma_f32_16x16x32") == expected, func
+        assert not [b for b in body if re.search(r"v_accvgpr_|scratch_", b)] and "scratch_" not in whole, func
+        lines = whole.split("\n")
+        label_at = {m.group(1): n for n, line in enumerate(lines) if (m := re.match(r"^(\.LBB\w+):", line))}
+        seen, checked, todo = set(), 0, [(n + 1, 0) for n, line in enumerate(lines) if "v_mfma" in line]
+        while todo:
+            n, nops = todo.pop()
+            while n < len(lines) and (n, nops) not in seen:
+                seen.add((n, nops))
+                line = lines[n]
+                if "v_mfma" in line or "s_endpgm" in line:
+                    break
+                nops += "s_nop 15" in line
+                if nops >= 2:
+                    checked += 1
+                    break
+                assert not re.search(r"[ ,]a\[?\d", line), f"{func}: {line.strip()} too early after the MFMAs"
+                m = re.match(r"^\s+s_(c?)branch\w*\s+(\.LBB\w+)", line)
+                if m:
+                    todo.append((label_at[m.group(2)], nops))
+                    if not m.group(1):
+                        break
+                n += 1
+        assert checked >= 1, func
