@@ -89,56 +89,160 @@ struct route_args
     float        scale;
 };
 
+// Consecutive elements of a row, `count` of COUNT, as fp32.  WHOLE: all of them, on an address that pieces of them start
+// on; else the others repeat the last one's address (a load is always in the row).
+template<class T, int COUNT, bool WHOLE>
+__device__ __forceinline__ void load_run(const T* from, int count, int last, float (&to)[COUNT])
+{
+    if constexpr(WHOLE)
+    {
+        constexpr int PIECE = COUNT * (int)sizeof(T) < 16 ? COUNT : 16 / (int)sizeof(T);
+        typedef T     piece_t __attribute__((ext_vector_type(PIECE)));
+#pragma unroll
+        for(int i = 0; i < COUNT; i += PIECE)
+        {
+            const piece_t v = *reinterpret_cast<const piece_t*>(from + i);
+#pragma unroll
+            for(int e = 0; e < PIECE; ++e)
+            {
+                to[i + e] = (float)v[e];
+            }
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < COUNT; ++i)
+        {
+            to[i] = (float)from[i < count ? i : last];
+        }
+    }
+}
+
+// e^t in fp64: t = n ln 2 + r with |r| <= ln 2 / 2, e^r by its series (the first term left out is 4e-18 of it), times 2^n.
+// Half the instructions of the library's, which also serves what is far from here.
+__device__ __forceinline__ double power_of_e(double t)
+{
+    constexpr double over_ln2 = 1.4426950408889634074, ln2 = 0.693147180559945309417, ln2_rest = 2.3190468138462996e-17;
+    const double     n = __builtin_rint(t * over_ln2);
+    const double     r = __builtin_fma(-n, ln2_rest, __builtin_fma(-n, ln2, t));
+    double           p = 1.0 / 6227020800.0; // 1 / 13!
+    p = __builtin_fma(p, r, 1.0 / 479001600.0);
+    p = __builtin_fma(p, r, 1.0 / 39916800.0);
+    p = __builtin_fma(p, r, 1.0 / 3628800.0);
+    p = __builtin_fma(p, r, 1.0 / 362880.0);
+    p = __builtin_fma(p, r, 1.0 / 40320.0);
+    p = __builtin_fma(p, r, 1.0 / 5040.0);
+    p = __builtin_fma(p, r, 1.0 / 720.0);
+    p = __builtin_fma(p, r, 1.0 / 120.0);
+    p = __builtin_fma(p, r, 1.0 / 24.0);
+    p = __builtin_fma(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    const double e = __builtin_ldexp(p, (int)n);
+    return t < -745.0 ? 0.0 : e; // (also of -infinity; no number stays none)
+}
+
+// 1 / d for d of ordinary size: the hardware's 2^-24 or better, doubled in digits twice.
+__device__ __forceinline__ double one_over(double d)
+{
+    double y = __builtin_amdgcn_rcp(d);
+    y        = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+    return __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+}
+
+// 1 / (1 + e^-x); 0 where e^-x leaves fp64.
+__device__ __forceinline__ double sigmoid(double x)
+{
+    const double e = power_of_e(-x);
+    return x < -709.0 ? 0.0 : one_over(1.0 + e);
+}
+
 // A choice as one number that v_max_f64 orders: the value, whose last 9 bits tell the expert, so that of equal
 // values the lower expert is more.  (The values that the bits can confuse differ by 2^-44 of themselves; logits, which
 // have 24 bits, none.)  No number counts as the lowest value.
-constexpr unsigned long long choice_bits = 511;
+constexpr int choice_bits = 511;
 __device__ __forceinline__ double choice_key(double value, int expert)
 {
     constexpr double most = 1.7976931348623157e308;
-    value = value >= -most ? value : -most;
-    value = (value <= most ? value : most) + 0.0;
-    unsigned long long b = __builtin_bit_cast(unsigned long long, value);
-    b = (b & ~choice_bits) | (unsigned long long)((b >> 63) != 0 ? expert : (int)choice_bits - expert);
-    return __builtin_bit_cast(double, b);
+    // (of a number and none, the maximum is the number; 0 is added for the sign of -0)
+    value = __builtin_fmin(__builtin_fmax(value, -most), most) + 0.0;
+    const unsigned long long b  = __builtin_bit_cast(unsigned long long, value);
+    const int                hi = (int)(b >> 32);
+    // below 0 the larger bits are the smaller number
+    const unsigned int lo = ((unsigned int)b & ~(unsigned int)choice_bits)
+                            | (unsigned int)((choice_bits - expert) ^ (hi >> 31 & choice_bits));
+    return __builtin_bit_cast(double, (unsigned long long)(unsigned int)hi << 32 | lo);
 }
 __device__ __forceinline__ int expert_of_key(double key)
 {
     const unsigned long long b = __builtin_bit_cast(unsigned long long, key);
-    return (b >> 63) != 0 ? (int)(b & choice_bits) : (int)(choice_bits - (b & choice_bits));
+    return choice_bits - (((int)b & choice_bits) ^ ((int)(b >> 32) >> 31 & choice_bits));
 }
 
-// Sixteen lanes a token, CHUNK experts a lane (args.chunk of them used).  Mathematics: scores s = softmax(x) or
-// 1 / (1 + e^-x); the k experts of the largest s + bias (of the largest x where there is no bias: the same order)
-// among the experts of the `kept` groups whose `best` largest s + bias sum to most; weights scale s, or scale s over the
-// sum of the chosen s.  Everything that decides is held in fp64, so that the choice is the definition's and not that of
-// a rounding: fp64 runs at the fp32 rate here.
-template<class InT, int CHUNK, bool SIGMOID>
+// Falling order by Batcher's merge of odd and even places: 63 exchanges for 16 keys.
+template<int COUNT>
+__device__ __forceinline__ void sort_falling(double (&key)[COUNT])
+{
+#pragma unroll
+    for(int p = 1; p < COUNT; p *= 2)
+    {
+#pragma unroll
+        for(int q = p; q >= 1; q /= 2)
+        {
+#pragma unroll
+            for(int j = q % p; j + q < COUNT; j += 2 * q)
+            {
+#pragma unroll
+                for(int i = 0; i < q; ++i)
+                {
+                    if(i + j + q < COUNT && (i + j) / (2 * p) == (i + j + q) / (2 * p))
+                    {
+                        const double a = key[i + j], b = key[i + j + q];
+                        key[i + j]     = __builtin_fmax(a, b);
+                        key[i + j + q] = __builtin_fmin(a, b);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Sixteen lanes a token, CHUNK experts a lane (args.chunk of them used; WHOLE: all, in every lane), at most MOST choices.
+//
+// Mathematics: scores s = softmax(x) or 1 / (1 + e^-x); the k experts of the largest s + bias (of the largest x where there is
+// no bias: the same order) among the experts of the `kept` groups whose `best` largest s + bias sum to most; weights scale s,
+// or scale s over the sum of the chosen s.  Everything that decides is held in fp64, so that the choice is the definition's
+// and not that of a rounding; fp64 runs at the fp32 rate here.
+//
+// Bound by the instructions: 8191 tokens over 256 experts in groups are 2 waves for every SIMD, whose 16 scores a lane, their sort and
+// eight rounds of a maximum over 16 lanes (four DPP steps) are some 1100 instructions.
+template<class InT, int CHUNK, bool SIGMOID, bool WHOLE, int MOST>
 __device__ __forceinline__ void route_token(const route_args& args, long long token, int lane)
 {
     const InT* const x     = static_cast<const InT*>(args.logits) + token * args.experts;
     const int        group = lane / args.spread, within = lane % args.spread * args.chunk;
-    const int        first = group * args.size + within; // this lane's experts: first .. first + count - 1
+    int              first = group * args.size + within; // this lane's experts: first .. first + count - 1
     int              count = args.size - within;
     count                  = count < args.chunk ? count : args.chunk;
     count                  = group < args.groups && count > 0 ? count : 0;
+    first                  = count > 0 ? first : 0;
+    const int last         = count > 0 ? count - 1 : 0;
     const double least = -__builtin_inf();
     float        logit[CHUNK];
-#pragma unroll
-    for(int i = 0; i < CHUNK; ++i)
-    {
-        logit[i] = i < count ? (float)x[first + i] : -__builtin_inff();
-    }
+    load_run<InT, CHUNK, WHOLE>(x + first, count, last, logit);
+    auto is = [&](int i) { return WHOLE || i < count; };
     const bool by_score = args.bias != nullptr || args.groups > 1;
     // softmax: its largest logit and sum, where the scores need them
-    double top = 0.0, total = 1.0;
+    double top = 0.0, over_total = 1.0;
     if constexpr(!SIGMOID)
     {
         float most = -__builtin_inff();
 #pragma unroll
         for(int i = 0; i < CHUNK; ++i)
         {
-            most = __builtin_fmaxf(most, logit[i]);
+            most = is(i) ? __builtin_fmaxf(most, logit[i]) : most;
         }
         most = join_row(most, route_lanes, [](float a, float b) { return __builtin_fmaxf(a, b); });
         top  = most > -__builtin_inff() ? (double)most : 0.0; // (no finite logit: all scores are 0)
@@ -148,30 +252,47 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
 #pragma unroll
             for(int i = 0; i < CHUNK; ++i)
             {
-                sum += i < count ? exp((double)logit[i] - top) : 0.0;
+                sum += is(i) ? power_of_e((double)logit[i] - top) : 0.0;
             }
-            sum   = sum_of_row(sum);
-            total = sum == 0.0 ? 1.0 : sum;
+            sum        = sum_of_row(sum);
+            over_total = sum == 0.0 ? 1.0 : 1.0 / sum;
         }
     }
-    auto score = [&](float l) {
-        return SIGMOID ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - top) / total;
-    };
+    auto score = [&](float l) { return SIGMOID ? sigmoid((double)l) : power_of_e((double)l - top) * over_total; };
     double key[CHUNK];
     double high = least, second = least; // the lane's two best values
-#pragma unroll
-    for(int i = 0; i < CHUNK; ++i)
+    if(by_score)
     {
-        double value = (double)logit[i];
-        if(by_score)
+        float bias[CHUNK];
+        if(args.bias != nullptr)
         {
-            const double s = i < count ? score(logit[i]) + (args.bias != nullptr ? (double)args.bias[first + i] : 0.0) : least;
-            const double v = s >= least ? s : least; // (no number: the lowest)
+            load_run<float, CHUNK, WHOLE>(args.bias + first, count, last, bias);
+        }
+        else
+        {
+#pragma unroll
+            for(int i = 0; i < CHUNK; ++i)
+            {
+                bias[i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for(int i = 0; i < CHUNK; ++i)
+        {
+            const double s = score(logit[i]) + (double)bias[i];
+            const double v = is(i) ? __builtin_fmax(s, least) : least; // (no number: the lowest)
             second         = __builtin_fmax(second, __builtin_fmin(high, v));
             high           = __builtin_fmax(high, v);
-            value          = args.bias != nullptr ? s : value;
+            key[i]         = is(i) ? choice_key(args.bias != nullptr ? s : (double)logit[i], first + i) : least;
         }
-        key[i] = i < count ? choice_key(value, first + i) : least;
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < CHUNK; ++i)
+        {
+            key[i] = is(i) ? choice_key((double)logit[i], first + i) : least;
+        }
     }
     if(args.groups > 1)
     {
@@ -209,42 +330,65 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
             }
         }
     }
-    // k times the largest of all lanes' keys
-    int mine[2] = {0, 0};
-    for(int j = 0; j < args.k; ++j)
-    {
-        double most = key[0];
+    // Every lane's keys in falling order; k times the largest of the lanes' first ones, whose lane moves its others up.  (No two
+    // keys that an expert has are equal.)
+    constexpr int DEPTH = CHUNK < MOST ? CHUNK : MOST; // keys of a lane that can be chosen
+    sort_falling(key);
+    int  mine[MOST > route_lanes ? 2 : 1] = {};
+    auto choose_one = [&](int j, int depth) {
+        const double most = join_row(key[0], route_lanes, [](double a, double b) { return __builtin_fmax(a, b); });
+        const bool   own  = key[0] == most;
 #pragma unroll
-        for(int i = 1; i < CHUNK; ++i)
+        for(int i = 0; i + 1 < DEPTH; ++i)
         {
-            most = __builtin_fmax(most, key[i]);
+            if(i < depth)
+            {
+                key[i] = own ? key[i + 1] : key[i];
+            }
         }
-        most = join_row(most, route_lanes, [](double a, double b) { return __builtin_fmax(a, b); });
-#pragma unroll
-        for(int i = 0; i < CHUNK; ++i)
-        {
-            key[i] = key[i] == most ? least : key[i];
-        }
+        key[DEPTH - 1] = own && depth >= DEPTH - 1 ? least : key[DEPTH - 1];
         const int e = expert_of_key(most);
         mine[0]     = lane == j ? e : mine[0];
-        mine[1]     = lane + route_lanes == j ? e : mine[1];
+        if constexpr(MOST > route_lanes)
+        {
+            mine[1] = lane + route_lanes == j ? e : mine[1];
+        }
+    };
+    if constexpr(MOST <= 8)
+    {
+#pragma unroll
+        for(int j = 0; j < MOST; ++j)
+        {
+            if(j < args.k)
+            {
+                choose_one(j, MOST - 1 - j < DEPTH - 1 ? MOST - 1 - j : DEPTH - 1); // (as many as may still be chosen)
+            }
+        }
+    }
+    else
+    {
+        for(int j = 0; j < args.k; ++j)
+        {
+            choose_one(j, DEPTH - 1);
+        }
     }
     // lane j: the j-th and the (16 + j)-th choice
     const bool real = args.mask == nullptr || args.mask[token] != 0;
-    double     s[2];
+    double     s[MOST > route_lanes ? 2 : 1], total = 0.0;
 #pragma unroll
-    for(int h = 0; h < 2; ++h)
+    for(int h = 0; h < (MOST > route_lanes ? 2 : 1); ++h)
     {
         s[h] = lane + h * route_lanes < args.k ? score((float)x[mine[h]]) : 0.0;
+        total += s[h];
     }
     double factor = args.scale;
     if(args.renormalize)
     {
-        const double sum = sum_of_row(s[0] + s[1]);
-        factor           = sum == 0.0 ? 0.0 : factor / sum;
+        total  = sum_of_row(total);
+        factor = total == 0.0 ? 0.0 : factor / total;
     }
 #pragma unroll
-    for(int h = 0; h < 2; ++h)
+    for(int h = 0; h < (MOST > route_lanes ? 2 : 1); ++h)
     {
         const int j = lane + h * route_lanes;
         if(j < args.k)
@@ -256,14 +400,14 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
 }
 
 // (all lanes of a token leave the loop together)
-template<class InT, int CHUNK, bool SIGMOID>
+template<class InT, int CHUNK, bool SIGMOID, bool WHOLE, int MOST>
 __global__ void __launch_bounds__(256) route(const route_args args)
 {
     constexpr int each = 256 / route_lanes; // tokens of a workgroup
     for(long long token = (long long)blockIdx.x * each + threadIdx.x / route_lanes; token < args.tokens;
         token += (long long)gridDim.x * each)
     {
-        route_token<InT, CHUNK, SIGMOID>(args, token, threadIdx.x % route_lanes);
+        route_token<InT, CHUNK, SIGMOID, WHOLE, MOST>(args, token, threadIdx.x % route_lanes);
     }
 }
 
@@ -274,17 +418,18 @@ struct route_back_args
     const int*   chosen; // tokens x k
     const void*  logits;
     long long    tokens;
-    int          experts, k, renormalize;
+    int          experts, k, renormalize, chunk; // experts of a lane
     float        scale;
 };
 
 // The gradient of the weights by the logits; the choice itself has none.  With ds_j = scale (dw_j - D) / sum, D = sum_i dw_i
 // w_i / scale, (renormalised; else scale dw_j): sigmoid dx_j = ds_j s_j (1 - s_j) for the chosen, 0 for the others; softmax
 // dx_e = s_e (ds_e - sum_j s_j ds_j), where the sum is 0 if the weights are renormalised, so that the logits
-// that were not chosen are not even read.  Sixteen lanes a token; a choice outside the experts has no gradient, one
-// that is listed twice has both.
-template<class InT, bool SIGMOID>
-__device__ __forceinline__ void route_back_token(const route_back_args& args, long long token, int lane)
+// that were not chosen are not even read.  Sixteen lanes a token, CHUNK experts a lane; a choice outside the experts has no
+// gradient, one that is listed twice has both.  Bound by memory: the gradient is written, and a cache line of logits
+// read for every choice.
+template<class InT, int CHUNK, bool SIGMOID, bool WHOLE>
+__device__ __forceinline__ void route_back_token(const route_back_args& args, long long token, int lane, float* row)
 {
     const InT* const x  = static_cast<const InT*>(args.logits) + token * args.experts;
     InT* const       dx = static_cast<InT*>(args.dlogits) + token * args.experts;
@@ -303,14 +448,20 @@ __device__ __forceinline__ void route_back_token(const route_back_args& args, lo
     }
     const bool none  = sum_of_row((e[0] >= 0 ? 1 : 0) + (e[1] >= 0 ? 1 : 0)) == 0; // (a token that went nowhere)
     const bool dense = !SIGMOID && !args.renormalize && !none;
-    float      top = 0.0f, total = 1.0f;
+    const int  first = lane * args.chunk; // this lane's experts
+    int        count = args.experts - first;
+    count            = count < args.chunk ? (count > 0 ? count : 0) : args.chunk;
+    float top = 0.0f, total = 1.0f;
+    float p[CHUNK]; // dense: the scores of the lane's experts
     if constexpr(!SIGMOID)
     {
         if(dense)
         {
-            for(int i = lane; i < args.experts; i += route_lanes)
+            load_run<InT, CHUNK, WHOLE>(x + (count > 0 ? first : 0), count, count > 0 ? count - 1 : 0, p);
+#pragma unroll
+            for(int i = 0; i < CHUNK; ++i)
             {
-                most = __builtin_fmaxf(most, (float)x[i]);
+                most = WHOLE || i < count ? __builtin_fmaxf(most, p[i]) : most;
             }
         }
         top = join_row(most, route_lanes, [](float a, float b) { return __builtin_fmaxf(a, b); });
@@ -318,9 +469,11 @@ __device__ __forceinline__ void route_back_token(const route_back_args& args, lo
         if(dense)
         {
             float sum = 0.0f;
-            for(int i = lane; i < args.experts; i += route_lanes)
+#pragma unroll
+            for(int i = 0; i < CHUNK; ++i)
             {
-                sum += expf((float)x[i] - top);
+                p[i] = WHOLE || i < count ? expf(p[i] - top) : 0.0f;
+                sum += p[i];
             }
             sum   = sum_of_row(sum);
             total = sum == 0.0f ? 1.0f : sum;
@@ -351,35 +504,90 @@ __device__ __forceinline__ void route_back_token(const route_back_args& args, lo
         own[h] = SIGMOID ? ds[h] * s[h] * (logit[h] > 0.0f ? expf(-logit[h]) * s[h] : 1.0f - s[h]) : s[h] * ds[h];
         own[h] = e[h] < 0 ? 0.0f : own[h];
     }
-    for(int base = 0; base < args.experts; base += route_lanes)
+    // The choices' parts go to their experts' places in LDS, one after the other (of equal ones all count, in their order; the
+    // sixteen lanes are of one wave, which LDS serves in order).
+    volatile float* const places = row;
+#pragma unroll
+    for(int i = 0; i < CHUNK; ++i)
     {
-        const int i = base + lane;
-        float     d = 0.0f;
-        if(dense && i < args.experts)
+        if(i < count)
         {
-            d = -all * (expf((float)x[i] - top) / total);
+            places[first + i] = 0.0f;
         }
+    }
+    bool twice = false;
+    for(int j = 0; j < args.k; ++j)
+    {
+        const int at = of_lane(j < route_lanes ? e[0] : e[1], j % route_lanes);
+        twice        = twice || (at >= 0 && ((e[0] == at && lane != j) || (e[1] == at && lane + route_lanes != j)));
+    }
+    if(__ballot(twice) == 0)
+    {
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+        {
+            if(e[h] >= 0)
+            {
+                places[e[h]] = own[h];
+            }
+        }
+    }
+    else
+    {
         for(int j = 0; j < args.k; ++j)
         {
-            const int   at  = of_lane(j < route_lanes ? e[0] : e[1], j % route_lanes);
-            const float add = of_lane(j < route_lanes ? own[0] : own[1], j % route_lanes);
-            d += at == i ? add : 0.0f;
+            const int h = j < route_lanes ? 0 : 1;
+            if(lane == j % route_lanes && e[h] >= 0)
+            {
+                places[e[h]] = places[e[h]] + own[h];
+            }
         }
-        if(i < args.experts)
+    }
+    float d[CHUNK];
+#pragma unroll
+    for(int i = 0; i < CHUNK; ++i)
+    {
+        d[i] = i < count ? places[first + i] : 0.0f;
+        d[i] = dense ? d[i] - all * (p[i] / total) : d[i];
+    }
+    if constexpr(WHOLE)
+    {
+        constexpr int PIECE = CHUNK * (int)sizeof(InT) < 16 ? CHUNK : 16 / (int)sizeof(InT);
+        typedef InT   piece_t __attribute__((ext_vector_type(PIECE)));
+#pragma unroll
+        for(int i = 0; i < CHUNK; i += PIECE)
         {
-            dx[i] = to_out<InT>(d);
+            piece_t o;
+#pragma unroll
+            for(int v = 0; v < PIECE; ++v)
+            {
+                o[v] = to_out<InT>(d[i + v]);
+            }
+            *reinterpret_cast<piece_t*>(dx + first + i) = o;
+        }
+    }
+    else
+    {
+#pragma unroll
+        for(int i = 0; i < CHUNK; ++i)
+        {
+            if(i < count)
+            {
+                dx[first + i] = to_out<InT>(d[i]);
+            }
         }
     }
 }
 
-template<class InT, bool SIGMOID>
+template<class InT, int CHUNK, bool SIGMOID, bool WHOLE>
 __global__ void __launch_bounds__(256) route_backward(const route_back_args args)
 {
-    constexpr int each = 256 / route_lanes;
+    constexpr int    each = 256 / route_lanes;
+    __shared__ float rows[each][route_lanes * CHUNK];
     for(long long token = (long long)blockIdx.x * each + threadIdx.x / route_lanes; token < args.tokens;
         token += (long long)gridDim.x * each)
     {
-        route_back_token<InT, SIGMOID>(args, token, threadIdx.x % route_lanes);
+        route_back_token<InT, CHUNK, SIGMOID, WHOLE>(args, token, threadIdx.x % route_lanes, rows[threadIdx.x / route_lanes]);
     }
 }
 

@@ -30,18 +30,69 @@ bool is_score(int code)
     return code == ROCM_WMMA_GEMM_SCORE_SOFTMAX || code == ROCM_WMMA_GEMM_SCORE_SIGMOID;
 }
 
+// Whether an address may be read in pieces of that many bytes (a power of two).
+bool starts_on(const void* p, size_t bytes)
+{
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+// Calls f with a number of a lane's experts as a type: the smallest power of two that holds them.
+template<class F>
+void by_chunk(int chunk, F&& f)
+{
+    chunk <= 1    ? f(std::integral_constant<int, 1>{})
+    : chunk <= 2  ? f(std::integral_constant<int, 2>{})
+    : chunk <= 4  ? f(std::integral_constant<int, 4>{})
+    : chunk <= 8  ? f(std::integral_constant<int, 8>{})
+    : chunk <= 16 ? f(std::integral_constant<int, 16>{})
+    : chunk <= 32 ? f(std::integral_constant<int, 32>{})
+                  : f(std::integral_constant<int, 64>{});
+}
+
+// A run of a lane's elements starts on its pieces: all of `chunk`, in every lane and row.
+template<class T, int CHUNK>
+bool whole_runs(const void* p, int chunk)
+{
+    return chunk == CHUNK && starts_on(p, std::min<size_t>(16, CHUNK * sizeof(T)));
+}
+
+dim3 token_groups(long long tokens)
+{
+    return dim3(static_cast<unsigned>(std::min(ceil_div(tokens, 256 / device::route_lanes), most_groups_x)));
+}
+
 template<class InT, bool SIGMOID>
 void launch_route(const device::route_args& a, hipStream_t stream)
 {
-    const dim3 grid(static_cast<unsigned>(std::min(ceil_div(a.tokens, 256 / device::route_lanes), most_groups_x)));
-    auto       with = [&](auto kernel) { follow(kernel, grid, dim3(256), stream, a); };
-    a.chunk <= 1    ? with(&device::route<InT, 1, SIGMOID>)
-    : a.chunk <= 2  ? with(&device::route<InT, 2, SIGMOID>)
-    : a.chunk <= 4  ? with(&device::route<InT, 4, SIGMOID>)
-    : a.chunk <= 8  ? with(&device::route<InT, 8, SIGMOID>)
-    : a.chunk <= 16 ? with(&device::route<InT, 16, SIGMOID>)
-    : a.chunk <= 32 ? with(&device::route<InT, 32, SIGMOID>)
-                    : with(&device::route<InT, 64, SIGMOID>);
+    by_chunk(a.chunk, [&](auto c) {
+        constexpr int CHUNK = decltype(c)::value;
+        const bool    lanes_full = a.spread * a.groups == device::route_lanes && a.size == a.spread * a.chunk;
+        const bool    whole = lanes_full && whole_runs<InT, CHUNK>(a.logits, a.chunk) && whole_runs<float, CHUNK>(a.bias, a.chunk);
+        auto with = [&](auto kernel) { follow(kernel, token_groups(a.tokens), dim3(256), stream, a); };
+        if(a.k <= 8)
+        {
+            whole ? with(&device::route<InT, CHUNK, SIGMOID, true, 8>) : with(&device::route<InT, CHUNK, SIGMOID, false, 8>);
+        }
+        else
+        {
+            with(&device::route<InT, CHUNK, SIGMOID, false, device::most_choices>);
+        }
+    });
+}
+
+template<class InT, bool SIGMOID>
+void launch_route_backward(const device::route_back_args& a, hipStream_t stream)
+{
+    by_chunk(a.chunk, [&](auto c) {
+        constexpr int CHUNK = decltype(c)::value;
+        if constexpr(CHUNK <= 32) // (512 experts on 16 lanes)
+        {
+            const bool whole = a.experts == a.chunk * device::route_lanes && whole_runs<InT, CHUNK>(a.logits, a.chunk)
+                               && whole_runs<InT, CHUNK>(a.dlogits, a.chunk);
+            follow(whole ? &device::route_backward<InT, CHUNK, SIGMOID, true> : &device::route_backward<InT, CHUNK, SIGMOID, false>,
+                   token_groups(a.tokens), dim3(256), stream, a);
+        }
+    });
 }
 
 int route(int type, int* chosen, float* weights, const void* logits, const rocm_wmma_gemm_routing& r, size_t M, size_t E,
@@ -101,19 +152,12 @@ int route_backward(int type, void* dlogits, const float* dweights, const int* ch
         return ROCM_WMMA_GEMM_ERR_ARGUMENT;
     }
     const device::route_back_args a{dlogits, dweights, chosen, logits, static_cast<long long>(M), static_cast<int>(E),
-                                    static_cast<int>(k), renormalize, scale};
+                                    static_cast<int>(k), renormalize, static_cast<int>(ceil_div(E, device::route_lanes)), scale};
     by_element(type, [&](auto* typed) {
         using in_t = std::remove_pointer_t<decltype(typed)>;
-        follow(score == ROCM_WMMA_GEMM_SCORE_SIGMOID ? &device::route_backward<in_t, true> : &device::route_backward<in_t, false>,
-               dim3(static_cast<unsigned>(std::min(ceil_div(M, 256 / device::route_lanes), most_groups_x))), dim3(256), stream, a);
+        score == ROCM_WMMA_GEMM_SCORE_SIGMOID ? launch_route_backward<in_t, true>(a, stream) : launch_route_backward<in_t, false>(a, stream);
     });
     return ROCM_WMMA_GEMM_OK;
-}
-
-// Whether an address may be read in pieces of that many bytes (a power of two).
-bool starts_on(const void* p, size_t bytes)
-{
-    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
 }
 
 int dispatch(int type, void* rows, int* offsets, int* places, const void* x, const int* chosen, size_t E, size_t M, size_t N,
