@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(256) route_backward(const route_back_args args
 // A stable counting sort of the choices by expert, 1024 threads a block, 64 choices a wave at a time: the lanes
 // with one expert find each other by nine ballots, one for each bit of its number, and their leader counts them in its
 // wave's row of the histogram.  Nothing depends on the order in which waves or blocks run.
-constexpr int sort_waves = 16, sort_rounds = 4, sort_block = sort_waves * 64 * sort_rounds; // choices of a block
+constexpr int sort_waves = 16, sort_round = sort_waves * 64, sort_rounds = 4, sort_block = sort_round * sort_rounds; // choices
 
 struct sort_tables
 {
@@ -606,20 +606,26 @@ struct sort_tables
 
 // The ranks of a block's choices within their expert and block, in rank[]; the block's counts by expert in
 // tables.first[0 .. experts - 1].  Choices outside the experts have rank -1.
+template<int ROUNDS>
 __device__ __forceinline__ void rank_choices(const int* chosen, long long begin, long long end, int experts, sort_tables& tables,
-                                             int (&expert)[sort_rounds], int (&rank)[sort_rounds])
+                                             int (&expert)[ROUNDS], int (&rank)[ROUNDS])
 {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for(int e = threadIdx.x; e < sort_waves * max_groups; e += 1024)
-    {
-        (&tables.counts[0][0])[e] = 0;
-    }
-    __syncthreads();
 #pragma unroll
-    for(int r = 0; r < sort_rounds; ++r)
+    for(int r = 0; r < ROUNDS; ++r)
     {
-        const long long at = begin + (wave * sort_rounds + r) * 64 + lane;
-        int             e  = at < end ? chosen[at] : -1;
+        const long long at = begin + (wave * ROUNDS + r) * 64 + lane;
+        expert[r]          = at < end ? chosen[at] : -1;
+    }
+    for(int e = lane; e < experts; e += 64)
+    {
+        tables.counts[wave][e] = 0; // (its own wave's: LDS serves a wave in order)
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for(int r = 0; r < ROUNDS; ++r)
+    {
+        const int       e  = expert[r];
         const bool      is = e >= 0 && e < experts;
         unsigned long long same = __ballot(is);
 #pragma unroll
@@ -660,7 +666,7 @@ __device__ __forceinline__ void rank_choices(const int* chosen, long long begin,
     }
     __syncthreads();
 #pragma unroll
-    for(int r = 0; r < sort_rounds; ++r)
+    for(int r = 0; r < ROUNDS; ++r)
     {
         rank[r] += expert[r] >= 0 ? tables.counts[wave][expert[r]] : 0;
     }
@@ -713,29 +719,93 @@ struct dispatch_args
     int         copy; // 0: rows are not wanted
 };
 
-// The counts of every block and the ranks within it (in places, until the bases are known).  A single block knows
-// all: it writes places and offsets.
-__global__ void __launch_bounds__(1024) dispatch_rank(const dispatch_args args)
+// A piece of a token's row to the places of its choices (place: of choice `lane`).
+template<class Piece>
+__device__ __forceinline__ void copy_row(const dispatch_args& args, long long token, int place, long long at, long long end)
+{
+    const long long    pieces = args.row_bytes / (long long)sizeof(Piece);
+    const Piece* const from   = static_cast<const Piece*>(args.x) + token * pieces;
+    Piece* const       to     = static_cast<Piece*>(args.rows);
+    // (four pieces of a lane on their way at a time)
+    for(; at < end; at += 256)
+    {
+        Piece v[4];
+#pragma unroll
+        for(int u = 0; u < 4; ++u)
+        {
+            v[u] = at + 64 * u < end ? from[at + 64 * u] : Piece{};
+        }
+        for(int j = 0; j < args.k; ++j)
+        {
+            const int p = __builtin_amdgcn_readlane(place, j);
+            if(p >= 0)
+            {
+#pragma unroll
+                for(int u = 0; u < 4; ++u)
+                {
+                    if(at + 64 * u < end)
+                    {
+                        to[p * pieces + at + 64 * u] = v[u];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// All of it in one launch, for up to ROUNDS * 1024 choices: every workgroup sorts all of them for itself and copies its share
+// of the rows, 64 pieces of a row a wave.  32 tokens of 8 choices, rows of 8 KB: 6.4 us, where two launches took 11.0.
+template<int ROUNDS, class Piece>
+__global__ void __launch_bounds__(1024) dispatch_few(const dispatch_args args)
 {
     __shared__ sort_tables tables;
-    int                    expert[sort_rounds], rank[sort_rounds];
-    const long long        begin = (long long)blockIdx.x * sort_block;
-    rank_choices(args.chosen, begin, args.slots, args.experts, tables, expert, rank);
-    const bool alone = args.blocks == 1;
-    if(alone)
+    __shared__ int         places[ROUNDS * sort_round];
+    int                    expert[ROUNDS], rank[ROUNDS];
+    rank_choices<ROUNDS>(args.chosen, 0, args.slots, args.experts, tables, expert, rank);
+    scan_experts(tables.first, args.experts);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for(int r = 0; r < ROUNDS; ++r)
     {
-        scan_experts(tables.first, args.experts);
+        const int at = (wave * ROUNDS + r) * 64 + lane;
+        places[at]   = expert[r] < 0 ? -1 : tables.first[expert[r]] + rank[r];
+        if(blockIdx.x == 0 && at < args.slots)
+        {
+            args.places[at] = places[at];
+        }
+    }
+    if(blockIdx.x == 0)
+    {
         for(int e = threadIdx.x; e <= args.experts; e += 1024)
         {
             args.offsets[e] = tables.first[e];
         }
     }
-    else
+    if(!args.copy)
     {
-        for(int e = threadIdx.x; e < args.experts; e += 1024)
-        {
-            args.counts[(long long)blockIdx.x * args.experts + e] = tables.first[e];
-        }
+        return;
+    }
+    __syncthreads();
+    const long long pieces = args.row_bytes / (long long)sizeof(Piece), runs = (pieces + 63) / 64, all = args.tokens * runs;
+    // (neighbouring runs on different compute units)
+    for(long long run = blockIdx.x + (long long)gridDim.x * wave; run < all; run += (long long)gridDim.x * sort_waves)
+    {
+        const long long token = run / runs, at = (run - token * runs) * 64 + lane;
+        const int       place = lane < args.k ? places[token * args.k + lane] : -1;
+        copy_row<Piece>(args, token, place, at, at < pieces ? at + 1 : at);
+    }
+}
+
+// The counts of every block, and the ranks within it in places, until it is known what lies before.
+__global__ void __launch_bounds__(1024) dispatch_rank(const dispatch_args args)
+{
+    __shared__ sort_tables tables;
+    int                    expert[sort_rounds], rank[sort_rounds];
+    const long long        begin = (long long)blockIdx.x * sort_block;
+    rank_choices<sort_rounds>(args.chosen, begin, args.slots, args.experts, tables, expert, rank);
+    for(int e = threadIdx.x; e < args.experts; e += 1024)
+    {
+        args.counts[(long long)blockIdx.x * args.experts + e] = tables.first[e];
     }
 #pragma unroll
     for(int r = 0; r < sort_rounds; ++r)
@@ -743,12 +813,13 @@ __global__ void __launch_bounds__(1024) dispatch_rank(const dispatch_args args)
         const long long at = begin + ((threadIdx.x >> 6) * sort_rounds + r) * 64 + (threadIdx.x & 63);
         if(at < args.slots)
         {
-            args.places[at] = expert[r] < 0 ? -1 : alone ? tables.first[expert[r]] + rank[r] : rank[r];
+            args.places[at] = expert[r] < 0 ? -1 : rank[r];
         }
     }
 }
 
-// Where every block's choices of every expert begin, and the offsets.  One workgroup.
+// Where every block's choices of every expert begin (in counts), and the offsets.  One workgroup; for tables that are too
+// large for dispatch_rows to add up.
 __global__ void __launch_bounds__(1024) dispatch_scan(const dispatch_args args)
 {
     __shared__ int first[max_groups + 1];
@@ -782,43 +853,74 @@ __global__ void __launch_bounds__(1024) dispatch_scan(const dispatch_args args)
     }
 }
 
-// A token's row to the places of its choices; a wave a token, PIECE bytes a lane.  With counts (several blocks) the
-// places are still ranks: their bases are added first.
-template<class Piece>
-__global__ void __launch_bounds__(256) dispatch_rows(const dispatch_args args)
+// Adds what lies before a block's choices of an expert to their ranks, and copies the rows.  A workgroup takes `each`
+// tokens in a row, whose choices lie in one block or in two neighbouring ones.  SCANNED: counts already say where the blocks' begin;
+// else every workgroup adds up the (small) table.  A wave a token.
+template<class Piece, bool SCANNED>
+__global__ void __launch_bounds__(256) dispatch_rows(const dispatch_args args, int each)
 {
-    const int lane = threadIdx.x & 63;
-    for(long long token = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); token < args.tokens; token += (long long)gridDim.x * 4)
+    __shared__ int  first[max_groups + 1], base[2][max_groups];
+    const long long token0 = (long long)blockIdx.x * each;
+    const int       block0 = (int)(token0 * args.k / sort_block);
+    if constexpr(SCANNED)
+    {
+        for(int e = threadIdx.x; e < args.experts; e += 256)
+        {
+            base[0][e] = args.counts[(long long)block0 * args.experts + e];
+            base[1][e] = block0 + 1 < args.blocks ? args.counts[(long long)(block0 + 1) * args.experts + e] : 0;
+        }
+    }
+    else
+    {
+        for(int e = threadIdx.x; e < args.experts; e += 256)
+        {
+            int all = 0, before = 0, own = 0;
+#pragma unroll 8
+            for(int b = 0; b < args.blocks; ++b)
+            {
+                const int count = args.counts[b * args.experts + e];
+                all += count;
+                before += b < block0 ? count : 0;
+                own += b == block0 ? count : 0;
+            }
+            first[e]   = all;
+            base[0][e] = before;
+            base[1][e] = before + own;
+        }
+        __syncthreads();
+        scan_experts(first, args.experts);
+        for(int e = threadIdx.x; e < args.experts; e += 256)
+        {
+            base[0][e] += first[e];
+            base[1][e] += first[e];
+        }
+        if(blockIdx.x == 0)
+        {
+            for(int e = threadIdx.x; e <= args.experts; e += 256)
+            {
+                args.offsets[e] = first[e];
+            }
+        }
+    }
+    __syncthreads();
+    const int       lane   = threadIdx.x & 63;
+    const long long token1 = token0 + each < args.tokens ? token0 + each : args.tokens;
+    for(long long token = token0 + (threadIdx.x >> 6); token < token1; token += 4)
     {
         const long long slot  = token * args.k + lane;
         int             place = -1;
         if(lane < args.k)
         {
             place = args.places[slot];
-            if(args.counts != nullptr && place >= 0)
+            if(place >= 0)
             {
-                place += args.counts[slot / sort_block * args.experts + args.chosen[slot]];
+                place += base[slot / sort_block - block0][args.chosen[slot]];
                 args.places[slot] = place;
             }
         }
-        if(!args.copy)
+        if(args.copy)
         {
-            continue;
-        }
-        const long long    pieces = args.row_bytes / (long long)sizeof(Piece);
-        const Piece* const from   = static_cast<const Piece*>(args.x) + token * pieces;
-        Piece* const       to     = static_cast<Piece*>(args.rows);
-        for(long long at = lane; at < pieces; at += 64)
-        {
-            const Piece v = from[at];
-            for(int j = 0; j < args.k; ++j)
-            {
-                const int p = __builtin_amdgcn_readlane(place, j);
-                if(p >= 0)
-                {
-                    to[p * pieces + at] = v;
-                }
-            }
+            copy_row<Piece>(args, token, place, lane, args.row_bytes / (long long)sizeof(Piece));
         }
     }
 }

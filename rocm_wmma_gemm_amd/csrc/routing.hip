@@ -160,6 +160,23 @@ int route_backward(int type, void* dlogits, const float* dweights, const int* ch
     return ROCM_WMMA_GEMM_OK;
 }
 
+// Calls f with a null pointer of a piece of a row.
+template<class F>
+void by_piece(size_t bytes, F&& f)
+{
+    switch(bytes)
+    {
+        case 16: f(static_cast<device::u32x4*>(nullptr)); break;
+        case 8: f(static_cast<unsigned long long*>(nullptr)); break;
+        case 4: f(static_cast<unsigned int*>(nullptr)); break;
+        default: f(static_cast<unsigned short*>(nullptr)); break;
+    }
+}
+
+// Counts that every workgroup adds up for itself rather than wait for a launch that does (8191 tokens of 6 choices
+// over 128 experts, 1536 counts: 59 us against 65).
+constexpr size_t most_added_up = 8192;
+
 int dispatch(int type, void* rows, int* offsets, int* places, const void* x, const int* chosen, size_t E, size_t M, size_t N,
              size_t k, hipStream_t stream)
 {
@@ -181,34 +198,42 @@ int dispatch(int type, void* rows, int* offsets, int* places, const void* x, con
                             static_cast<long long>(N * element_size(type)), static_cast<int>(E), static_cast<int>(k), 1, copy};
     const size_t blocks = std::max<size_t>(1, ceil_div(slots, device::sort_block));
     a.blocks            = static_cast<int>(blocks);
-    workspace_lease lease;
-    if(blocks > 1)
+    size_t piece        = 16;
+    while(piece > 2 && (a.row_bytes % piece != 0 || !starts_on(x, piece) || !starts_on(rows, piece)))
     {
-        a.counts = reinterpret_cast<int*>(lease.acquire(blocks * std::max<size_t>(1, E) * sizeof(int), stream));
-        if(a.counts == nullptr)
-        {
-            return ROCM_WMMA_GEMM_ERR_SCRATCH;
-        }
+        piece /= 2;
+    }
+    if(blocks == 1)
+    {
+        // (a run of 64 pieces a wave, spread over the compute units)
+        const size_t runs = M * ceil_div(a.row_bytes / piece, 64);
+        const dim3   grid(static_cast<unsigned>(copy ? std::min<size_t>(std::max<size_t>(1, ceil_div(runs, 4)), compute_units()) : 1));
+        by_piece(piece, [&](auto* typed) {
+            using piece_t = std::remove_pointer_t<decltype(typed)>;
+            follow(slots <= device::sort_round ? &device::dispatch_few<1, piece_t> : &device::dispatch_few<device::sort_rounds, piece_t>,
+                   grid, dim3(1024), stream, a);
+        });
+        return ROCM_WMMA_GEMM_OK;
+    }
+    workspace_lease lease;
+    a.counts = reinterpret_cast<int*>(lease.acquire(blocks * std::max<size_t>(1, E) * sizeof(int), stream));
+    if(a.counts == nullptr)
+    {
+        return ROCM_WMMA_GEMM_ERR_SCRATCH;
     }
     follow(&device::dispatch_rank, dim3(static_cast<unsigned>(blocks)), dim3(1024), stream, a);
-    if(blocks > 1)
+    const bool scanned = blocks * E > most_added_up;
+    if(scanned)
     {
         follow(&device::dispatch_scan, dim3(1), dim3(1024), stream, a);
     }
-    if(copy || blocks > 1)
-    {
-        size_t piece = 16;
-        while(piece > 1 && (a.row_bytes % piece != 0 || !starts_on(x, piece) || !starts_on(rows, piece)))
-        {
-            piece /= 2;
-        }
-        const dim3 grid(static_cast<unsigned>(std::min<size_t>(ceil_div(M, 4), size_t{1} << 16)));
-        follow(piece == 16  ? &device::dispatch_rows<device::u32x4>
-               : piece == 8 ? &device::dispatch_rows<unsigned long long>
-               : piece == 4 ? &device::dispatch_rows<unsigned int>
-                            : &device::dispatch_rows<unsigned short>,
-               grid, dim3(256), stream, a);
-    }
+    // (eight workgroups a compute unit where there are so many tokens; their choices end in the next block at the latest)
+    const size_t each = std::min(std::max<size_t>(4, ceil_div(M, 8 * compute_units())), device::sort_block / k);
+    by_piece(piece, [&](auto* typed) {
+        using piece_t = std::remove_pointer_t<decltype(typed)>;
+        follow(scanned ? &device::dispatch_rows<piece_t, true> : &device::dispatch_rows<piece_t, false>,
+               dim3(static_cast<unsigned>(ceil_div(M, each))), dim3(256), stream, a, static_cast<int>(each));
+    });
     return ROCM_WMMA_GEMM_OK;
 }
 

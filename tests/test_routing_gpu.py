@@ -238,7 +238,7 @@ def choices(M, k, E, seed, outside=0.0):
     return c.cuda()
 
 
-DISPATCHES = [(1, 8, 1, 1), (1, 5120, 8, 64), (5, 7, 3, 2), (32, 4096, 8, 64), (63, 100, 2, 512), (129, 33, 32, 5), (512, 64, 8, 16),
+DISPATCHES = [(1, 8, 1, 1), (1, 5120, 8, 64), (5, 7, 3, 2), (32, 4096, 8, 64), (63, 100, 2, 512), (129, 33, 32, 5), (512, 64, 8, 16), (128, 1000, 8, 11), (129, 520, 8, 11),
               (513, 8, 8, 17), (2000, 24, 6, 130), (3, 1, 1, 300), (4097, 3, 3, 9)]
 
 
@@ -268,9 +268,10 @@ def test_dispatch(loader, size, dtype):
         within(dx, sums.sum(1), (UNIT[dtype] + (k + 2) * E32) * sums.abs().sum(1) + LEAST[dtype], "gradient of x")
 
 
-def test_dispatch_of_many_choices(loader):
-    """More blocks than one round of the scan, against a stable sort."""
-    M, N, k, E = 70001, 8, 8, 256
+@pytest.mark.parametrize("size", [(70001, 8, 8, 256), (30000, 8, 8, 100), (3000, 8, 31, 512)], ids=_id)
+def test_dispatch_of_many_choices(loader, size):
+    """Tables of counts that the scan adds up and that every workgroup does, against a stable sort."""
+    M, N, k, E = size
     chosen, x = choices(M, k, E, 3, 0.1), rnd((M, N), F16, 4)
     rows, places = torch.zeros((M * k, N), dtype=F16, device="cuda"), torch.empty((M, k), dtype=torch.int32, device="cuda")
     offsets = torch.empty(E + 1, dtype=torch.int32, device="cuda")

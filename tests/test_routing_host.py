@@ -93,12 +93,14 @@ def test_every_launch_of_routing_fits_the_grid(recorded):  # noqa: F811
 
 
 def test_nothing_of_a_dispatch_follows_a_launch_that_failed(recorded):  # noqa: F811
-    call = ["dispatch", [1, "p", "p", "p", "p", "p", 64, 5000, 64, 4, None]]
-    (status, whole), = recorded(call)
-    assert status == 0 and len(whole) == 3
-    for n in range(3):
-        (status, launches), = recorded(["fail", n], call)
-        assert status == -4 and len(launches) == n + 1
+    # few choices, a table of counts that every workgroup adds up, one that is added up by a launch of its own
+    for m, e, steps in ((1000, 64, 1), (5000, 64, 2), (70000, 512, 3)):
+        call = ["dispatch", [1, "p", "p", "p", "p", "p", e, m, 64, 4, None]]
+        (status, whole), = recorded(call)
+        assert status == 0 and len(whole) == steps
+        for n in range(steps):
+            (status, launches), = recorded(["fail", n], call)
+            assert status == -4 and len(launches) == n + 1
 
 
 ROUTES = """
