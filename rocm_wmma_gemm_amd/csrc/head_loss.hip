@@ -23,10 +23,8 @@ constexpr size_t piece_bytes = size_t{128} << 20;
 // A piece of their gradient in 16 bits.
 constexpr size_t slope_bytes = size_t{512} << 20;
 // The statistics of rows that go together.
-constexpr size_t parts_bytes = size_t{256} << 20;
+constexpr size_t parts_bytes = size_t{256} << 20, most_parts_bytes = size_t{4} << 30;
 constexpr size_t least_piece = 1024, piece_grain = 256; // columns
-// Fewer rows stream the weights through the few-row kernels, which write their logits.
-constexpr size_t least_fused_rows = 192;
 
 // An operand's rows in memory.
 struct operand
@@ -179,12 +177,13 @@ step logits_of(const head& h, int finish, const operand& a, const operand& b, si
     return s;
 }
 
-// Whether the logits' products end in a tile's statistics or gradients, or write the logits for a pass of their own: few
-// rows, and rows too long for the tiles' offsets.
-bool fuses(const head& h, const operand& a, const operand& b)
+// How the logits' products run where they end in a tile's statistics (finish_parts) or gradients (finish_slope); no kernel
+// where they write the logits for a pass of their own: rows too long for the tiles' offsets, and few rows against weights
+// that would have to be copied first, which cost more than that pass.
+launch_choice fused_plan(const head& h, int finish, const operand& a, const operand& b, size_t cols)
 {
-    return h.M >= least_fused_rows && h.N != 0
-           && logits_of(h, finish_slope, a, b, 0, h.N, nullptr, round_up8(h.N)).plan(compute_units()).kernel.fn != nullptr;
+    const launch_choice c = logits_of(h, finish, a, b, 0, cols, nullptr, round_up8(cols)).plan(compute_units());
+    return c.copy_a || c.copy_b ? launch_choice{} : c;
 }
 
 // dA += dz B^T for a piece, rows `pitch` apart
@@ -277,7 +276,7 @@ head rows_of(const head& h, size_t row0, size_t rows)
     return p;
 }
 
-// The listed logits where no logits are written.
+// The listed logits where no logits are written and the tiles do not look for them.
 void pick(const head& h, const operand& a, const operand& b, float* picked, hipStream_t stream)
 {
     const bool     nk = h.layout_b == 1;
@@ -298,24 +297,30 @@ void pick(const head& h, const operand& a, const operand& b, float* picked, hipS
 // loss, lse and (a list) the listed logits of some rows, from operands whose copies are made
 struct loss_plan
 {
-    bool   fused;
+    bool   fused, gathers; // its tiles end in statistics; the listed logits are worked out on their own
     pieces p;
     size_t each, all; // parts of a piece, of a row
     size_t z_at, parts_at, picked_at, product_at, product;
     launch_choice tiles; // fused
     loss_plan(const head& h, const operand& a, const operand& b, bool own_picked, room r)
-        // (a column of weights that are stored K x N is gathered element by element: a list of them is picked from the logits)
-        : fused((h.layout_b == 1 || h.want.teacher == nullptr) && fuses(h, a, b)), p(h.N, fused ? h.N : piece_bytes / (4 * h.M))
+        : fused(false), p(0, 0)
     {
         product = 0;
+        tiles   = fused_plan(h, finish_parts, a, b, h.N);
+        // (the few-row kernels look for the listed entries themselves; a column of weights that are stored K x N is gathered
+        // element by element, so a list of them is picked from the logits)
+        gathers = tiles.kernel.per_cu != 0;
+        fused   = tiles.kernel.fn != nullptr && (!gathers || h.layout_b == 1 || h.want.teacher == nullptr);
+        p       = pieces(h.N, fused ? h.N : piece_bytes / (4 * h.M));
         if(fused)
         {
-            tiles   = logits_of(h, finish_parts, a, b, 0, h.N, nullptr, round_up8(h.N)).plan(compute_units());
-            each    = ceil_div(h.N, tiles.kernel.block_n / 2); // (a wave's columns)
-            all     = each;
-            product = tiles.scratch();
+            // (a wave's columns of a tile, or a tile of the few-row kernels)
+            each  = ceil_div(h.N, tiles.kernel.per_cu != 0 ? tiles.kernel.block_n / 2 : tiles.kernel.block_n);
+            all   = each;
+            fused = h.M * all * sizeof(device::softmax_part) <= most_parts_bytes;
+            p     = fused ? p : pieces(h.N, piece_bytes / (4 * h.M));
         }
-        else
+        if(!fused)
         {
             each = ceil_div(p.cols, device::part_cols);
             all  = h.N != 0 ? each * p.count : 0;
@@ -350,12 +355,19 @@ int loss_of_rows(const head& h, const loss_plan& plan, const operand& a, const o
         step s              = logits_of(h, finish_parts, a, b, 0, h.N, nullptr, round_up8(h.N));
         s.args.parts        = parts;
         s.args.parts_of_row = static_cast<int>(plan.all);
-        const int rc        = launch_product(s.types, s.finish, plan.tiles, s.args, plan.product != 0 ? scratch : nullptr, stream);
+        s.args.entries      = h.want.entries;
+        s.args.wide_entries = h.want.wide;
+        s.args.listed       = h.want.k;
+        s.args.picked       = of_targets;
+        const int rc        = launch_product(s.types, s.finish, plan.tiles, s.args, nullptr, stream);
         if(rc != ROCM_WMMA_GEMM_OK)
         {
             return rc;
         }
-        pick(h, a, b, of_targets, stream);
+        if(plan.gathers)
+        {
+            pick(h, a, b, of_targets, stream);
+        }
     }
     const unsigned pick_groups = static_cast<unsigned>(std::min<size_t>(ceil_div(h.M * h.want.k, 256), 4096));
     for(size_t v0 = 0; !plan.fused && v0 < std::max<size_t>(h.N, 1); v0 += plan.p.cols)
@@ -393,7 +405,7 @@ int loss_of(const head& h, float* loss, float* lse, float* picked, hipStream_t s
         return ROCM_WMMA_GEMM_ERR_ARGUMENT;
     }
     // rows have nothing to do with each other: as many go together as leave the statistics their room (64 columns a part)
-    const size_t some = std::min(h.M, std::max<size_t>(4096, parts_bytes / sizeof(device::softmax_part) / (h.N / 64 + 1)));
+    const size_t some = std::min(h.M, std::max<size_t>(256, parts_bytes / sizeof(device::softmax_part) / (h.N / 64 + 1)));
     room         r;
     const copies c(h, pieces(h.N, piece_bytes / (4 * some)).count, r);
     const loss_plan first(rows_of(h, 0, some), c.plan_a(h), c.plan_b(h), picked == nullptr, r);
@@ -456,7 +468,7 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     room         r;
     const copies c(h, pieces(h.N, slope_bytes / (2 * rows)).count, r);
     const operand plan_a = c.plan_a(h), plan_b = c.plan_b(h);
-    const bool   fused = fuses(h, plan_a, plan_b);
+    const bool   fused = h.N != 0 && fused_plan(h, finish_slope, plan_a, plan_b, h.N).kernel.fn != nullptr;
     const pieces p(h.N, fused ? slope_bytes / (2 * rows) : piece_bytes / (4 * rows));
     const size_t pitch = p.pitch(), k_pitch = round_up8(h.K);
     const size_t z_at = fused ? 0 : r.take(h.M * pitch * 4), dz_at = r.take(h.M * pitch * 2),

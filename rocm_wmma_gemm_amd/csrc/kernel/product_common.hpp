@@ -61,6 +61,13 @@ struct loss_record
     int   unused; // (16 bytes)
 };
 
+// A column that a list names, -1 where it is none of a matrix' `cols`.
+__device__ __forceinline__ int listed_column(const void* entries, int wide, long long at, int cols)
+{
+    const long long v = wide ? static_cast<const long long*>(entries)[at] : (long long)static_cast<const int*>(entries)[at];
+    return v >= 0 && v < cols ? (int)v : -1;
+}
+
 struct act_args
 {
     act_kind kind;
@@ -90,8 +97,11 @@ struct product_args
     const float* alpha_at; // nullptr, or where on the device alpha is (finish_back)
     const loss_record* records; // one a row
     softmax_part* parts; // rows x parts_of_row
-    int          parts_of_row, part0; // the launch's first part
+    int          parts_of_row;
     int          col_base; // the first column's number in the matrix that B is a block of
+    const void*  entries; // rows x listed columns whose logits go to picked (loss_use::parts), of 32 or 64 bits
+    int          listed, wide_entries; // (the few-row kernels; the tiled ones leave their statistics alone)
+    float*       picked; // rows x listed
     act_args     act;
     int          keep_sum; // kept holds 0: alpha A B + bias, before the activation (A's type);
                            // 1: the finished value, C's, in A's type

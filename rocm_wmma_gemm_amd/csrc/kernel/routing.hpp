@@ -598,6 +598,25 @@ __global__ void __launch_bounds__(256) route_backward(const route_back_args args
 // wave's row of the histogram.  Nothing depends on the order in which waves or blocks run.
 constexpr int sort_waves = 16, sort_round = sort_waves * 64, sort_rounds = 4, sort_block = sort_round * sort_rounds; // choices
 
+// Rows of this many bytes are written past the caches: they are not in the 256 MB memory-side cache when they are read next.
+// With a reader behind them, 256 MB of rows: 124.4 us against 125.5, 512 MB 253 against 266; but 128 MB 69 against 59, and
+// the gradients of 128 MB, 256 MB and 512 MB 77 against 79, 182 against 189 and 353 against 360.
+constexpr long long streamed_bytes = 256ll << 20;
+
+// (a template argument: the compiler joins the two stores of a branch, without the hint)
+template<bool STREAMED, class Piece>
+__device__ __forceinline__ void put(Piece* to, const Piece& v)
+{
+    if constexpr(STREAMED)
+    {
+        __builtin_nontemporal_store(v, to);
+    }
+    else
+    {
+        *to = v;
+    }
+}
+
 struct sort_tables
 {
     int counts[sort_waves][max_groups]; // of a wave, then what lies before it in its block
@@ -720,7 +739,7 @@ struct dispatch_args
 };
 
 // A piece of a token's row to the places of its choices (place: of choice `lane`).
-template<class Piece>
+template<class Piece, bool STREAMED>
 __device__ __forceinline__ void copy_row(const dispatch_args& args, long long token, int place, long long at, long long end)
 {
     const long long    pieces = args.row_bytes / (long long)sizeof(Piece);
@@ -745,7 +764,7 @@ __device__ __forceinline__ void copy_row(const dispatch_args& args, long long to
                 {
                     if(at + 64 * u < end)
                     {
-                        to[p * pieces + at + 64 * u] = v[u];
+                        put<STREAMED>(to + p * pieces + at + 64 * u, v[u]);
                     }
                 }
             }
@@ -792,7 +811,7 @@ __global__ void __launch_bounds__(1024) dispatch_few(const dispatch_args args)
     {
         const long long token = run / runs, at = (run - token * runs) * 64 + lane;
         const int       place = lane < args.k ? places[token * args.k + lane] : -1;
-        copy_row<Piece>(args, token, place, at, at < pieces ? at + 1 : at);
+        copy_row<Piece, false>(args, token, place, at, at < pieces ? at + 1 : at);
     }
 }
 
@@ -856,7 +875,7 @@ __global__ void __launch_bounds__(1024) dispatch_scan(const dispatch_args args)
 // Adds what lies before a block's choices of an expert to their ranks, and copies the rows.  A workgroup takes `each`
 // tokens in a row, whose choices lie in one block or in two neighbouring ones.  SCANNED: counts already say where the blocks' begin;
 // else every workgroup adds up the (small) table.  A wave a token.
-template<class Piece, bool SCANNED>
+template<class Piece, bool SCANNED, bool STREAMED>
 __global__ void __launch_bounds__(256) dispatch_rows(const dispatch_args args, int each)
 {
     __shared__ int  first[max_groups + 1], base[2][max_groups];
@@ -920,7 +939,7 @@ __global__ void __launch_bounds__(256) dispatch_rows(const dispatch_args args, i
         }
         if(args.copy)
         {
-            copy_row<Piece>(args, token, place, lane, args.row_bytes / (long long)sizeof(Piece));
+            copy_row<Piece, STREAMED>(args, token, place, lane, args.row_bytes / (long long)sizeof(Piece));
         }
     }
 }
@@ -1003,7 +1022,7 @@ __global__ void __launch_bounds__(256) combine(const combine_args args, int bloc
 
 // The gradients: of a row, weight * dout; of a weight, the product of dout with its row.  A wave a choice: the k waves
 // of a token share dout in the caches.
-template<class InT, class OutT, int WIDTH>
+template<class InT, class OutT, int WIDTH, bool STREAMED>
 __global__ void __launch_bounds__(256) combine_backward(const combine_args args)
 {
     const int lane = threadIdx.x & 63;
@@ -1039,7 +1058,7 @@ __global__ void __launch_bounds__(256) combine_backward(const combine_args args)
                     {
                         o[v] = to_out<InT>(w * (float)d[v]);
                     }
-                    *reinterpret_cast<vec_of<InT, WIDTH>*>(to + col) = o;
+                    put<STREAMED>(reinterpret_cast<vec_of<InT, WIDTH>*>(to + col), o);
                 }
             }
         }

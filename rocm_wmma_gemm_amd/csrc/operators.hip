@@ -209,6 +209,7 @@ float round_us(const form_cost& f, size_t tiles, size_t cus, int per_cu, float k
 
 launch_choice choose(int types, int layout, int finish, const product_args& given, size_t cus)
 {
+    const bool         logits    = finish == finish_parts || finish == finish_slope; // (whole tiles)
     const bool         symmetric = finish == finish_square || finish == finish_poly;
     const starts_on_16 aligned   = alignment_of(given);
     const bool         copy_a = !aligned.a, copy_b = !aligned.b;
@@ -330,7 +331,7 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
             for(const size_t slices : {1, 2, 4})
             {
                 const launch_choice s = slices == 1 ? c : with_slices(c, slices);
-                if(slices > 1 && (batch || s.k_slices == 1 || tiles * slices > slots))
+                if(slices > 1 && (batch || logits || s.k_slices == 1 || tiles * slices > slots))
                 {
                     continue;
                 }

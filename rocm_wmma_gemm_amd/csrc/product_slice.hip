@@ -22,6 +22,8 @@ using res_t = std::conditional_t<kTypes == types_steps_f16 || kTypes == types_st
 
 constexpr product_kernel kNone{nullptr, 0, 0, 0, nullptr, nullptr, 0};
 constexpr bool           kSteps = kTypes >= types_steps_square;
+// logits that leave their statistics or gradient: C has the operands' type, or there is none
+constexpr bool kLogits = kTypes == types_f16_f16 || kTypes == types_bf16_bf16;
 
 template<class Impl>
 product_kernel made(int block_m, int block_n, int per_cu)
@@ -66,7 +68,7 @@ product_kernel tiled_finish(int finish)
             case finish_logistic: return tiled<LAYOUT, BM, BN, device::epilogue_logistic>();
             default: break;
         }
-        if constexpr(kTypes == types_f16_f16 || kTypes == types_bf16_bf16) // logits: C has the operands' type, or there is none
+        if constexpr(kLogits)
         {
             switch(finish)
             {
@@ -117,8 +119,18 @@ product_kernel narrow(int finish)
     }
 }
 
+template<int LAYOUT, int BM, int BN, device::loss_use LOSS>
+product_kernel skinny_of()
+{
+    using impl       = device::skinny_product<kIn, out_t, res_t, BM, BN, LAYOUT == layout_kk, false, LOSS>;
+    using once       = device::skinny_product<kIn, out_t, res_t, BM, BN, LAYOUT == layout_kk, true, LOSS>;
+    product_kernel k = made<impl>(BM, BN, 0);
+    k.once           = &device::product_entry<once>;
+    return k;
+}
+
 template<int LAYOUT, int BM, int BN>
-product_kernel skinny()
+product_kernel skinny(int finish)
 {
     if constexpr(kSteps && LAYOUT == (kTypes == types_steps_square ? layout_kk : layout_kn) && BM >= 32 && BN >= 32)
     {
@@ -127,11 +139,18 @@ product_kernel skinny()
     constexpr bool built = (BN == 64 && BM < 64) ? LAYOUT == layout_kn : BN == 16 ? LAYOUT == layout_kk : true;
     if constexpr(!kSteps && LAYOUT != layout_mn && built)
     {
-        using impl       = device::skinny_product<kIn, out_t, res_t, BM, BN, LAYOUT == layout_kk, false>;
-        using once       = device::skinny_product<kIn, out_t, res_t, BM, BN, LAYOUT == layout_kk, true>;
-        product_kernel k = made<impl>(BM, BN, 0);
-        k.once           = &device::product_entry<once>;
-        return k;
+        if constexpr(kLogits)
+        {
+            if(finish == finish_parts)
+            {
+                return skinny_of<LAYOUT, BM, BN, device::loss_use::parts>();
+            }
+            if(finish == finish_slope)
+            {
+                return skinny_of<LAYOUT, BM, BN, device::loss_use::slope>();
+            }
+        }
+        return skinny_of<LAYOUT, BM, BN, device::loss_use::none>();
     }
     else
     {
@@ -160,7 +179,8 @@ product_kernel general(int form)
 template<int LAYOUT>
 product_kernel in_layout(int form, int finish)
 {
-    if((finish == finish_parts || finish == finish_slope) && (form < form_tiled_256 || form > form_tiled_192))
+    // (logits: the general kernel and the narrow one are not built)
+    if((finish == finish_parts || finish == finish_slope) && (!kLogits || form < form_tiled_256 || form == form_narrow_128))
     {
         return kNone;
     }
@@ -183,13 +203,13 @@ product_kernel in_layout(int form, int finish)
             }
             return kNone;
         case form_narrow_128: return narrow<LAYOUT>(finish);
-        case form_skinny_16x32: return skinny<LAYOUT, 16, 32>();
-        case form_skinny_16x64: return skinny<LAYOUT, 16, 64>();
-        case form_skinny_32x32: return skinny<LAYOUT, 32, 32>();
-        case form_skinny_32x64: return skinny<LAYOUT, 32, 64>();
-        case form_skinny_64x32: return skinny<LAYOUT, 64, 32>();
-        case form_skinny_64x64: return skinny<LAYOUT, 64, 64>();
-        case form_skinny_32x16: return skinny<LAYOUT, 32, 16>();
+        case form_skinny_16x32: return skinny<LAYOUT, 16, 32>(finish);
+        case form_skinny_16x64: return skinny<LAYOUT, 16, 64>(finish);
+        case form_skinny_32x32: return skinny<LAYOUT, 32, 32>(finish);
+        case form_skinny_32x64: return skinny<LAYOUT, 32, 64>(finish);
+        case form_skinny_64x32: return skinny<LAYOUT, 64, 32>(finish);
+        case form_skinny_64x64: return skinny<LAYOUT, 64, 64>(finish);
+        case form_skinny_32x16: return skinny<LAYOUT, 32, 16>(finish);
         default: return kNone;
     }
 }

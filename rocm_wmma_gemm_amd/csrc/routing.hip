@@ -228,10 +228,12 @@ int dispatch(int type, void* rows, int* offsets, int* places, const void* x, con
         follow(&device::dispatch_scan, dim3(1), dim3(1024), stream, a);
     }
     // (eight workgroups a compute unit where there are so many tokens; their choices end in the next block at the latest)
+    const bool   streamed = slots * N * element_size(type) >= device::streamed_bytes;
     const size_t each = std::min(std::max<size_t>(4, ceil_div(M, 8 * compute_units())), device::sort_block / k);
     by_piece(piece, [&](auto* typed) {
         using piece_t = std::remove_pointer_t<decltype(typed)>;
-        follow(scanned ? &device::dispatch_rows<piece_t, true> : &device::dispatch_rows<piece_t, false>,
+        follow(streamed ? (scanned ? &device::dispatch_rows<piece_t, true, true> : &device::dispatch_rows<piece_t, false, true>)
+                        : (scanned ? &device::dispatch_rows<piece_t, true, false> : &device::dispatch_rows<piece_t, false, false>),
                dim3(static_cast<unsigned>(ceil_div(M, each))), dim3(256), stream, a, static_cast<int>(each));
     });
     return ROCM_WMMA_GEMM_OK;
@@ -277,10 +279,13 @@ int combine_backward(int rows_type, int out_type, const device::combine_args& a,
 {
     const size_t in = element_size(rows_type), out = element_size(out_type);
     const bool   eight = a.cols % 8 == 0 && starts_on(a.rows, 8 * in) && starts_on(a.drows, 8 * in) && starts_on(a.dout, 8 * out);
+    const bool   streamed = eight && static_cast<size_t>(a.slots) * a.cols * in >= device::streamed_bytes;
     by_pair(rows_type, out_type, [&](auto* in_typed, auto* out_typed) {
         using in_t  = std::remove_pointer_t<decltype(in_typed)>;
         using out_t = std::remove_pointer_t<decltype(out_typed)>;
-        follow(eight ? &device::combine_backward<in_t, out_t, 8> : &device::combine_backward<in_t, out_t, 1>,
+        follow(streamed ? &device::combine_backward<in_t, out_t, 8, true>
+               : eight  ? &device::combine_backward<in_t, out_t, 8, false>
+                        : &device::combine_backward<in_t, out_t, 1, false>,
                dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(a.slots, 4), most_groups_x))), dim3(256), stream, a);
     });
     return ROCM_WMMA_GEMM_OK;
