@@ -389,7 +389,8 @@ int loss_of_rows(const head& h, const loss_plan& plan, const operand& a, const o
             follow(&device::softmax_parts, dim3(static_cast<unsigned>(h.M), static_cast<unsigned>(plan.each)), dim3(256), stream, args);
         }
     }
-    follow(&device::join_rows, dim3(row_groups(h.M)), dim3(256), stream,
+    const bool few = h.M < 1024;
+    follow(few ? &device::join_rows<4> : &device::join_rows<1>, dim3(few ? static_cast<unsigned>(h.M) : row_groups(h.M)), dim3(256), stream,
            device::join_args{h.want, parts, of_targets, loss, lse, static_cast<int>(plan.all)});
     return ROCM_WMMA_GEMM_OK;
 }
@@ -507,10 +508,16 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     char* const   scratch = ws + product_at;
     const device::record_args f{h.want, dloss, lse, reinterpret_cast<device::loss_record*>(ws + records_at),
                                 reinterpret_cast<float*>(ws + unit_at)};
-    follow(&device::gradient_unit, dim3(1), dim3(1024), stream, f);
-    if(h.M != 0)
+    if(h.M > device::most_alone)
     {
-        follow(&device::gradient_records, dim3(row_groups(h.M)), dim3(256), stream, f);
+        follow(&device::gradient_unit, dim3(1), dim3(1024), stream, f);
+        follow(&device::gradient_records<false>, dim3(row_groups(h.M)), dim3(256), stream, f);
+    }
+    else
+    {
+        // (at most four workgroups a compute unit look for the largest)
+        const unsigned groups = static_cast<unsigned>(std::min<size_t>(row_groups(rows), 4 * cus));
+        follow(&device::gradient_records<true>, dim3(groups), dim3(256), stream, f);
     }
     int rc = ROCM_WMMA_GEMM_OK;
     for(size_t v0 = 0; v0 < std::max<size_t>(h.N, 1) && rc == ROCM_WMMA_GEMM_OK; v0 += p.cols)

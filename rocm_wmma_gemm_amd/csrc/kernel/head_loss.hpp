@@ -235,15 +235,18 @@ struct join_args
     int                 all;
 };
 
-// The loss of a row from its parts: a wave a row.
+// The loss of a row from its parts: a wave a row, or (WAVES 4) a workgroup a row, where there are few with many parts.
+template<int WAVES>
 __global__ void __launch_bounds__(256) join_rows(const join_args args)
 {
-    const int lane = threadIdx.x & 63;
-    for(long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < args.want.rows; row += (long long)gridDim.x * 4)
+    __shared__ softmax_part of_wave[4];
+    const int               lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long         step = (long long)gridDim.x * (4 / WAVES);
+    for(long long row = (long long)blockIdx.x * (4 / WAVES) + wave / WAVES; row < args.want.rows; row += step)
     {
         softmax_part all{-__builtin_inff(), 0.0f};
 #pragma unroll 4
-        for(int p = lane; p < args.all; p += 64)
+        for(int p = wave % WAVES * 64 + lane; p < args.all; p += 64 * WAVES)
         {
             all = joined(all, args.parts[row * args.all + p]);
         }
@@ -252,6 +255,18 @@ __global__ void __launch_bounds__(256) join_rows(const join_args args)
         {
             const softmax_part other{__shfl_xor(all.top, d), __shfl_xor(all.sum, d)};
             all = joined(all, other);
+        }
+        if constexpr(WAVES == 4)
+        {
+            // (a workgroup's rows are its own: every thread is in the loop as often)
+            __syncthreads();
+            of_wave[wave] = all;
+            __syncthreads();
+            all = joined(joined(of_wave[0], of_wave[1]), joined(of_wave[2], of_wave[3]));
+            if(wave != 0)
+            {
+                continue;
+            }
         }
         // (what lies between the largest logit and a listed one first: it is exact where the two are near)
         const float rest = log2f(all.sum);
@@ -300,13 +315,14 @@ struct record_args
     float*       unit; // [0]: unit, [1]: most
 };
 
-// (one workgroup: the largest of all rows)
-__global__ void __launch_bounds__(1024) gradient_unit(const record_args args)
+// The largest T |dloss| of all rows, 1 if there is none; by all threads of a workgroup.
+template<int THREADS>
+__device__ __forceinline__ float largest_gradient(const record_args& args)
 {
-    __shared__ float of_wave[16];
+    __shared__ float of_wave[THREADS / 64];
     float            most = 0.0f;
 #pragma unroll 8
-    for(int row = threadIdx.x; row < args.want.rows; row += 1024)
+    for(int row = threadIdx.x; row < args.want.rows; row += THREADS)
     {
         const float d = __builtin_fabsf(args.dloss[row] / args.want.scale);
         most          = d > most && d < __builtin_inff() ? d : most;
@@ -321,23 +337,50 @@ __global__ void __launch_bounds__(1024) gradient_unit(const record_args args)
         of_wave[threadIdx.x >> 6] = most;
     }
     __syncthreads();
+    most = of_wave[0];
+    for(int w = 1; w < THREADS / 64; ++w)
+    {
+        most = __builtin_fmaxf(most, of_wave[w]);
+    }
+    return most > 0.0f ? most : 1.0f;
+}
+
+__device__ __forceinline__ void write_unit(const record_args& args, float most)
+{
+    args.unit[0] = most * 0x1p-14f;
+    args.unit[1] = most;
+}
+
+// (one workgroup)
+__global__ void __launch_bounds__(1024) gradient_unit(const record_args args)
+{
+    const float most = largest_gradient<1024>(args);
     if(threadIdx.x == 0)
     {
-        for(int w = 1; w < 16; ++w)
-        {
-            most = __builtin_fmaxf(most, of_wave[w]);
-        }
-        most         = most > 0.0f ? most : 1.0f;
-        args.unit[0] = most * 0x1p-14f;
-        args.unit[1] = most;
+        write_unit(args, most);
     }
 }
 
-// A wave a row (a list has to be looked through for an entry).
+// A wave a row (a list has to be looked through for an entry).  ALONE: every workgroup looks for the largest gradient itself, where
+// that is less than waiting for a launch that does (4 us; 64 KB of dloss are read in less).
+constexpr int most_alone = 16384; // rows
+template<bool ALONE>
 __global__ void __launch_bounds__(256) gradient_records(const record_args args)
 {
-    const int   lane = threadIdx.x & 63;
-    const float most = args.unit[1];
+    const int lane = threadIdx.x & 63;
+    float     most;
+    if constexpr(ALONE)
+    {
+        most = largest_gradient<256>(args);
+        if(blockIdx.x == 0 && threadIdx.x == 0)
+        {
+            write_unit(args, most);
+        }
+    }
+    else
+    {
+        most = args.unit[1];
+    }
     for(long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < args.want.rows; row += (long long)gridDim.x * 4)
     {
         bool      is;
@@ -354,7 +397,9 @@ __global__ void __launch_bounds__(256) gradient_records(const record_args args)
         }
         if(lane == 0)
         {
-            args.records[row] = {args.lse[row] * log2_of_e, is ? args.dloss[row] / args.want.scale / most * 0x1p14f : 0.0f, (int)target, 0};
+            const float factor = args.dloss[row] / args.want.scale / most * 0x1p14f;
+            args.records[row]  = is ? loss_record{args.lse[row] * log2_of_e, factor, (int)target, 0}
+                                    : loss_record{__builtin_inff(), 0.0f, -1, 0};
         }
     }
 }
@@ -392,7 +437,7 @@ __global__ void __launch_bounds__(256) softmax_slope(const softmax_slope_args ar
     {
         const float p = __builtin_amdgcn_exp2f((e < 4 ? lo[e & 3] : hi[e & 3]) * args.want.scale2 - own.lse);
         const float d = own.factor * (p - (target == col + e ? 1.0f : 0.0f));
-        o[e]          = to_out<InT>(own.factor == 0.0f || col + e >= args.cols ? 0.0f : d);
+        o[e]          = to_out<InT>(col + e >= args.cols ? 0.0f : d);
     }
     *reinterpret_cast<in8*>(static_cast<InT*>(args.dz) + row * args.pitch + col) = o;
 }

@@ -55,8 +55,8 @@ struct softmax_part
 
 struct loss_record
 {
-    float lse; // log2 of the sum of 2^(alpha z)
-    float factor; // 0: the row's gradient is 0, whatever its logits are
+    float lse; // log2 of the sum of 2^(alpha z); infinity: the row has no gradient
+    float factor; // 0 then
     int   target; // a column (of the matrix that B is a block of), or -1
     int   unused; // (16 bytes)
 };

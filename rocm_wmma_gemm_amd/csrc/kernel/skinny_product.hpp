@@ -107,7 +107,7 @@ struct skinny_product
                 {
                     const float p = __builtin_amdgcn_exp2f(sum_of(piece * 8 + e) * args.alpha - own.lse);
                     const float d = own.factor * (p - (target == col + e ? 1.0f : 0.0f));
-                    o[e]          = to_out<OutT>(own.factor == 0.0f || col + e >= args.N ? 0.0f : d);
+                    o[e]          = to_out<OutT>(col + e >= args.N ? 0.0f : d);
                 }
                 *reinterpret_cast<out8*>(static_cast<OutT*>(args.C) + (long long)row * args.ldc + col) = o;
             }

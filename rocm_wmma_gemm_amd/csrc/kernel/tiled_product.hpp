@@ -574,15 +574,13 @@ struct tiled_product
                         y[e] = z[e];
                         if constexpr(SLOPE)
                         {
-                            // (the power is the hardware's, 1 ulp; below 2^-126 it gives 0)
+                            // (the power is the hardware's, 1 ulp; below 2^-126 it gives 0, as for a row without a gradient,
+                            // whose lse is infinite)
                             const u32x4        r = record[block % AHEAD][q];
                             const unsigned int lse_bits = r[0], factor_bits = r[1];
-                            const float        lse = __builtin_bit_cast(float, lse_bits);
-                            const float        factor = __builtin_bit_cast(float, factor_bits);
-                            const int          hit = (int)r[2] - (number0 + p * HALF * 16 + piece_col[q]);
-                            const float        power
-                                = __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], args.alpha, past_edge[p][q][e]) - lse);
-                            y[e] = factor == 0.0f ? 0.0f : factor * (power - (hit == e ? 1.0f : 0.0f));
+                            y[e] = __builtin_bit_cast(float, factor_bits)
+                                   * __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], args.alpha, past_edge[p][q][e])
+                                                            - __builtin_bit_cast(float, lse_bits));
                         }
                         if constexpr(EPI::logistic)
                         {
@@ -603,6 +601,21 @@ struct tiled_product
                             else
                             {
                                 y[e] += EPI::scaled ? args.beta * r : r;
+                            }
+                        }
+                    }
+                    if constexpr(SLOPE)
+                    {
+                        // (few pieces hold their row's target)
+                        const u32x4        r = record[block % AHEAD][q];
+                        const unsigned int factor_bits = r[1];
+                        const int          hit = (int)r[2] - (number0 + p * HALF * 16 + piece_col[q]);
+                        if(__any(hit >= 0 && hit < PIECE))
+                        {
+#pragma unroll
+                            for(int e = 0; e < PIECE; ++e)
+                            {
+                                y[e] -= hit == e ? __builtin_bit_cast(float, factor_bits) : 0.0f;
                             }
                         }
                     }
