@@ -59,10 +59,14 @@ using epilogue_parts    = product_epilogue<false, false, false, false, false, fa
 using epilogue_slope    = product_epilogue<false, false, false, false, false, false, diagonal_use::none, false, loss_use::slope>;
 
 // NARROW: rows of C, the residual, the second output or the bias do not start on 16 bytes: they go
-// element by element, a lane a column, so that a store instruction still writes runs of a row.
-template<in_kind IN, class OutT, class ResT, bool A_KMAJOR, bool B_KMAJOR, int BM, int BN, class EPI, bool NARROW = false>
+// element by element, a lane a column, so that a store instruction still writes runs of a row.  ANYWHERE: 16-byte pieces on
+// whatever address they start (buffer accesses need no alignment here), element by element in the last column of tiles alone,
+// where a piece may reach past its row: dB of 1999 x 32003 x 999, rows of 32003, 189 us, where elements on 128 x 128 tiles took 207.
+template<in_kind IN, class OutT, class ResT, bool A_KMAJOR, bool B_KMAJOR, int BM, int BN, class EPI, bool NARROW = false,
+         bool ANYWHERE = false>
 struct tiled_product
 {
+    static_assert(!ANYWHERE || (NARROW && !EPI::mirror && EPI::loss == loss_use::none), "whole pieces of rows that start anywhere");
     using loop = solo_gemm<IN, OutT, A_KMAJOR, B_KMAJOR, BM, BN, 64, 2, 2, 2, true>;
     using InT  = typename loop::InT;
     static constexpr int THREADS = loop::THREADS, TM = loop::TM, TN = loop::TN, BK = 64;
@@ -354,11 +358,11 @@ struct tiled_product
 
     // The wave's part of a finished tile, corner (row_w, col_w) in the workgroup's; MIRRORED: its
     // transpose, to the mirrored place (see has_mirror).
-    template<bool MIRRORED>
+    template<bool MIRRORED, bool BY_ELEMENT = NARROW>
     __device__ __forceinline__ static void write(const product_args& args, const work& w, f32x4 (&acc)[TM][TN],
                                                  int row_w, int col_w, int lane, lds_char_ptr strip)
     {
-        constexpr int PIECE = NARROW ? 1 : 16 / (int)sizeof(OutT); // columns of a piece
+        constexpr int PIECE = BY_ELEMENT ? 1 : 16 / (int)sizeof(OutT); // columns of a piece
         constexpr int PR    = HALF * 16 / PIECE; // pieces of a strip row
         constexpr int READS = (16 * PR + 63) / 64;
         constexpr bool UNEVEN = 16 * PR % 64 != 0; // the last read has lanes to spare
@@ -427,7 +431,7 @@ struct tiled_product
                     typedef unsigned int u2 __attribute__((ext_vector_type(2)));
                     constexpr int        PAIRS = PIECE / 4;
                     const unsigned int   from_at = col < cols ? (unsigned int)col * 2 : loop::STORE_RANGE;
-                    if constexpr(NARROW)
+                    if constexpr(BY_ELEMENT)
                     {
                         const unsigned short b = __builtin_amdgcn_raw_buffer_load_b16(bias_from, from_at, 0, 0);
                         bias[p][q][0]          = (float)__builtin_bit_cast(InT, b);
@@ -468,7 +472,7 @@ struct tiled_product
         }
         // residual pieces (and, by rows, what they are multiplied by) of AHEAD blocks are on their way
         constexpr int WANT = sizeof(OutT) == 4 || sizeof(ResT) == 4 || PER_CU > 1 || EPI::mirror ? 2 : 4;
-        constexpr int AHEAD = NARROW ? 1 : BLOCKS < WANT ? BLOCKS : WANT;
+        constexpr int AHEAD = BY_ELEMENT ? 1 : BLOCKS < WANT ? BLOCKS : WANT;
         piece<ResT, PIECE> residual[EPI::residual ? AHEAD : 1][PASSES][READS];
         float              by_row[EPI::diagonal == diagonal_use::rows ? AHEAD : 1][READS];
         u32x4              record[SLOPE ? AHEAD : 1][READS];
@@ -548,7 +552,7 @@ struct tiled_product
                 for(int q = 0; q < READS; ++q)
                 {
                     float z[PIECE], y[PIECE];
-                    if constexpr(NARROW)
+                    if constexpr(BY_ELEMENT)
                     {
                         const float v = *reinterpret_cast<const lds_float*>(strip + strip_at[q]);
                         z[0]          = EPI::scaled ? alpha * v : v;
@@ -962,6 +966,10 @@ struct tiled_product
                 {
                     // (read next by the kernel that adds the slices up: no streaming hint)
                     write_partial(cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
+                }
+                else if(ANYWHERE && cur.x.col0 + BN <= args.N)
+                {
+                    write<false, NARROW && !ANYWHERE>(args, cur, acc, wave_m * loop::WTM, wave_n * loop::WTN, lane, strip);
                 }
                 else
                 {

@@ -163,6 +163,8 @@ constexpr form_cost tiled_costs[] = {
     {form_tiled_192, 8.0f, 0.70f, 0.90f, 2.9e6f},
 };
 constexpr form_cost narrow_cost = {form_narrow_128, 6.0f, 0.64f, 1.0f, 2.9e6f};
+// (finish_back's, 128 x 256 with pieces that start anywhere; on 256 x 256 the two ways to end a tile spill)
+constexpr form_cost narrow_back_cost = {form_narrow_128, 7.0f, 0.64f, 0.85f, 3.5e6f};
 // The general kernel, by layout: FLOP per us where there is enough to do (it gathers operands that are contiguous
 // along M or N two bytes at a time), and us per 64 of K of a tile on its own.
 constexpr float general_flops[num_product_layouts] = {2.0e8f, 8.5e7f, 6.5e7f};
@@ -310,7 +312,7 @@ launch_choice choose(int types, int layout, int finish, const product_args& give
     }
     else
     {
-        consider_tiled(narrow_cost);
+        consider_tiled(finish == finish_back ? narrow_back_cost : narrow_cost);
     }
     // (the few-row kernel's offsets within a weight that is contiguous along N have 31 bits)
     const bool batch = args.kind == product_kind::batch;

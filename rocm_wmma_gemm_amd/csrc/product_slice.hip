@@ -31,11 +31,11 @@ product_kernel made(int block_m, int block_n, int per_cu)
     return {&device::product_entry<Impl>, block_m, block_n, Impl::THREADS, nullptr, nullptr, per_cu};
 }
 
-template<int LAYOUT, int BM, int BN, class EPI, bool NARROW = false>
+template<int LAYOUT, int BM, int BN, class EPI, bool NARROW = false, bool ANYWHERE = false>
 product_kernel tiled()
 {
     constexpr bool AK = LAYOUT != layout_mn, BK = LAYOUT == layout_kk;
-    using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, BM, BN, EPI, NARROW>;
+    using impl        = device::tiled_product<kIn, out_t, res_t, AK, BK, BM, BN, EPI, NARROW, ANYWHERE>;
     product_fn finish = nullptr;
     // (the steps' products are not cut: their scratch memory holds matrices; logits leave whole tiles)
     if constexpr(!kSteps && EPI::loss == device::loss_use::none)
@@ -109,7 +109,7 @@ product_kernel narrow(int finish)
     }
     else if constexpr(LAYOUT == layout_mn)
     {
-        return finish == finish_back ? tiled<LAYOUT, 128, 128, device::epilogue_back, true>()
+        return finish == finish_back ? tiled<LAYOUT, 128, 256, device::epilogue_back, true, true>()
                                      : tiled<LAYOUT, 128, 128, device::epilogue_add, true>();
     }
     else

@@ -45,7 +45,7 @@ enum product_form
     form_tiled_128, // persistent 128 x 128 tiles
     form_tiled_128x256,
     form_tiled_192, // symmetric products of K-contiguous operands only
-    form_narrow_128, // 128 x 128 tiles for rows of C that do not start on 16 bytes
+    form_narrow_128, // 128 x 128 tiles for rows of C that do not start on 16 bytes (128 x 256 with finish_back)
     // whole sums of few rows, rows x columns of a tile
     form_skinny_16x32,
     form_skinny_16x64, // B contiguous along N only: a k row of 64 columns is a whole cache line

@@ -162,6 +162,19 @@ def detect_arch() -> str:
     return name.split(":", 1)[0]
 
 
+_TORCH = None
+
+
+def _torch():
+    """torch, imported with the first tensor that is passed (a statement in every call costs more than this)."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+
+        _TORCH = torch
+    return _TORCH
+
+
 _SLOTS = {}
 
 
@@ -389,6 +402,8 @@ class Loader:
     @staticmethod
     def _held(name, t, need, dtype, device):
         """Address of a packed tensor on `device` that holds `need` elements of `dtype`."""
+        if t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.numel() >= need:
+            return t.data_ptr()
         if t.get_device() != device:
             raise ValueError(f"{name} must be a device tensor" if not t.is_cuda else
                              f"{name} is on device {t.get_device()}, the other operands on {device}")
@@ -396,25 +411,21 @@ class Loader:
             raise ValueError(f"{name} must be densely packed")
         if t.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-        if t.numel() < need:
-            raise ValueError(f"{name} holds {t.numel()} elements, the problem needs {need}")
-        return t.data_ptr()
+        raise ValueError(f"{name} holds {t.numel()} elements, the problem needs {need}")
 
     @staticmethod
     def _stream_on(stream, device):
         """Handle of `stream`, or of torch's current one on `device` (whose stream object takes 3 us
         to make, a third of a small call)."""
         if stream is None:
-            import torch
-
+            torch = _torch()
             raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
             return raw(device) if raw is not None else int(torch.cuda.current_stream(device).cuda_stream)
         return Loader._stream_handle(stream)
 
     @staticmethod
     def _device_of(name, t):
-        import torch
-
+        torch = _torch()
         device = t.get_device()
         if device < 0:
             raise ValueError(f"{name} must be a device tensor")
@@ -424,6 +435,11 @@ class Loader:
 
     @staticmethod
     def _sizes(*sizes):
+        all_bits = 0
+        for v in sizes:
+            all_bits |= v  # (negative if one is, past 31 bits if one is)
+        if 0 <= all_bits <= 0x7FFFFFFF:
+            return
         for v in sizes:
             if v < 0 or v > 0x7FFFFFFF:
                 raise ValueError(f"a size of {v} does not fit in 31 bits")
@@ -576,8 +592,7 @@ class Loader:
 
     @staticmethod
     def _plain_types():
-        import torch
-
+        torch = _TORCH or _torch()
         return torch.int32, torch.float32
 
     def _handle_on(self, stream, device):
@@ -594,17 +609,12 @@ class Loader:
         experts form so many groups of neighbours, of which those ``kept_groups`` (all) take part whose
         ``group_best`` (1 or 2) best biased scores sum to most.  renormalize: a token's weights are divided by their sum; then
         multiplied by ``scale``.  mask (M, bool or uint8): tokens where it is 0 go nowhere: experts -1, weights 0."""
-        import torch
-
         self._sizes(M, E, k)
         int32, f32 = self._plain_types()
         held, device = self._held, self._device_of("logits", logits)
-        if mask is not None and mask.dtype is not torch.bool:
-            mask_type = torch.uint8
-        else:
-            mask_type = torch.bool
         r = _RoutingC(_score(score), None if bias is None else held("bias", bias, E, f32, device),
-                      None if mask is None else held("mask", mask, M, mask_type, device), groups,
+                      None if mask is None else held("mask", mask, M, _torch().uint8 if mask.dtype is not _torch().bool
+                                                     else _torch().bool, device), groups,
                       groups if kept_groups is None else kept_groups, group_best, 1 if renormalize else 0, scale)
         self._done("route", self._lib.rocm_wmma_gemm_route(
             self._element("logits", logits), held("chosen", chosen, M * k, int32, device),

@@ -17,3 +17,5 @@ SHAPED(f16, _Float16, true, true, 128, 128, epilogue_slope)
 SHAPED(bf16, __bf16, true, false, 128, 256, epilogue_slope)
 SHAPED(bf16, __bf16, false, false, 256, 256, epilogue_back)
 SHAPED(f16, float, false, false, 128, 256, epilogue_back)
+template __global__ void device::tiled_product_entry<device::tiled_product<device::in_kind::f16, _Float16, _Float16, false, false, 128, 256, device::epilogue_back, true, true>>(device::product_args);
+template __global__ void device::tiled_product_entry<device::tiled_product<device::in_kind::bf16, float, float, false, false, 128, 256, device::epilogue_back, true, true>>(device::product_args);

@@ -251,6 +251,31 @@ def test_gradients_that_are_added_to_and_wanted_alone(loader, types):
         check_gradients(dA, None, a, w, layout, x, dx, q, real, dloss, 1.0)
 
 
+@pytest.mark.parametrize("types", PAIRS, ids=_id)
+@pytest.mark.parametrize("odd", [0, 1])
+def test_weight_gradients_whose_rows_start_anywhere(loader, types, odd):
+    """Rows of odd lengths, several tiles of them: every element is right, also where it is added to, and nothing around
+    the gradient is written."""
+    ab, out = types
+    for (M, N, K), layout in (((700, 1501, 301), R.row_major), ((513, 300, 1031), R.col_major), ((300, 5003, 130), R.row_major),
+                              ((400, 2305, 259), R.col_major), ((260, 513, 255), R.row_major)):
+        a, w, B = problem(M, N, K, ab, layout, 1)
+        targets, dloss = targets_of(M, N, 2), rnd((M,), F32, 5)
+        q, real = one_hot(targets, N)
+        x, dx = logits64(a, w)
+        loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+        loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K, layout)
+        for accumulate in (False, True):
+            flat = rnd((B.numel() + 2048 + odd,), out, 6)
+            kept = flat.clone()
+            dB = flat[1024 + odd:1024 + odd + B.numel()].view(B.shape)
+            loader.linear_cross_entropy_backward(None, dB, dloss, lse, a, B, targets, M, N, K, layout, accumulate=accumulate)
+            before = kept[1024 + odd:1024 + odd + B.numel()].view(B.shape) if accumulate else None
+            check_gradients(None, dB, a, w, layout, x, dx, q, real, dloss, 1.0, before)
+            assert torch.equal(flat[:1024 + odd], kept[:1024 + odd])
+            assert torch.equal(flat[1024 + odd + B.numel():], kept[1024 + odd + B.numel():])
+
+
 @pytest.mark.parametrize("which", range(4))
 def test_operands_that_start_anywhere(loader, which):
     for (M, N, K), layout in (((40, 520, 72), R.col_major), ((300, 520, 72), R.row_major), ((300, 1000, 136), R.col_major)):

@@ -112,7 +112,7 @@ def test_tiled_products_behind_a_loss_keep_accumulators_in_place(tmp_path):
     for f, body in _mfma_loops(text):
         if "tiled_product" in f and (f not in loops or len(body) < len(loops[f])):
             loops[f] = body
-    assert len(loops) == 10
+    assert len(loops) == 12
     for func, body in loops.items():
         whole = text[text.index(func + ":"):]
         whole = whole[:whole.index(".Lfunc_end")]
