@@ -241,7 +241,7 @@ struct pieces
 int check_head(const head& h, bool listed)
 {
     if((h.in != ROCM_WMMA_GEMM_ELEMENT_F16 && h.in != ROCM_WMMA_GEMM_ELEMENT_BF16) || (h.layout_b & ~1) || (h.want.wide & ~1)
-       || !(h.want.scale > 0.0f) || !std::isfinite(h.want.scale) || !std::isfinite(1.0f / h.want.scale)
+       || !(h.want.scale > 0.0f) || !std::isfinite(h.want.scale2) || !std::isfinite(1.0f / h.want.scale)
        || (listed && h.want.k < 1))
     {
         return ROCM_WMMA_GEMM_ERR_ARGUMENT;
@@ -467,7 +467,7 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     const size_t size = f32 ? 4 : 2, cus = compute_units(), rows = std::max<size_t>(h.M, 1);
     const int    types = f32 ? h.to_f32() : h.to_16();
     room         r;
-    const copies c(h, pieces(h.N, slope_bytes / (2 * rows)).count, r);
+    const copies c(h, pieces(h.N, piece_bytes / (4 * rows)).count, r); // (the smaller of the pieces there may be)
     const operand plan_a = c.plan_a(h), plan_b = c.plan_b(h);
     const bool   fused = h.N != 0 && fused_plan(h, finish_slope, plan_a, plan_b, h.N).kernel.fn != nullptr;
     const pieces p(h.N, fused ? slope_bytes / (2 * rows) : piece_bytes / (4 * rows));

@@ -152,11 +152,11 @@ __device__ __forceinline__ double one_over(double d)
     return __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
 }
 
-// 1 / (1 + e^-x); 0 where e^-x leaves fp64.
+// 1 / (1 + e^-x); 0 below 1e-304, where 1 over it leaves fp64's ordinary numbers.
 __device__ __forceinline__ double sigmoid(double x)
 {
     const double e = power_of_e(-x);
-    return x < -709.0 ? 0.0 : one_over(1.0 + e);
+    return x < -700.0 ? 0.0 : one_over(1.0 + e);
 }
 
 // A choice as one number that v_max_f64 orders: the value, whose last 9 bits tell the expert, so that of equal

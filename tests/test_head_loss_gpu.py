@@ -233,6 +233,26 @@ def test_many_pieces_of_the_vocabulary(loader, ab):
         del q, x, dx
 
 
+def test_few_rows_and_many_columns_that_start_anywhere(loader):
+    """Weights stored K x N whose rows start on odd elements, few rows, more columns than a piece of their logits has (131584):
+    every piece is a block of columns of longer rows."""
+    M, N, K = 255, 132001, 24
+    for ab in (F16, BF16):
+        a, w, B = problem(M, N, K, ab, R.row_major, 1)
+        targets, dloss = targets_of(M, N, 2), rnd((M,), F32, 5)
+        targets[0] = N - 1
+        q, real = one_hot(targets, N)
+        x, dx = logits64(a, w)
+        loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+        loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K, R.row_major)
+        check_loss(loss, lse, x, dx, q, torch.zeros_like(q), real, 1.0)
+        dA, dB = torch.empty((M, K), dtype=F32, device="cuda"), torch.empty(B.shape, dtype=ab, device="cuda")
+        loader.linear_cross_entropy_backward(dA, None, dloss, lse, a, B, targets, M, N, K, R.row_major)
+        check_gradients(dA, None, a, w, R.row_major, x, dx, q, real, dloss, 1.0)
+        loader.linear_cross_entropy_backward(None, dB, dloss, lse, a, B, targets, M, N, K, R.row_major)
+        check_gradients(None, dB, a, w, R.row_major, x, dx, q, real, dloss, 1.0)
+
+
 @pytest.mark.parametrize("types", PAIRS, ids=_id)
 def test_gradients_that_are_added_to_and_wanted_alone(loader, types):
     ab, out = types

@@ -42,7 +42,7 @@ def test_losses_refuse(library):
     assert back(0, p, p, p, p, p, None, p, 0, 4, 16, 8, 1, 0) == ARGUMENT
     assert back(0, None, None, p, p, p, p, p, 0, 4, 16, 8, 1, 0) == OK  # nothing wanted
     far = lambda *a: library.rocm_wmma_gemm_linear_distillation(*a, None)  # noqa: E731
-    for temperature in (0.0, -1.0, nan, inf, 1e-45):
+    for temperature in (0.0, -1.0, nan, inf, 1e-45, 4.2e-39):
         assert far(0, p, p, p, p, p, p, 0, p, 4, 16, 8, 2, temperature, 1) == ARGUMENT
     assert far(0, p, p, None, p, p, p, 0, p, 4, 16, 8, 2, 1.0, 1) == ARGUMENT
     assert far(0, p, p, p, p, p, p, 0, None, 4, 16, 8, 2, 1.0, 1) == ARGUMENT
