@@ -77,49 +77,36 @@ struct room
     }
 };
 
-// Copies of the operands whose rows do not start on 16 bytes, where all of a call's products read them: A always (it is
-// small next to the products), B where there are enough rows to pay for reading and writing it, and where pieces of its
-// columns would have to be copied out of longer rows.
+// Copies of the operands whose rows do not start on 16 bytes, which all of a call's products read, in one launch.  (Few rows
+// too: 35 of 5787 elements against 55790 take 1040 us on the kernel that reads any address, a copy and the product 350.)
 struct copies
 {
     bool   a, b;
     size_t a_at = 0, b_at = 0;
-    copies(const head& h, size_t pieces, room& r)
+    copies(const head& h, room& r)
         : a(h.M != 0 && h.K != 0 && (h.K % 8 != 0 || !aligned16(h.A))),
-          b(h.N != 0 && h.K != 0 && (h.b_length() % 8 != 0 || !aligned16(h.B)) && (h.M >= 256 || (h.layout_b == 0 && pieces > 1)))
+          b(h.N != 0 && h.M != 0 && h.K != 0 && (h.b_length() % 8 != 0 || !aligned16(h.B)))
     {
         a_at = a ? r.take(h.M * round_up8(h.K) * 2) : 0;
         b_at = b ? r.take(h.b_rows() * round_up8(h.b_length()) * 2) : 0;
     }
-    operand run(bool copied, const void* given, size_t rows, size_t length, char* to, hipStream_t stream) const
+    // the operands, and (ws) their copies made; before anything is launched an aligned address stands for a copy
+    void make(const head& h, operand* to_a, operand* to_b, char* ws, hipStream_t stream) const
     {
-        if(!copied)
+        auto job = [&](const void* given, size_t rows, size_t length, size_t at) {
+            return device::pack_job{given, ws + at, static_cast<int>(rows), static_cast<int>(length), static_cast<int>(rows),
+                                    static_cast<int>(round_up8(length)), 0, 0};
+        };
+        const device::pack_job ja = job(h.A, h.M, h.K, a_at), jb = job(h.B, h.b_rows(), h.b_length(), b_at);
+        if(ws != nullptr && (a || b))
         {
-            return {given, length};
+            const size_t pieces = std::max(a ? h.M * round_up8(h.K) / 8 : 0, b ? h.b_rows() * round_up8(h.b_length()) / 8 : 0);
+            follow(&device::pack_padded<unsigned short>,
+                   dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(pieces, 256), 8192)), a && b ? 2 : 1), dim3(256), stream, a ? ja : jb,
+                   b ? jb : ja);
         }
-        const size_t           padded = round_up8(length);
-        const device::pack_job job{given, to, static_cast<int>(rows), static_cast<int>(length), static_cast<int>(rows),
-                                   static_cast<int>(padded), 0, 0};
-        follow(&device::pack_padded<unsigned short>,
-               dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(rows * padded / 8, 256), 8192))), dim3(256), stream, job, job);
-        return {to, padded};
-    }
-    operand run_a(const head& h, char* ws, hipStream_t stream) const
-    {
-        return run(a, h.A, h.M, h.K, ws + a_at, stream);
-    }
-    operand run_b(const head& h, char* ws, hipStream_t stream) const
-    {
-        return run(b, h.B, h.b_rows(), h.b_length(), ws + b_at, stream);
-    }
-    // the same as run() leaves, before anything is launched (an aligned address stands for the copies)
-    operand plan_a(const head& h) const
-    {
-        return a ? operand{nullptr, round_up8(h.K)} : operand{h.A, h.K};
-    }
-    operand plan_b(const head& h) const
-    {
-        return b ? operand{nullptr, round_up8(h.b_length())} : operand{h.B, h.b_length()};
+        *to_a = a ? operand{ws != nullptr ? ws + a_at : nullptr, round_up8(h.K)} : operand{h.A, h.K};
+        *to_b = b ? operand{ws != nullptr ? ws + b_at : nullptr, round_up8(h.b_length())} : operand{h.B, h.b_length()};
     }
 };
 
@@ -178,8 +165,7 @@ step logits_of(const head& h, int finish, const operand& a, const operand& b, si
 }
 
 // How the logits' products run where they end in a tile's statistics (finish_parts) or gradients (finish_slope); no kernel
-// where they write the logits for a pass of their own: rows too long for the tiles' offsets, and few rows against weights
-// that would have to be copied first, which cost more than that pass.
+// where they write the logits for a pass of their own: rows too long for the tiles' offsets.
 launch_choice fused_plan(const head& h, int finish, const operand& a, const operand& b, size_t cols)
 {
     const launch_choice c = logits_of(h, finish, a, b, 0, cols, nullptr, round_up8(cols)).plan(compute_units());
@@ -220,6 +206,64 @@ step weights_of(const head& h, const operand& a, const void* dz, size_t dz_pitch
     s.args.alpha_at = unit;
     return s;
 }
+
+// The weights' gradient of few rows is an outer product, bound by its stores; past these a tile's sums are long enough.
+constexpr size_t most_outer = 64;
+
+void launch_outer(const head& h, int out, const operand& a, const void* dz, size_t dz_pitch, size_t cols, void* to, const float* unit,
+                  bool add, hipStream_t stream)
+{
+    const bool nk = h.layout_b == 1;
+    device::outer_args o{nk ? dz : a.at, nk ? a.at : dz, to, unit, static_cast<long long>(nk ? dz_pitch : a.ld),
+                         static_cast<long long>(nk ? a.ld : dz_pitch), static_cast<long long>(nk ? h.K : h.N),
+                         static_cast<long long>(nk ? cols : h.K), static_cast<long long>(nk ? h.K : cols), static_cast<int>(h.M), add ? 1 : 0};
+    auto run = [&](auto* in_typed, auto* out_typed) {
+        using in_t  = std::remove_pointer_t<decltype(in_typed)>;
+        using out_t = std::remove_pointer_t<decltype(out_typed)>;
+        // (a launch has 2^32 threads along x, so 2^24 blocks of rows are enough for any extent; 65535 blocks of columns are not)
+        in_parts(ceil_div(o.cols, device::outer_cols), most_groups_y, [&](int block0, unsigned blocks) {
+            device::outer_args part = o;
+            const long long    skip = static_cast<long long>(block0) * device::outer_cols;
+            part.Q                  = static_cast<const in_t*>(o.Q) + skip;
+            part.C                  = static_cast<out_t*>(o.C) + skip;
+            part.cols               = o.cols - skip;
+            follow(h.M <= 32 ? &device::outer_product<in_t, out_t, 1> : &device::outer_product<in_t, out_t, 2>,
+                   dim3(static_cast<unsigned>(ceil_div(o.rows, device::outer_rows)), blocks), dim3(256), stream, part);
+        });
+    };
+    const bool f32 = out == ROCM_WMMA_GEMM_ELEMENT_F32;
+    if(h.bf16())
+    {
+        __bf16* in = nullptr;
+        f32 ? run(in, static_cast<float*>(nullptr)) : run(in, in);
+    }
+    else
+    {
+        _Float16* in = nullptr;
+        f32 ? run(in, static_cast<float*>(nullptr)) : run(in, in);
+    }
+}
+
+// Few rows of dA are sums over the whole vocabulary on few tiles: the vocabulary goes in `count` segments of `cols` columns, as
+// a batch of products whose sums are added up as they are brought back, and a rest.
+struct segments
+{
+    size_t count = 0, cols = 0;
+    segments(const head& h, size_t all, size_t cus)
+    {
+        // (tiles of 32 columns, two workgroups a compute unit)
+        const size_t wanted = std::min<size_t>(16, 2 * cus / std::max<size_t>(1, ceil_div(h.K, 32)));
+        if(h.M <= most_outer && wanted >= 4 && all >= wanted * 1024)
+        {
+            cols  = all / wanted / piece_grain * piece_grain;
+            count = wanted;
+        }
+    }
+    size_t parts() const
+    {
+        return count + 1;
+    }
+};
 
 struct pieces
 {
@@ -408,17 +452,19 @@ int loss_of(const head& h, float* loss, float* lse, float* picked, hipStream_t s
     // rows have nothing to do with each other: as many go together as leave the statistics their room (64 columns a part)
     const size_t some = std::min(h.M, std::max<size_t>(256, parts_bytes / sizeof(device::softmax_part) / (h.N / 64 + 1)));
     room         r;
-    const copies c(h, pieces(h.N, piece_bytes / (4 * some)).count, r);
-    const loss_plan first(rows_of(h, 0, some), c.plan_a(h), c.plan_b(h), picked == nullptr, r);
+    const copies c(h, r);
+    operand      a, b;
+    c.make(h, &a, &b, nullptr, stream);
+    const loss_plan first(rows_of(h, 0, some), a, b, picked == nullptr, r);
     const size_t    rest = h.M % some;
-    const loss_plan last  = rest != 0 ? loss_plan(rows_of(h, 0, rest), c.plan_a(h), c.plan_b(h), picked == nullptr, r) : first;
+    const loss_plan last  = rest != 0 ? loss_plan(rows_of(h, 0, rest), a, b, picked == nullptr, r) : first;
     workspace_lease lease;
     char*           ws = lease.acquire(std::max(first.bytes(), last.bytes()), stream);
     if(ws == nullptr)
     {
         return ROCM_WMMA_GEMM_ERR_SCRATCH;
     }
-    const operand a = c.run_a(h, ws, stream), b = c.run_b(h, ws, stream);
+    c.make(h, &a, &b, ws, stream);
     for(size_t row = 0; row < h.M; row += some)
     {
         const size_t  rows = std::min(some, h.M - row);
@@ -467,14 +513,18 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     const size_t size = f32 ? 4 : 2, cus = compute_units(), rows = std::max<size_t>(h.M, 1);
     const int    types = f32 ? h.to_f32() : h.to_16();
     room         r;
-    const copies c(h, pieces(h.N, piece_bytes / (4 * rows)).count, r); // (the smaller of the pieces there may be)
-    const operand plan_a = c.plan_a(h), plan_b = c.plan_b(h);
+    const copies c(h, r);
+    operand      plan_a, plan_b;
+    c.make(h, &plan_a, &plan_b, nullptr, stream);
     const bool   fused = h.N != 0 && fused_plan(h, finish_slope, plan_a, plan_b, h.N).kernel.fn != nullptr;
     const pieces p(h.N, fused ? slope_bytes / (2 * rows) : piece_bytes / (4 * rows));
     const size_t pitch = p.pitch(), k_pitch = round_up8(h.K);
-    const size_t z_at = fused ? 0 : r.take(h.M * pitch * 4), dz_at = r.take(h.M * pitch * 2),
+    const bool   outer = h.M <= most_outer && h.M != 0;
+    // (segments of a single piece: few rows have no more)
+    const segments seg = p.count == 1 ? segments(h, h.N, cus) : segments(h, 0, cus);
+    const size_t z_at = fused ? 0 : r.take(h.M * pitch * 4), dz_at = r.take(h.M * pitch * 2 + (seg.count != 0 ? h.N * 2 : 0)), // (a segment's loads may reach so far past the last row)
                  records_at = r.take(h.M * sizeof(device::loss_record)), unit_at = r.take(8),
-                 sum_at = wants_a ? r.take(h.M * k_pitch * 4) : 0, product_at = r.bytes;
+                 sum_at = wants_a ? r.take(seg.parts() * h.M * k_pitch * 4) : 0, product_at = r.bytes;
     auto logits = [&](const operand& a, const operand& b, size_t v0, size_t cols, char* ws) {
         step s = logits_of(h, fused ? finish_slope : finish_plain, a, b, v0, cols, ws != nullptr ? ws + (fused ? dz_at : z_at) : nullptr, pitch);
         s.args.records = ws != nullptr ? reinterpret_cast<const device::loss_record*>(ws + records_at) : nullptr;
@@ -489,13 +539,46 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
                           static_cast<char*>(dB) + v0 * (h.layout_b == 1 ? h.K : 1) * size, h.b_length(), accumulate,
                           ws != nullptr ? reinterpret_cast<const float*>(ws + unit_at) : nullptr);
     };
+    // part 0: all segments in one launch (seg.count of them), part 1: the rest behind them; without segments part 0 is all
+    auto states_part = [&](const operand& b, size_t v0, size_t cols, size_t part, char* ws) {
+        if(seg.count == 0)
+        {
+            return states(b, v0, cols, ws);
+        }
+        if(part == 0)
+        {
+            step s          = states(b, 0, seg.cols, ws);
+            s.args.kind     = product_kind::batch;
+            s.args.groups   = static_cast<int>(seg.count);
+            s.args.stride_a = static_cast<long long>(seg.cols);
+            s.args.stride_b = static_cast<long long>(seg.cols * (h.layout_b == 1 ? b.ld : 1));
+            s.args.stride_c = static_cast<long long>(h.M * k_pitch);
+            // (a block of columns ends with the last row of the matrix, not of the block's rows)
+            s.args.b_skip = h.layout_b == 1 ? 0 : static_cast<long long>((seg.count - 1) * seg.cols);
+            return s;
+        }
+        const size_t first = seg.count * seg.cols;
+        step         s     = states(b, first, cols - first, ws);
+        if(ws != nullptr)
+        {
+            s.args.A = static_cast<const char*>(s.args.A) + first * 2;
+            s.args.C = static_cast<char*>(s.args.C) + seg.count * h.M * k_pitch * 4;
+        }
+        s.finish        = finish_plain;
+        s.args.residual = nullptr;
+        return s;
+    };
+    const size_t launches = seg.count == 0 || seg.count * seg.cols == h.N ? 1 : 2;
     size_t product = 0;
     for(size_t v0 = 0; v0 < std::max<size_t>(h.N, 1); v0 += p.cols)
     {
         const size_t cols = std::min(p.cols, h.N - v0);
         product = std::max(product, logits(plan_a, plan_b, v0, cols, nullptr).plan(cus).scratch());
-        product = std::max(product, wants_a ? states(plan_b, v0, cols, nullptr).plan(cus).scratch() : 0);
-        product = std::max(product, wants_b ? weights(plan_a, v0, cols, nullptr).plan(cus).scratch() : 0);
+        for(size_t part = 0; wants_a && part < launches; ++part)
+        {
+            product = std::max(product, states_part(plan_b, v0, cols, part, nullptr).plan(cus).scratch());
+        }
+        product = std::max(product, wants_b && !outer ? weights(plan_a, v0, cols, nullptr).plan(cus).scratch() : 0);
         v0 = v0 == p.cols && p.count > 3 ? (p.count - 2) * p.cols : v0; // (the first, one behind it, the last)
     }
     workspace_lease lease;
@@ -504,7 +587,8 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     {
         return ROCM_WMMA_GEMM_ERR_SCRATCH;
     }
-    const operand a = c.run_a(h, ws, stream), b = c.run_b(h, ws, stream);
+    operand       a, b;
+    c.make(h, &a, &b, ws, stream);
     char* const   scratch = ws + product_at;
     const device::record_args f{h.want, dloss, lse, reinterpret_cast<device::loss_record*>(ws + records_at),
                                 reinterpret_cast<float*>(ws + unit_at)};
@@ -534,21 +618,31 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
                                                static_cast<long long>(v0), static_cast<int>(cols), f.records, picked};
             h.bf16() ? launch_slope<__bf16>(s, fused, stream) : launch_slope<_Float16>(s, fused, stream);
         }
-        if(wants_a)
+        for(size_t part = 0; wants_a && rc == ROCM_WMMA_GEMM_OK && part < launches; ++part)
         {
-            rc = states(b, v0, cols, ws).run(scratch, stream);
+            rc = states_part(b, v0, cols, part, ws).run(scratch, stream);
         }
         if(wants_b && rc == ROCM_WMMA_GEMM_OK)
         {
-            rc = weights(a, v0, cols, ws).run(scratch, stream);
+            if(outer && cols != 0)
+            {
+                launch_outer(h, out, a, ws + dz_at, pitch, cols, static_cast<char*>(dB) + v0 * (h.layout_b == 1 ? h.K : 1) * size, f.unit,
+                             accumulate, stream);
+            }
+            else
+            {
+                rc = weights(a, v0, cols, ws).run(scratch, stream);
+            }
         }
     }
     if(rc == ROCM_WMMA_GEMM_OK && wants_a)
     {
+        const size_t sums = seg.count == 0 ? 1 : seg.count + launches - 1;
         by_element(out, [&](auto* typed) {
             using out_t = std::remove_pointer_t<decltype(typed)>;
             follow(&device::scaled_rows<out_t>, dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(h.M * k_pitch, 1024), 8192))), dim3(256),
-                   stream, reinterpret_cast<const float*>(ws + sum_at), static_cast<long long>(k_pitch), static_cast<out_t*>(dA),
+                   stream, reinterpret_cast<const float*>(ws + sum_at), static_cast<int>(sums), static_cast<long long>(h.M * k_pitch),
+                   static_cast<long long>(k_pitch), static_cast<out_t*>(dA),
                    static_cast<long long>(h.M), static_cast<long long>(h.K), f.unit);
         });
     }

@@ -492,11 +492,138 @@ __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args arg
     }
 }
 
-// out (rows of `cols` elements) = from (pitch apart) * unit.
+// The weights' gradient from few rows: C_ij = unit sum_t P_ti Q_tj (+ C_ij), P and Q row by row t, at most 32 DEPTH of them.
+// Bound by C's stores.  A wave holds 64 columns of Q as four operands of the 16x16x32 MFMA and walks down C's rows, 16 at a
+// time; which column an operand's row stands for is chosen so that a lane's four results of four columns are 16 columns in a
+// row.  (The tiles of the layer products spend a round of their ring on so short a sum: 2 rows of 100848 x 1288, 260 MB, 202 us.)
+struct outer_args
+{
+    const void*  P; // t x rows, p_pitch apart
+    const void*  Q; // t x cols
+    void*        C; // rows x cols, c_pitch apart
+    const float* unit;
+    long long    p_pitch, q_pitch, c_pitch;
+    long long    rows, cols;
+    int          t, add;
+};
+
+constexpr int outer_rows = 256, outer_cols = 256; // of a workgroup
+
+__device__ __forceinline__ f32x4 multiply_outer(__bf16 __attribute__((ext_vector_type(8))) a, __bf16 __attribute__((ext_vector_type(8))) b,
+                                                f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 multiply_outer(_Float16 __attribute__((ext_vector_type(8))) a,
+                                                _Float16 __attribute__((ext_vector_type(8))) b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+template<class InT, class OutT, int DEPTH>
+__global__ void __launch_bounds__(256) outer_product(const outer_args args)
+{
+    typedef InT     in8 __attribute__((ext_vector_type(8)));
+    constexpr int   PIECE = 16 / (int)sizeof(OutT); // columns of a store
+    typedef OutT    piece_t __attribute__((ext_vector_type(PIECE)));
+    typedef piece_t piece_anywhere __attribute__((aligned(sizeof(OutT))));
+    const int       lane = threadIdx.x & 63, c16 = lane & 15, g = lane >> 4;
+    const long long col0 = (long long)blockIdx.y * outer_cols + (threadIdx.x >> 6) * 64;
+    if(col0 >= args.cols)
+    {
+        return;
+    }
+    // element [t][at] of an operand, 0 outside (the address is always inside)
+    auto element = [&](const void* from, long long pitch, int t, long long at, long long end) {
+        const bool is = t < args.t && at < end;
+        const InT  v  = static_cast<const InT*>(from)[is ? t * pitch + at : 0];
+        return is ? v : (InT)0.0f;
+    };
+    in8 q[4][DEPTH];
+#pragma unroll
+    for(int f = 0; f < 4; ++f)
+    {
+#pragma unroll
+        for(int d = 0; d < DEPTH; ++d)
+        {
+#pragma unroll
+            for(int u = 0; u < 8; ++u)
+            {
+                q[f][d][u] = element(args.Q, args.q_pitch, d * 32 + g * 8 + u, col0 + (c16 >> 2) * 16 + f * 4 + (c16 & 3), args.cols);
+            }
+        }
+    }
+    const float     unit = *args.unit;
+    const long long end  = (long long)(blockIdx.x + 1) * outer_rows < args.rows ? (long long)(blockIdx.x + 1) * outer_rows : args.rows;
+    const long long col  = col0 + g * 16; // this lane's 16
+    for(long long row0 = (long long)blockIdx.x * outer_rows; row0 < end; row0 += 16)
+    {
+        in8 p[DEPTH];
+#pragma unroll
+        for(int d = 0; d < DEPTH; ++d)
+        {
+#pragma unroll
+            for(int u = 0; u < 8; ++u)
+            {
+                p[d][u] = element(args.P, args.p_pitch, d * 32 + g * 8 + u, row0 + c16, end);
+            }
+        }
+        float y[16];
+#pragma unroll
+        for(int f = 0; f < 4; ++f)
+        {
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for(int d = 0; d < DEPTH; ++d)
+            {
+                sum = multiply_outer(q[f][d], p[d], sum);
+            }
+#pragma unroll
+            for(int e = 0; e < 4; ++e)
+            {
+                y[4 * f + e] = unit * sum[e];
+            }
+        }
+        if(row0 + c16 >= end)
+        {
+            continue;
+        }
+        OutT* const to = static_cast<OutT*>(args.C) + (row0 + c16) * args.c_pitch + col;
+#pragma unroll
+        for(int s = 0; s < 16; s += PIECE)
+        {
+            if(col + s + PIECE <= args.cols)
+            {
+                piece_t o{};
+                if(args.add)
+                {
+                    o = *reinterpret_cast<const piece_anywhere*>(to + s);
+                }
+#pragma unroll
+                for(int e = 0; e < PIECE; ++e)
+                {
+                    o[e] = to_out<OutT>(args.add ? y[s + e] + (float)o[e] : y[s + e]);
+                }
+                *reinterpret_cast<piece_anywhere*>(to + s) = o;
+                continue;
+            }
+#pragma unroll
+            for(int e = 0; e < PIECE; ++e)
+            {
+                if(col + s + e < args.cols)
+                {
+                    to[s + e] = to_out<OutT>(args.add ? y[s + e] + (float)to[s + e] : y[s + e]);
+                }
+            }
+        }
+    }
+}
+
+// out (rows of `cols` elements) = the sum of `parts` (part_size apart, rows pitch apart), in their order, times unit.
 template<class OutT>
 __global__ void __launch_bounds__(256)
-    scaled_rows(const float* __restrict__ from, long long pitch, OutT* __restrict__ out, long long rows, long long cols,
-                const float* __restrict__ unit)
+    scaled_rows(const float* __restrict__ from, int parts, long long part_size, long long pitch, OutT* __restrict__ out, long long rows,
+                long long cols, const float* __restrict__ unit)
 {
     const float     by     = *unit;
     const long long pieces = (cols + 3) / 4, total = rows * pieces; // (from's rows are padded to whole pieces)
@@ -505,16 +632,21 @@ __global__ void __launch_bounds__(256)
     for(long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long long)gridDim.x * 256)
     {
         const long long row = at / pieces, col = (at - row * pieces) * 4;
-        const f32x4     v   = *reinterpret_cast<const f32x4*>(from + row * pitch + col);
-        OutT* const     to  = out + row * cols + col;
+        f32x4           v   = *reinterpret_cast<const f32x4*>(from + row * pitch + col);
+#pragma unroll 4
+        for(int part = 1; part < parts; ++part)
+        {
+            v += *reinterpret_cast<const f32x4*>(from + part * part_size + row * pitch + col);
+        }
+        OutT* const to = out + row * cols + col;
+        out4        o;
+#pragma unroll
+        for(int e = 0; e < 4; ++e)
+        {
+            o[e] = to_out<OutT>(v[e] * by);
+        }
         if(whole)
         {
-            out4 o;
-#pragma unroll
-            for(int e = 0; e < 4; ++e)
-            {
-                o[e] = to_out<OutT>(v[e] * by);
-            }
             *reinterpret_cast<out4*>(to) = o;
             continue;
         }
@@ -523,7 +655,7 @@ __global__ void __launch_bounds__(256)
         {
             if(col + e < cols)
             {
-                to[e] = to_out<OutT>(v[e] * by);
+                to[e] = o[e];
             }
         }
     }

@@ -233,9 +233,34 @@ def test_many_pieces_of_the_vocabulary(loader, ab):
         del q, x, dx
 
 
+@pytest.mark.parametrize("types", PAIRS, ids=_id)
+@pytest.mark.parametrize("size", [(1, 16384, 64), (3, 20000, 72), (33, 17001, 136), (64, 40000, 40), (40, 4099, 1030), (65, 20000, 72),
+                                  (2, 70000, 9)], ids=_id)
+def test_gradients_of_few_rows(loader, size, types):
+    """Outer products, and sums over a vocabulary that goes in segments, a whole number of them or not."""
+    M, N, K = size
+    ab, out = types
+    for layout in (R.col_major, R.row_major):
+        a, w, B = problem(M, N, K, ab, layout, 1)
+        targets, dloss = targets_of(M, N, 2), rnd((M,), F32, 5)
+        targets[-1] = N - 1
+        q, real = one_hot(targets, N)
+        x, dx = logits64(a, w)
+        loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+        loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K, layout)
+        check_loss(loss, lse, x, dx, q, torch.zeros_like(q), real, 1.0)
+        for accumulate in (False, True):
+            flat = rnd((B.numel() + 64,), out, 6)
+            kept = flat.clone()
+            dA, dB = torch.full((M, K), math.nan, dtype=out, device="cuda"), flat[32:32 + B.numel()].view(B.shape)
+            loader.linear_cross_entropy_backward(dA, dB, dloss, lse, a, B, targets, M, N, K, layout, accumulate=accumulate)
+            before = kept[32:32 + B.numel()].view(B.shape) if accumulate else None
+            check_gradients(dA, dB, a, w, layout, x, dx, q, real, dloss, 1.0, before)
+            assert torch.equal(flat[:32], kept[:32]) and torch.equal(flat[32 + B.numel():], kept[32 + B.numel():])
+
+
 def test_few_rows_and_many_columns_that_start_anywhere(loader):
-    """Weights stored K x N whose rows start on odd elements, few rows, more columns than a piece of their logits has (131584):
-    every piece is a block of columns of longer rows."""
+    """Weights stored K x N whose rows start on odd elements, few rows, many columns."""
     M, N, K = 255, 132001, 24
     for ab in (F16, BF16):
         a, w, B = problem(M, N, K, ab, R.row_major, 1)
