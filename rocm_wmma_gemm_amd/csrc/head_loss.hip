@@ -216,7 +216,12 @@ void launch_outer(const head& h, int out, const operand& a, const void* dz, size
     const bool nk = h.layout_b == 1;
     device::outer_args o{nk ? dz : a.at, nk ? a.at : dz, to, unit, static_cast<long long>(nk ? dz_pitch : a.ld),
                          static_cast<long long>(nk ? a.ld : dz_pitch), static_cast<long long>(nk ? h.K : h.N),
-                         static_cast<long long>(nk ? cols : h.K), static_cast<long long>(nk ? h.K : cols), static_cast<int>(h.M), add ? 1 : 0};
+                         static_cast<long long>(nk ? cols : h.K), static_cast<long long>(nk ? h.K : cols), static_cast<int>(h.M), add ? 1 : 0, device::outer_rows};
+    // (fewer rows a workgroup where there would be less than two for every compute unit: 1788 x 740 16.8 us with 256)
+    while(o.each > 16 && ceil_div(o.rows, o.each) * ceil_div(o.cols, device::outer_cols) < 2 * compute_units())
+    {
+        o.each /= 2;
+    }
     auto run = [&](auto* in_typed, auto* out_typed) {
         using in_t  = std::remove_pointer_t<decltype(in_typed)>;
         using out_t = std::remove_pointer_t<decltype(out_typed)>;
@@ -228,7 +233,7 @@ void launch_outer(const head& h, int out, const operand& a, const void* dz, size
             part.C                  = static_cast<out_t*>(o.C) + skip;
             part.cols               = o.cols - skip;
             follow(h.M <= 32 ? &device::outer_product<in_t, out_t, 1> : &device::outer_product<in_t, out_t, 2>,
-                   dim3(static_cast<unsigned>(ceil_div(o.rows, device::outer_rows)), blocks), dim3(256), stream, part);
+                   dim3(static_cast<unsigned>(ceil_div(o.rows, o.each)), blocks), dim3(256), stream, part);
         });
     };
     const bool f32 = out == ROCM_WMMA_GEMM_ELEMENT_F32;

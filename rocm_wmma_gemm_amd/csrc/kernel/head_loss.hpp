@@ -505,9 +505,10 @@ struct outer_args
     long long    p_pitch, q_pitch, c_pitch;
     long long    rows, cols;
     int          t, add;
+    int          each; // rows of a workgroup, a multiple of 16
 };
 
-constexpr int outer_rows = 256, outer_cols = 256; // of a workgroup
+constexpr int outer_rows = 256, outer_cols = 256; // of a workgroup, at most
 
 __device__ __forceinline__ f32x4 multiply_outer(__bf16 __attribute__((ext_vector_type(8))) a, __bf16 __attribute__((ext_vector_type(8))) b,
                                                 f32x4 c)
@@ -554,9 +555,9 @@ __global__ void __launch_bounds__(256) outer_product(const outer_args args)
         }
     }
     const float     unit = *args.unit;
-    const long long end  = (long long)(blockIdx.x + 1) * outer_rows < args.rows ? (long long)(blockIdx.x + 1) * outer_rows : args.rows;
+    const long long row1 = (long long)(blockIdx.x + 1) * args.each, end = row1 < args.rows ? row1 : args.rows;
     const long long col  = col0 + g * 16; // this lane's 16
-    for(long long row0 = (long long)blockIdx.x * outer_rows; row0 < end; row0 += 16)
+    for(long long row0 = (long long)blockIdx.x * args.each; row0 < end; row0 += 16)
     {
         in8 p[DEPTH];
 #pragma unroll

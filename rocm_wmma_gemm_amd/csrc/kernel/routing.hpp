@@ -609,13 +609,32 @@ __device__ __forceinline__ void put(Piece* to, const Piece& v)
 {
     if constexpr(STREAMED)
     {
-        __builtin_nontemporal_store(v, to);
+        __builtin_nontemporal_store(v.v, &to->v);
     }
     else
     {
-        *to = v;
+        to->v = v.v;
     }
 }
+
+// 16 bytes, 2, or 8 elements, that may start on any element: accesses of vectors need no alignment here.  (Structures: the
+// alignment of a plain vector type gets lost where templates take it.)
+struct piece16
+{
+    typedef u32x4 vector __attribute__((aligned(2)));
+    vector        v;
+};
+struct piece2
+{
+    unsigned short v;
+};
+template<class T>
+struct eight
+{
+    typedef T vector __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    vector    v;
+};
+static_assert(alignof(piece16) == 2 && sizeof(piece16) == 16 && alignof(eight<float>) == 4 && sizeof(eight<_Float16>) == 16, "anywhere");
 
 struct sort_tables
 {
@@ -738,13 +757,15 @@ struct dispatch_args
     int         copy; // 0: rows are not wanted
 };
 
-// A piece of a token's row to the places of its choices (place: of choice `lane`).
+// A run of pieces of a token's row to the places of its choices (place: of choice `lane`).  The last piece ends with the row: it
+// may overlap the one before, whose bytes are the same.
 template<class Piece, bool STREAMED>
 __device__ __forceinline__ void copy_row(const dispatch_args& args, long long token, int place, long long at, long long end)
 {
-    const long long    pieces = args.row_bytes / (long long)sizeof(Piece);
-    const Piece* const from   = static_cast<const Piece*>(args.x) + token * pieces;
-    Piece* const       to     = static_cast<Piece*>(args.rows);
+    const char* const from = static_cast<const char*>(args.x) + token * args.row_bytes;
+    char* const       to   = static_cast<char*>(args.rows);
+    const long long   last = args.row_bytes - (long long)sizeof(Piece);
+    auto start = [&](long long piece) { return piece * (long long)sizeof(Piece) < last ? piece * (long long)sizeof(Piece) : last; };
     // (four pieces of a lane on their way at a time)
     for(; at < end; at += 256)
     {
@@ -752,24 +773,31 @@ __device__ __forceinline__ void copy_row(const dispatch_args& args, long long to
 #pragma unroll
         for(int u = 0; u < 4; ++u)
         {
-            v[u] = at + 64 * u < end ? from[at + 64 * u] : Piece{};
+            v[u].v = at + 64 * u < end ? reinterpret_cast<const Piece*>(from + start(at + 64 * u))->v : decltype(v[u].v){};
         }
         for(int j = 0; j < args.k; ++j)
         {
             const int p = __builtin_amdgcn_readlane(place, j);
             if(p >= 0)
             {
+                char* const row = to + p * args.row_bytes;
 #pragma unroll
                 for(int u = 0; u < 4; ++u)
                 {
                     if(at + 64 * u < end)
                     {
-                        put<STREAMED>(to + p * pieces + at + 64 * u, v[u]);
+                        put<STREAMED>(reinterpret_cast<Piece*>(row + start(at + 64 * u)), v[u]);
                     }
                 }
             }
         }
     }
+}
+
+template<class Piece>
+__device__ __forceinline__ long long pieces_of_row(const dispatch_args& args)
+{
+    return (args.row_bytes + (long long)sizeof(Piece) - 1) / (long long)sizeof(Piece);
 }
 
 // All of it in one launch, for up to ROUNDS * 1024 choices: every workgroup sorts all of them for itself and copies its share
@@ -805,7 +833,7 @@ __global__ void __launch_bounds__(1024) dispatch_few(const dispatch_args args)
         return;
     }
     __syncthreads();
-    const long long pieces = args.row_bytes / (long long)sizeof(Piece), runs = (pieces + 63) / 64, all = args.tokens * runs;
+    const long long pieces = pieces_of_row<Piece>(args), runs = (pieces + 63) / 64, all = args.tokens * runs;
     // (neighbouring runs on different compute units)
     for(long long run = blockIdx.x + (long long)gridDim.x * wave; run < all; run += (long long)gridDim.x * sort_waves)
     {
@@ -939,7 +967,7 @@ __global__ void __launch_bounds__(256) dispatch_rows(const dispatch_args args, i
         }
         if(args.copy)
         {
-            copy_row<Piece, STREAMED>(args, token, place, lane, args.row_bytes / (long long)sizeof(Piece));
+            copy_row<Piece, STREAMED>(args, token, place, lane, pieces_of_row<Piece>(args));
         }
     }
 }
@@ -961,71 +989,85 @@ struct combine_args
     const void*  dout;
 };
 
-template<class T, int WIDTH>
-using vec_of = T __attribute__((ext_vector_type(WIDTH)));
-
-// out = sum over the choices of weight * row (+ residual), in fp32 in the order of the choices, rounded once.  WIDTH
-// elements a thread; blockIdx.x: the token, blockIdx.y: 256 pieces of its row.
-template<class InT, class OutT, int WIDTH>
+// out = sum over the choices of weight * row (+ residual), in fp32 in the order of the choices, rounded once.  Eight columns a
+// thread, the last ones of a row one by one; blockIdx.x: the token, blockIdx.y: 256 pieces of its row.
+template<class InT, class OutT>
 __global__ void __launch_bounds__(256) combine(const combine_args args, int block0)
 {
+    const long long col = ((long long)(block0 + blockIdx.y) * 256 + threadIdx.x) * 8;
+    if(col >= args.cols)
+    {
+        return;
+    }
+    const bool whole = col + 8 <= args.cols;
+    const int  count = whole ? 8 : (int)(args.cols - col);
     for(long long token = blockIdx.x; token < args.tokens; token += gridDim.x)
     {
-        const long long col = ((long long)(block0 + blockIdx.y) * 256 + threadIdx.x) * WIDTH;
-        if(col >= args.cols)
-        {
-            return;
-        }
-        float sum[WIDTH];
-#pragma unroll
-        for(int v = 0; v < WIDTH; ++v)
-        {
-            sum[v] = 0.0f;
-        }
+        float sum[8] = {};
         const int*   places  = args.places + token * args.k;
         const float* weights = args.weights != nullptr ? args.weights + token * args.k : nullptr;
-#pragma unroll 8
-        for(int j = 0; j < args.k; ++j)
+        const InT*   rows    = static_cast<const InT*>(args.rows) + col;
+        const long long at   = token * args.cols + col;
+        OutT* const  out     = static_cast<OutT*>(args.out) + at;
+        const OutT*  added   = args.residual != nullptr ? static_cast<const OutT*>(args.residual) + at : nullptr;
+        if(whole)
         {
-            const int p = places[j];
-            if(p >= 0 && p < args.slots)
+#pragma unroll 8
+            for(int j = 0; j < args.k; ++j)
             {
-                const float            w = weights != nullptr ? weights[j] : 1.0f;
-                const vec_of<InT, WIDTH> y
-                    = *reinterpret_cast<const vec_of<InT, WIDTH>*>(static_cast<const InT*>(args.rows) + p * args.cols + col);
-#pragma unroll
-                for(int v = 0; v < WIDTH; ++v)
+                const int p = places[j];
+                if(p >= 0 && p < args.slots)
                 {
-                    sum[v] += w * (float)y[v];
+                    const float      w = weights != nullptr ? weights[j] : 1.0f;
+                    const eight<InT> y{reinterpret_cast<const eight<InT>*>(rows + p * args.cols)->v};
+#pragma unroll
+                    for(int v = 0; v < 8; ++v)
+                    {
+                        sum[v] += w * (float)y.v[v];
+                    }
                 }
             }
-        }
-        const long long at = token * args.cols + col;
-        if(args.residual != nullptr)
-        {
-            const vec_of<OutT, WIDTH> r = *reinterpret_cast<const vec_of<OutT, WIDTH>*>(static_cast<const OutT*>(args.residual) + at);
-#pragma unroll
-            for(int v = 0; v < WIDTH; ++v)
+            if(added != nullptr)
             {
-                sum[v] += (float)r[v];
-            }
-        }
-        vec_of<OutT, WIDTH> o;
+                const eight<OutT> r{reinterpret_cast<const eight<OutT>*>(added)->v};
 #pragma unroll
-        for(int v = 0; v < WIDTH; ++v)
-        {
-            o[v] = to_out<OutT>(sum[v]);
+                for(int v = 0; v < 8; ++v)
+                {
+                    sum[v] += (float)r.v[v];
+                }
+            }
+            eight<OutT> o;
+#pragma unroll
+            for(int v = 0; v < 8; ++v)
+            {
+                o.v[v] = to_out<OutT>(sum[v]);
+            }
+            reinterpret_cast<eight<OutT>*>(out)->v = o.v;
+            continue;
         }
-        *reinterpret_cast<vec_of<OutT, WIDTH>*>(static_cast<OutT*>(args.out) + at) = o;
+        for(int v = 0; v < count; ++v)
+        {
+            float s = 0.0f;
+            for(int j = 0; j < args.k; ++j)
+            {
+                const int p = places[j];
+                if(p >= 0 && p < args.slots)
+                {
+                    s += (weights != nullptr ? weights[j] : 1.0f) * (float)rows[p * args.cols + v];
+                }
+            }
+            out[v] = to_out<OutT>(added != nullptr ? s + (float)added[v] : s);
+        }
     }
 }
 
 // The gradients: of a row, weight * dout; of a weight, the product of dout with its row.  A wave a choice: the k waves
 // of a token share dout in the caches.
-template<class InT, class OutT, int WIDTH, bool STREAMED>
+template<class InT, class OutT, bool STREAMED>
 __global__ void __launch_bounds__(256) combine_backward(const combine_args args)
 {
-    const int lane = threadIdx.x & 63;
+    const int       lane  = threadIdx.x & 63;
+    const long long whole = args.cols / 8 * 8, own = whole + lane; // this lane's column of the last ones
     for(long long slot = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); slot < args.slots; slot += (long long)gridDim.x * 4)
     {
         const int  p  = args.places[slot];
@@ -1033,32 +1075,41 @@ __global__ void __launch_bounds__(256) combine_backward(const combine_args args)
         float      dot = 0.0f;
         if(is)
         {
-            const float       w    = args.weights != nullptr ? args.weights[slot] : 1.0f;
-            const OutT* const d0   = static_cast<const OutT*>(args.dout) + slot / args.k * args.cols;
-            const InT* const  y0   = static_cast<const InT*>(args.rows) + p * args.cols;
-            InT* const        to   = static_cast<InT*>(args.drows) + p * args.cols;
+            const float       w  = args.weights != nullptr ? args.weights[slot] : 1.0f;
+            const OutT* const d0 = static_cast<const OutT*>(args.dout) + slot / args.k * args.cols;
+            const InT* const  y0 = static_cast<const InT*>(args.rows) + p * args.cols;
+            InT* const        to = static_cast<InT*>(args.drows) + p * args.cols;
 #pragma unroll 4
-            for(long long col = lane * WIDTH; col < args.cols; col += 64 * WIDTH)
+            for(long long col = lane * 8; col < whole; col += 512)
             {
-                const vec_of<OutT, WIDTH> d = *reinterpret_cast<const vec_of<OutT, WIDTH>*>(d0 + col);
+                const eight<OutT> d{reinterpret_cast<const eight<OutT>*>(d0 + col)->v};
                 if(args.dweights != nullptr)
                 {
-                    const vec_of<InT, WIDTH> y = *reinterpret_cast<const vec_of<InT, WIDTH>*>(y0 + col);
+                    const eight<InT> y{reinterpret_cast<const eight<InT>*>(y0 + col)->v};
 #pragma unroll
-                    for(int v = 0; v < WIDTH; ++v)
+                    for(int v = 0; v < 8; ++v)
                     {
-                        dot += (float)d[v] * (float)y[v];
+                        dot += (float)d.v[v] * (float)y.v[v];
                     }
                 }
                 if(args.drows != nullptr)
                 {
-                    vec_of<InT, WIDTH> o;
+                    eight<InT> o;
 #pragma unroll
-                    for(int v = 0; v < WIDTH; ++v)
+                    for(int v = 0; v < 8; ++v)
                     {
-                        o[v] = to_out<InT>(w * (float)d[v]);
+                        o.v[v] = to_out<InT>(w * (float)d.v[v]);
                     }
-                    put<STREAMED>(reinterpret_cast<vec_of<InT, WIDTH>*>(to + col), o);
+                    put<STREAMED>(reinterpret_cast<eight<InT>*>(to + col), o);
+                }
+            }
+            if(own < args.cols)
+            {
+                const float d = (float)d0[own];
+                dot += args.dweights != nullptr ? d * (float)y0[own] : 0.0f;
+                if(args.drows != nullptr)
+                {
+                    to[own] = to_out<InT>(w * d);
                 }
             }
         }

@@ -160,17 +160,11 @@ int route_backward(int type, void* dlogits, const float* dweights, const int* ch
     return ROCM_WMMA_GEMM_OK;
 }
 
-// Calls f with a null pointer of a piece of a row.
+// Calls f with a null pointer of a piece of a row: 16 bytes on any element, or an element of a shorter row.
 template<class F>
 void by_piece(size_t bytes, F&& f)
 {
-    switch(bytes)
-    {
-        case 16: f(static_cast<device::u32x4*>(nullptr)); break;
-        case 8: f(static_cast<unsigned long long*>(nullptr)); break;
-        case 4: f(static_cast<unsigned int*>(nullptr)); break;
-        default: f(static_cast<unsigned short*>(nullptr)); break;
-    }
+    bytes == 16 ? f(static_cast<device::piece16*>(nullptr)) : f(static_cast<device::piece2*>(nullptr));
 }
 
 // Counts that every workgroup adds up for itself rather than wait for a launch that does (8191 tokens of 6 choices
@@ -198,15 +192,11 @@ int dispatch(int type, void* rows, int* offsets, int* places, const void* x, con
                             static_cast<long long>(N * element_size(type)), static_cast<int>(E), static_cast<int>(k), 1, copy};
     const size_t blocks = std::max<size_t>(1, ceil_div(slots, device::sort_block));
     a.blocks            = static_cast<int>(blocks);
-    size_t piece        = 16;
-    while(piece > 2 && (a.row_bytes % piece != 0 || !starts_on(x, piece) || !starts_on(rows, piece)))
-    {
-        piece /= 2;
-    }
+    const size_t piece  = a.row_bytes >= 16 ? 16 : 2;
     if(blocks == 1)
     {
         // (a run of 64 pieces a wave, spread over the compute units)
-        const size_t runs = M * ceil_div(a.row_bytes / piece, 64);
+        const size_t runs = M * ceil_div(ceil_div(a.row_bytes, piece), 64);
         const dim3   grid(static_cast<unsigned>(copy ? std::min<size_t>(std::max<size_t>(1, ceil_div(runs, 4)), compute_units()) : 1));
         by_piece(piece, [&](auto* typed) {
             using piece_t = std::remove_pointer_t<decltype(typed)>;
@@ -261,15 +251,12 @@ int check_rows(size_t M, size_t N, size_t k)
 
 int combine(int rows_type, int out_type, const device::combine_args& a, hipStream_t stream)
 {
-    // (elements of a piece: 16 bytes of a 16-bit type, or one)
-    const size_t in = element_size(rows_type), out = element_size(out_type);
-    const bool   eight = a.cols % 8 == 0 && starts_on(a.rows, 8 * in) && starts_on(a.out, 8 * out) && starts_on(a.residual, 8 * out);
     by_pair(rows_type, out_type, [&](auto* in_typed, auto* out_typed) {
         using in_t  = std::remove_pointer_t<decltype(in_typed)>;
         using out_t = std::remove_pointer_t<decltype(out_typed)>;
-        in_parts(ceil_div(a.cols, eight ? 2048 : 256), most_groups_y, [&](int block0, unsigned blocks) {
-            follow(eight ? &device::combine<in_t, out_t, 8> : &device::combine<in_t, out_t, 1>,
-                   dim3(static_cast<unsigned>(std::min<long long>(a.tokens, most_groups_x)), blocks), dim3(256), stream, a, block0);
+        in_parts(ceil_div(a.cols, 2048), most_groups_y, [&](int block0, unsigned blocks) {
+            follow(&device::combine<in_t, out_t>, dim3(static_cast<unsigned>(std::min<long long>(a.tokens, most_groups_x)), blocks), dim3(256),
+                   stream, a, block0);
         });
     });
     return ROCM_WMMA_GEMM_OK;
@@ -277,15 +264,11 @@ int combine(int rows_type, int out_type, const device::combine_args& a, hipStrea
 
 int combine_backward(int rows_type, int out_type, const device::combine_args& a, hipStream_t stream)
 {
-    const size_t in = element_size(rows_type), out = element_size(out_type);
-    const bool   eight = a.cols % 8 == 0 && starts_on(a.rows, 8 * in) && starts_on(a.drows, 8 * in) && starts_on(a.dout, 8 * out);
-    const bool   streamed = eight && static_cast<size_t>(a.slots) * a.cols * in >= device::streamed_bytes;
+    const bool streamed = static_cast<size_t>(a.slots) * a.cols * element_size(rows_type) >= device::streamed_bytes;
     by_pair(rows_type, out_type, [&](auto* in_typed, auto* out_typed) {
         using in_t  = std::remove_pointer_t<decltype(in_typed)>;
         using out_t = std::remove_pointer_t<decltype(out_typed)>;
-        follow(streamed ? &device::combine_backward<in_t, out_t, 8, true>
-               : eight  ? &device::combine_backward<in_t, out_t, 8, false>
-                        : &device::combine_backward<in_t, out_t, 1, false>,
+        follow(streamed ? &device::combine_backward<in_t, out_t, true> : &device::combine_backward<in_t, out_t, false>,
                dim3(static_cast<unsigned>(std::min<size_t>(ceil_div(a.slots, 4), most_groups_x))), dim3(256), stream, a);
     });
     return ROCM_WMMA_GEMM_OK;
