@@ -505,3 +505,103 @@ def test_losses_refuse(loader):
     for temperature in (0.0, -1.0, math.inf, math.nan):
         with pytest.raises(R.GemmLibraryError):
             loader.linear_distillation(loss, lse, loss, a, B, entries, teacher, M, N, K, temperature=temperature)
+
+
+def slopes64(x, dx, lse, d_lse, q, real, dloss, dtype):
+    """The gradient of some columns of logits and its bound, as in check_gradients, from the lse of whole rows (up to 2^20
+    columns) and the largest of their logits' bounds."""
+    p = torch.exp(x - lse[:, None])
+    g = (dloss.double() * real.double())[:, None]
+    dz = g * (p - q)
+    rel = dx + d_lse[:, None] + (80 + 1024 + 8 * (x.abs() + lse.abs()[:, None])) * E32
+    err = g.abs() * (p * rel + (p + q) * 40 * E32) * 1.01
+    err = err + UNIT[dtype] * (dz.abs() + err)
+    return dz, torch.where(real[:, None], err, torch.zeros_like(err))
+
+
+@pytest.mark.parametrize("size", [(9, 540001, R.col_major), (300, 540000, R.col_major), (9, 540000, R.row_major),
+                                  (300, 540001, R.row_major)], ids=_id)
+def test_weights_past_32_bits(loader, size):
+    """More than 2^31 weights, 4.4 GB, on few rows and on tiles; their gradient at the ends and on both sides of 2^31 elements."""
+    (M, N, layout), K, ab = size, 4096, BF16
+    assert N * K > 1 << 31
+    a = rnd((M, K), ab, 1)
+    B = torch.empty((N, K) if layout == R.col_major else (K, N), dtype=ab, device="cuda")
+    w = B if layout == R.col_major else B.t()
+    x, dx = (torch.empty((M, N), dtype=torch.float64, device="cuda") for _ in range(2))
+    for v0 in range(0, N, 65536):
+        w[v0:v0 + 65536] = rnd((min(65536, N - v0), K), ab, v0 + 2, 2.0 / math.sqrt(K))
+        x[:, v0:v0 + 65536], dx[:, v0:v0 + 65536] = logits64(a, w[v0:v0 + 65536])
+    targets = targets_of(M, N, 2)
+    targets[1], targets[2] = N - 1, (1 << 31) // K
+    q, real = one_hot(targets, N)
+    loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K, layout)
+    check_loss(loss, lse, x, dx, q, torch.zeros_like(q), real, 1.0)
+    dloss = rnd((M,), F32, 5)
+    dA, dB = torch.full((M, K), math.nan, dtype=ab, device="cuda"), torch.full(B.shape, math.nan, dtype=ab, device="cuda")
+    loader.linear_cross_entropy_backward(dA, dB, dloss, lse, a, B, targets, M, N, K, layout)
+    lse64, A = torch.logsumexp(x, 1), a.double()
+    want, size64, tol = (torch.zeros((M, K), dtype=torch.float64, device="cuda") for _ in range(3))
+    got_b = dB if layout == R.col_major else dB.t()
+    for v0 in range(0, N, 65536):
+        at = slice(v0, min(v0 + 65536, N))
+        dz, err = slopes64(x[:, at], dx[:, at], lse64, dx.max(1)[0], q[:, at], real, dloss, ab)
+        W = w[at].double()
+        want += dz @ W
+        tol += err @ W.abs()
+        size64 += (dz.abs() + err) @ W.abs()
+        want_b = dz.t() @ A
+        tol_b = err.t() @ A.abs() + (M + 16) * SUM * ((dz.abs() + err).t() @ A.abs())
+        within(got_b[at], want_b, tol_b + UNIT[ab] * (want_b.abs() + tol_b) + LEAST[ab], f"dB from {v0} on")
+    tol += (N + 16) * SUM * size64
+    within(dA, want, tol + UNIT[ab] * (want.abs() + tol) + LEAST[ab], "dA")
+
+
+def test_logits_past_32_bits(loader):
+    """More than 2^32 logits: rows that go together for their statistics, and pieces of their gradient."""
+    M, N, K, ab = 70001, 66000, 64, F16
+    assert M * N > 1 << 32
+    a, w, B = problem(M, N, K, ab, R.col_major, 1)
+    targets = targets_of(M, N, 2)
+    targets[-1] = N - 1
+    dloss = torch.where(rnd((M,), F32, 5) > 0, 1.0, -0.5)  # (of one size, so that f16's least number counts for nothing)
+    loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K)
+    dA, dB = torch.full((M, K), math.nan, device="cuda"), torch.full((N, K), math.nan, device="cuda")
+    loader.linear_cross_entropy_backward(dA, dB, dloss, lse, a, B, targets, M, N, K)
+    want_b, tol_b, size_b = (torch.zeros((N, K), dtype=torch.float64, device="cuda") for _ in range(3))
+    W = w.double()
+    for row in range(0, M, 4096):
+        at = slice(row, min(row + 4096, M))
+        x, dx = logits64(a[at], w)
+        q, real = one_hot(targets[at], N)
+        check_loss(loss[at], lse[at], x, dx, q, torch.zeros_like(q), real, 1.0)
+        dz, err = slopes64(x, dx, torch.logsumexp(x, 1), dx.max(1)[0], q, real, dloss[at], ab)
+        err = err + 2.0 ** -38 * real[:, None]
+        want, A = dz @ W, a[at].double()
+        tol = err @ W.abs() + (N + 16) * SUM * ((dz.abs() + err) @ W.abs())
+        within(dA[at], want, tol + UNIT[F32] * (want.abs() + tol) + LEAST[F32], f"dA from {row} on")
+        want_b += dz.t() @ A
+        tol_b += err.t() @ A.abs()
+        size_b += (dz.abs() + err).t() @ A.abs()
+    tol_b += (M + 16) * SUM * size_b
+    within(dB, want_b, tol_b + UNIT[F32] * (want_b.abs() + tol_b) + LEAST[F32], "dB")
+
+
+@pytest.mark.parametrize("layout", [R.col_major, R.row_major], ids=_id)
+@pytest.mark.parametrize("size", [(3, 2100001, 40), (100, 2200000, 24)], ids=_id)
+def test_vocabularies_of_more_than_two_million(loader, size, layout):
+    """Rows of 2^21 logits and more, which are too long for the tiles' offsets."""
+    (M, N, K), ab = size, BF16
+    a, w, B = problem(M, N, K, ab, layout, 1)
+    targets, dloss = targets_of(M, N, 2), rnd((M,), F32, 5)
+    targets[-1] = N - 1
+    q, real = one_hot(targets, N)
+    x, dx = logits64(a, w)
+    loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K, layout)
+    check_loss(loss, lse, x, dx, q, torch.zeros_like(q), real, 1.0)
+    dA, dB = torch.full((M, K), math.nan, dtype=ab, device="cuda"), torch.full(B.shape, math.nan, dtype=ab, device="cuda")
+    loader.linear_cross_entropy_backward(dA, dB, dloss, lse, a, B, targets, M, N, K, layout)
+    check_gradients(dA, dB, a, w, layout, x, dx, q, real, dloss, 1.0)

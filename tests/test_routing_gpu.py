@@ -428,3 +428,42 @@ def test_routing_refuses(loader):
         loader.combine_backward(None, None, x, None, i, 4, 8, 2)
     with pytest.raises(R.GemmLibraryError):
         loader.combine(x.half(), rnd((8, 8), BF16, 1), i, 4, 8, 2)
+
+
+def test_rows_past_32_bits(loader):
+    """More than 2^31 elements of sorted rows, 4.6 GB: dispatch, combine and its gradients, all of it or both ends."""
+    M, N, k, E, dtype = 70001, 8192, 4, 64, BF16
+    assert M * k * N > 1 << 31
+    chosen, x = choices(M, k, E, 1, 0.02), rnd((M, N), dtype, 2)
+    rows = torch.zeros((M * k, N), dtype=dtype, device="cuda")
+    places, offsets = torch.empty((M, k), dtype=torch.int32, device="cuda"), torch.empty(E + 1, dtype=torch.int32, device="cuda")
+    loader.dispatch(rows, offsets, places, x, chosen, M, N, k)
+    flat = torch.where((chosen < 0) | (chosen >= E), E, chosen).flatten().long()
+    order = torch.argsort(flat, stable=True)
+    n = int((flat < E).sum())
+    assert n * N > 1 << 31 and int(offsets[-1]) == n
+    want = torch.full_like(flat, -1)
+    want[order[:n]] = torch.arange(n, device="cuda")
+    assert torch.equal(places.flatten().long(), want)
+    for at in range(0, n, 32768):
+        assert torch.equal(rows[at:min(at + 32768, n)], x[order[at:min(at + 32768, n)] // k]), at
+    assert (rows[n:] == 0).all()
+    w, dC = rnd((M, k), F32, 3), rnd((M, N), dtype, 5)
+    C = torch.full((M, N), math.nan, dtype=dtype, device="cuda")
+    loader.combine(C, rows, places, M, N, k, weights=w)
+    drows, dw = torch.full_like(rows, 77.0), torch.full((M, k), math.nan, device="cuda")
+    loader.combine_backward(drows, dw, dC, rows, places, M, N, k, weights=w)
+    assert (drows[n:] == 77.0).all()
+    for token in range(0, M, 8192):
+        at = slice(token, min(token + 8192, M))
+        there = (places[at] >= 0).double()
+        # (every row is its token's: the sum is the token's row times its weights')
+        factor, x64, d64 = w[at].double() * there, x[at].double(), dC[at].double()
+        total = factor.sum(1, keepdim=True) * x64
+        within(C[at], total, UNIT[dtype] * total.abs() + LEAST[dtype] + (k + 3) * E32 * factor.abs().sum(1, keepdim=True) * x64.abs(), "sum")
+        dot = (x64 * d64).sum(1, keepdim=True) * there
+        within(dw[at], dot, (N + 8) * E32 * (x64 * d64).abs().sum(1, keepdim=True) * there, "gradient of the weights")
+        for j in range(k):
+            is_there = places[at][:, j] >= 0
+            d = (factor[:, j:j + 1] * d64)[is_there]
+            within(drows[places[at][:, j][is_there].long()], d, (UNIT[dtype] + E32) * 1.01 * d.abs() + LEAST[dtype], "gradient of the rows")
