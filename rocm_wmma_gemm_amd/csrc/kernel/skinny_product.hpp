@@ -24,7 +24,7 @@ namespace device
 {
 
 // Logits leave their tile's statistics, with the logits that lists name, or their gradient, straight from the sums
-// (loss_use): 17 rows against 50001 entries of 2048 take 42 us instead of 51 with passes of their own.
+// (loss_use): 17 rows against 50001 entries of 2048 take 45.5 us (the weights at 5.3 TB/s and 4.3 us that join the parts) instead of 51 with passes of their own.
 //
 // ONCE: the weight's loads carry the non-temporal hint (product_kernel::once).
 template<in_kind IN, class OutT, class ResT, int BM, int BN, bool B_KMAJOR, bool ONCE, loss_use LOSS = loss_use::none>
