@@ -448,8 +448,9 @@ __global__ void __launch_bounds__(256) softmax_slope(const softmax_slope_args ar
 template<class InT>
 __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args args)
 {
-    __shared__ long long entries[4][most_entries];
-    __shared__ float     shares[4][most_entries];
+    typedef int      i32x4 __attribute__((ext_vector_type(4)));
+    __shared__ int   entries[4][most_entries] __attribute__((aligned(16)));
+    __shared__ float shares[4][most_entries] __attribute__((aligned(16)));
     const int            lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int            k    = args.want.k;
     const long long      step = (long long)gridDim.x * 4;
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args arg
 #pragma unroll
             for(int r = 0; r < list_rounds; ++r)
             {
-                entries[wave][r * 64 + lane] = l.entry[r];
+                entries[wave][r * 64 + lane] = (int)l.entry[r]; // (-1 past the list's end)
                 shares[wave][r * 64 + lane]  = l.e[r] * norm;
             }
         }
@@ -476,13 +477,20 @@ __global__ void __launch_bounds__(256) listed_slope(const softmax_slope_args arg
         {
             for(int j = lane; j < k; j += 64)
             {
-                const long long v = entries[wave][j];
+                const int v = entries[wave][j];
                 if(v >= args.col0 && v < args.col0 + args.cols)
                 {
                     float q = 0.0f;
-                    for(int i = 0; i < k; ++i)
+#pragma unroll 4
+                    for(int i = 0; i < k; i += 4)
                     {
-                        q += entries[wave][i] == v ? shares[wave][i] : 0.0f;
+                        const i32x4 listed = *reinterpret_cast<const i32x4*>(&entries[wave][i]);
+                        const f32x4 share  = *reinterpret_cast<const f32x4*>(&shares[wave][i]);
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            q += listed[e] == v ? share[e] : 0.0f;
+                        }
                     }
                     const float p = __builtin_amdgcn_exp2f(args.picked[row * k + j] * args.want.scale2 - own.lse);
                     static_cast<InT*>(args.dz)[row * args.pitch + (v - args.col0)] = to_out<InT>(factor * (p - q));
