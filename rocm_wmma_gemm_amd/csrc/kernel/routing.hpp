@@ -425,9 +425,37 @@ struct route_back_args
 // The gradient of the weights by the logits; the choice itself has none.  With ds_j = scale (dw_j - D) / sum, D = sum_i dw_i
 // w_i / scale, (renormalised; else scale dw_j): sigmoid dx_j = ds_j s_j (1 - s_j) for the chosen, 0 for the others; softmax
 // dx_e = s_e (ds_e - sum_j s_j ds_j), where the sum is 0 if the weights are renormalised, so that the logits
-// that were not chosen are not even read.  Sixteen lanes a token, CHUNK experts a lane; a choice outside the experts has no
-// gradient, one that is listed twice has both.  Bound by memory: the gradient is written, and a cache line of logits
-// read for every choice: 16384 tokens of 128 experts in bf16 take 6.5 us, 8 choices each.
+// that were not chosen are not even read.  Softmax's largest score of the chosen is 1 before it is divided by anything, so
+// fp32 holds all of it.  A sigmoid's scores may all be far below fp32's least number, and their shares of the sum are ordinary
+// numbers all the same: they are worked out in fp64, as for the weights, and nothing but the result is rounded to fp32.
+// Sixteen lanes a token, CHUNK experts a lane; a choice outside the experts has no gradient, one that is listed twice has both.
+// Bound by the latency of a token's chain (its choices, their logits, the joins over 16 lanes, the places in LDS): 16384 tokens of
+// 128 experts in bf16, 8 choices each, take 6.4 us, 9 MB at 1.4 TB/s; 6.5 us by sigmoid (6.1 with
+// its scores in fp32, which gave 0 and infinities for logits of -80 and below).
+__device__ __forceinline__ void sigmoid_gradients(const route_back_args& args, const float (&logit)[2], const float (&dw)[2],
+                                                  float (&own)[2])
+{
+    double s[2], rest[2], ds[2]; // 1 / (1 + e^-x) and 1 / (1 + e^x), each with all its digits; 0 as in sigmoid()
+#pragma unroll
+    for(int h = 0; h < 2; ++h)
+    {
+        const double x = (double)logit[h], e = power_of_e(-__builtin_fabs(x)), near_one = one_over(1.0 + e), small = e * near_one;
+        s[h]    = x < -700.0 ? 0.0 : x < 0.0 ? small : near_one;
+        rest[h] = x < 0.0 ? near_one : small;
+        ds[h]   = (double)args.scale * (double)dw[h];
+    }
+    double dot = 0.0;
+    if(args.renormalize)
+    {
+        const double sum = sum_of_row(s[0] + s[1]), over = sum == 0.0 ? 0.0 : 1.0 / sum;
+        s[0] *= over;
+        s[1] *= over;
+        dot = sum_of_row(s[0] * ds[0] + s[1] * ds[1]);
+    }
+    own[0] = (float)(s[0] * (ds[0] - dot) * rest[0]);
+    own[1] = (float)(s[1] * (ds[1] - dot) * rest[1]);
+}
+
 template<class InT, int CHUNK, bool SIGMOID, bool WHOLE>
 __device__ __forceinline__ void route_back_token(const route_back_args& args, long long token, int lane, float* row)
 {
@@ -479,29 +507,36 @@ __device__ __forceinline__ void route_back_token(const route_back_args& args, lo
             total = sum == 0.0f ? 1.0f : sum;
         }
     }
-    float s[2], ds[2];
-#pragma unroll
-    for(int h = 0; h < 2; ++h)
-    {
-        s[h]  = e[h] < 0 ? 0.0f : SIGMOID ? 1.0f / (1.0f + expf(-logit[h])) : expf(logit[h] - top) / total;
-        ds[h] = args.scale * dw[h];
-    }
-    if(args.renormalize)
-    {
-        const float sum  = sum_of_row(s[0] + s[1]);
-        const float rest = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const float dot  = sum_of_row(ds[0] * s[0] * rest + ds[1] * s[1] * rest);
-        ds[0]            = (ds[0] - dot) * rest;
-        ds[1]            = (ds[1] - dot) * rest;
-    }
     // what every chosen logit gets, and what all get
-    float       own[2];
-    const float all = dense ? sum_of_row(s[0] * ds[0] + s[1] * ds[1]) : 0.0f;
+    float own[2], all = 0.0f;
+    if constexpr(SIGMOID)
+    {
+        sigmoid_gradients(args, logit, dw, own);
+    }
+    else
+    {
+        float s[2], ds[2];
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+        {
+            s[h]  = e[h] < 0 ? 0.0f : expf(logit[h] - top) / total;
+            ds[h] = args.scale * dw[h];
+        }
+        if(args.renormalize)
+        {
+            const float sum  = sum_of_row(s[0] + s[1]);
+            const float rest = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float dot  = sum_of_row(ds[0] * s[0] * rest + ds[1] * s[1] * rest);
+            ds[0]            = (ds[0] - dot) * rest;
+            ds[1]            = (ds[1] - dot) * rest;
+        }
+        own[0] = s[0] * ds[0];
+        own[1] = s[1] * ds[1];
+        all    = dense ? sum_of_row(s[0] * ds[0] + s[1] * ds[1]) : 0.0f;
+    }
 #pragma unroll
     for(int h = 0; h < 2; ++h)
     {
-        // (1 - s of a sigmoid: e^-x s, which keeps its digits where s is near 1)
-        own[h] = SIGMOID ? ds[h] * s[h] * (logit[h] > 0.0f ? expf(-logit[h]) * s[h] : 1.0f - s[h]) : s[h] * ds[h];
         own[h] = e[h] < 0 ? 0.0f : own[h];
     }
     // The choices' parts go to their experts' places in LDS, one after the other (of equal ones all count, in their order; the

@@ -467,3 +467,27 @@ def test_rows_past_32_bits(loader):
             is_there = places[at][:, j] >= 0
             d = (factor[:, j:j + 1] * d64)[is_there]
             within(drows[places[at][:, j][is_there].long()], d, (UNIT[dtype] + E32) * 1.01 * d.abs() + LEAST[dtype], "gradient of the rows")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=_id)
+@pytest.mark.parametrize("centre", [-640.0, -100.0, -90.0, -88.0, -86.0, -80.0, 0.0, 30.0, 600.0])
+def test_gradient_of_sigmoid_weights_wherever_the_logits_lie(loader, centre, dtype):
+    """All of a token's logits near `centre`, gradients as large as a scaled loss has them: a token's weights are shares of the
+    sum of its scores, which is far below fp32's least number for most of these, and so is 1 - s for the last.
+
+    The kernel works in fp64 and rounds to fp32, then to the logits' type; what is made of differences (dw_j - D) is off by
+    some 2^-48 of the numbers subtracted."""
+    M, E, k, size = 65, 40, 6, 4096.0 if dtype is not F16 else 256.0
+    x, dw = (rnd((M, E), F32, 1, 1.5) + centre).to(dtype), rnd((M, k), F32, 2, size)
+    s, rest = (1 / (1 + torch.exp(-v * x.double())) for v in (1, -1))  # s and 1 - s
+    for renormalize, scale in ((True, 2.5), (False, 0.5)):
+        chosen, weights = routed(loader, x, k, score=SIGMOID, renormalize=renormalize, scale=scale)
+        p, q = s.gather(1, chosen.long()), rest.gather(1, chosen.long())
+        w = p / p.sum(1, keepdim=True) if renormalize else p
+        within(weights, scale * w, E32 * scale * w * 1.001 + LEAST[F32], "weights")
+        dot, most = ((w * v).sum(1, keepdim=True) if renormalize else 0.0 for v in (dw.double(), dw.double().abs()))
+        want = torch.zeros_like(s).scatter_(1, chosen.long(), scale * w * (dw.double() - dot) * q)
+        part = torch.zeros_like(s).scatter_(1, chosen.long(), scale * w * (dw.double().abs() + most) * q)
+        dx = torch.full((M, E), math.nan, dtype=dtype, device="cuda")
+        loader.route_backward(dx, dw, chosen, x, M, E, k, score=SIGMOID, renormalize=renormalize, scale=scale)
+        within(dx, want, (UNIT[dtype] + E32) * 1.01 * want.abs() + 2.0 ** -48 * part + LEAST[dtype] + LEAST[F32], "gradient of the logits")
