@@ -384,7 +384,7 @@ int rocm_wmma_gemm_linear_cross_entropy(int element, float* loss, float* lse, co
 
 /* dz = dloss (softmax(z) - [v = target]), 0 in rows that are left out; dA = dz B^T (M x K), dB = A^T dz in B's layout; a NULL result is
  * not computed.  accumulate 1: dB is added to.  type_idx: the types of dA and dB, and of A and B.  dz is rounded to A's
- * type before it is multiplied, in units of 2^-14 of the largest |dloss|. */
+ * type before it is multiplied, in units of 2^-14 of the largest |dloss| of the rows that are not left out. */
 int rocm_wmma_gemm_linear_cross_entropy_backward(int type_idx, void* dA, void* dB, const float* dloss, const float* lse,
                                                  const void* A, const void* B, const void* targets, int wide_targets, size_t M,
                                                  size_t N, size_t K, int layout_b, int accumulate, void* stream);

@@ -530,6 +530,7 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     const segments seg = p.count == 1 ? segments(h, h.N, cus) : segments(h, 0, cus);
     const size_t z_at = fused ? 0 : r.take(h.M * pitch * 4), dz_at = r.take(h.M * pitch * 2 + (seg.count != 0 ? h.N * 2 : 0)), // (a segment's loads may reach so far past the last row)
                  records_at = r.take(h.M * sizeof(device::loss_record)), unit_at = r.take(8),
+                 counted_at = h.want.teacher != nullptr ? r.take(h.M * sizeof(float)) : 0,
                  sum_at = wants_a ? r.take(seg.parts() * h.M * k_pitch * 4) : 0, product_at = r.bytes;
     auto logits = [&](const operand& a, const operand& b, size_t v0, size_t cols, char* ws) {
         step s = logits_of(h, fused ? finish_slope : finish_plain, a, b, v0, cols, ws != nullptr ? ws + (fused ? dz_at : z_at) : nullptr, pitch);
@@ -596,17 +597,22 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
     operand       a, b;
     c.make(h, &a, &b, ws, stream);
     char* const   scratch = ws + product_at;
-    const device::record_args f{h.want, dloss, lse, reinterpret_cast<device::loss_record*>(ws + records_at),
-                                reinterpret_cast<float*>(ws + unit_at)};
+    device::record_args f{h.want, dloss, lse, reinterpret_cast<device::loss_record*>(ws + records_at),
+                          reinterpret_cast<float*>(ws + unit_at)};
+    if(h.want.teacher != nullptr && h.M != 0)
+    {
+        float* const counted = reinterpret_cast<float*>(ws + counted_at);
+        follow(&device::counted_gradients, dim3(row_groups(h.M)), dim3(256), stream, h.want, dloss, counted);
+        f.dloss = counted;
+    }
+    const unsigned groups = static_cast<unsigned>(ceil_div(rows, 256));
     if(h.M > device::most_alone)
     {
         follow(&device::gradient_unit, dim3(1), dim3(1024), stream, f);
-        follow(&device::gradient_records<false>, dim3(row_groups(h.M)), dim3(256), stream, f);
+        follow(&device::gradient_records<false>, dim3(groups), dim3(256), stream, f);
     }
     else
     {
-        // (at most four workgroups a compute unit look for the largest)
-        const unsigned groups = static_cast<unsigned>(std::min<size_t>(row_groups(rows), 4 * cus));
         follow(&device::gradient_records<true>, dim3(groups), dim3(256), stream, f);
     }
     int rc = ROCM_WMMA_GEMM_OK;

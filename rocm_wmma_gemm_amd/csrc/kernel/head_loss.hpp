@@ -302,31 +302,73 @@ __global__ void __launch_bounds__(256) join_rows(const join_args args)
 
 // ------------------------------------------------------------------ the gradient
 
-// The gradient of a row's logits is worked out as T dloss / most 2^14 (p - q), with `most` the largest T |dloss| of all
-// rows, and 0 for a row that is compared with nothing; the products' sums are brought back by unit = most 2^-14 as they are
-// rounded.  It is held in 16 bits, whose smallest number in f16 is 6e-8 (p - q is at most 1, so 2^14 stays in range), and where
+// The gradient of a row's logits is worked out as T dloss / most 2^14 (p - q), with `most` the largest T |dloss| of the
+// rows that are compared with something, and 0 for the others, whatever their dloss; the products' sums are brought back by
+// unit = most 2^-14 as they are rounded.  It is held in 16 bits, whose smallest number in f16 is 6e-8 (p - q is at most 1, so 2^14 stays in range), and where
 // all rows have one dloss, as under a mean, its rounding leaves p - q of a target with a small p as it is: against 64 bits a bf16
 // gradient is 1.9e-3 off instead of 2.6e-3 with dloss itself in it.
 struct record_args
 {
     wanted_args  want;
-    const float* dloss;
+    const float* dloss; // (of lists: counted_gradients')
     const float* lse;
     loss_record* records;
     float*       unit; // [0]: unit, [1]: most
 };
 
-// The largest T |dloss| of all rows, 1 if there is none; by all threads of a workgroup.
+// dloss of the rows whose list has a share, 0 of the others: a list takes a wave to look through, so it is done once, before
+// all rows are looked through for the largest.  A wave a row.
+__global__ void __launch_bounds__(256)
+    counted_gradients(const wanted_args want, const float* __restrict__ dloss, float* __restrict__ counted)
+{
+    for(long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < want.rows; row += (long long)gridDim.x * 4)
+    {
+        const float sum = read_list(want, row).sum;
+        if((threadIdx.x & 63) == 0)
+        {
+            counted[row] = sum > 0.0f || sum != sum ? dloss[row] : 0.0f;
+        }
+    }
+}
+
+// The largest T |dloss| of the rows that count, 1 if there is none; by all threads of a workgroup.
 template<int THREADS>
 __device__ __forceinline__ float largest_gradient(const record_args& args)
 {
     __shared__ float of_wave[THREADS / 64];
     float            most = 0.0f;
-#pragma unroll 8
-    for(int row = threadIdx.x; row < args.want.rows; row += THREADS)
+    auto look = [&](auto entry) { // (a loop for every width of an index: the loads of eight rows go out together)
+        const int last = args.want.rows - 1;
+        for(int first = threadIdx.x; first <= last; first += 8 * THREADS)
+        {
+            float     said[8];
+            long long v[8];
+#pragma unroll
+            for(int u = 0; u < 8; ++u)
+            {
+                const int row = first + u * THREADS < last ? first + u * THREADS : last; // (the last row again changes nothing)
+                said[u]       = args.dloss[row];
+                v[u]          = entry(row);
+            }
+#pragma unroll
+            for(int u = 0; u < 8; ++u)
+            {
+                const float d = __builtin_fabsf(said[u] / args.want.scale);
+                most = v[u] >= 0 && v[u] < args.want.vocabulary && d > most && d < __builtin_inff() ? d : most;
+            }
+        }
+    };
+    if(args.want.teacher != nullptr)
     {
-        const float d = __builtin_fabsf(args.dloss[row] / args.want.scale);
-        most          = d > most && d < __builtin_inff() ? d : most;
+        look([](int) { return 0ll; }); // (with a list that counts there is a vocabulary)
+    }
+    else if(args.want.wide)
+    {
+        look([&](int row) { return static_cast<const long long*>(args.want.entries)[row]; });
+    }
+    else
+    {
+        look([&](int row) { return (long long)static_cast<const int*>(args.want.entries)[row]; });
     }
 #pragma unroll
     for(int d = 1; d < 64; d *= 2)
@@ -362,14 +404,13 @@ __global__ void __launch_bounds__(1024) gradient_unit(const record_args args)
     }
 }
 
-// A wave a row (a list has to be looked through for an entry).  ALONE: every workgroup looks for the largest gradient itself, where
-// that is less than waiting for a launch that does (4 us; 64 KB of dloss are read in less).
+// A thread a row.  ALONE: every workgroup looks for the largest gradient itself, where that is less than waiting for a launch that
+// does (4 us; 64 KB of dloss and the targets are read in less).
 constexpr int most_alone = 16384; // rows
 template<bool ALONE>
 __global__ void __launch_bounds__(256) gradient_records(const record_args args)
 {
-    const int lane = threadIdx.x & 63;
-    float     most;
+    float most;
     if constexpr(ALONE)
     {
         most = largest_gradient<256>(args);
@@ -382,26 +423,15 @@ __global__ void __launch_bounds__(256) gradient_records(const record_args args)
     {
         most = args.unit[1];
     }
-    for(long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); row < args.want.rows; row += (long long)gridDim.x * 4)
+    for(long long row = (long long)blockIdx.x * 256 + threadIdx.x; row < args.want.rows; row += (long long)gridDim.x * 256)
     {
-        bool      is;
-        long long target = -1;
-        if(args.want.teacher == nullptr)
-        {
-            target = entry_of(args.want, row);
-            is     = target >= 0;
-        }
-        else
-        {
-            const float sum = read_list(args.want, row).sum;
-            is              = sum > 0.0f || sum != sum;
-        }
-        if(lane == 0)
-        {
-            const float factor = args.dloss[row] / args.want.scale / most * 0x1p14f;
-            args.records[row]  = is ? loss_record{args.lse[row] * log2_of_e, factor, (int)target, 0}
+        const bool      listed = args.want.teacher != nullptr;
+        const long long target = listed ? -1 : entry_of(args.want, row);
+        const float     dloss  = args.dloss[row];
+        const bool      is     = listed ? dloss != 0.0f : target >= 0;
+        const float     factor = dloss / args.want.scale / most * 0x1p14f;
+        args.records[row]      = is ? loss_record{args.lse[row] * log2_of_e, factor, (int)target, 0}
                                     : loss_record{__builtin_inff(), 0.0f, -1, 0};
-        }
     }
 }
 

@@ -605,3 +605,34 @@ def test_vocabularies_of_more_than_two_million(loader, size, layout):
     dA, dB = torch.full((M, K), math.nan, dtype=ab, device="cuda"), torch.full(B.shape, math.nan, dtype=ab, device="cuda")
     loader.linear_cross_entropy_backward(dA, dB, dloss, lse, a, B, targets, M, N, K, layout)
     check_gradients(dA, dB, a, w, layout, x, dx, q, real, dloss, 1.0)
+
+
+@pytest.mark.parametrize("ab", [F16, BF16], ids=_id)
+@pytest.mark.parametrize("size", [(40, 700, 64), (300, 1000, 72), (1500, 520, 64), (16385, 264, 40)], ids=_id)
+def test_whatever_dloss_says_of_rows_that_are_left_out(loader, size, ab):
+    """Large, infinite and unset values there change no bit of the gradients."""
+    (M, N, K), k = size, 5
+    a, w, B = problem(M, N, K, ab, R.col_major, 1)
+    dloss = rnd((M,), F32, 5, 1e-4)
+    targets = targets_of(M, N, 2)
+    entries, teacher = lists_of(M, N, k, 3)
+    entries[5::3] = -1
+    teacher[7::9] = -math.inf  # (a list without a share)
+    loss, lse, picked = torch.empty(M, device="cuda"), torch.empty(M, device="cuda"), torch.empty((M, k), device="cuda")
+    out = {}
+    for kind in ("target", "list"):
+        out_of = ~one_hot(targets, N)[1] if kind == "target" else ~((entries >= 0) & (entries < N) & (teacher > -math.inf)).any(1)
+        assert out_of.any() and not out_of.all()
+        for said in (0.0, 1.0, 1e8, 3e38, math.inf, math.nan):
+            d = torch.where(out_of, torch.full_like(dloss, said), dloss)
+            dA, dB = torch.full((M, K), math.nan, dtype=ab, device="cuda"), torch.full((N, K), math.nan, dtype=ab, device="cuda")
+            if kind == "target":
+                loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K)
+                loader.linear_cross_entropy_backward(dA, dB, d, lse, a, B, targets, M, N, K)
+            else:
+                loader.linear_distillation(loss, lse, picked, a, B, entries, teacher, M, N, K)
+                loader.linear_distillation_backward(dA, dB, d, lse, picked, a, B, entries, teacher, M, N, K)
+            assert (dA[out_of] == 0).all() and dA.abs().max() > 0
+            if said == 0.0:
+                out[kind] = dA, dB
+            assert torch.equal(dA, out[kind][0]) and torch.equal(dB, out[kind][1]), (kind, said)
