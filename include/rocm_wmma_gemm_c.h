@@ -373,7 +373,8 @@ int rocm_wmma_gemm_combine_backward(int rows_type, int out_type, void* drows, fl
  * (temperature 1 for cross entropy), which the backward pass reads.  Softmax, sums and losses are worked out in fp32.  M up to
  * 2^20, N and K up to 2^31 - 256; a size of 0 is no error.  Rows of A that are left out must hold numbers all the same (they are
  * multiplied by 0).  The calls enqueue on *stream and return; they work in the library's scratch buffer and return
- * ROCM_WMMA_GEMM_ERR_SCRATCH where it cannot be had (on a capturing stream: make one eager call first).
+ * ROCM_WMMA_GEMM_ERR_SCRATCH where it cannot be had (on a capturing stream: make one eager call first; operands whose rows do
+ * not start on 16 bytes are copied, and the whole has to fit 16 GiB).
  * --------------------------------------------------------------------------------------- */
 
 /* loss_t = lse_t - z_t,target; 0 for a row whose target lies outside 0 .. N - 1 (it is left out).  targets: M values of 32 bits, or

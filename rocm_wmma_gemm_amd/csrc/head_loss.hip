@@ -16,7 +16,7 @@ using device::product_args;
 using device::product_kind;
 using device::wanted_args;
 
-constexpr size_t most_rows = size_t{1} << 20; // (a piece of 1024 columns of them fits the scratch buffer)
+constexpr size_t most_rows = size_t{1} << 20; // (a piece of 1024 columns of them fits the scratch buffer; their dA in fp32 may not: see gradients_of)
 
 // A piece of the logits in fp32 is read back from the memory-side cache where it is not larger than this.
 constexpr size_t piece_bytes = size_t{128} << 20;
@@ -503,8 +503,12 @@ void launch_slope(const device::softmax_slope_args& s, bool fused, hipStream_t s
 //
 // What is rounded, and why: dz to A's type, as both products need it, in the units of record_args.  dA's parts are added up in
 // fp32 over the pieces.
+//
+// A million rows of thousands of elements in fp32 are more than the scratch buffer may hold: then dB is worked out for itself, from all
+// rows, so that its sums are rounded once, and dA behind it in blocks of rows, which have nothing to do with each other, at the
+// price of the logits a third time.  asked: only whether there is room, nothing is launched.
 int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss, const float* lse, const float* picked, bool accumulate,
-                 hipStream_t stream)
+                 hipStream_t stream, bool asked = false)
 {
     const bool wants_a = dA != nullptr && h.M != 0 && h.K != 0, wants_b = dB != nullptr && h.N != 0 && h.K != 0;
     if(!wants_a && !wants_b)
@@ -587,6 +591,39 @@ int gradients_of(const head& h, int out, void* dA, void* dB, const float* dloss,
         }
         product = std::max(product, wants_b && !outer ? weights(plan_a, v0, cols, nullptr).plan(cus).scratch() : 0);
         v0 = v0 == p.cols && p.count > 3 ? (p.count - 2) * p.cols : v0; // (the first, one behind it, the last)
+    }
+    if(product_at + product > workspace_limit_bytes)
+    {
+        if(!wants_a || (!wants_b && h.M == 1))
+        {
+            return ROCM_WMMA_GEMM_ERR_SCRATCH;
+        }
+        auto parts = [&](bool only_asked) {
+            if(wants_b)
+            {
+                const int rc = gradients_of(h, out, nullptr, dB, dloss, lse, picked, accumulate, stream, only_asked);
+                return rc != ROCM_WMMA_GEMM_OK ? rc
+                                               : gradients_of(h, out, dA, nullptr, dloss, lse, picked, false, stream, only_asked);
+            }
+            const size_t half = ceil_div(h.M, 2);
+            for(size_t row = 0; row < h.M; row += half)
+            {
+                const int rc = gradients_of(rows_of(h, row, std::min(half, h.M - row)), out, static_cast<char*>(dA) + row * h.K * size, nullptr,
+                                            dloss + row, lse + row, picked != nullptr ? picked + row * h.want.k : nullptr, false, stream,
+                                            only_asked);
+                if(rc != ROCM_WMMA_GEMM_OK || only_asked) // (the second half is no larger)
+                {
+                    return rc;
+                }
+            }
+            return ROCM_WMMA_GEMM_OK;
+        };
+        const int rc = parts(true);
+        return rc != ROCM_WMMA_GEMM_OK || asked ? rc : parts(false);
+    }
+    if(asked)
+    {
+        return ROCM_WMMA_GEMM_OK;
     }
     workspace_lease lease;
     char*           ws = lease.acquire(product_at + product, stream);

@@ -636,3 +636,43 @@ def test_whatever_dloss_says_of_rows_that_are_left_out(loader, size, ab):
             if said == 0.0:
                 out[kind] = dA, dB
             assert torch.equal(dA, out[kind][0]) and torch.equal(dB, out[kind][1]), (kind, said)
+
+
+@pytest.mark.parametrize("layout", [R.col_major, R.row_major], ids=_id)
+def test_gradients_of_a_million_long_rows(loader, layout):
+    """2^20 rows of 4096 elements: dA in fp32 would fill the scratch buffer, so the rows go in blocks."""
+    M, N, K, ab = 1 << 20, 264, 4096, BF16
+    w = rnd((N, K), ab, 2, 2.0 / math.sqrt(K))
+    B = w if layout == R.col_major else w.t().contiguous()
+    a = torch.empty((M, K), dtype=ab, device="cuda")
+    for row in range(0, M, 1 << 16):
+        a[row:row + (1 << 16)] = rnd((1 << 16, K), ab, row + 3)
+    targets, dloss = targets_of(M, N, 2), rnd((M,), F32, 5)
+    loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+    loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K, layout)
+    before = rnd(B.shape, F32, 6)
+    dA, dB = torch.full((M, K), math.nan, dtype=ab, device="cuda"), torch.full(B.shape, math.nan, dtype=ab, device="cuda")
+    alone, added = torch.full_like(dA, math.nan), before.clone()
+    loader.linear_cross_entropy_backward(dA, dB, dloss, lse, a, B, targets, M, N, K, layout)
+    loader.linear_cross_entropy_backward(alone, None, dloss, lse, a, B, targets, M, N, K, layout)
+    assert torch.equal(alone, dA)
+    del alone
+    loader.linear_cross_entropy_backward(None, added, dloss, lse, a, B, targets, M, N, K, layout, accumulate=True)
+    W = w.double()
+    want_b, tol_b, size_b = (torch.zeros((N, K), dtype=torch.float64, device="cuda") for _ in range(3))
+    for row in range(0, M, 1 << 15):
+        at = slice(row, row + (1 << 15))
+        x, dx = logits64(a[at], w)
+        q, real = one_hot(targets[at], N)
+        dz, err = slopes64(x, dx, torch.logsumexp(x, 1), dx.max(1)[0], q, real, dloss[at], ab)
+        want, A = dz @ W, a[at].double()
+        tol = err @ W.abs() + (N + 16) * SUM * ((dz.abs() + err) @ W.abs())
+        within(dA[at], want, tol + UNIT[ab] * (want.abs() + tol) + LEAST[ab], f"dA from {row} on")
+        want_b += dz.t() @ A
+        tol_b += err.t() @ A.abs()
+        size_b += (dz.abs() + err).t() @ A.abs()
+    tol_b += (M + 16) * SUM * size_b
+    got = (dB, added) if layout == R.col_major else (dB.t(), added.t())
+    within(got[0], want_b, tol_b + UNIT[ab] * (want_b.abs() + tol_b) + LEAST[ab], "dB")
+    more = (before if layout == R.col_major else before.t()).double()
+    within(got[1], want_b + more, tol_b + UNIT[F32] * (want_b.abs() + tol_b) + 2 * E32 * (want_b.abs() + more.abs()) + LEAST[F32], "dB added to")

@@ -141,3 +141,32 @@ def test_tiled_products_behind_a_loss_keep_accumulators_in_place(tmp_path):
                         break
                 n += 1
         assert checked >= 1, func
+
+
+def test_only_copies_of_operands_are_more_than_the_scratch_buffer_holds(recorded):  # noqa: F811
+    """Sizes up to the documented ones are launched, a gradient of 2^20 rows of 4096 and more elements in blocks of rows.  Only operands
+    whose rows do not start on 16 bytes, and whose copies take more than 16 GiB, are refused, before anything is launched."""
+    most = (1 << 31) - 256
+    for m, n, k in ((1, 1, 1), (300, 1001, 77), (4096, 131072, 4096), (1, most, 8), (3, 1 << 27, 3), (1 << 20, 5000, 8), (1 << 20, 40000, 16),
+                    (1 << 20, 264, 4096), (1 << 20, 32000, 4096), (1 << 19, 32000, 8192), (1 << 20, 128, 8192), (1 << 20, 1000, 4095),
+                    (1 << 16, 131072, 16384), (2, 8, most), (64, 1000, 1 << 26), (1, 1, most), (1 << 20, 128, 8201), (1 << 19, 72, 16385)):
+        calls, large = [], []
+        for kind, layout in ((0, 0), (1, 1)):
+            calls += calls_of(kind, m, n, k, layout)
+            padded = lambda rows, length: rows * ((length + 7) // 8) * 16 if length % 8 else 0  # noqa: E731
+            copied = padded(m, k) + (padded(k, n) if layout == 0 else padded(n, k))
+            # (a gradient of the states alone goes in blocks of rows: half of the states' copies at a time, or less)
+            alone = padded(m // 4, k) + (padded(k, n) if layout == 0 else padded(n, k))
+            large += [copied > 1 << 34] * 3 + [alone > 1 << 34] + [copied > 1 << 34]
+        for call, refused, (status, launches) in zip(calls, large, recorded(*calls)):
+            assert (status, bool(launches)) == ((SCRATCH, False) if refused else (OK, True)), (call, status, len(launches))
+            assert not any(failed for *_, failed in launches), (call, launches)
+
+
+def test_nothing_of_a_gradient_in_blocks_follows_a_launch_that_failed(recorded):  # noqa: F811
+    for call in calls_of(1, 1 << 20, 264, 4096, 1)[1::2]:
+        (status, whole), = recorded(call)
+        assert status == OK and len(whole) >= 14  # (of every block: the unit, records, logits, dA's product, its rounding; more of lists)
+        for n in range(0, len(whole), 5):
+            (status, launches), = recorded(["fail", n], call)
+            assert status == -4 and len(launches) == n + 1, (call[0], n)
