@@ -269,9 +269,15 @@ __global__ void __launch_bounds__(256) join_rows(const join_args args)
                 continue;
             }
         }
-        // (what lies between the largest logit and a listed one first: it is exact where the two are near)
+        // What lies between the largest logit and a listed one first: it is exact where the two are near, 0 where they are one
+        // (z scale2 is rounded as it was for the largest: no multiply-add).  Where tiles leave the statistics the listed logit comes
+        // from pick_products, whose sum has another order: it may be a rounding above the largest, but -log p is not below 0.
         const float rest = log2f(all.sum);
-        auto        less_log_p = [&](float z) { return ((all.top - z * args.want.scale2) + rest) * log_of_2; };
+        auto        less_log_p = [&](float z) {
+#pragma clang fp contract(off)
+            const float x = z * args.want.scale2, bits = (all.top - x) + rest;
+            return (bits < 0.0f ? 0.0f : bits) * log_of_2;
+        };
         float       loss = 0.0f;
         if(args.want.teacher == nullptr)
         {

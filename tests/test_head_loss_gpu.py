@@ -676,3 +676,30 @@ def test_gradients_of_a_million_long_rows(loader, layout):
     within(got[0], want_b, tol_b + UNIT[ab] * (want_b.abs() + tol_b) + LEAST[ab], "dB")
     more = (before if layout == R.col_major else before.t()).double()
     within(got[1], want_b + more, tol_b + UNIT[F32] * (want_b.abs() + tol_b) + 2 * E32 * (want_b.abs() + more.abs()) + LEAST[F32], "dB added to")
+
+
+def test_a_row_that_is_sure_of_its_target_has_no_negative_loss(loader):
+    """-log p is 0 or more.  Where the vocabulary is one entry, or all others are far below, the largest logit is the target's: the
+    kernels that pick it from the logits they add up (few rows, logits that are written) leave exactly 0, tiles whose target is
+    added up on its own are at most the two sums' difference above."""
+    for ab in (F16, BF16):
+        for M, N, K, layout in ((64, 1, 96, R.col_major), (40, 600, 64, R.row_major), (64, 600, 264, R.col_major),
+                                (2000, 1, 520, R.col_major), (2000, 777, 264, R.col_major), (1000, 1000, 136, R.row_major)):
+            a, w, B = problem(M, N, K, ab, layout, 1)
+            targets = torch.randint(N, (M,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+            a = (w[targets].float() * torch.linspace(25, 90, M, device="cuda")[:, None]).to(ab)
+            x, dx = logits64(a, w)
+            others = x.scatter(1, targets[:, None], -math.inf).max(1)[0]
+            sure = x.gather(1, targets[:, None])[:, 0] - others > 40 + 2 * dx.max(1)[0]  # (e^-40: nothing in fp32)
+            assert sure.sum() > M // 2
+            loss, lse = torch.empty(M, device="cuda"), torch.empty(M, device="cuda")
+            loader.linear_cross_entropy(loss, lse, a, B, targets, M, N, K, layout)
+            assert (loss >= 0).all(), (M, N, K, loss.min().item())
+            if M <= 64:
+                assert (loss[sure] == 0).all(), (M, N, K, loss[sure].max().item())
+            else:
+                assert (loss[sure] <= 2 * dx.max(1)[0][sure]).all()
+            # a list of the one entry is the same distance
+            picked = torch.empty((M, 1), device="cuda")
+            loader.linear_distillation(loss, lse, picked, a, B, targets[:, None].contiguous(), torch.zeros((M, 1), device="cuda"), M, N, K, layout)
+            assert (loss >= 0).all() and (M > 64 and layout == R.col_major or (loss[sure] == 0).all())
