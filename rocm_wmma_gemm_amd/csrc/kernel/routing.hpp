@@ -234,8 +234,9 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
     load_run<InT, CHUNK, WHOLE>(x + first, count, last, logit);
     auto is = [&](int i) { return WHOLE || i < count; };
     const bool by_score = args.bias != nullptr || args.groups > 1;
-    // softmax: its largest logit and sum, where the scores need them
-    double top = 0.0, over_total = 1.0;
+    // softmax: its largest logit and sum, where the scores need them.  A logit that is no number adds nothing to the sum, so that
+    // the others are chosen by their scores; the weights' sum is none with it.
+    double top = 0.0, over_total = 1.0, over_weights = 1.0;
     if constexpr(!SIGMOID)
     {
         float most = -__builtin_inff();
@@ -249,16 +250,21 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
         if(by_score || !args.renormalize)
         {
             double sum = 0.0;
+            int    bad = 0;
 #pragma unroll
             for(int i = 0; i < CHUNK; ++i)
             {
-                sum += is(i) ? power_of_e((double)logit[i] - top) : 0.0;
+                // (of a number and none, the maximum is the number)
+                sum += is(i) ? power_of_e(__builtin_fmax((double)logit[i] - top, least)) : 0.0;
+                bad |= is(i) && logit[i] != logit[i] ? 1 : 0;
             }
-            sum        = sum_of_row(sum);
-            over_total = sum == 0.0 ? 1.0 : 1.0 / sum;
+            sum          = sum_of_row(sum);
+            bad          = join_row(bad, route_lanes, [](int a, int b) { return a | b; });
+            over_total   = sum == 0.0 ? 1.0 : 1.0 / sum;
+            over_weights = bad ? __builtin_nan("") : over_total;
         }
     }
-    auto score = [&](float l) { return SIGMOID ? sigmoid((double)l) : power_of_e((double)l - top) * over_total; };
+    auto score = [&](float l, double over) { return SIGMOID ? sigmoid((double)l) : power_of_e((double)l - top) * over; };
     double key[CHUNK];
     double high = least, second = least; // the lane's two best values
     if(by_score)
@@ -279,7 +285,7 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
 #pragma unroll
         for(int i = 0; i < CHUNK; ++i)
         {
-            const double s = score(logit[i]) + (double)bias[i];
+            const double s = score(logit[i], over_total) + (double)bias[i];
             const double v = is(i) ? __builtin_fmax(s, least) : least; // (no number: the lowest)
             second         = __builtin_fmax(second, __builtin_fmin(high, v));
             high           = __builtin_fmax(high, v);
@@ -378,7 +384,7 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
 #pragma unroll
     for(int h = 0; h < (MOST > route_lanes ? 2 : 1); ++h)
     {
-        s[h] = lane + h * route_lanes < args.k ? score((float)x[mine[h]]) : 0.0;
+        s[h] = lane + h * route_lanes < args.k ? score((float)x[mine[h]], over_weights) : 0.0;
         total += s[h];
     }
     double factor = args.scale;

@@ -491,3 +491,31 @@ def test_gradient_of_sigmoid_weights_wherever_the_logits_lie(loader, centre, dty
         dx = torch.full((M, E), math.nan, dtype=dtype, device="cuda")
         loader.route_backward(dx, dw, chosen, x, M, E, k, score=SIGMOID, renormalize=renormalize, scale=scale)
         within(dx, want, (UNIT[dtype] + E32) * 1.01 * want.abs() + 2.0 ** -48 * part + LEAST[dtype] + LEAST[F32], "gradient of the logits")
+
+
+@pytest.mark.parametrize("sizes", [(20, 1), (24, 4), (512, 1), (48, 16)], ids=_id)
+def test_a_logit_that_is_no_number_is_chosen_last(loader, sizes):
+    """The other experts are chosen as without it: by their scores among the numbers, with a bias, in groups, by every score."""
+    E, groups = sizes
+    M, k, each = 50, 6, E // groups
+    kept = max(1, groups // 2) if each * (groups // 2) >= k + 2 else groups
+    for score in (SOFTMAX, SIGMOID):
+        for bias in (None, rnd((E,), F32, 3, 0.05 if score == SIGMOID else 0.01)):
+            x = rnd((M, E), F32, 1, 1.5)
+            gone = torch.randint(E, (M,), generator=torch.Generator().manual_seed(2)).cuda()
+            bad = x.scatter(1, gone[:, None], math.nan)
+            s = scores64(x.scatter(1, gone[:, None], -math.inf), score)  # (of the numbers; the one that is none counts 0 in their sum)
+            value = (s if bias is None else s + bias.double()).scatter(1, gone[:, None], -math.inf)
+            rank = value if bias is not None else x.double().scatter(1, gone[:, None], -math.inf)
+            if groups > 1:
+                of = value.view(M, groups, each).sort(2, descending=True)[0][:, :, :2].sum(2)
+                best = of.sort(dim=1, descending=True, stable=True)[1][:, :kept]
+                allowed = torch.zeros((M, groups), dtype=torch.bool, device="cuda").scatter_(1, best, True)
+                rank = torch.where(allowed.repeat_interleave(each, 1), rank, -math.inf)
+            want = rank.sort(dim=1, descending=True, stable=True)[1][:, :k]
+            chosen, _ = routed(loader, bad, k, score=score, bias=bias, groups=groups, kept_groups=kept)
+            assert torch.equal(chosen.long(), want), (score, bias is not None)
+    if groups == 1 and E <= 32:
+        for bias in (None, torch.zeros(E, device="cuda")):
+            chosen, _ = routed(loader, bad, E, score=SOFTMAX, bias=bias)
+            assert torch.equal(chosen[:, -1].long(), gone)
