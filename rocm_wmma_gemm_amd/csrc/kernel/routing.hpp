@@ -320,7 +320,8 @@ __device__ __forceinline__ void route_token(const route_args& args, long long to
         {
             meet(from_row<0x141>(high), from_row<0x141>(second));
         }
-        const double of_group = args.best > 1 && args.size > 1 ? high + second : high;
+        // (infinite biases: of a sum that is none, the lowest, or the group would be one more than `kept`)
+        const double of_group = __builtin_fmax(args.best > 1 && args.size > 1 ? high + second : high, least);
         int          better   = 0;
         for(int g = 0; g < args.groups; ++g)
         {

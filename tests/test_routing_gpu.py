@@ -519,3 +519,14 @@ def test_a_logit_that_is_no_number_is_chosen_last(loader, sizes):
         for bias in (None, torch.zeros(E, device="cuda")):
             chosen, _ = routed(loader, bad, E, score=SOFTMAX, bias=bias)
             assert torch.equal(chosen[:, -1].long(), gone)
+
+
+def test_no_more_groups_are_kept_than_asked_for(loader):
+    """A group whose two best biased scores are infinite both ways has no sum: it is the lowest, not one more."""
+    E, groups, kept, k = 16, 8, 1, 2
+    x = rnd((40, E), F32, 1)
+    bias = torch.zeros(E, device="cuda")
+    bias[4], bias[5] = math.inf, -math.inf
+    for score in (SOFTMAX, SIGMOID):
+        chosen, _ = routed(loader, x, k, score=score, bias=bias, groups=groups, kept_groups=kept)
+        assert (chosen // 2 == chosen[:, :1] // 2).all() and (chosen // 2 != 2).all(), score
