@@ -703,3 +703,25 @@ def test_a_row_that_is_sure_of_its_target_has_no_negative_loss(loader):
             picked = torch.empty((M, 1), device="cuda")
             loader.linear_distillation(loss, lse, picked, a, B, targets[:, None].contiguous(), torch.zeros((M, 1), device="cuda"), M, N, K, layout)
             assert (loss >= 0).all() and (M > 64 and layout == R.col_major or (loss[sure] == 0).all())
+
+
+def test_gradients_of_lists_in_blocks_of_rows(loader):
+    """The states' gradient of 2^20 rows with lists, which goes in two blocks, has the bits of two calls of half of the rows."""
+    M, N, K, k, t = 1 << 20, 72, 4096, 3, 2.0
+    w = rnd((N, K), BF16, 2, 2.0 / math.sqrt(K))
+    a = torch.empty((M, K), dtype=BF16, device="cuda")
+    for row in range(0, M, 1 << 16):
+        a[row:row + (1 << 16)] = rnd((1 << 16, K), BF16, row + 3)
+    entries, teacher = lists_of(M, N, k, 4)
+    dloss = rnd((M,), F32, 5)
+    loss, lse, picked = torch.empty(M, device="cuda"), torch.empty(M, device="cuda"), torch.empty((M, k), device="cuda")
+    for index in (torch.int64, torch.int32):
+        listed = entries.to(index)
+        loader.linear_distillation(loss, lse, picked, a, w, listed, teacher, M, N, K, temperature=t)
+        dA, halves = torch.full((M, K), math.nan, dtype=BF16, device="cuda"), torch.full((M, K), math.nan, dtype=BF16, device="cuda")
+        loader.linear_distillation_backward(dA, None, dloss, lse, picked, a, w, listed, teacher, M, N, K, temperature=t)
+        for row in (0, M // 2):
+            at = slice(row, row + M // 2)
+            loader.linear_distillation_backward(halves[at], None, dloss[at], lse[at], picked[at], a[at], w, listed[at], teacher[at], M // 2, N, K,
+                                                temperature=t)
+        assert torch.isfinite(dA[::4099].float()).all() and torch.equal(dA, halves)
