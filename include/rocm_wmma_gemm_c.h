@@ -333,7 +333,7 @@ typedef struct rocm_wmma_gemm_routing
 
 /* chosen (M x k): the experts of the largest biased score, of the largest logit where there is no bias, the best
  * first; of equal ones the lower expert.  weights (M x k): their scores, without the bias.  What decides is worked out in
- * fp64.  A masked token's experts are -1, its weights 0.  A logit of -infinity has the score 0; a token whose chosen
+ * fp64; biased scores that differ by less than 2^-43 of themselves may count as equal.  A masked token's experts are -1, its weights 0.  A logit of -infinity has the score 0; a token whose chosen
  * scores are all 0 has weights 0.  A logit that is no number counts as the lowest value: the others are chosen as without it,
  * and its token's weights may be no numbers. */
 int rocm_wmma_gemm_route(int logits_type, int* chosen, float* weights, const void* logits,

@@ -160,8 +160,8 @@ __device__ __forceinline__ double sigmoid(double x)
 }
 
 // A choice as one number that v_max_f64 orders: the value, whose last 9 bits tell the expert, so that of equal
-// values the lower expert is more.  (The values that the bits can confuse differ by 2^-44 of themselves; logits, which
-// have 24 bits, none.)  No number counts as the lowest value.
+// values the lower expert is more.  (Values that differ by less than 2^-43 of themselves may count as equal: 9 bits of 52; logits, which
+// have 24 bits, are told apart.)  No number counts as the lowest value.
 constexpr int choice_bits = 511;
 __device__ __forceinline__ double choice_key(double value, int expert)
 {
@@ -214,7 +214,7 @@ __device__ __forceinline__ void sort_falling(double (&key)[COUNT])
 // Mathematics: scores s = softmax(x) or 1 / (1 + e^-x); the k experts of the largest s + bias (of the largest x where there is
 // no bias: the same order) among the experts of the `kept` groups whose `best` largest s + bias sum to most; weights scale s,
 // or scale s over the sum of the chosen s.  Everything that decides is held in fp64, so that the choice is the definition's
-// and not that of a rounding; fp64 runs at the fp32 rate here.
+// and not that of fp32's roundings; fp64 runs at the fp32 rate here.
 //
 // Bound by the instructions: 8191 tokens over 256 experts in groups are 2 waves for every SIMD, whose 16 scores a lane, their sort and
 // eight rounds of a maximum over 16 lanes (four DPP steps) are some 1100 instructions: 7.9 us a call (8.4 MB, 1.1 TB/s).
@@ -429,16 +429,8 @@ struct route_back_args
     float        scale;
 };
 
-// The gradient of the weights by the logits; the choice itself has none.  With ds_j = scale (dw_j - D) / sum, D = sum_i dw_i
-// w_i / scale, (renormalised; else scale dw_j): sigmoid dx_j = ds_j s_j (1 - s_j) for the chosen, 0 for the others; softmax
-// dx_e = s_e (ds_e - sum_j s_j ds_j), where the sum is 0 if the weights are renormalised, so that the logits
-// that were not chosen are not even read.  Softmax's largest score of the chosen is 1 before it is divided by anything, so
-// fp32 holds all of it.  A sigmoid's scores may all be far below fp32's least number, and their shares of the sum are ordinary
-// numbers all the same: they are worked out in fp64, as for the weights, and nothing but the result is rounded to fp32.
-// Sixteen lanes a token, CHUNK experts a lane; a choice outside the experts has no gradient, one that is listed twice has both.
-// Bound by the latency of a token's chain (its choices, their logits, the joins over 16 lanes, the places in LDS): 16384 tokens of
-// 128 experts in bf16, 8 choices each, take 6.4 us, 9 MB at 1.4 TB/s; 6.5 us by sigmoid (6.1 with
-// its scores in fp32, which gave 0 and infinities for logits of -80 and below).
+// What a lane's two choices get by sigmoid scores (see route_back_token); a choice that is none has a logit of -infinity and a
+// gradient of 0.
 __device__ __forceinline__ void sigmoid_gradients(const route_back_args& args, const float (&logit)[2], const float (&dw)[2],
                                                   float (&own)[2])
 {
@@ -463,6 +455,16 @@ __device__ __forceinline__ void sigmoid_gradients(const route_back_args& args, c
     own[1] = (float)(s[1] * (ds[1] - dot) * rest[1]);
 }
 
+// The gradient of the weights by the logits; the choice itself has none.  With ds_j = scale (dw_j - D) / sum, D = sum_i dw_i
+// w_i / scale, (renormalised; else scale dw_j): sigmoid dx_j = ds_j s_j (1 - s_j) for the chosen, 0 for the others; softmax
+// dx_e = s_e (ds_e - sum_j s_j ds_j), where the sum is 0 if the weights are renormalised, so that the logits
+// that were not chosen are not even read.  Softmax's largest score of the chosen is 1 before it is divided by anything, so
+// fp32 holds all of it.  A sigmoid's scores may all be far below fp32's least number, and their shares of the sum are ordinary
+// numbers all the same: they are worked out in fp64, as for the weights, and nothing but the result is rounded to fp32.
+// Sixteen lanes a token, CHUNK experts a lane; a choice outside the experts has no gradient, one that is listed twice has both.
+// Bound by the latency of a token's chain (its choices, their logits, the joins over 16 lanes, the places in LDS): 16384 tokens of
+// 128 experts in bf16, 8 choices each, take 6.4 us, 9 MB at 1.4 TB/s; 6.5 us by sigmoid (6.1 with
+// its scores in fp32, which gave 0 and infinities for logits of -80 and below).
 template<class InT, int CHUNK, bool SIGMOID, bool WHOLE>
 __device__ __forceinline__ void route_back_token(const route_back_args& args, long long token, int lane, float* row)
 {
