@@ -333,9 +333,10 @@ typedef struct rocm_wmma_gemm_routing
 
 /* chosen (M x k): the experts of the largest biased score, of the largest logit where there is no bias, the best
  * first; of equal ones the lower expert.  weights (M x k): their scores, without the bias.  What decides is worked out in
- * fp64; biased scores that differ by less than 2^-43 of themselves may count as equal.  A masked token's experts are -1, its weights 0.  A logit of -infinity has the score 0; a token whose chosen
- * scores are all 0 has weights 0.  A logit that is no number counts as the lowest value: the others are chosen as without it,
- * and its token's weights may be no numbers. */
+ * fp64; biased scores that differ by less than 2^-43 of themselves may count as equal.  A masked token's experts are -1, its
+ * weights 0.  A logit of -infinity has the score 0; a token whose chosen scores are all 0 has weights 0.  A logit that is no
+ * number counts as the lowest value: the others are chosen as without it, and its token's weights may be no numbers.  (The
+ * softmax of a token with a logit of +infinity has no value: with a bias or groups its choice means nothing.) */
 int rocm_wmma_gemm_route(int logits_type, int* chosen, float* weights, const void* logits,
                          const rocm_wmma_gemm_routing* routing, size_t M, size_t E, size_t k, void* stream);
 

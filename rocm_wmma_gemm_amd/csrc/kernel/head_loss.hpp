@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(256) join_rows(const join_args args)
 
 // The gradient of a row's logits is worked out as T dloss / most 2^14 (p - q), with `most` the largest T |dloss| of the
 // rows that are compared with something, and 0 for the others, whatever their dloss; the products' sums are brought back by
-// unit = most 2^-14 as they are rounded.  It is held in 16 bits, whose smallest number in f16 is 6e-8 (p - q is at most 1, so 2^14 stays in range), and where
-// all rows have one dloss, as under a mean, its rounding leaves p - q of a target with a small p as it is: against 64 bits a bf16
+// unit = most 2^-14 as they are rounded.  It is held in 16 bits, whose smallest number in f16 is 6e-8 (p - q is at most 1, so 2^14
+// stays in range), and where all rows have one dloss, as under a mean, its rounding leaves p - q of a target with a small p as it is: against 64 bits a bf16
 // gradient is 1.9e-3 off instead of 2.6e-3 with dloss itself in it (1.7e-3 is its own last rounding).  Gradients in fp32 hold no more
 // of it: they are 8.4e-4 off from bf16 operands and 1.3e-4 from f16 (4096 x 65536 x 4096, 2048 x 32000 x 2048).  More bits would take
 // the products of both dA and dB twice.
